@@ -15,6 +15,9 @@ in libdynconv.so, reached through a C ABI (include/dynconv.h).
 from .headwise import headwise_dynamic_convolution, _HeadwiseDynamicConvolutionFn  # noqa: F401
 from .lowrank import lowrank_dynamic_convolution, _LowrankDynamicConvolutionFn  # noqa: F401
 from .lowrank import lowrank_dynamic_convolution_grouped  # noqa: F401
+from .lowrank import lowrank_dynamic_convolution_step, lowrank_dynamic_convolution_step_grouped  # noqa: F401
+from .linattn import linear_attention, linear_attention_step  # noqa: F401
+from .norm import group_norm  # noqa: F401
 from .modules import LowRankDynamicShortConvolution, GroupedLowRankDynamicShortConvolution  # noqa: F401
 from ._capi import LIB_PATH, load as load_library  # noqa: F401
 
@@ -22,6 +25,11 @@ __all__ = [
     "headwise_dynamic_convolution",
     "lowrank_dynamic_convolution",
     "lowrank_dynamic_convolution_grouped",
+    "lowrank_dynamic_convolution_step",
+    "lowrank_dynamic_convolution_step_grouped",
+    "linear_attention",
+    "linear_attention_step",
+    "group_norm",
     "LowRankDynamicShortConvolution",
     "GroupedLowRankDynamicShortConvolution",
     "load_library",

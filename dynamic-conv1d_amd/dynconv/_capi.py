@@ -1,4 +1,4 @@
-"""ctypes binding of libdynconv.so (C ABI declared in include/dynconv.h).
+"""ctypes binding of libdynconv.so (C ABI declared in include/dynconv.h and include/dynconv_layer.h).
 
 The library is loaded lazily after `import torch`, so it binds to the HIP
 runtime torch has already mapped (both carry SONAME libamdhip64.so.7).
@@ -52,6 +52,23 @@ SIGNATURES = {
                                + [_c_vp, _c_i64] + [_c_i64] * 5 + [_c_int, _c_int, _c_vp]),
 }
 
+# name -> (restype, argtypes); mirrors include/dynconv_layer.h.
+_c_st = ctypes.POINTER(_c_i64)  # host array of strides
+_c_f = ctypes.c_float
+LAYER_SIGNATURES = {
+    "dc_linear_attention_ws_bytes": (_c_i64, [_c_i64] * 5 + [_c_int, _c_int]),
+    "dc_linear_attention_fwd": (_c_int, [_c_vp, _c_st] * 3 + [_c_vp] * 4 + [_c_st] + [_c_vp] * 2 + [_c_i64] * 6
+                                + [_c_f, _c_int, _c_vp]),
+    "dc_linear_attention_bwd": (_c_int, [_c_vp, _c_st] * 3 + [_c_vp] * 4 + [_c_st] + [_c_vp] + [_c_vp, _c_st] * 3
+                                + [_c_vp] * 2 + [_c_i64] * 6 + [_c_f, _c_int, _c_vp]),
+    "dc_linear_attention_step": (_c_int, [_c_vp, _c_st] * 3 + [_c_vp] * 4 + [_c_i64] * 5 + [_c_f, _c_int, _c_vp]),
+    "dc_group_norm_fwd": (_c_int, [_c_vp] * 5 + [_c_i64] * 3 + [_c_f] + [_c_int] * 3 + [_c_vp]),
+    "dc_group_norm_bwd_ws_bytes": (_c_i64, [_c_i64] * 3 + [_c_int]),
+    "dc_group_norm_bwd": (_c_int, [_c_vp] * 10 + [_c_i64] * 4 + [_c_f] + [_c_int] * 3 + [_c_vp]),
+    "dc_lowrank_step_grouped": (_c_int, [_c_i64, _c_vp, _c_i64] + [_c_pp] * 3 + [_c_vp] * 2 + [_c_pp] + [_c_i64] * 5
+                                + [_c_int, _c_int, _c_vp]),
+}
+
 _lib = None
 _lock = threading.Lock()
 # The native autograd binding (csrc/torch_binding.cpp, built beside the library),
@@ -94,7 +111,7 @@ def load(path: str = LIB_PATH):
                 "`python dynamic-conv1d_amd/build.py` (or __graft_entry__.build())"
             )
         lib = ctypes.CDLL(path)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **LAYER_SIGNATURES}.items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
@@ -130,6 +147,11 @@ def ptr_array(ts):
     return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
 
 
+def int64_array(values):
+    """A host array of int64 (a `const int64_t*` argument)."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
 # torch's current-stream handle without building a Stream object (2 us -> 0.1 us per call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _get_device = getattr(torch._C, "_cuda_getDevice", None)
@@ -154,6 +176,12 @@ def on_tensor_device(fn):
             return fn(ctx, *args)
 
     return wrapper
+
+
+def on_first_device(fn):
+    """on_tensor_device for a plain function whose first argument is a tensor."""
+    run = on_tensor_device(lambda ctx, *args: fn(*args))
+    return functools.wraps(fn)(lambda *args: run(None, *args))
 
 
 def stream_of(t: torch.Tensor):

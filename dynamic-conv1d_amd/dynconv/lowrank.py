@@ -267,3 +267,89 @@ def lowrank_dynamic_convolution_grouped(
     assert hd == 0 or (0 < hd <= D and D % hd == 0), "head_dim must divide D"
     params = z + U + (static_w if has_static else [])
     return _GroupedLowrankDynamicConvolutionFn.apply(x, residual, G, has_static, hd, *params)
+
+
+@_capi.on_first_device
+def _step_grouped(x, z, U, state, static_w, residual, slots, W):
+    N, C = x.shape
+    G = len(z)
+    D = C // G
+    y = torch.empty(G, N, D, dtype=x.dtype, device=x.device)
+    ys = y.unbind(0)
+    status = _capi.load().dc_lowrank_step_grouped(
+        G, _capi.ptr(x), x.stride(0), _capi.ptr_array(z), _capi.ptr_array(U), _capi.ptr_array(static_w),
+        _capi.ptr(state), _capi.ptr(slots), _capi.ptr_array(ys), N, D, z[0].shape[-1], W, state.shape[0],
+        _capi.dtype_code(x.dtype), int(bool(residual)), _capi.stream_of(x))
+    _capi.check(status, "lowrank step")
+    return ys
+
+
+def lowrank_dynamic_convolution_step_grouped(
+    x: torch.Tensor,
+    z,
+    U,
+    state: torch.Tensor,
+    static_w=None,
+    residual: bool = False,
+    slots: torch.Tensor | None = None,
+):
+    """lowrank_dynamic_convolution_grouped for one more token of each of N sequences; `state` is updated in place.
+
+    Args:
+        x:        [N, G*D], the new token's fused projection, channels contiguous.
+        z:        G tensors [N, R], contiguous.
+        U:        G tensors [R, W*D], contiguous; static_w: None, or G tensors [W, D].
+        state:    [slots, W-1, G*D] of x's dtype, contiguous: each sequence's last W-1 rows of x, oldest first (zeros
+                  before its first token).  The oldest goes, x comes in behind the others.
+        slots:    [N] int32 on the device, the row of `state` of each sequence; distinct, except that ids outside the
+                  cache (-1) mark sequences that take no part: their outputs are zero.  None: row n.
+
+    Returns:
+        a tuple of G tensors [N, D]: row t of what the whole-sequence operator gives for the sequence so far.
+        Serving only: no gradients.
+    """
+    z, U = list(z), list(U)
+    G = len(z)
+    assert 1 <= G <= 4, "between 1 and 4 groups"
+    assert len(U) == G and (static_w is None or len(static_w) == G), "one U (and static_w) per group"
+    assert x.is_cuda and x.dim() == 2 and x.shape[0] > 0 and x.shape[1] > 0 and x.shape[1] % G == 0, "x must be [N, G*D]"
+    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    N, C = x.shape
+    D, R = C // G, z[0].shape[-1]
+    rank = R if static_w is None else R + 1
+    assert rank & (rank - 1) == 0, "rank R must be a power of 2. If static_w is set R+1 must be a power of 2."
+    W = U[0].shape[-1] // D
+    tensors = [*z, *U, state] + ([] if static_w is None else list(static_w))
+    assert all(t.device == x.device and t.is_contiguous() for t in tensors), "contiguous tensors on x's device"
+    assert all(t.dtype == x.dtype for t in tensors), "x, z, U, static_w and state must share one dtype"
+    assert not (torch.is_grad_enabled() and any(t.requires_grad for t in [x, *tensors])), \
+        "the step has no gradient: call it under torch.no_grad()"
+    for g in range(G):
+        assert tuple(z[g].shape) == (N, R), "every z must be [N, R]"
+        assert U[g].dim() == 2 and tuple(U[g].shape) == (R, W * D) and W > 0, "every U must be [R, W*D]"
+        assert static_w is None or tuple(static_w[g].shape) == (W, D), "every static_w must be [W, D]"
+    assert state.dim() == 3 and tuple(state.shape[1:]) == (W - 1, C), "state must be [slots, W-1, G*D]"
+    if slots is None:
+        assert N <= state.shape[0], "more sequences than rows of state"
+    else:
+        assert slots.device == x.device and slots.dtype in (torch.int32, torch.int64) and tuple(slots.shape) == (N,), \
+            "slots must be int32 [N], on x's device"
+        slots = slots.to(torch.int32).contiguous()
+    return _step_grouped(x, z, U, state, None if static_w is None else list(static_w), residual, slots, W)
+
+
+def lowrank_dynamic_convolution_step(
+    x: torch.Tensor,
+    z: torch.Tensor,
+    U: torch.Tensor,
+    state: torch.Tensor,
+    static_w: torch.Tensor | None = None,
+    residual: bool = False,
+    slots: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """lowrank_dynamic_convolution for one more token of each sequence: x [N, D], z [N, R], state [slots, W-1, D].
+
+    One group of lowrank_dynamic_convolution_step_grouped (see there); returns y [N, D]."""
+    sw = None if static_w is None else [static_w]
+    return lowrank_dynamic_convolution_step_grouped(x, [z], [U], state, static_w=sw, residual=residual, slots=slots)[0]
