@@ -1,122 +1,178 @@
-// Linear attention with a decay for each head (include/dynconv_layer.h).
+// Linear attention with a decay for each head: passes, segments and launches
+// (kernels: linattn_mfma.h).
 //
-//   S_t = g S_{t-1} + skv k_t^T v_t,    o_t = so q_t S_t,    g = exp(log_decay[h])
+//   S_t = g S_{t-1} + k_t^T v_t,    o_t = s q_t S_t,    g = exp(log_decay[h])
 //
 // The forward is one pass of this recurrence; the backward is three more, each
 // the same recurrence on other tensors:
 //   dq_t = s (S_t do_t)             forward in time on (do, v, k): state S^T
-//   dk_t = (dS_t v_t)               backward in time on (v, do, q): state dS^T
-//   dv_t = (k_t dS_t)               backward in time on (k, q, do): state dS
+//   dk_t = (dS_t v_t)               against time on (v, do, q): state dS^T
+//   dv_t = (k_t dS_t)               against time on (k, q, do): state dS
 // with dS_t = g dS_{t+1} + s q_t^T do_t.  The gradient of the final state enters
 // dS at the last token without a factor, and g dS_0 is the initial state's.
 //
-// This kernel walks the tokens one by one: a workgroup holds 64 columns of one
-// head's state in registers, four threads to a column.
-#include "dc_common.h"
+// Where batch x heads leave CUs idle, tokens are cut into segments: one launch
+// forms each segment's state from zero (k and v are read), a second carries the
+// states from segment to segment, the third runs the chunks of every segment from
+// its state.  dk and dv walk the same states, turned over.
 #include "layer_launch.h"
+#include "linattn_mfma.h"
 
 namespace dc {
 namespace {
 
-constexpr int kCols = 64, kRowGroups = 4, kTile = 16;
+using la::Args;
 
-template <typename T, int KR>
-__global__ __launch_bounds__(256) void la_recurrent(LaProblem P) {
-  constexpr int KP = KR * kRowGroups;
-  __shared__ float sq[kTile][KP], sk[kTile][KP], sv[kTile][kCols], part[kTile][kRowGroups][kCols];
-  const LaPass& p = P.pass[blockIdx.z];
-  const int64_t b = blockIdx.x / P.H, h = blockIdx.x % P.H;
-  const int n = threadIdx.x % kCols, rg = threadIdx.x / kCols;
-  const int col0 = blockIdx.y * kCols, col = col0 + n;
-  if (col0 >= p.V) return;
-  const float g = expf(P.log_decay[h]);
-  const int nt_all = (int)P.T;
-  const int len = P.lengths ? min(max(P.lengths[b], 0), nt_all) : nt_all;
-  const int64_t sbase = (int64_t)blockIdx.x * p.K * p.V;
+int cover(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : 256; }
 
-  float S[KR];
-#pragma unroll
-  for (int i = 0; i < KR; ++i) {
-    const int a = rg * KR + i;
-    S[i] = p.s_in && a < p.K && col < p.V ? p.s_in[sbase + a * p.s_row + col * p.s_col] : 0.f;
-  }
-  const T* q = (const T*)p.q + b * p.qs[0] + h * p.qs[1];
-  const T* k = (const T*)p.k + b * p.ks[0] + h * p.ks[1];
-  const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
-  T* o = (T*)p.o + b * p.os[0] + h * p.os[1];
+struct Cut {
+  int seg, nseg;
+};
 
-  for (int t0 = 0; t0 < len; t0 += kTile) {
-    const int nt = min(kTile, len - t0);
-    for (int i = threadIdx.x; i < nt * KP; i += 256) {
-      const int r = i / KP, a = i % KP;
-      const int64_t t = p.rev ? len - 1 - t0 - r : t0 + r;
-      sq[r][a] = a < p.K ? (float)q[t * p.qs[2] + a] : 0.f;
-      sk[r][a] = a < p.K ? (float)k[t * p.ks[2] + a] : 0.f;
-    }
-    for (int i = threadIdx.x; i < nt * kCols; i += 256) {
-      const int r = i / kCols, c = i % kCols;
-      const int64_t t = p.rev ? len - 1 - t0 - r : t0 + r;
-      sv[r][c] = col0 + c < p.V ? (float)v[t * p.vs[2] + col0 + c] * p.skv : 0.f;
-    }
-    __syncthreads();
-    for (int r = 0; r < nt; ++r) {
-      const float d = p.rev && t0 + r == 0 ? 1.f : g, vn = sv[r][n];
-      float acc = 0.f;
-#pragma unroll
-      for (int i = 0; i < KR; ++i) {
-        S[i] = d * S[i] + sk[r][rg * KR + i] * vn;
-        acc += sq[r][rg * KR + i] * S[i];
-      }
-      part[r][rg][n] = acc;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < nt * kCols; i += 256) {
-      const int r = i / kCols, c = i % kCols;
-      const int64_t t = p.rev ? len - 1 - t0 - r : t0 + r;
-      if (col0 + c < p.V)
-        o[t * p.os[2] + col0 + c] = (T)(p.so * ((part[r][0][c] + part[r][1][c]) + (part[r][2][c] + part[r][3][c])));
-    }
-  }
-  for (int64_t i = threadIdx.x; i < (int64_t)(nt_all - len) * kCols; i += 256) {
-    const int64_t t = len + i / kCols;
-    const int c = i % kCols;
-    if (col0 + c < p.V) o[t * p.os[2] + col0 + c] = (T)0.f;
-  }
-  if (p.s_out) {
-    const float d = p.rev && len > 0 ? g : 1.f;
-#pragma unroll
-    for (int i = 0; i < KR; ++i) {
-      const int a = rg * KR + i;
-      if (a < p.K && col < p.V) p.s_out[sbase + a * p.s_row + col * p.s_col] = d * S[i];
-    }
-  }
+// Segments of a launch: 512 workgroups (two on a CU) where the tokens allow segments of 256.
+Cut cut_of(const LaProblem& p) {
+  int64_t wgs = 0;
+  for (int i = 0; i < p.npass; ++i) wgs += p.B * p.H * ((p.pass[i].V + 127) / 128);
+  const int64_t want = (512 + wgs - 1) / wgs, most = p.T / 256;
+  const int64_t n = want < most ? want : most;
+  if (n <= 1) return {(int)((p.T + 63) / 64 * 64), 1};
+  const int64_t seg = ((p.T + n - 1) / n + 63) / 64 * 64;
+  return {(int)seg, (int)((p.T + seg - 1) / seg)};
 }
 
-template <typename T>
-hipError_t launch_recurrent(const LaProblem& p) {
-  int K = 0, V = 0;
-  for (int i = 0; i < p.npass; ++i) {
-    K = max(K, p.pass[i].K);
-    V = max(V, p.pass[i].V);
+// Sets of segment states: the forward's one; the backward's two (dq's, and dv's that dk shares).
+int sets_of(const LaProblem& p) { return p.npass == 3 ? 2 : 1; }
+
+// States from segment to segment: states[s] <- the state before segment s.
+struct Carry {
+  const float* log_decay;
+  const int32_t* lengths;
+  float* states[2];
+  const float* s_in[2];
+  float* s_out[2];
+  int rev[2];
+  int64_t H, T, n;  // n: elements of a state
+  int seg, nseg;
+};
+
+__global__ __launch_bounds__(256) void la_carry(Carry A) {
+  const int set = blockIdx.z, rev = A.rev[set];
+  const int64_t bh = blockIdx.y, e = ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  if (e >= A.n) return;
+  const int T = (int)A.T;
+  const int len = A.lengths ? min(max(A.lengths[bh / A.H], 0), T) : T;
+  const double lam = A.log_decay[bh % A.H];
+  float* st = A.states[set] + bh * A.nseg * A.n + e;
+  float run = A.s_in[set] ? A.s_in[set][bh * A.n + e] : 0.f;
+  const float full = (float)exp(lam * A.seg);
+  for (int s = 0; s < A.nseg; ++s) {
+    const bool last = s == A.nseg - 1;
+    const float own = last && !A.s_out[set] ? 0.f : st[s * A.n];
+    st[s * A.n] = run;
+    const int cnt = min(max(len - s * A.seg, 0), A.seg) - (rev && s == 0 && len > 0 ? 1 : 0);
+    const float g = cnt == 0 ? 1.f : cnt == A.seg ? full : (float)exp(lam * cnt);
+    run = g * run + own;
   }
-  const dim3 grid((unsigned)(p.B * p.H), (unsigned)((V + kCols - 1) / kCols), (unsigned)p.npass);
-  if (K <= 32) la_recurrent<T, 8><<<grid, 256, 0, p.stream>>>(p);
-  else if (K <= 64) la_recurrent<T, 16><<<grid, 256, 0, p.stream>>>(p);
-  else if (K <= 128) la_recurrent<T, 32><<<grid, 256, 0, p.stream>>>(p);
-  else la_recurrent<T, 64><<<grid, 256, 0, p.stream>>>(p);
-  return hipGetLastError();
+  if (A.s_out[set]) A.s_out[set][bh * A.n + e] = rev && len > 0 ? (float)(run * exp(lam)) : run;
+}
+
+// Rows of whole 16-byte pieces, 64 of which stay within the 2^30 bytes of a buffer's range.
+bool whole16(const void* t, const int64_t (&st)[3], int width, int es) {
+  const int64_t n = 16 / es;
+  return reinterpret_cast<uintptr_t>(t) % 16 == 0 && st[0] % n == 0 && st[1] % n == 0 && st[2] % n == 0 && width % n == 0 &&
+         st[2] >= width && st[2] * es < (1 << 24);
+}
+
+// Rows of every tensor of a pass are whole 16-byte pieces.
+bool whole(const LaPass& a, int es, bool states) {
+  return whole16(a.k, a.ks, a.K, es) && whole16(a.v, a.vs, a.V, es) &&
+         (states || (whole16(a.q, a.qs, a.K, es) && whole16(a.o, a.os, a.V, es)));
+}
+
+// The passes whose kernel is the same go in one launch.
+hipError_t launch(const LaProblem& p, const Cut& c, float* const* states_of, bool states) {
+  const int es = dtype_size(p.dtype);
+  bool done[kLaMaxPasses] = {};
+  for (int i = 0; i < p.npass; ++i) {
+    if (done[i]) continue;
+    Args a{};
+    a.p = p;
+    a.seg = c.seg;
+    a.nseg = c.nseg;
+    const int kp = cover(p.pass[i].K), nw = p.pass[i].V <= 64 ? 2 : 4;
+    const bool w = whole(p.pass[i], es, states);
+    a.nvb = 1;
+    for (int j = i; j < p.npass; ++j) {
+      const LaPass& b = p.pass[j];
+      if (done[j] || cover(b.K) != kp || (b.V <= 64 ? 2 : 4) != nw || whole(b, es, states) != w) continue;
+      done[j] = true;
+      a.p.pass[a.npass] = b;
+      a.states[a.npass++] = c.nseg > 1 ? states_of[j] : nullptr;
+      const int nvb = (b.V + nw * 32 - 1) / (nw * 32);
+      if (nvb > a.nvb) a.nvb = nvb;
+    }
+    const int64_t nblk = p.B * p.H * c.nseg * a.nvb;
+    if (nblk > 0x7fffffff) return hipErrorInvalidValue;
+    a.nblk = (int)nblk;
+    hipError_t e;
+    switch (p.dtype) {
+      case kBF16: e = la::launch<bf16>(a, kp, nw, w, states, p.stream); break;
+      case kFP16: e = la::launch<fp16>(a, kp, nw, w, states, p.stream); break;
+      default: e = la::launch<float>(a, kp, nw, w, states, p.stream); break;
+    }
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
 
-int64_t la_ws_bytes(const LaProblem&) { return 0; }
+int64_t la_ws_bytes(const LaProblem& p) {
+  const Cut c = cut_of(p);
+  if (c.nseg == 1) return 0;
+  return sets_of(p) * p.B * p.H * c.nseg * (int64_t)p.pass[0].K * p.pass[0].V * (int64_t)sizeof(float);
+}
 
 hipError_t la_run(const LaProblem& p) {
-  switch (p.dtype) {
-    case kBF16: return launch_recurrent<bf16>(p);
-    case kFP16: return launch_recurrent<fp16>(p);
-    default: return launch_recurrent<float>(p);
+  const Cut c = cut_of(p);
+  float* of[kLaMaxPasses] = {};
+  if (c.nseg > 1) {
+    const int sets = sets_of(p);
+    const int64_t n = (int64_t)p.pass[0].K * p.pass[0].V, set = p.B * p.H * c.nseg * n;
+    float* ws = static_cast<float*>(p.ws);
+    of[0] = ws;
+    of[1] = of[2] = ws + set;
+    // a set's states are formed by the pass whose state lies row by row: dq's k and v change places, dv's stay
+    LaProblem f = p;
+    f.npass = sets;
+    if (sets == 2) f.pass[1] = p.pass[2];
+    Carry y{};
+    for (int i = 0; i < sets; ++i) {
+      LaPass& a = f.pass[i];
+      if (a.s_col != 1) {
+        const LaPass t = a;
+        a.k = t.v; a.v = t.k;
+        for (int d = 0; d < 3; ++d) {
+          a.ks[d] = t.vs[d];
+          a.vs[d] = t.ks[d];
+        }
+        a.K = t.V; a.V = t.K; a.s_row = t.s_col; a.s_col = 1;
+      }
+      y.states[i] = of[i];
+      y.s_in[i] = a.s_in;
+      y.s_out[i] = a.s_out;
+      y.rev[i] = a.rev;
+    }
+    hipError_t e = launch(f, c, of, true);
+    if (e != hipSuccess) return e;
+    y.log_decay = p.log_decay;
+    y.lengths = p.lengths;
+    y.H = p.H; y.T = p.T; y.n = n;
+    y.seg = c.seg; y.nseg = c.nseg;
+    la_carry<<<dim3((unsigned)((n + 255) / 256), (unsigned)(p.B * p.H), (unsigned)sets), 256, 0, p.stream>>>(y);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
   }
+  return launch(p, c, of, false);
 }
 
 }  // namespace dc

@@ -1,0 +1,4 @@
+// The fp16 linear attention kernels (linattn_mfma.h).
+#include "linattn_mfma.h"
+
+template hipError_t dc::la::launch<dc::fp16>(const dc::la::Args&, int, int, bool, bool, hipStream_t);

@@ -1,0 +1,445 @@
+// Linear attention with a decay for each head, in chunks of tokens on matrix
+// cores (include/dynconv_layer.h).  One pass (LaPass) is, for each head,
+//
+//   S_t = g S_{t-1} + skv k_t^T v_t,    o_t = so q_t S_t
+//
+// and over a chunk of C tokens with the state S before it, i, j = 0 .. C-1:
+//
+//   o_i = so ( g^{i+1} q_i S + sum_{j<=i} g^{i-j} (q_i . k_j) skv v_j )
+//   S  <- g^C S + sum_j k_j^T (skv g^{C-1-j} v_j)
+//
+// Four matrix products: scores, scores * v, q * S, k^T * v.  The forward is one
+// pass; dq, dk and dv are passes on other tensors (linattn.hip), those of dk and
+// dv against time, where the tokens are loaded in turned order and all else is
+// alike.  The state that enters a pass against time (the gradient of the final
+// state) meets its first token without a decay.
+//
+// Layout.  A workgroup takes one segment of one head's tokens, chunk after
+// chunk, and NW * 32 columns of v; a wavefront keeps its 32 columns of S in
+// float32 accumulators for the whole segment.  v_mfma_f32_32x32x16 leaves
+// element (row, col) of its result in lane col + 32 ((row/4) % 2), register
+// row%4 + 4 (row/8); an operand wants 8 values of the summed index in a lane.
+// Every product here sums in the order that results come in (step s: 16 s +
+// 8 (e/4) + 4 half + e%4 for element e), so scores and S go from results to
+// operands without leaving their lane: scores are formed as k q^T (column i in
+// lane i), S as k^T v (column n in lane n), o as (v^T scores^T + S^T q^T), whose
+// column i sits in lane i with four neighbouring channels to a store.  q and k
+// rows are read from LDS 4 values at a time in that order, v and k columns
+// through transposing reads.  The scores are formed by each of the NW
+// wavefronts: 24 of its 78 products at 128 channels, against an exchange
+// through LDS and a barrier.
+//
+// Precision.  Scores and S are rounded to the inputs' type as operands (relative
+// 2^-8 / 2^-11 of single terms, below the rounding of o); the products that make
+// S take v g^{C-1-j} in two parts of the type (16 or 22 bits), so that a returned
+// state is a float32 result; fp16 operands that would come near that type's end
+// are made 2^-16 smaller (a wavefront's scores or S together, where one of them
+// passes 2^15).  float32 inputs take float32 matrix products throughout.  All
+// sums and S are float32.
+#pragma once
+
+#include "lowrank_mfma.h"
+#include "layer_launch.h"
+
+namespace dc {
+namespace la {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// Kernel arguments: the problem, segments of seg tokens (a multiple of the
+// chunk), and the states before each segment, [B * H][nseg][K * V] per set.
+struct Args {
+  LaProblem p;
+  int npass, seg, nseg, nvb;
+  int nblk;
+  // what a pass starts its segments from / a state pass writes: one set of states (null: one segment, s_in / s_out)
+  float* states[kLaMaxPasses];
+};
+
+// Tokens of a chunk: 64, or 32 where three tiles of 64 float32 rows would pass the LDS.
+__host__ __device__ constexpr int chunk_tokens(int es, int kp) { return es == 4 && kp > 128 ? 32 : 64; }
+
+template <typename T> struct Ops {  // 16-bit types
+  typedef u32x4 Frag;
+  static constexpr bool kSplit = true, kNarrow = __is_same(T, fp16);  // two parts; float32 values may not fit
+  __device__ static __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+    if constexpr (__is_same(T, bf16))
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+  }
+  // 16 channels of row `row` (this lane's half): p points at the row's first of them
+  __device__ static __forceinline__ Frag rows(const T* p, int half) {
+    const u32x2 a = *reinterpret_cast<const u32x2*>(p + 4 * half);
+    const u32x2 b = *reinterpret_cast<const u32x2*>(p + 8 + 4 * half);
+    return Frag{a[0], a[1], b[0], b[1]};
+  }
+  // column lane%32 of 16 rows: p points at (row 0, column 0) of the 16 x 32 block, rows rs elements apart
+  __device__ static __forceinline__ Frag cols(const T* p, int rs, int lane) {
+    const T* q = p + (4 * (lane / 32) + (lane % 16) / 4) * rs + 16 * ((lane / 16) % 2) + 4 * (lane % 4);
+    const u32x2 a = lds_read_tr16(q), b = lds_read_tr16(q + 8 * rs);
+    return Frag{a[0], a[1], b[0], b[1]};
+  }
+  __device__ static __forceinline__ Frag pack(const float* v) {
+    return Frag{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])};
+  }
+  __device__ static __forceinline__ void unpack(Frag f, float* v) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = Mma16<T>::to_f(elem16(f, e));
+  }
+};
+template <> struct Ops<float> {
+  struct Frag { float v[8]; };
+  static constexpr bool kSplit = false, kNarrow = false;
+  __device__ static __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
+    return c;
+  }
+  __device__ static __forceinline__ Frag rows(const float* p, int half) {
+    Frag f;
+    load_vals<float, 4>(p + 4 * half, f.v);
+    load_vals<float, 4>(p + 8 + 4 * half, f.v + 4);
+    return f;
+  }
+  __device__ static __forceinline__ Frag cols(const float* p, int rs, int lane) {
+    Frag f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = p[(8 * (e / 4) + 4 * (lane / 32) + e % 4) * rs + lane % 32];
+    return f;
+  }
+  __device__ static __forceinline__ Frag pack(const float* v) {
+    Frag f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = v[e];
+    return f;
+  }
+  __device__ static __forceinline__ void unpack(Frag f, float* v) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = f.v[e];
+  }
+};
+
+// Elements from a row of a tile to the next in LDS: rows start 4, 12 or 36 banks
+// after each other (mod 64), which keeps both the row reads (16 rows x 8 bytes at
+// once; float32: 8 x 16) and the transposing ones (4 rows x 32 bytes) apart.
+template <typename T, int N>
+constexpr int row_elems() {
+  return N + (sizeof(T) == 4 ? 16 : N % 128 == 0 ? 48 : 16) / (int)sizeof(T);
+}
+
+// g^k, g = 2^lam2; g^0 = 1 also where lam2 is minus infinity.
+__device__ __forceinline__ float power(float lam2, int k) { return k == 0 ? 1.f : exp2f(lam2 * (float)k); }
+
+// The end of a phase: what it has read of LDS is read again by the next one, and nothing moves across.  Without it the
+// compiler keeps operands for the following phases, and spills.
+__device__ __forceinline__ void phase() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// One tile of C rows of N channels on its way from memory to LDS, in 16-byte
+// pieces, which wait in registers through the chunk before.  WHOLE: every piece of
+// a row lies inside or outside of it, 16-byte aligned, rows within 32-bit offsets of
+// each other: buffer loads, whose range drops the rows past `end`.  Otherwise
+// pieces are gathered element by element.
+constexpr int kOut = 0x7FFFFFF0;  // an offset past every range
+template <typename T, int C, int N, int NT, bool WHOLE>
+struct Tile {
+  static constexpr int VE = 16 / (int)sizeof(T), PR = N / VE, NV = C * PR / NT, RPI = NT / PR;
+  static_assert(C * PR % NT == 0 && NT % PR == 0, "whole pieces and rows to every thread");
+  u32x4 v[NV];
+  // row r of the tile is token p0 + r of a head (base), or turn - (p0 + r) where turn >= 0; rows at `end` and past it are zero
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int width, int p0, int end, int turn) {
+    const int r0 = (int)threadIdx.x / PR, c = ((int)threadIdx.x % PR) * VE;
+    if constexpr (WHOLE) {
+      // the range starts at the tile's first token in memory; a row past the end falls behind it, or (turned) before it
+      const int n = min(end - p0, C);
+      const T* first = base + (int64_t)(turn >= 0 ? turn - (p0 + n - 1) : p0) * stride;
+      const int sb = (int)stride * (int)sizeof(T);
+      const rsrc_t rs = make_rsrc_wave<(int64_t(1) << 30)>(first, ((int64_t)(n - 1) * stride + width) * (int64_t)sizeof(T));
+      const int step = turn >= 0 ? -sb : sb;
+      int off = c < width ? (turn >= 0 ? (n - 1 - r0) * sb : r0 * sb) + c * (int)sizeof(T) : kOut;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] = bload128(rs, c < width ? off + i * RPI * step : kOut);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int p = p0 + r0 + i * RPI;
+        v[i] = u32x4{0, 0, 0, 0};
+        if (p < end && c < width) {
+          const T* q = base + (int64_t)(turn >= 0 ? turn - p : p) * stride + c;
+          T e[VE];
+#pragma unroll
+          for (int j = 0; j < VE; ++j) e[j] = c + j < width ? q[j] : (T)0.f;
+          __builtin_memcpy(&v[i], e, 16);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* lds) const {
+    const int r0 = (int)threadIdx.x / PR, c = ((int)threadIdx.x % PR) * VE;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) *reinterpret_cast<u32x4*>(lds + (r0 + i * RPI) * row_elems<T, N>() + c) = v[i];
+  }
+};
+
+// The power of two that a wavefront's operands are made smaller by: one of N values passes 2^15.
+template <typename O, int N>
+__device__ __forceinline__ float shrink(const float* v) {
+  if constexpr (!O::kNarrow) return 1.f;
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]));
+  return __any(m > 32768.f) ? 1.f / 65536 : 1.f;
+}
+
+// STATES: only the state after each segment, from zero, for states[pass].
+template <typename T, int KP, int NW, int C, bool WHOLE, bool STATES>
+__global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void la_chunks(Args A) {
+  typedef Ops<T> O;
+  typedef typename O::Frag Frag;
+  constexpr int NT = NW * 64, NB = C / 32, KB = KP / 32, RK = row_elems<T, KP>(), RV = row_elems<T, NW * 32>();
+  __shared__ __align__(16) T sk[C * RK];
+  __shared__ __align__(16) T sv[C * RV];
+  __shared__ __align__(16) T sq[STATES ? 8 : C * RK];
+
+  const LaPass& P = A.p.pass[blockIdx.z];
+  int blk = xcd_remap(blockIdx.x, A.nblk);
+  const int vb = blk % A.nvb;
+  blk /= A.nvb;
+  const int seg = blk % A.nseg, bh = blk / A.nseg;
+  const int b = bh / (int)A.p.H, hd = bh % (int)A.p.H;
+  const int lane = threadIdx.x % 64, half = lane / 32, col = lane % 32, wv = wave_id();
+  const int n0 = vb * NW * 32 + wv * 32;  // first column of this wavefront
+  if (vb * NW * 32 >= P.V) return;
+  if (STATES && seg == A.nseg - 1 && !P.s_out) return;  // nothing reads the last segment's
+  const bool mine = n0 < P.V;
+  const float lam = A.p.log_decay[hd], lam2 = lam * 1.44269504088896f;
+  const int T_ = (int)A.p.T;
+  const int len = A.p.lengths ? min(max(A.p.lengths[b], 0), T_) : T_;
+  const int lo = seg * A.seg, top = min(T_, lo + A.seg), hi = min(len, top);
+  const int turn = P.rev ? len - 1 : -1;
+  const T* k = (const T*)P.k + b * P.ks[0] + hd * P.ks[1];
+  const T* v = (const T*)P.v + b * P.vs[0] + hd * P.vs[1] + vb * NW * 32;
+  const T* q = (const T*)P.q + b * P.qs[0] + hd * P.qs[1];
+  T* o = (T*)P.o + b * P.os[0] + hd * P.os[1];
+  const int vw = P.V - vb * NW * 32;
+
+  float* states = A.states[blockIdx.z];
+  if (states) states += ((int64_t)bh * A.nseg + seg) * P.K * P.V;
+  const int64_t sbase = (int64_t)bh * P.K * P.V;
+
+  f32x16 S[KB];
+  {
+    const float* from = STATES ? nullptr : states ? states : P.s_in ? P.s_in + sbase : nullptr;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int a = kb * 32 + 8 * (r / 4) + 4 * half + r % 4;
+        S[kb][r] = from && a < P.K && n0 + col < P.V ? from[a * P.s_row + (n0 + col) * P.s_col] : 0.f;
+      }
+  }
+
+  // weights that every full chunk has, element e of a step (or register r of a result) at row(e): of the last 16
+  // tokens for S, and of a score on the diagonal
+  auto row = [&](int e) { return 8 * (e / 4) + 4 * half + e % 4; };
+  float vlast[8], diag[STATES ? 1 : 16];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) vlast[e] = P.skv * power(lam2, 15 - row(e));
+  if constexpr (!STATES)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) diag[r] = row(r) <= col ? P.skv * P.so * power(lam2, col - row(r)) : 0.f;
+  const float g16 = power(lam2, 16), gcol = STATES ? 0.f : P.so * power(lam2, col + 1);
+  // g^C in two floats: a state kept over many chunks would gather the rounding of one
+  const double gc = exp((double)lam * C);
+  const float gc_hi = (float)gc, gc_lo = (float)(gc - (double)gc_hi);
+
+  Tile<T, C, KP, NT, WHOLE> tk, tq;
+  Tile<T, C, NW * 32, NT, WHOLE> tv;
+  if (lo < hi) {
+    tk.load(k, P.ks[2], P.K, lo, hi, turn);
+    tv.load(v, P.vs[2], vw, lo, hi, turn);
+    if constexpr (!STATES) tq.load(q, P.qs[2], P.K, lo, hi, turn);
+  }
+  for (int p0 = lo; p0 < hi; p0 += C) {
+    __syncthreads();  // the chunk before has been read
+    tk.store(sk);
+    tv.store(sv);
+    if constexpr (!STATES) tq.store(sq);
+    __syncthreads();
+    if (p0 + C < hi) {
+      tk.load(k, P.ks[2], P.K, p0 + C, hi, turn);
+      tv.load(v, P.vs[2], vw, p0 + C, hi, turn);
+      if constexpr (!STATES) tq.load(q, P.qs[2], P.K, p0 + C, hi, turn);
+    }
+    if (!mine) continue;
+    // weights below are products with these; opaque, or the compiler would form all of them before the loop and spill
+    float gl = gcol, g1 = g16;
+    asm volatile("" : "+v"(gl), "+v"(g1));
+    const int cl = min(C, hi - p0);            // tokens of this chunk
+    const int early = P.rev && p0 == 0 ? 1 : 0;  // the entering state meets the first token without a decay
+
+    if constexpr (!STATES) {
+      float sdown = 1.f;
+      if constexpr (O::kNarrow) {
+        sdown = shrink<O, 16>(reinterpret_cast<const float*>(&S[0]));
+#pragma unroll
+        for (int kb = 1; kb < KB; ++kb) sdown = fminf(sdown, shrink<O, 16>(reinterpret_cast<const float*>(&S[kb])));
+      }
+#pragma unroll
+      for (int ib = 0; ib < NB; ++ib) {
+        phase();
+        if (ib * 32 >= cl) break;
+        f32x16 acc = {}, sc[NB] = {};
+#pragma unroll
+        for (int s = 0; s < KP / 16; ++s) {
+          const Frag qf = O::rows(sq + (ib * 32 + col) * RK + s * 16, half);
+          float t[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) t[e] = O::kNarrow ? S[s / 2][8 * (s % 2) + e] * sdown : S[s / 2][8 * (s % 2) + e];
+          acc = O::mma(O::pack(t), qf, acc);
+#pragma unroll
+          for (int jb = 0; jb <= ib; ++jb) sc[jb] = O::mma(O::rows(sk + (jb * 32 + col) * RK + s * 16, half), qf, sc[jb]);
+        }
+        const float w = P.so / sdown * power(lam2, ib * 32 + col + 1 - early);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] *= w;
+        float up = 1.f;
+#pragma unroll
+        for (int jb = 0; jb <= ib; ++jb) {
+          float t[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r)  // g^{i-j}: on the diagonal, or by way of the block's last token
+            t[r] = sc[jb][r] * (jb == ib ? diag[r] : vlast[r % 8] * (r < 8 ? g1 * gl : gl));
+          if constexpr (O::kNarrow) {
+            const float d = shrink<O, 16>(t);
+            if (d != 1.f) {  // o in the same smaller units
+              for (int r = 0; r < 16; ++r) {
+                t[r] *= d;
+                acc[r] *= d;
+              }
+              up /= d;
+            } else if (up != 1.f) {
+              for (int r = 0; r < 16; ++r) t[r] /= up;
+            }
+          }
+#pragma unroll
+          for (int s = 0; s < 2; ++s) acc = O::mma(O::cols(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane), O::pack(t + 8 * s), acc);
+        }
+        const int i = ib * 32 + col;
+        if (i < cl) {
+          T* to = o + (int64_t)(turn >= 0 ? turn - p0 - i : p0 + i) * P.os[2] + n0 + 4 * half;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float out[4] = {acc[4 * g] * up, acc[4 * g + 1] * up, acc[4 * g + 2] * up, acc[4 * g + 3] * up};
+            const int n = n0 + 8 * g + 4 * half;
+            if constexpr (WHOLE) {
+              if (n < P.V) store_vals<T, 4>(to + 8 * g, out);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (n + j < P.V) to[8 * g + j] = (T)out[j];
+            }
+          }
+        }
+      }
+    }
+
+    phase();
+    // S <- g^cl S + k^T (skv g^{cl-1-j} v)
+    if (cl == C && !early) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[kb][r] = S[kb][r] * gc_hi + S[kb][r] * gc_lo;
+    } else {
+      const float g = power(lam2, cl - early);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[kb][r] *= g;
+    }
+#pragma unroll
+    for (int s = 0; s < C / 16; ++s) {
+      float t[8];
+      O::unpack(O::cols(sv + s * 16 * RV + wv * 32, RV, lane), t);
+      if (cl == C) {
+        float g = 1.f;  // g^{C-16-16s}
+#pragma unroll
+        for (int i = s + 1; i < C / 16; ++i) g *= g1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] *= vlast[e] * g;
+      } else {  // rows past the chunk's tokens are zero: any finite weight
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          t[e] *= P.skv * power(lam2, max(cl - 1 - 16 * s - row(e), 0));
+      }
+      const Frag v1 = O::pack(t);
+      Frag v2;
+      if constexpr (O::kSplit) {
+        float u[8];
+        O::unpack(v1, u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = t[e] - u[e];
+        v2 = O::pack(u);
+      }
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const Frag kf = O::cols(sk + s * 16 * RK + kb * 32, RK, lane);
+        S[kb] = O::mma(kf, v1, S[kb]);
+        if constexpr (O::kSplit) S[kb] = O::mma(kf, v2, S[kb]);
+      }
+    }
+  }
+
+  // the final state of a head in one segment, or the segment's own
+  float* to = STATES ? states : states ? nullptr : P.s_out ? P.s_out + sbase : nullptr;
+  if (to) {
+    const float g = !STATES && P.rev && len > 0 ? power(lam2, 1) : 1.f;
+    // opaque to the compiler, which would otherwise keep the addresses and masks of the first
+    // state's loads in registers through the whole segment (100 spilled registers)
+    int h4 = 4 * half, c = n0 + col;
+    asm volatile("" : "+v"(h4), "+v"(c));
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int a = kb * 32 + 8 * (r / 4) + h4 + r % 4;
+        if (a < P.K && c < P.V) to[a * P.s_row + c * P.s_col] = S[kb][r] * g;
+      }
+  }
+  if constexpr (!STATES) {  // rows past the sequence's length
+    const int z0 = max(len, lo), w = min(vw, NW * 32);
+    for (int64_t i = threadIdx.x; i < (int64_t)(top - z0) * w; i += NT)
+      o[(z0 + i / w) * P.os[2] + vb * NW * 32 + i % w] = (T)0.f;
+  }
+}
+
+// The kernel of a type for these sizes (instantiated in linattn_<type>.hip).
+template <typename T, int KP, int NW>
+void launch_dims(const Args& a, bool whole, bool states, hipStream_t st) {
+  constexpr int C = chunk_tokens(sizeof(T), KP);
+  const dim3 grid((unsigned)a.nblk, 1, (unsigned)a.npass);
+  if (states) {
+    if (whole) la_chunks<T, KP, NW, C, true, true><<<grid, NW * 64, 0, st>>>(a);
+    else la_chunks<T, KP, NW, C, false, true><<<grid, NW * 64, 0, st>>>(a);
+  } else {
+    if (whole) la_chunks<T, KP, NW, C, true, false><<<grid, NW * 64, 0, st>>>(a);
+    else la_chunks<T, KP, NW, C, false, false><<<grid, NW * 64, 0, st>>>(a);
+  }
+}
+template <typename T>
+hipError_t launch(const Args& a, int kp, int nw, bool whole, bool states, hipStream_t st) {
+  if (kp == 64) nw == 2 ? launch_dims<T, 64, 2>(a, whole, states, st) : launch_dims<T, 64, 4>(a, whole, states, st);
+  else if (kp == 128) nw == 2 ? launch_dims<T, 128, 2>(a, whole, states, st) : launch_dims<T, 128, 4>(a, whole, states, st);
+  else nw == 2 ? launch_dims<T, 256, 2>(a, whole, states, st) : launch_dims<T, 256, 4>(a, whole, states, st);
+  return hipGetLastError();
+}
+extern template hipError_t launch<bf16>(const Args&, int, int, bool, bool, hipStream_t);
+extern template hipError_t launch<fp16>(const Args&, int, int, bool, bool, hipStream_t);
+extern template hipError_t launch<float>(const Args&, int, int, bool, bool, hipStream_t);
+
+}  // namespace la
+}  // namespace dc
