@@ -29,19 +29,48 @@ struct Cut {
   int seg, nseg;
 };
 
-// Segments of a launch: 512 workgroups (two on a CU) where the tokens allow segments of 256.
-Cut cut_of(const LaProblem& p) {
-  int64_t wgs = 0;
-  for (int i = 0; i < p.npass; ++i) wgs += p.B * p.H * ((p.pass[i].V + 127) / 128);
-  const int64_t want = (512 + wgs - 1) / wgs, most = p.T / 256;
-  const int64_t n = want < most ? want : most;
-  if (n <= 1) return {(int)((p.T + 63) / 64 * 64), 1};
-  const int64_t seg = ((p.T + n - 1) / n + 63) / 64 * 64;
-  return {(int)seg, (int)((p.T + seg - 1) / seg)};
-}
-
 // Sets of segment states: the forward's one; the backward's two (dq's, and dv's that dk shares).
 int sets_of(const LaProblem& p) { return p.npass == 3 ? 2 : 1; }
+
+// Workgroups of a pass that a CU holds at once: by registers two wavefronts on a SIMD in 16 bits up to 128 channels, else
+// one; by LDS three tiles each.
+int resident(const LaPass& p, int dtype) {
+  const int kp = cover(p.K), nw = p.V <= 64 ? 2 : 4;
+  if (dtype == kFP32) return nw == 2 && kp == 64 ? 2 : 1;
+  if (kp == 256) return 1;
+  return nw == 4 ? 2 : kp == 64 ? 4 : 3;
+}
+
+// Segments of a problem: the count with the least estimated time, in units of a round of chunks on every CU.  A launch
+// takes whole rounds of resident workgroups; segments cost the states' launch (0.4 of a chunk's time for each of its
+// chunks, measured 72 us against 172) and carrying them (one unit for 25 MB).  Against filling 512 workgroups by division
+// alone: B2 H32 T8192 hd128 backward 9 rounds of 12 chunks for 576 workgroups, now 3 of 16.
+Cut cut_of(const LaProblem& p) {
+  const int C = la::chunk_tokens(dtype_size(p.dtype), cover(p.pass[0].K));
+  const int64_t chunks = (p.T + C - 1) / C;
+  const int sets = sets_of(p);
+  double best = 0;
+  int64_t seg = chunks;
+  for (int64_t n = 1; n <= 128 && n <= (chunks + 1) / 2; ++n) {
+    const int64_t len = (chunks + n - 1) / n;
+    if (n > 1 && (chunks + len - 1) / len != n) continue;  // the same segments as fewer
+    double t = 0, wgs = 0;
+    for (int i = 0; i < p.npass; ++i) {
+      const LaPass& a = p.pass[i];
+      const double w = (double)p.B * p.H * n * ((a.V + 127) / 128) / (256 * resident(a, p.dtype));
+      wgs += w;
+      if (n > 1 && (p.npass == 1 || i != 1)) t += 0.4 * (w < 1 ? 1 : w) * len;
+    }
+    t += (wgs <= 1 ? 1 : __builtin_ceil(wgs)) * len;
+    if (n > 1) t += 1 + 4e-8 * sets * 4 * (double)p.B * p.H * n * p.pass[0].K * p.pass[0].V;
+    if (n == 1 || t < best) {
+      best = t;
+      seg = len;
+    }
+  }
+  if (seg < 1) seg = 1;
+  return {(int)(seg * C), (int)(chunks > 0 ? (chunks + seg - 1) / seg : 1)};
+}
 
 // States from segment to segment: states[s] <- the state before segment s.
 struct Carry {
@@ -108,6 +137,7 @@ hipError_t launch(const LaProblem& p, const Cut& c, float* const* states_of, boo
       done[j] = true;
       a.p.pass[a.npass] = b;
       a.states[a.npass++] = c.nseg > 1 ? states_of[j] : nullptr;
+      a.returned |= b.s_out && states == (c.nseg > 1);
       const int nvb = (b.V + nw * 32 - 1) / (nw * 32);
       if (nvb > a.nvb) a.nvb = nvb;
     }

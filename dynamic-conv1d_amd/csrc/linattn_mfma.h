@@ -8,6 +8,9 @@
 //   o_i = so ( g^{i+1} q_i S + sum_{j<=i} g^{i-j} (q_i . k_j) skv v_j )
 //   S  <- g^C S + sum_j k_j^T (skv g^{C-1-j} v_j)
 //
+// A chunk that is not full holds its tokens in its last rows, behind rows of zeros,
+// so that the weights of k^T v are those of every chunk.
+//
 // Four matrix products: scores, scores * v, q * S, k^T * v.  The forward is one
 // pass; dq, dk and dv are passes on other tensors (linattn.hip), those of dk and
 // dv against time, where the tokens are loaded in turned order and all else is
@@ -31,8 +34,8 @@
 //
 // Precision.  Scores and S are rounded to the inputs' type as operands (relative
 // 2^-8 / 2^-11 of single terms, below the rounding of o); the products that make
-// S take v g^{C-1-j} in two parts of the type (16 or 22 bits), so that a returned
-// state is a float32 result; fp16 operands that would come near that type's end
+// S take v g^{C-1-j} in two parts of the type (16 or 22 bits), bf16 in three where
+// the state is returned, which so is a float32 result; fp16 operands that would come near that type's end
 // are made 2^-16 smaller (a wavefront's scores or S together, where one of them
 // passes 2^15).  float32 inputs take float32 matrix products throughout.  All
 // sums and S are float32.
@@ -52,6 +55,7 @@ struct Args {
   LaProblem p;
   int npass, seg, nseg, nvb;
   int nblk;
+  bool returned;  // a state formed by this launch is the caller's result
   // what a pass starts its segments from / a state pass writes: one set of states (null: one segment, s_in / s_out)
   float* states[kLaMaxPasses];
 };
@@ -149,26 +153,26 @@ struct Tile {
   static constexpr int VE = 16 / (int)sizeof(T), PR = N / VE, NV = C * PR / NT, RPI = NT / PR;
   static_assert(C * PR % NT == 0 && NT % PR == 0, "whole pieces and rows to every thread");
   u32x4 v[NV];
-  // row r of the tile is token p0 + r of a head (base), or turn - (p0 + r) where turn >= 0; rows at `end` and past it are zero
+  // the tile's last row is token `end` - 1 (or p0 + C - 1), rows before token p0 are zero; token p of a head sits at row p
+  // of `base`, or turn - p where turn >= 0
   __device__ __forceinline__ void load(const T* base, int64_t stride, int width, int p0, int end, int turn) {
-    const int r0 = (int)threadIdx.x / PR, c = ((int)threadIdx.x % PR) * VE;
+    const int n = min(end - p0, C), r0 = (int)threadIdx.x / PR - (C - n), c = ((int)threadIdx.x % PR) * VE;
     if constexpr (WHOLE) {
-      // the range starts at the tile's first token in memory; a row past the end falls behind it, or (turned) before it
-      const int n = min(end - p0, C);
+      // the range holds the n tokens: the rows before them fall in front of it, or (turned) behind
       const T* first = base + (int64_t)(turn >= 0 ? turn - (p0 + n - 1) : p0) * stride;
       const int sb = (int)stride * (int)sizeof(T);
       const rsrc_t rs = make_rsrc_wave<(int64_t(1) << 30)>(first, ((int64_t)(n - 1) * stride + width) * (int64_t)sizeof(T));
       const int step = turn >= 0 ? -sb : sb;
-      int off = c < width ? (turn >= 0 ? (n - 1 - r0) * sb : r0 * sb) + c * (int)sizeof(T) : kOut;
+      const int off = (turn >= 0 ? (n - 1 - r0) * sb : r0 * sb) + c * (int)sizeof(T);
 #pragma unroll
       for (int i = 0; i < NV; ++i) v[i] = bload128(rs, c < width ? off + i * RPI * step : kOut);
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int p = p0 + r0 + i * RPI;
+        const int r = r0 + i * RPI;
         v[i] = u32x4{0, 0, 0, 0};
-        if (p < end && c < width) {
-          const T* q = base + (int64_t)(turn >= 0 ? turn - p : p) * stride + c;
+        if (r >= 0 && c < width) {
+          const T* q = base + (int64_t)(turn >= 0 ? turn - p0 - r : p0 + r) * stride + c;
           T e[VE];
 #pragma unroll
           for (int j = 0; j < VE; ++j) e[j] = c + j < width ? q[j] : (T)0.f;
@@ -184,18 +188,24 @@ struct Tile {
   }
 };
 
-// The power of two that a wavefront's operands are made smaller by: one of N values passes 2^15.
-template <typename O, int N>
-__device__ __forceinline__ float shrink(const float* v) {
-  if constexpr (!O::kNarrow) return 1.f;
-  float m = 0.f;
+// Whether one of a wavefront's N values comes near the end of fp16: they then take part 2^-16 smaller.
+constexpr float kSmaller = 1.f / 65536;
+template <int N>
+__device__ __forceinline__ float largest(const float* v, float m = 0.f) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]));
-  return __any(m > 32768.f) ? 1.f / 65536 : 1.f;
+  for (int i = 0; i < N; i += 2) m = fmaxf(fmaxf(m, fabsf(v[i])), fabsf(v[i + 1]));
+  return m;
+}
+__device__ __forceinline__ bool near_end(float m) { return __any(!(m <= 32768.f)); }
+template <int N>
+__device__ __forceinline__ void scale(float* v, float by) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] *= by;
 }
 
-// STATES: only the state after each segment, from zero, for states[pass].
-template <typename T, int KP, int NW, int C, bool WHOLE, bool STATES>
+// STATES: only the state after each segment, from zero, for states[pass].  RETURNED: a state that is formed here is the
+// caller's result (three parts in bf16; in every kernel they cost the common one 10% by spilled registers).
+template <typename T, int KP, int NW, int C, bool WHOLE, bool STATES, bool RETURNED>
 __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void la_chunks(Args A) {
   typedef Ops<T> O;
   typedef typename O::Frag Frag;
@@ -251,10 +261,10 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
   if constexpr (!STATES)
 #pragma unroll
     for (int r = 0; r < 16; ++r) diag[r] = row(r) <= col ? P.skv * P.so * power(lam2, col - row(r)) : 0.f;
-  const float g16 = power(lam2, 16), gcol = STATES ? 0.f : P.so * power(lam2, col + 1);
-  // g^C in two floats: a state kept over many chunks would gather the rounding of one
-  const double gc = exp((double)lam * C);
-  const float gc_hi = (float)gc, gc_lo = (float)(gc - (double)gc_hi);
+  const float g16 = power(lam2, 16), gcol = P.so * power(lam2, col + 1);
+  const float gC = power(lam2, C);
+
+  constexpr bool three = __is_same(T, bf16) && RETURNED;
 
   Tile<T, C, KP, NT, WHOLE> tk, tq;
   Tile<T, C, NW * 32, NT, WHOLE> tv;
@@ -275,72 +285,88 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
       if constexpr (!STATES) tq.load(q, P.qs[2], P.K, p0 + C, hi, turn);
     }
     if (!mine) continue;
-    // weights below are products with these; opaque, or the compiler would form all of them before the loop and spill
-    float gl = gcol, g1 = g16;
-    asm volatile("" : "+v"(gl), "+v"(g1));
-    const int cl = min(C, hi - p0);            // tokens of this chunk
-    const int early = P.rev && p0 == 0 ? 1 : 0;  // the entering state meets the first token without a decay
+    const int cl = min(C, hi - p0), shift = C - cl;  // tokens of this chunk: its last rows
+    const int early = P.rev && p0 == 0 ? 1 : 0;      // the entering state meets the first token without a decay
+    // opaque, or the compiler forms every product of these weights before the loop, and spills
+    float g1 = g16;
+    asm volatile("" : "+v"(g1));
+    float* const Sf = reinterpret_cast<float*>(S);
 
     if constexpr (!STATES) {
-      float sdown = 1.f;
+      f32x16 acc[NB] = {};
+      bool small = false;
       if constexpr (O::kNarrow) {
-        sdown = shrink<O, 16>(reinterpret_cast<const float*>(&S[0]));
-#pragma unroll
-        for (int kb = 1; kb < KB; ++kb) sdown = fminf(sdown, shrink<O, 16>(reinterpret_cast<const float*>(&S[kb])));
+        small = near_end(largest<KB * 16>(Sf));
+        if (small) scale<KB * 16>(Sf, kSmaller);
       }
+#pragma unroll
+      for (int s = 0; s < KP / 16; ++s) {
+        const Frag sf = O::pack(Sf + s * 8);
+#pragma unroll
+        for (int ib = 0; ib < NB; ++ib) acc[ib] = O::mma(sf, O::rows(sq + (ib * 32 + col) * RK + s * 16, half), acc[ib]);
+      }
+      if constexpr (O::kNarrow)
+        if (small) {
+          scale<KB * 16>(Sf, 1.f / kSmaller);
+#pragma unroll
+          for (int ib = 0; ib < NB; ++ib) scale<16>(reinterpret_cast<float*>(&acc[ib]), 1.f / kSmaller);
+        }
 #pragma unroll
       for (int ib = 0; ib < NB; ++ib) {
         phase();
-        if (ib * 32 >= cl) break;
-        f32x16 acc = {}, sc[NB] = {};
+        if (ib * 32 + 31 < shift) continue;
+        const int jb0 = shift / 32;  // the first block with tokens
+        float* const af = reinterpret_cast<float*>(&acc[ib]);
+        f32x16 sc[NB] = {};
 #pragma unroll
         for (int s = 0; s < KP / 16; ++s) {
           const Frag qf = O::rows(sq + (ib * 32 + col) * RK + s * 16, half);
-          float t[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) t[e] = O::kNarrow ? S[s / 2][8 * (s % 2) + e] * sdown : S[s / 2][8 * (s % 2) + e];
-          acc = O::mma(O::pack(t), qf, acc);
 #pragma unroll
           for (int jb = 0; jb <= ib; ++jb) sc[jb] = O::mma(O::rows(sk + (jb * 32 + col) * RK + s * 16, half), qf, sc[jb]);
         }
-        const float w = P.so / sdown * power(lam2, ib * 32 + col + 1 - early);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[r] *= w;
-        float up = 1.f;
-#pragma unroll
-        for (int jb = 0; jb <= ib; ++jb) {
-          float t[16];
-#pragma unroll
-          for (int r = 0; r < 16; ++r)  // g^{i-j}: on the diagonal, or by way of the block's last token
-            t[r] = sc[jb][r] * (jb == ib ? diag[r] : vlast[r % 8] * (r < 8 ? g1 * gl : gl));
+        bool tiny = false;  // acc is held smaller
+        auto add = [&](float* t, int jb) {
           if constexpr (O::kNarrow) {
-            const float d = shrink<O, 16>(t);
-            if (d != 1.f) {  // o in the same smaller units
-              for (int r = 0; r < 16; ++r) {
-                t[r] *= d;
-                acc[r] *= d;
-              }
-              up /= d;
-            } else if (up != 1.f) {
-              for (int r = 0; r < 16; ++r) t[r] /= up;
+            if (tiny) scale<16>(t, kSmaller);
+            else if (near_end(largest<16>(t))) {
+              tiny = true;
+              scale<16>(t, kSmaller);
+              scale<16>(af, kSmaller);
             }
           }
 #pragma unroll
-          for (int s = 0; s < 2; ++s) acc = O::mma(O::cols(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane), O::pack(t + 8 * s), acc);
+          for (int s = 0; s < 2; ++s)
+            acc[ib] = O::mma(O::cols(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane), O::pack(t + 8 * s), acc[ib]);
+        };
+        if (NB > 1 && ib > jb0) {
+          // the state and the block before by way of its last token: g^{i+1} = g^{32} g^{col+1}, g^{i-j} = g^{col+1} g^{31-j}
+          scale<16>(af, power(lam2, 32 - early - shift));
+          float t[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) t[r] = sc[0][r] * (r < 8 ? vlast[r] * g1 : vlast[r - 8]);
+          add(t, 0);
+          scale<16>(af, gcol);
+        } else {
+          scale<16>(af, P.so * power(lam2, max(ib * 32 + col + 1 - early - shift, 0)));
         }
-        const int i = ib * 32 + col;
-        if (i < cl) {
+        float t[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t[r] = sc[ib][r] * diag[r];
+        add(t, ib);
+        if constexpr (O::kNarrow)
+          if (tiny) scale<16>(af, 1.f / kSmaller);
+        const int i = ib * 32 + col - shift;
+        if (i >= 0) {
           T* to = o + (int64_t)(turn >= 0 ? turn - p0 - i : p0 + i) * P.os[2] + n0 + 4 * half;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const float out[4] = {acc[4 * g] * up, acc[4 * g + 1] * up, acc[4 * g + 2] * up, acc[4 * g + 3] * up};
             const int n = n0 + 8 * g + 4 * half;
             if constexpr (WHOLE) {
-              if (n < P.V) store_vals<T, 4>(to + 8 * g, out);
+              if (n < P.V) store_vals<T, 4>(to + 8 * g, af + 4 * g);
             } else {
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                if (n + j < P.V) to[8 * g + j] = (T)out[j];
+                if (n + j < P.V) to[8 * g + j] = (T)af[4 * g + j];
             }
           }
         }
@@ -348,48 +374,37 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
     }
 
     phase();
-    // S <- g^cl S + k^T (skv g^{cl-1-j} v)
-    if (cl == C && !early) {
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) S[kb][r] = S[kb][r] * gc_hi + S[kb][r] * gc_lo;
-    } else {
-      const float g = power(lam2, cl - early);
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) S[kb][r] *= g;
-    }
+    // S <- g^cl S + k^T (skv g^{C-1-row} v)
+    scale<KB * 16>(Sf, cl == C && !early ? gC : power(lam2, cl - early));
 #pragma unroll
     for (int s = 0; s < C / 16; ++s) {
-      float t[8];
+      float t[8], g = 1.f;  // g^{C-16-16s}
+#pragma unroll
+      for (int i = s + 1; i < C / 16; ++i) g *= g1;
       O::unpack(O::cols(sv + s * 16 * RV + wv * 32, RV, lane), t);
-      if (cl == C) {
-        float g = 1.f;  // g^{C-16-16s}
 #pragma unroll
-        for (int i = s + 1; i < C / 16; ++i) g *= g1;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] *= vlast[e] * g;
-      } else {  // rows past the chunk's tokens are zero: any finite weight
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          t[e] *= P.skv * power(lam2, max(cl - 1 - 16 * s - row(e), 0));
-      }
+      for (int e = 0; e < 8; ++e) t[e] *= vlast[e] * g;
       const Frag v1 = O::pack(t);
-      Frag v2;
+      Frag v2, v3;
       if constexpr (O::kSplit) {
         float u[8];
         O::unpack(v1, u);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[e] = t[e] - u[e];
-        v2 = O::pack(u);
+        for (int e = 0; e < 8; ++e) t[e] -= u[e];
+        v2 = O::pack(t);
+        if (three) {
+          O::unpack(v2, u);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) t[e] -= u[e];
+          v3 = O::pack(t);
+        }
       }
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const Frag kf = O::cols(sk + s * 16 * RK + kb * 32, RK, lane);
         S[kb] = O::mma(kf, v1, S[kb]);
         if constexpr (O::kSplit) S[kb] = O::mma(kf, v2, S[kb]);
+        if (three) S[kb] = O::mma(kf, v3, S[kb]);
       }
     }
   }
@@ -422,12 +437,14 @@ template <typename T, int KP, int NW>
 void launch_dims(const Args& a, bool whole, bool states, hipStream_t st) {
   constexpr int C = chunk_tokens(sizeof(T), KP);
   const dim3 grid((unsigned)a.nblk, 1, (unsigned)a.npass);
+  const bool returned = __is_same(T, bf16) && a.returned;
+  auto run = [&](auto kernel) { kernel<<<grid, NW * 64, 0, st>>>(a); };
   if (states) {
-    if (whole) la_chunks<T, KP, NW, C, true, true><<<grid, NW * 64, 0, st>>>(a);
-    else la_chunks<T, KP, NW, C, false, true><<<grid, NW * 64, 0, st>>>(a);
+    if (returned) run(whole ? la_chunks<T, KP, NW, C, true, true, __is_same(T, bf16)> : la_chunks<T, KP, NW, C, false, true, __is_same(T, bf16)>);
+    else run(whole ? la_chunks<T, KP, NW, C, true, true, false> : la_chunks<T, KP, NW, C, false, true, false>);
   } else {
-    if (whole) la_chunks<T, KP, NW, C, true, false><<<grid, NW * 64, 0, st>>>(a);
-    else la_chunks<T, KP, NW, C, false, false><<<grid, NW * 64, 0, st>>>(a);
+    if (returned) run(whole ? la_chunks<T, KP, NW, C, true, false, __is_same(T, bf16)> : la_chunks<T, KP, NW, C, false, false, __is_same(T, bf16)>);
+    else run(whole ? la_chunks<T, KP, NW, C, true, false, false> : la_chunks<T, KP, NW, C, false, false, false>);
   }
 }
 template <typename T>
