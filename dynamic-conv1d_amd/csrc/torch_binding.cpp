@@ -1,4 +1,4 @@
-// Native autograd binding of the C ABI (include/dynconv.h) for PyTorch: the
+// Native autograd binding of the C ABI (include/dynconv.h, dynconv_layer.h) for PyTorch: the
 // operators' autograd Functions as C++ nodes, called from dynconv/*.py.
 //
 // A small or medium call is bound by its host path.  Through Python's
@@ -19,6 +19,8 @@
 
 #include <dlfcn.h>
 
+#include <cmath>
+
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
@@ -31,6 +33,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include "dynconv.h"
+#include "dynconv_layer.h"
 
 namespace {
 
@@ -55,6 +58,14 @@ struct Abi {
   decltype(&dc_proj_in_fwd) proj_in_fwd;
   decltype(&dc_proj_in_bwd_ws_bytes) proj_in_bwd_ws_bytes;
   decltype(&dc_proj_in_bwd) proj_in_bwd;
+  decltype(&dc_linear_attention_ws_bytes) linear_attention_ws_bytes;
+  decltype(&dc_linear_attention_fwd) linear_attention_fwd;
+  decltype(&dc_linear_attention_bwd) linear_attention_bwd;
+  decltype(&dc_linear_attention_step) linear_attention_step;
+  decltype(&dc_group_norm_fwd) group_norm_fwd;
+  decltype(&dc_group_norm_bwd_ws_bytes) group_norm_bwd_ws_bytes;
+  decltype(&dc_group_norm_bwd) group_norm_bwd;
+  decltype(&dc_lowrank_step_grouped) lowrank_step_grouped;
 };
 Abi abi{};
 bool ready = false;
@@ -275,6 +286,112 @@ struct GroupedModuleFn : public Function<GroupedModuleFn> {
   }
 };
 
+// ------------------------------------------------------- linear attention
+struct LinearAttentionFn : public Function<LinearAttentionFn> {
+  // o over token-major memory, and the final state if it is wanted
+  static variable_list run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const Tensor& s0,
+                           const Tensor& lengths, double scale, bool want_state) {
+    const int64_t B = q.size(0), H = q.size(1), T = q.size(2), K = q.size(3), V = v.size(3);
+    const int dt = dtype_code(q);
+    Tensor o = at::empty({B, T, H, V}, q.options()).transpose(1, 2);
+    Tensor st = want_state ? at::empty({B, H, K, V}, lam.options()) : Tensor();
+    const int64_t n = abi.linear_attention_ws_bytes(B, H, T, K, V, dt, 0);
+    check(n, "linear attention workspace query");
+    const Tensor ws = bytes_like(q, n);
+    check(abi.linear_attention_fwd(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(),
+                                   static_cast<float*>(ptr(lam)), static_cast<float*>(ptr(s0)),
+                                   static_cast<int32_t*>(ptr(lengths)), ptr(o), o.strides().data(),
+                                   static_cast<float*>(ptr(st)), ptr(ws), n, B, H, T, K, V, (float)scale, dt,
+                                   stream_of(q)),
+          "linear attention forward");
+    variable_list out{o};
+    if (want_state) out.push_back(st);
+    return out;
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                               const std::optional<Tensor>& s0, const Tensor& lam, const std::optional<Tensor>& lengths,
+                               double scale, bool want_state) {
+    const Tensor s = s0.value_or(Tensor()), n = lengths.value_or(Tensor());
+    variable_list out = run(q, k, v, lam, s, n, scale, want_state);
+    ctx->save_for_backward({q, k, v, s, lam, n});
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &s0 = saved[3], &lam = saved[4], &lengths = saved[5];
+    const c10::DeviceGuard guard(q.device());
+    const int64_t B = q.size(0), H = q.size(1), T = q.size(2), K = q.size(3), V = v.size(3);
+    const int dt = dtype_code(q);
+    // an output that did not reach the loss has no gradient
+    Tensor d = grads[0].defined() ? grads[0].to(q.scalar_type()) : at::zeros({B, H, T, V}, q.options());
+    if (V > 1 && d.stride(3) != 1) d = d.contiguous();
+    const Tensor ds = grads.size() > 1 && grads[1].defined() ? grad_in(grads[1], at::kFloat) : Tensor();
+    Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
+    Tensor ds0 = s0.defined() && ctx->needs_input_grad(3) ? at::empty_like(s0) : Tensor();
+    const int64_t n = abi.linear_attention_ws_bytes(B, H, T, K, V, dt, 1);
+    check(n, "linear attention backward workspace query");
+    const Tensor ws = bytes_like(q, n);
+    check(abi.linear_attention_bwd(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(),
+                                   static_cast<float*>(ptr(lam)), static_cast<float*>(ptr(s0)),
+                                   static_cast<int32_t*>(ptr(lengths)), ptr(d), d.strides().data(),
+                                   static_cast<float*>(ptr(ds)), ptr(dq), dq.strides().data(), ptr(dk),
+                                   dk.strides().data(), ptr(dv), dv.strides().data(), static_cast<float*>(ptr(ds0)),
+                                   ptr(ws), n, B, H, T, K, V, (float)ctx->saved_data["scale"].toDouble(), dt,
+                                   stream_of(q)),
+          "linear attention backward");
+    return {dq, dk, dv, ds0, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// -------------------------------------------------------------- group norm
+struct GroupNormFn : public Function<GroupNormFn> {
+  static int param_code(const Tensor& x, const Tensor& w, const Tensor& b) {
+    return dtype_code(w.defined() ? w : b.defined() ? b : x);
+  }
+  static Tensor run(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& gate, int64_t groups, int64_t act,
+                    double eps) {
+    Tensor y = at::empty_like(x);
+    const int64_t D = x.size(-1);
+    check(abi.group_norm_fwd(ptr(x), ptr(w), ptr(b), ptr(gate), ptr(y), x.numel() / D, D, groups, (float)eps, (int)act,
+                             dtype_code(x), param_code(x, w, b), stream_of(x)),
+          "group norm forward");
+    return y;
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& w,
+                        const std::optional<Tensor>& b, const std::optional<Tensor>& gate, int64_t groups, int64_t act,
+                        double eps) {
+    const Tensor wt = w.value_or(Tensor()), bt = b.value_or(Tensor()), gt = gate.value_or(Tensor());
+    Tensor y = run(x, wt, bt, gt, groups, act, eps);
+    ctx->save_for_backward({x, wt, bt, gt});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &gate = saved[3];
+    const c10::DeviceGuard guard(x.device());
+    const int64_t D = x.size(-1), M = x.numel() / D, groups = ctx->saved_data["groups"].toInt();
+    const Tensor dy = grad_in(grads[0], x.scalar_type());
+    Tensor dx = at::empty_like(x), dgate = gate.defined() ? at::empty_like(gate) : Tensor();
+    Tensor dw = w.defined() && ctx->needs_input_grad(1) ? at::empty_like(w) : Tensor();
+    // an input that is None has no place among the indexes
+    Tensor db = b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1) ? at::empty_like(b) : Tensor();
+    const int dt = dtype_code(x);
+    const int64_t n = dw.defined() || db.defined() ? abi.group_norm_bwd_ws_bytes(M, D, groups, dt) : 0;
+    check(n, "group norm backward workspace query");
+    const Tensor ws = bytes_like(x, n);
+    check(abi.group_norm_bwd(ptr(x), ptr(w), ptr(b), ptr(gate), ptr(dy), ptr(dx), ptr(dgate), ptr(dw), ptr(db), ptr(ws),
+                             n, M, D, groups, (float)ctx->saved_data["eps"].toDouble(),
+                             (int)ctx->saved_data["act"].toInt(), dt, param_code(x, w, b), stream_of(x)),
+          "group norm backward");
+    return {dx, dw, db, dgate, Tensor(), Tensor(), Tensor()};
+  }
+};
+
 // ------------------------------------------------------------ entry points
 // No function transform, dispatch mode or tracer is looking at this call.
 bool plain_call() {
@@ -311,6 +428,21 @@ bool any_requires_grad(std::initializer_list<const Tensor*> ts) {
   if (!(cond)) Py_RETURN_NONE
 
 std::optional<Tensor> opt(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+// A tuple of tensors.
+PyObject* wrap_all(variable_list ts) {
+  PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
+  if (!out) return nullptr;
+  for (size_t i = 0; i < ts.size(); ++i) {
+    PyObject* o = THPVariable_Wrap(std::move(ts[i]));
+    if (!o) {
+      Py_DECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, (Py_ssize_t)i, o);
+  }
+  return out;
+}
 
 // headwise(x, weight, static_w or None, residual) -> y, or None (not taken)
 PyObject* py_headwise(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -399,17 +531,182 @@ PyObject* py_grouped_module(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
       ys = GroupedModuleFn::run(x, pre, w_in, U, sw, hd, s, GroupedModuleFn::z_buffer(x, s), Tensor(), 0);
     }
   }
-  PyObject* out = PyTuple_New((Py_ssize_t)ys.size());
-  if (!out) return nullptr;
-  for (size_t g = 0; g < ys.size(); ++g) {
-    PyObject* o = THPVariable_Wrap(std::move(ys[g]));
-    if (!o) {
-      Py_DECREF(out);
-      return nullptr;
-    }
-    PyTuple_SET_ITEM(out, (Py_ssize_t)g, o);
+  return wrap_all(std::move(ys));
+  END_HANDLE_TH_ERRORS
+}
+
+// None (t stays undefined), or a plain tensor on like's device.
+bool optional_tensor(PyObject* o, Tensor* t, const Tensor& like) {
+  return o == Py_None || (plain_tensor(o, t) && t->device() == like.device());
+}
+
+bool rows_whole(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
+
+// log_decay [H] and the scale of linear attention's calls; false: not taken (err: an exception is set)
+bool decay_and_scale(PyObject* decay, PyObject* scale, const Tensor& q, Tensor* lam, double* s, bool* err) {
+  if (!plain_tensor(decay, lam) || lam->device() != q.device() || lam->scalar_type() != at::kFloat || lam->dim() != 1 ||
+      lam->size(0) != q.size(1) || !lam->is_contiguous() || any_requires_grad({lam}))
+    return false;
+  if (scale == Py_None) {
+    *s = 1.0 / std::sqrt((double)q.size(-1));
+  } else {
+    *s = PyFloat_AsDouble(scale);
+    *err = *s == -1.0 && PyErr_Occurred();
   }
-  return out;
+  return !*err;
+}
+
+bool int_vector(const Tensor& t, int64_t n) {
+  return !t.defined() || (t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous());
+}
+
+// linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_state) -> o or (o, state), or None (not taken)
+PyObject* py_linear_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v, lam, s0, lengths;
+  DC_DECLINE_UNLESS(nargs == 8 && plain_call() && plain_tensor(args[0], &q) && plain_tensor(args[1], &k, &q) &&
+                    plain_tensor(args[2], &v, &q));
+  DC_DECLINE_UNLESS(dtype_code(q) >= 0 && q.dim() == 4 && v.dim() == 4 && k.sizes() == q.sizes());
+  const int64_t B = q.size(0), H = q.size(1), K = q.size(3), V = v.size(3);
+  DC_DECLINE_UNLESS(v.size(0) == B && v.size(1) == H && v.size(2) == q.size(2) && K <= DC_LA_MAX_DIM && V <= DC_LA_MAX_DIM);
+  DC_DECLINE_UNLESS(rows_whole(q) && rows_whole(k) && rows_whole(v));
+  DC_DECLINE_UNLESS(optional_tensor(args[5], &s0, q) && optional_tensor(args[6], &lengths, q) && int_vector(lengths, B));
+  DC_DECLINE_UNLESS(!s0.defined() || (s0.scalar_type() == at::kFloat && s0.is_contiguous() && s0.dim() == 4 &&
+                                      s0.size(0) == B && s0.size(1) == H && s0.size(2) == K && s0.size(3) == V));
+  double scale = 0;
+  bool err = false;
+  if (!decay_and_scale(args[3], args[4], q, &lam, &scale, &err)) {
+    if (err) return nullptr;
+    Py_RETURN_NONE;
+  }
+  const int want = PyObject_IsTrue(args[7]);
+  if (want < 0) return nullptr;
+  variable_list out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(q.device());
+    out = any_requires_grad({&q, &k, &v, &s0}) ? LinearAttentionFn::apply(q, k, v, opt(s0), lam, opt(lengths), scale, want != 0)
+                                               : LinearAttentionFn::run(q, k, v, lam, s0, lengths, scale, want != 0);
+  }
+  return want ? wrap_all(std::move(out)) : THPVariable_Wrap(std::move(out[0]));
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_attention_step(q, k, v, log_decay, state, scale, slots) -> o, or None (not taken)
+PyObject* py_linear_attention_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v, lam, state, slots;
+  DC_DECLINE_UNLESS(nargs == 7 && plain_call() && plain_tensor(args[0], &q) && plain_tensor(args[1], &k, &q) &&
+                    plain_tensor(args[2], &v, &q) && plain_tensor(args[4], &state) && state.device() == q.device());
+  DC_DECLINE_UNLESS(dtype_code(q) >= 0 && q.dim() == 3 && v.dim() == 3 && k.sizes() == q.sizes());
+  const int64_t B = q.size(0), H = q.size(1), K = q.size(2), V = v.size(2);
+  DC_DECLINE_UNLESS(v.size(0) == B && v.size(1) == H && K <= DC_LA_MAX_DIM && V <= DC_LA_MAX_DIM);
+  DC_DECLINE_UNLESS(rows_whole(q) && rows_whole(k) && rows_whole(v) && !any_requires_grad({&q, &k, &v, &state}));
+  DC_DECLINE_UNLESS(state.scalar_type() == at::kFloat && state.is_contiguous() && state.dim() == 4 && state.size(1) == H &&
+                    state.size(2) == K && state.size(3) == V);
+  DC_DECLINE_UNLESS(optional_tensor(args[6], &slots, q) && int_vector(slots, B) &&
+                    (slots.defined() || B <= state.size(0)));
+  double scale = 0;
+  bool err = false;
+  if (!decay_and_scale(args[3], args[5], q, &lam, &scale, &err)) {
+    if (err) return nullptr;
+    Py_RETURN_NONE;
+  }
+  Tensor o;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(q.device());
+    o = at::empty({B, H, V}, q.options());
+    check(abi.linear_attention_step(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(),
+                                    static_cast<float*>(ptr(lam)), static_cast<float*>(ptr(state)),
+                                    static_cast<int32_t*>(ptr(slots)), ptr(o), B, H, K, V, state.size(0), (float)scale,
+                                    dtype_code(q), stream_of(q)),
+          "linear attention step");
+  }
+  return THPVariable_Wrap(std::move(o));
+  END_HANDLE_TH_ERRORS
+}
+
+// group_norm(x, groups, weight, bias, gate, activation code, eps) -> y, or None (not taken)
+PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor x, w, b, gate;
+  DC_DECLINE_UNLESS(nargs == 7 && plain_call() && plain_tensor(args[0], &x) && dtype_code(x) >= 0 && x.dim() >= 1 &&
+                    x.is_contiguous());
+  DC_DECLINE_UNLESS(PyLong_CheckExact(args[1]) && PyLong_CheckExact(args[5]));
+  DC_DECLINE_UNLESS(optional_tensor(args[2], &w, x) && optional_tensor(args[3], &b, x));
+  DC_DECLINE_UNLESS(args[4] == Py_None || (plain_tensor(args[4], &gate, &x) && gate.is_contiguous() && gate.sizes() == x.sizes()));
+  const int64_t D = x.size(-1), groups = PyLong_AsLongLong(args[1]), act = PyLong_AsLongLong(args[5]);
+  const double eps = PyFloat_AsDouble(args[6]);
+  if (PyErr_Occurred()) return nullptr;
+  DC_DECLINE_UNLESS(groups > 0 && D % groups == 0 && D / groups <= 4096);
+  for (const Tensor* p : {&w, &b})
+    DC_DECLINE_UNLESS(!p->defined() || (p->dim() == 1 && p->size(0) == D && p->is_contiguous() &&
+                                        (p->scalar_type() == at::kFloat || p->scalar_type() == x.scalar_type())));
+  DC_DECLINE_UNLESS(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type());
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(x.device());
+    y = any_requires_grad({&x, &w, &b, &gate}) ? GroupNormFn::apply(x, opt(w), opt(b), opt(gate), groups, act, eps)
+                                               : GroupNormFn::run(x, w, b, gate, groups, act, eps);
+  }
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// lowrank_step(x, z list, U list, state, static_w list or None, residual, slots) -> tuple of G tensors, or None (not taken)
+PyObject* py_lowrank_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor x, state, slots, z[DC_MAX_GROUPS], U[DC_MAX_GROUPS], sw[DC_MAX_GROUPS];
+  DC_DECLINE_UNLESS(nargs == 7 && plain_call() && plain_tensor(args[0], &x) && plain_tensor(args[3], &state, &x) &&
+                    dtype_code(x) >= 0 && x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= x.size(1));
+  const bool has_static = args[4] != Py_None;
+  DC_DECLINE_UNLESS(PyList_CheckExact(args[1]) && PyList_CheckExact(args[2]) && (!has_static || PyList_CheckExact(args[4])));
+  const int64_t G = PyList_GET_SIZE(args[1]);
+  DC_DECLINE_UNLESS(G >= 1 && G <= DC_MAX_GROUPS && PyList_GET_SIZE(args[2]) == G &&
+                    (!has_static || PyList_GET_SIZE(args[4]) == G) && x.size(1) % G == 0);
+  const int64_t N = x.size(0), D = x.size(1) / G;
+  int64_t R = 0, W = 0;
+  for (int64_t g = 0; g < G; ++g) {
+    DC_DECLINE_UNLESS(plain_tensor(PyList_GET_ITEM(args[1], g), &z[g], &x) && plain_tensor(PyList_GET_ITEM(args[2], g), &U[g], &x) &&
+                      (!has_static || plain_tensor(PyList_GET_ITEM(args[4], g), &sw[g], &x)));
+    if (g == 0) {
+      DC_DECLINE_UNLESS(z[0].dim() == 2 && U[0].dim() == 2);
+      R = z[0].size(1);
+      W = U[0].size(1) / D;
+    }
+    DC_DECLINE_UNLESS(z[g].dim() == 2 && z[g].size(0) == N && z[g].size(1) == R && z[g].is_contiguous());
+    DC_DECLINE_UNLESS(U[g].dim() == 2 && U[g].size(0) == R && U[g].size(1) == W * D && U[g].is_contiguous());
+    DC_DECLINE_UNLESS(!has_static || (sw[g].dim() == 2 && sw[g].size(0) == W && sw[g].size(1) == D && sw[g].is_contiguous()));
+    DC_DECLINE_UNLESS(!any_requires_grad({&z[g], &U[g], &sw[g]}));
+  }
+  const int64_t rank = R + (has_static ? 1 : 0);
+  DC_DECLINE_UNLESS(W > 1 && (rank & (rank - 1)) == 0 && !any_requires_grad({&x, &state}));
+  DC_DECLINE_UNLESS(state.is_contiguous() && state.dim() == 3 && state.size(1) == W - 1 && state.size(2) == G * D);
+  DC_DECLINE_UNLESS(optional_tensor(args[6], &slots, x) && int_vector(slots, N) && (slots.defined() || N <= state.size(0)));
+  const int residual = PyObject_IsTrue(args[5]);
+  if (residual < 0) return nullptr;
+  variable_list ys;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(x.device());
+    const void *zp[DC_MAX_GROUPS], *Up[DC_MAX_GROUPS], *sp[DC_MAX_GROUPS];
+    void* yp[DC_MAX_GROUPS];
+    const Tensor y = at::empty({G, N, D}, x.options());
+    for (int64_t g = 0; g < G; ++g) {
+      zp[g] = ptr(z[g]);
+      Up[g] = ptr(U[g]);
+      sp[g] = ptr(sw[g]);
+      ys.push_back(y.select(0, g));
+      yp[g] = ptr(ys.back());
+    }
+    check(abi.lowrank_step_grouped(G, ptr(x), x.stride(0), zp, Up, has_static ? sp : nullptr, ptr(state),
+                                   static_cast<int32_t*>(ptr(slots)), yp, N, D, R, W, state.size(0), dtype_code(x),
+                                   residual != 0, stream_of(x)),
+          "lowrank step");
+  }
+  return wrap_all(std::move(ys));
   END_HANDLE_TH_ERRORS
 }
 
@@ -438,6 +735,14 @@ PyObject* py_init(PyObject*, PyObject* path) {
   sym(abi.proj_in_fwd, "dc_proj_in_fwd");
   sym(abi.proj_in_bwd_ws_bytes, "dc_proj_in_bwd_ws_bytes");
   sym(abi.proj_in_bwd, "dc_proj_in_bwd");
+  sym(abi.linear_attention_ws_bytes, "dc_linear_attention_ws_bytes");
+  sym(abi.linear_attention_fwd, "dc_linear_attention_fwd");
+  sym(abi.linear_attention_bwd, "dc_linear_attention_bwd");
+  sym(abi.linear_attention_step, "dc_linear_attention_step");
+  sym(abi.group_norm_fwd, "dc_group_norm_fwd");
+  sym(abi.group_norm_bwd_ws_bytes, "dc_group_norm_bwd_ws_bytes");
+  sym(abi.group_norm_bwd, "dc_group_norm_bwd");
+  sym(abi.lowrank_step_grouped, "dc_lowrank_step_grouped");
   ready = true;
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
@@ -449,6 +754,14 @@ PyMethodDef methods[] = {
     {"lowrank", (PyCFunction)(void*)py_lowrank, METH_FASTCALL, "lowrank(x, z, U, static_w, residual)"},
     {"grouped_module", (PyCFunction)(void*)py_grouped_module, METH_FASTCALL,
      "grouped_module(x, pre_z, w_in, proj_out, proj_out_bias, head_dim)"},
+    {"linear_attention", (PyCFunction)(void*)py_linear_attention, METH_FASTCALL,
+     "linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_state)"},
+    {"linear_attention_step", (PyCFunction)(void*)py_linear_attention_step, METH_FASTCALL,
+     "linear_attention_step(q, k, v, log_decay, state, scale, slots)"},
+    {"group_norm", (PyCFunction)(void*)py_group_norm, METH_FASTCALL,
+     "group_norm(x, groups, weight, bias, gate, activation, eps)"},
+    {"lowrank_step", (PyCFunction)(void*)py_lowrank_step, METH_FASTCALL,
+     "lowrank_step(x, z, U, state, static_w, residual, slots)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

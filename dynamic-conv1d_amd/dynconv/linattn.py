@@ -34,7 +34,7 @@ def _like(t):
 
 
 class _LinearAttentionFn(torch.autograd.Function):
-    """o, and the final state where it is asked for."""
+    """o, and the final state where it is asked for.  Plain calls take its native form (_capi.binding)."""
 
     @staticmethod
     @_capi.on_tensor_device
@@ -132,6 +132,10 @@ def linear_attention(
 
     Products of 16-bit inputs run on matrix cores with float32 sums; the state is float32 throughout.
     """
+    if _capi.binding is not None:
+        out = _capi.binding.linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_state)
+        if out is not None:
+            return out
     assert q.is_cuda and q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k, v must be [B, H, T, .] on the GPU"
     B, H, T, K = q.shape
     assert k.shape == q.shape, "k must have q's shape"
@@ -173,6 +177,10 @@ def linear_attention_step(
     Returns:
         o [B, H, V] in q's dtype.  Serving only: no gradients.
     """
+    if _capi.binding is not None:
+        o = _capi.binding.linear_attention_step(q, k, v, log_decay, state, scale, slots)
+        if o is not None:
+            return o
     assert q.is_cuda and q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k, v must be [B, H, .] on the GPU"
     B, H, K = q.shape
     assert k.shape == q.shape and v.shape[:2] == q.shape[:2], "k must have q's shape, v must be [B, H, V]"

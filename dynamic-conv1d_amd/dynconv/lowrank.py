@@ -309,6 +309,11 @@ def lowrank_dynamic_convolution_step_grouped(
         Serving only: no gradients.
     """
     z, U = list(z), list(U)
+    static_w = None if static_w is None else list(static_w)
+    if _capi.binding is not None:
+        ys = _capi.binding.lowrank_step(x, z, U, state, static_w, residual, slots)
+        if ys is not None:
+            return ys
     G = len(z)
     assert 1 <= G <= 4, "between 1 and 4 groups"
     assert len(U) == G and (static_w is None or len(static_w) == G), "one U (and static_w) per group"
@@ -320,7 +325,7 @@ def lowrank_dynamic_convolution_step_grouped(
     rank = R if static_w is None else R + 1
     assert rank & (rank - 1) == 0, "rank R must be a power of 2. If static_w is set R+1 must be a power of 2."
     W = U[0].shape[-1] // D
-    tensors = [*z, *U, state] + ([] if static_w is None else list(static_w))
+    tensors = [*z, *U, state] + ([] if static_w is None else static_w)
     assert all(t.device == x.device and t.is_contiguous() for t in tensors), "contiguous tensors on x's device"
     assert all(t.dtype == x.dtype for t in tensors), "x, z, U, static_w and state must share one dtype"
     assert not (torch.is_grad_enabled() and any(t.requires_grad for t in [x, *tensors])), \
@@ -336,7 +341,7 @@ def lowrank_dynamic_convolution_step_grouped(
         assert slots.device == x.device and slots.dtype in (torch.int32, torch.int64) and tuple(slots.shape) == (N,), \
             "slots must be int32 [N], on x's device"
         slots = slots.to(torch.int32).contiguous()
-    return _step_grouped(x, z, U, state, None if static_w is None else list(static_w), residual, slots, W)
+    return _step_grouped(x, z, U, state, static_w, residual, slots, W)
 
 
 def lowrank_dynamic_convolution_step(

@@ -15,13 +15,16 @@ MAX_GROUP = 4096  # channels of a group
 
 
 class _GroupNormFn(torch.autograd.Function):
+    """Plain calls take its native form (_capi.binding)."""
+
     @staticmethod
     @_capi.on_tensor_device
     def forward(ctx, x, weight, bias, gate, groups, act, eps):
         D = x.shape[-1]
         M = x.numel() // D
         y = torch.empty_like(x)
-        pdtype = _capi.dtype_code(x.dtype if weight is None and bias is None else (weight if weight is not None else bias).dtype)
+        param = weight if weight is not None else bias
+        pdtype = _capi.dtype_code(x.dtype if param is None else param.dtype)
         dtype = _capi.dtype_code(x.dtype)
         if M > 0:
             status = _capi.load().dc_group_norm_fwd(
@@ -84,6 +87,10 @@ def group_norm(
     Returns:
         y like x.  Statistics and sums are float32; results are the same run to run.
     """
+    if _capi.binding is not None and activation in ACTIVATIONS:
+        y = _capi.binding.group_norm(x, groups, weight, bias, gate, ACTIVATIONS[activation], eps)
+        if y is not None:
+            return y
     assert x.is_cuda and x.dim() >= 1 and x.is_contiguous(), "x must be contiguous, on the GPU"
     _capi.dtype_code(x.dtype)
     D = x.shape[-1]

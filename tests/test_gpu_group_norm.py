@@ -176,6 +176,28 @@ def test_graph():
             assert torch.equal(a, b)
 
 
+def test_native_binding_and_python_functions_agree(monkeypatch):
+    from dynconv import _capi
+
+    _capi.load()
+    if _capi.binding is None:
+        pytest.skip("no native binding")
+    g = gen(9)
+    x, gate, dy = (randn(g, 30, 128).to(BF).to(DEV) for _ in range(3))
+    w, b = torch.randn(128, device=DEV), torch.randn(128, device=DEV)
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, gate)]
+        y = group_norm(leaves[0], 4, leaves[1], leaves[2], leaves[3])
+        z = group_norm(leaves[0], 4, activation=None, eps=1e-3)
+        return [y, z, *torch.autograd.grad(y, leaves, dy), *torch.autograd.grad(z, leaves[:1], dy)], y.grad_fn.name()
+
+    a, name = run()
+    monkeypatch.setattr(_capi, "binding", None)
+    c, other = run()
+    assert name != other and all(torch.equal(p, q) for p, q in zip(a, c))
+
+
 def test_refusals():
     x = torch.randn(4, 64, device=DEV)
     w = torch.ones(64, device=DEV)

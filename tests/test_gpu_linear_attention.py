@@ -384,6 +384,38 @@ def test_step_in_a_cache_past_32_bits():
     assert torch.equal(a, b) and torch.equal(state[ids.long()], small)
 
 
+def test_native_binding_and_python_functions_agree(monkeypatch):
+    """The native nodes (where built) and the Python Functions launch the same kernels: bitwise equal results."""
+    from dynconv import _capi
+
+    _capi.load()
+    if _capi.binding is None:
+        pytest.skip("no native binding")
+    g = gen(14)
+    lam = _decays(2, 5).to(DEV)
+    x = [randn(g, 2, 2, 90, 32).to(BF).to(DEV) for _ in range(4)]
+    S0, dS = randn(g, 2, 2, 32, 32).to(DEV), randn(g, 2, 2, 32, 32).to(DEV)
+    n = torch.tensor([90, 17], dtype=torch.int32, device=DEV)
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (*x[:3], S0)]
+        o, S = linear_attention(*leaves[:3], lam, 0.5, leaves[3], n, return_state=True)
+        grads = torch.autograd.grad((o, S), leaves, (x[3], dS))
+        alone = torch.autograd.grad(linear_attention(*leaves[:3], lam), leaves[:3], x[3])
+        with torch.no_grad():
+            S1 = S0.clone()
+            one = linear_attention_step(x[0][:, :, 0], x[1][:, :, 0], x[2][:, :, 0], lam, S1, slots=n % 2)
+            quiet = linear_attention(*x[:3], lam)
+        return [o, S, *grads, *alone, one, S1, quiet], o.grad_fn.name()
+
+    a, name = run()
+    monkeypatch.setattr(_capi, "binding", None)
+    b, other = run()
+    assert name != other, "the native node takes the plain call"
+    for p, q in zip(a, b):
+        assert torch.equal(p, q) and p.stride() == q.stride()
+
+
 def test_refusals():
     lam = torch.zeros(2, device=DEV)
     q = torch.randn(1, 2, 4, 8, device=DEV)

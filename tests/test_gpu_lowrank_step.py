@@ -117,6 +117,22 @@ def test_graph():
         assert all(torch.equal(a, b) for a, b in zip(outs, want)) and torch.equal(state, end)
 
 
+def test_native_binding_and_python_function_agree(monkeypatch):
+    from dynconv import _capi
+
+    _capi.load()
+    x, z, U, sw, state = (_dev(t) for t in _inputs(gen(35), 2, 6, 64, 7, 4, True, 9, HF))
+    ids = torch.tensor([8, 1, -1, 3, 0, 5], dtype=torch.int32, device=DEV)
+
+    def run():
+        s = state.clone()
+        return [*lowrank_dynamic_convolution_step_grouped(x, z, U, s, static_w=sw, residual=True, slots=ids), s]
+
+    a = run()
+    monkeypatch.setattr(_capi, "binding", None)
+    assert all(torch.equal(p, q) for p, q in zip(a, run()))
+
+
 def test_refusals():
     x, z, U, sw, state = (_dev(t) for t in _inputs(gen(34), 2, 3, 64, 7, 4, True, 3, BF))
     step = lowrank_dynamic_convolution_step_grouped
