@@ -27,7 +27,8 @@
 // operands without leaving their lane: scores are formed as k q^T (column i in
 // lane i), S as k^T v (column n in lane n), o as (v^T scores^T + S^T q^T), whose
 // column i sits in lane i with four neighbouring channels to a store.  q and k
-// rows are read from LDS 4 values at a time in that order, v and k columns
+// rows lie in LDS so that a lane's 8 values of that order are neighbours (16-byte
+// reads; two 8-byte reads took twice the LDS's time), v and k columns are read
 // through transposing reads.  The scores are formed by each of the NW
 // wavefronts: 24 of its 78 products at 128 channels, against an exchange
 // through LDS and a barrier.
@@ -63,6 +64,10 @@ struct Args {
 // Tokens of a chunk: 64, or 32 where three tiles of 64 float32 rows would pass the LDS.
 __host__ __device__ constexpr int chunk_tokens(int es, int kp) { return es == 4 && kp > 128 ? 32 : 64; }
 
+// Where channel c of a row of q or k lies in LDS: of each 16 channels the second and third quads change places, so that
+// the 8 channels of a lane's half, 4 half .. + 3 and 8 + 4 half .. + 3, are neighbours.
+__host__ __device__ constexpr int quad(int c) { return (c & ~12) | ((c & 4) << 1) | ((c & 8) >> 1); }
+
 template <typename T> struct Ops {  // 16-bit types
   typedef u32x4 Frag;
   static constexpr bool kSplit = true, kNarrow = __is_same(T, fp16);  // two parts; float32 values may not fit
@@ -72,15 +77,14 @@ template <typename T> struct Ops {  // 16-bit types
     else
       return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
   }
-  // 16 channels of row `row` (this lane's half): p points at the row's first of them
-  __device__ static __forceinline__ Frag rows(const T* p, int half) {
-    const u32x2 a = *reinterpret_cast<const u32x2*>(p + 4 * half);
-    const u32x2 b = *reinterpret_cast<const u32x2*>(p + 8 + 4 * half);
-    return Frag{a[0], a[1], b[0], b[1]};
-  }
-  // column lane%32 of 16 rows: p points at (row 0, column 0) of the 16 x 32 block, rows rs elements apart
+  // this lane's half of 16 channels of a row: p points at the first of them
+  __device__ static __forceinline__ Frag rows(const T* p, int half) { return *reinterpret_cast<const Frag*>(p + 8 * half); }
+  // column lane%32 of 16 rows: p points at (row 0, column 0) of the 16 x 32 block, rows rs elements apart; TURNED: the
+  // rows' channels lie in quad() order
+  template <bool TURNED>
   __device__ static __forceinline__ Frag cols(const T* p, int rs, int lane) {
-    const T* q = p + (4 * (lane / 32) + (lane % 16) / 4) * rs + 16 * ((lane / 16) % 2) + 4 * (lane % 4);
+    const int c = 4 * (lane % 4);
+    const T* q = p + (4 * (lane / 32) + (lane % 16) / 4) * rs + 16 * ((lane / 16) % 2) + (TURNED ? quad(c) : c);
     const u32x2 a = lds_read_tr16(q), b = lds_read_tr16(q + 8 * rs);
     return Frag{a[0], a[1], b[0], b[1]};
   }
@@ -102,14 +106,15 @@ template <> struct Ops<float> {
   }
   __device__ static __forceinline__ Frag rows(const float* p, int half) {
     Frag f;
-    load_vals<float, 4>(p + 4 * half, f.v);
-    load_vals<float, 4>(p + 8 + 4 * half, f.v + 4);
+    load_vals<float, 8>(p + 8 * half, f.v);
     return f;
   }
+  template <bool TURNED>
   __device__ static __forceinline__ Frag cols(const float* p, int rs, int lane) {
     Frag f;
+    const int c = TURNED ? quad(lane % 32) : lane % 32;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.v[e] = p[(8 * (e / 4) + 4 * (lane / 32) + e % 4) * rs + lane % 32];
+    for (int e = 0; e < 8; ++e) f.v[e] = p[(8 * (e / 4) + 4 * (lane / 32) + e % 4) * rs + c];
     return f;
   }
   __device__ static __forceinline__ Frag pack(const float* v) {
@@ -124,13 +129,15 @@ template <> struct Ops<float> {
   }
 };
 
-// Elements from a row of a tile to the next in LDS: rows start 4, 12 or 36 banks
-// after each other (mod 64), which keeps both the row reads (16 rows x 8 bytes at
-// once; float32: 8 x 16) and the transposing ones (4 rows x 32 bytes) apart.
-template <typename T, int N>
+// Elements from a row of a tile to the next in LDS.  Measured over 16 bytes of padding by 16, eight wavefronts: row
+// reads of 16 bytes take 2048 cycles a KB of reads without padding, 370 with an odd multiple of 16 bytes; transposing
+// reads 4 cycles each from 32 bytes on, under 3 with 64.  Rows of q and k take 48, v's (only read by columns) 64.
+template <typename T, int N, bool TURNED>
 constexpr int row_elems() {
-  return N + (sizeof(T) == 4 ? 16 : N % 128 == 0 ? 48 : 16) / (int)sizeof(T);
+  return N + (sizeof(T) == 4 ? 16 : !TURNED ? (N % 128 == 0 ? 64 : 32) : N % 128 == 0 ? 48 : 16) / (int)sizeof(T);
 }
+
+constexpr int kOut = 0x7FFFFFF0;  // a byte offset past every buffer's range
 
 // g^k, g = 2^lam2; g^0 = 1 also where lam2 is minus infinity.
 __device__ __forceinline__ float power(float lam2, int k) { return k == 0 ? 1.f : exp2f(lam2 * (float)k); }
@@ -147,7 +154,6 @@ __device__ __forceinline__ void phase() {
 // a row lies inside or outside of it, 16-byte aligned, rows within 32-bit offsets of
 // each other: buffer loads, whose range drops the rows past `end`.  Otherwise
 // pieces are gathered element by element.
-constexpr int kOut = 0x7FFFFFF0;  // an offset past every range
 template <typename T, int C, int N, int NT, bool WHOLE>
 struct Tile {
   static constexpr int VE = 16 / (int)sizeof(T), PR = N / VE, NV = C * PR / NT, RPI = NT / PR;
@@ -181,10 +187,20 @@ struct Tile {
       }
     }
   }
+  // TURNED: channels in quad() order
+  template <bool TURNED>
   __device__ __forceinline__ void store(T* lds) const {
-    const int r0 = (int)threadIdx.x / PR, c = ((int)threadIdx.x % PR) * VE;
+    const int c = ((int)threadIdx.x % PR) * VE;
+    T* to = lds + (int)threadIdx.x / PR * row_elems<T, N, TURNED>() + (TURNED ? quad(c) : c);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) *reinterpret_cast<u32x4*>(lds + (r0 + i * RPI) * row_elems<T, N>() + c) = v[i];
+    for (int i = 0; i < NV; ++i, to += RPI * row_elems<T, N, TURNED>()) {
+      if constexpr (TURNED && VE == 8) {  // two quads, which part
+        *reinterpret_cast<u32x2*>(to) = u32x2{v[i][0], v[i][1]};
+        *reinterpret_cast<u32x2*>(to + 8) = u32x2{v[i][2], v[i][3]};
+      } else {
+        *reinterpret_cast<u32x4*>(to) = v[i];
+      }
+    }
   }
 };
 
@@ -209,7 +225,7 @@ template <typename T, int KP, int NW, int C, bool WHOLE, bool STATES, bool RETUR
 __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void la_chunks(Args A) {
   typedef Ops<T> O;
   typedef typename O::Frag Frag;
-  constexpr int NT = NW * 64, NB = C / 32, KB = KP / 32, RK = row_elems<T, KP>(), RV = row_elems<T, NW * 32>();
+  constexpr int NT = NW * 64, NB = C / 32, KB = KP / 32, RK = row_elems<T, KP, true>(), RV = row_elems<T, NW * 32, false>();
   __shared__ __align__(16) T sk[C * RK];
   __shared__ __align__(16) T sv[C * RV];
   __shared__ __align__(16) T sq[STATES ? 8 : C * RK];
@@ -240,16 +256,21 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
   if (states) states += ((int64_t)bh * A.nseg + seg) * P.K * P.V;
   const int64_t sbase = (int64_t)bh * P.K * P.V;
 
+  // element (a, n0 + col) of a state of this head, a = row + 4 half, through a buffer of the state's range
+  const int K = P.K, V = P.V, srow = (int)P.s_row * 4, scol = (int)P.s_col * 4, srange = K * V * 4;
+  auto at = [=](int a, int c) {
+    const int off = a * srow + c * scol;
+    return ((a < K) & (c < V)) ? off : kOut;
+  };
   f32x16 S[KB];
   {
     const float* from = STATES ? nullptr : states ? states : P.s_in ? P.s_in + sbase : nullptr;
+    const rsrc_t rs = make_rsrc_wave(from, from ? srange : 0);  // no state: zeros
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int a = kb * 32 + 8 * (r / 4) + 4 * half + r % 4;
-        S[kb][r] = from && a < P.K && n0 + col < P.V ? from[a * P.s_row + (n0 + col) * P.s_col] : 0.f;
-      }
+      for (int r = 0; r < 16; ++r)
+        S[kb][r] = __uint_as_float(bload32(rs, at(kb * 32 + 8 * (r / 4) + 4 * half + r % 4, n0 + col)));
   }
 
   // weights that every full chunk has, element e of a step (or register r of a result) at row(e): of the last 16
@@ -275,9 +296,9 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
   }
   for (int p0 = lo; p0 < hi; p0 += C) {
     __syncthreads();  // the chunk before has been read
-    tk.store(sk);
-    tv.store(sv);
-    if constexpr (!STATES) tq.store(sq);
+    tk.template store<true>(sk);
+    tv.template store<false>(sv);
+    if constexpr (!STATES) tq.template store<true>(sq);
     __syncthreads();
     if (p0 + C < hi) {
       tk.load(k, P.ks[2], P.K, p0 + C, hi, turn);
@@ -336,7 +357,7 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
           }
 #pragma unroll
           for (int s = 0; s < 2; ++s)
-            acc[ib] = O::mma(O::cols(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane), O::pack(t + 8 * s), acc[ib]);
+            acc[ib] = O::mma(O::template cols<false>(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane), O::pack(t + 8 * s), acc[ib]);
         };
         if (NB > 1 && ib > jb0) {
           // the state and the block before by way of its last token: g^{i+1} = g^{32} g^{col+1}, g^{i-j} = g^{col+1} g^{31-j}
@@ -381,7 +402,7 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
       float t[8], g = 1.f;  // g^{C-16-16s}
 #pragma unroll
       for (int i = s + 1; i < C / 16; ++i) g *= g1;
-      O::unpack(O::cols(sv + s * 16 * RV + wv * 32, RV, lane), t);
+      O::unpack(O::template cols<false>(sv + s * 16 * RV + wv * 32, RV, lane), t);
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[e] *= vlast[e] * g;
       const Frag v1 = O::pack(t);
@@ -401,7 +422,7 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
       }
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const Frag kf = O::cols(sk + s * 16 * RK + kb * 32, RK, lane);
+        const Frag kf = O::template cols<true>(sk + s * 16 * RK + kb * 32, RK, lane);
         S[kb] = O::mma(kf, v1, S[kb]);
         if constexpr (O::kSplit) S[kb] = O::mma(kf, v2, S[kb]);
         if (three) S[kb] = O::mma(kf, v3, S[kb]);
@@ -413,17 +434,16 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
   float* to = STATES ? states : states ? nullptr : P.s_out ? P.s_out + sbase : nullptr;
   if (to) {
     const float g = !STATES && P.rev && len > 0 ? power(lam2, 1) : 1.f;
-    // opaque to the compiler, which would otherwise keep the addresses and masks of the first
+    const rsrc_t rs = make_rsrc_wave(to, srange);
+    // opaque to the compiler, which would otherwise keep the offsets of the first
     // state's loads in registers through the whole segment (100 spilled registers)
     int h4 = 4 * half, c = n0 + col;
     asm volatile("" : "+v"(h4), "+v"(c));
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int a = kb * 32 + 8 * (r / 4) + h4 + r % 4;
-        if (a < P.K && c < P.V) to[a * P.s_row + c * P.s_col] = S[kb][r] * g;
-      }
+      for (int r = 0; r < 16; ++r)
+        BufUnit<4>::template store<false>(__float_as_uint(S[kb][r] * g), rs, at(kb * 32 + 8 * (r / 4) + h4 + r % 4, c));
   }
   if constexpr (!STATES) {  // rows past the sequence's length
     const int z0 = max(len, lo), w = min(vw, NW * 32);
