@@ -87,8 +87,8 @@ int dc_linear_attention_bwd(const void* q, const int64_t* q_strides, const void*
                             const float* initial_state, const int32_t* lengths, const void* d_o,
                             const int64_t* do_strides, const float* d_final_state, void* dq,
                             const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
-                            const int64_t* dv_strides, float* d_initial_state, void* workspace, int64_t ws_bytes,
-                            int64_t B, int64_t H, int64_t T, int64_t K, int64_t V, float scale, int dtype,
+                            const int64_t* dv_strides, float* d_initial_state, const void* fwd_workspace,
+                            void* workspace, int64_t ws_bytes, int64_t B, int64_t H, int64_t T, int64_t K, int64_t V, float scale, int dtype,
                             void* stream) {
   const int64_t need = dc_linear_attention_ws_bytes(B, H, T, K, V, dtype, 1);
   if (need < 0) return (int)need;
@@ -100,6 +100,7 @@ int dc_linear_attention_bwd(const void* q, const int64_t* q_strides, const void*
                         (const void*)d_initial_state, (const void*)lengths})
     if (!aligned_to(t, 4)) return DC_ERR_ALIGN;
   if (need > 0 && (!workspace || ws_bytes < need || !aligned_to(workspace, 16))) return DC_ERR_WORKSPACE;
+  if (!aligned_to(fwd_workspace, 16)) return DC_ERR_WORKSPACE;
   for (const int64_t* t : {q_strides, k_strides, v_strides, do_strides, dq_strides, dk_strides, dv_strides})
     if (!t) return DC_ERR_NULL;
   int s = device_status();
@@ -124,6 +125,7 @@ int dc_linear_attention_bwd(const void* q, const int64_t* q_strides, const void*
   c.s_in = d_final_state; c.s_out = d_initial_state; c.s_row = V; c.s_col = 1;
   c.K = (int)K; c.V = (int)V; c.rev = 1; c.so = 1.f; c.skv = scale;
   p.npass = 3;
+  p.fwd_states = static_cast<const float*>(fwd_workspace);
   p.log_decay = log_decay; p.lengths = lengths;
   p.B = B; p.H = H; p.T = T; p.dtype = dtype;
   p.ws = workspace; p.ws_bytes = ws_bytes; p.stream = (hipStream_t)stream;

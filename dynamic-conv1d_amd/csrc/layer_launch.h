@@ -37,6 +37,7 @@ struct LaProblem {
   int dtype;
   void* ws;
   int64_t ws_bytes;
+  const float* fwd_states;  // backward: the states before each segment that the forward left in its workspace (null: none)
   hipStream_t stream;
 };
 int64_t la_ws_bytes(const LaProblem& p);

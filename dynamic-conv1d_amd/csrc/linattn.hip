@@ -29,46 +29,37 @@ struct Cut {
   int seg, nseg;
 };
 
-// Sets of segment states: the forward's one; the backward's two (dq's, and dv's that dk shares).
-int sets_of(const LaProblem& p) { return p.npass == 3 ? 2 : 1; }
-
-// Workgroups of a pass that a CU holds at once: by registers two wavefronts on a SIMD in 16 bits up to 128 channels, else
-// one; by LDS three tiles each.
-int resident(const LaPass& p, int dtype) {
-  const int kp = cover(p.K), nw = p.V <= 64 ? 2 : 4;
-  if (dtype == kFP32) return nw == 2 && kp == 64 ? 2 : 1;
-  if (kp == 256) return 1;
-  return nw == 4 ? 2 : kp == 64 ? 4 : 3;
+// Time of one chunk of a workgroup that has a CU to itself, in us (measured; only ratios matter).  Two workgroups on a CU
+// take nearly twice as long.
+double chunk_us(int K, int V, int dtype) {
+  const int kp = cover(K);
+  const double t = kp == 64 ? 2.5 : kp == 128 ? 3.5 : 7;
+  return dtype == kFP32 ? 5 * t : t;
 }
 
-// Segments of a problem: the count with the least estimated time, in units of a round of chunks on every CU.  A launch
-// takes whole rounds of resident workgroups; segments cost the states' launch (0.4 of a chunk's time for each of its
-// chunks, measured 72 us against 172) and carrying them (one unit for 25 MB).  Against filling 512 workgroups by division
-// alone: B2 H32 T8192 hd128 backward 9 rounds of 12 chunks for 576 workgroups, now 3 of 16.
+// Segments of a problem, the forward's and the backward's alike: the count with the least estimated time of the forward.
+// The chunks run in rounds of one workgroup to a CU; segments cost half a chunk's time to form each of their states, all
+// but the last one's, and the carrying of states of float32 at 4.5 TB/s.  B2 H32 T8192 hd128, forward and backward, us:
+// 4 segments 200 + 478, 8 208 + 510, 5 250 + 503, 1 455 + 550.  B8 H32 T4096 hd64: 1 segment 159 + 322, 2 195 + 446.
 Cut cut_of(const LaProblem& p) {
-  const int C = la::chunk_tokens(dtype_size(p.dtype), cover(p.pass[0].K));
+  // dq's pass of a backward has K and V the other way round: the same cut
+  const int K = p.npass == 3 ? p.pass[0].V : p.pass[0].K, V = p.npass == 3 ? p.pass[0].K : p.pass[0].V;
+  const int es = dtype_size(p.dtype);
+  const int C = max(la::chunk_tokens(es, cover(K)), la::chunk_tokens(es, cover(V)));
   const int64_t chunks = (p.T + C - 1) / C;
-  const int sets = sets_of(p);
+  const double heads = (double)p.B * p.H * ((V + 127) / 128), us = chunk_us(K, V, p.dtype);
   double best = 0;
-  int64_t seg = chunks;
+  int64_t seg = chunks < 1 ? 1 : chunks;
   for (int64_t n = 1; n <= 128 && n <= (chunks + 1) / 2; ++n) {
     const int64_t len = (chunks + n - 1) / n;
-    if (n > 1 && (chunks + len - 1) / len != n) continue;  // the same segments as fewer
-    double t = 0, wgs = 0;
-    for (int i = 0; i < p.npass; ++i) {
-      const LaPass& a = p.pass[i];
-      const double w = (double)p.B * p.H * n * ((a.V + 127) / 128) / (256 * resident(a, p.dtype));
-      wgs += w;
-      if (n > 1 && (p.npass == 1 || i != 1)) t += 0.4 * (w < 1 ? 1 : w) * len;
-    }
-    t += (wgs <= 1 ? 1 : __builtin_ceil(wgs)) * len;
-    if (n > 1) t += 1 + 4e-8 * sets * 4 * (double)p.B * p.H * n * p.pass[0].K * p.pass[0].V;
+    if ((chunks + len - 1) / len != n) continue;  // the same segments as fewer
+    double t = us * len * __builtin_ceil(heads * n / 256);
+    if (n > 1) t += 5 + 0.5 * us * len * __builtin_ceil(heads * (n - 1) / 256) + heads * n * K * V * 8 / 4.5e6;
     if (n == 1 || t < best) {
       best = t;
       seg = len;
     }
   }
-  if (seg < 1) seg = 1;
   return {(int)(seg * C), (int)(chunks > 0 ? (chunks + seg - 1) / seg : 1)};
 }
 
@@ -81,12 +72,13 @@ struct Carry {
   float* s_out[2];
   int rev[2];
   int64_t H, T, n;  // n: elements of a state
+  int64_t bh0;      // first head of the launch
   int seg, nseg;
 };
 
 __global__ __launch_bounds__(256) void la_carry(Carry A) {
   const int set = blockIdx.z, rev = A.rev[set];
-  const int64_t bh = blockIdx.y, e = ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  const int64_t bh = A.bh0 + blockIdx.y, e = ((int64_t)blockIdx.x * 256 + threadIdx.x);
   if (e >= A.n) return;
   const int T = (int)A.T;
   const int len = A.lengths ? min(max(A.lengths[bh / A.H], 0), T) : T;
@@ -141,7 +133,7 @@ hipError_t launch(const LaProblem& p, const Cut& c, float* const* states_of, boo
       const int nvb = (b.V + nw * 32 - 1) / (nw * 32);
       if (nvb > a.nvb) a.nvb = nvb;
     }
-    const int64_t nblk = p.B * p.H * c.nseg * a.nvb;
+    const int64_t nblk = p.B * p.H * c.nseg * a.nvb * a.npass;
     if (nblk > 0x7fffffff) return hipErrorInvalidValue;
     a.nblk = (int)nblk;
     hipError_t e;
@@ -157,29 +149,35 @@ hipError_t launch(const LaProblem& p, const Cut& c, float* const* states_of, boo
 
 }  // namespace
 
+// Sets of states before each segment: the forward's one, and for the backward dv's, that dk shares, behind dq's, which is
+// the forward's where the caller has kept it.
 int64_t la_ws_bytes(const LaProblem& p) {
   const Cut c = cut_of(p);
   if (c.nseg == 1) return 0;
-  return sets_of(p) * p.B * p.H * c.nseg * (int64_t)p.pass[0].K * p.pass[0].V * (int64_t)sizeof(float);
+  return (p.npass == 3 ? 2 : 1) * p.B * p.H * c.nseg * (int64_t)p.pass[0].K * p.pass[0].V * (int64_t)sizeof(float);
 }
 
 hipError_t la_run(const LaProblem& p) {
   const Cut c = cut_of(p);
   float* of[kLaMaxPasses] = {};
   if (c.nseg > 1) {
-    const int sets = sets_of(p);
-    const int64_t n = (int64_t)p.pass[0].K * p.pass[0].V, set = p.B * p.H * c.nseg * n;
+    const int64_t n = (int64_t)p.pass[0].K * p.pass[0].V;
     float* ws = static_cast<float*>(p.ws);
     of[0] = ws;
-    of[1] = of[2] = ws + set;
-    // a set's states are formed by the pass whose state lies row by row: dq's k and v change places, dv's stay
+    if (p.npass == 3) {
+      of[1] = of[2] = ws + p.B * p.H * c.nseg * n;
+      if (p.fwd_states) of[0] = const_cast<float*>(p.fwd_states);
+    }
+    // the passes that form states, and where
     LaProblem f = p;
-    f.npass = sets;
-    if (sets == 2) f.pass[1] = p.pass[2];
+    float* at[2];
+    f.npass = 0;
     Carry y{};
-    for (int i = 0; i < sets; ++i) {
-      LaPass& a = f.pass[i];
-      if (a.s_col != 1) {
+    for (int i = 0; i < p.npass; i += 2) {
+      if (i == 0 && p.npass == 3 && p.fwd_states) continue;
+      LaPass& a = f.pass[f.npass];
+      a = p.pass[i];
+      if (a.s_col != 1) {  // dq's state lies turned over: its k and v change places
         const LaPass t = a;
         a.k = t.v; a.v = t.k;
         for (int d = 0; d < 3; ++d) {
@@ -188,19 +186,24 @@ hipError_t la_run(const LaProblem& p) {
         }
         a.K = t.V; a.V = t.K; a.s_row = t.s_col; a.s_col = 1;
       }
-      y.states[i] = of[i];
-      y.s_in[i] = a.s_in;
-      y.s_out[i] = a.s_out;
-      y.rev[i] = a.rev;
+      at[f.npass] = y.states[f.npass] = of[i];
+      y.s_in[f.npass] = a.s_in;
+      y.s_out[f.npass] = a.s_out;
+      y.rev[f.npass++] = a.rev;
     }
-    hipError_t e = launch(f, c, of, true);
+    hipError_t e = launch(f, c, at, true);
     if (e != hipSuccess) return e;
     y.log_decay = p.log_decay;
     y.lengths = p.lengths;
     y.H = p.H; y.T = p.T; y.n = n;
     y.seg = c.seg; y.nseg = c.nseg;
-    la_carry<<<dim3((unsigned)((n + 255) / 256), (unsigned)(p.B * p.H), (unsigned)sets), 256, 0, p.stream>>>(y);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
+    const unsigned per = 65535;  // heads to a launch: the grid's second axis
+    for (int64_t h0 = 0; h0 < p.B * p.H; h0 += per) {
+      y.bh0 = h0;
+      const unsigned nh = (unsigned)(p.B * p.H - h0 < per ? p.B * p.H - h0 : per);
+      la_carry<<<dim3((unsigned)((n + 255) / 256), nh, (unsigned)f.npass), 256, 0, p.stream>>>(y);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
   }
   return launch(p, c, of, false);
 }

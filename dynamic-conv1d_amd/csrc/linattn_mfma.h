@@ -219,10 +219,16 @@ __device__ __forceinline__ void scale(float* v, float by) {
   for (int i = 0; i < N; ++i) v[i] *= by;
 }
 
+// Wavefronts on a SIMD that leave a kernel's registers unspilled.
+constexpr int waves_per_simd(int es, int kp, int nw, bool states) {
+  if (es == 4 || kp > 128) return 1;
+  return states ? (kp == 64 ? 3 : 2) : kp == 128 && nw == 2 ? 1 : 2;
+}
+
 // STATES: only the state after each segment, from zero, for states[pass].  RETURNED: a state that is formed here is the
 // caller's result (three parts in bf16; in every kernel they cost the common one 10% by spilled registers).
 template <typename T, int KP, int NW, int C, bool WHOLE, bool STATES, bool RETURNED>
-__global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void la_chunks(Args A) {
+__global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES)) void la_chunks(Args A) {
   typedef Ops<T> O;
   typedef typename O::Frag Frag;
   constexpr int NT = NW * 64, NB = C / 32, KB = KP / 32, RK = row_elems<T, KP, true>(), RV = row_elems<T, NW * 32, false>();
@@ -230,11 +236,14 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
   __shared__ __align__(16) T sv[C * RV];
   __shared__ __align__(16) T sq[STATES ? 8 : C * RK];
 
-  const LaPass& P = A.p.pass[blockIdx.z];
+  // the passes of one segment run side by side: what one reads, the others find in the last-level cache
   int blk = xcd_remap(blockIdx.x, A.nblk);
   const int vb = blk % A.nvb;
   blk /= A.nvb;
-  const int seg = blk % A.nseg, bh = blk / A.nseg;
+  const int pass = blk % A.npass;
+  blk /= A.npass;
+  const LaPass& P = A.p.pass[pass];
+  const int seg = P.rev ? A.nseg - 1 - blk % A.nseg : blk % A.nseg, bh = blk / A.nseg;
   const int b = bh / (int)A.p.H, hd = bh % (int)A.p.H;
   const int lane = threadIdx.x % 64, half = lane / 32, col = lane % 32, wv = wave_id();
   const int n0 = vb * NW * 32 + wv * 32;  // first column of this wavefront
@@ -252,7 +261,7 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
   T* o = (T*)P.o + b * P.os[0] + hd * P.os[1];
   const int vw = P.V - vb * NW * 32;
 
-  float* states = A.states[blockIdx.z];
+  float* states = A.states[pass];
   if (states) states += ((int64_t)bh * A.nseg + seg) * P.K * P.V;
   const int64_t sbase = (int64_t)bh * P.K * P.V;
 
@@ -287,25 +296,25 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
 
   constexpr bool three = __is_same(T, bf16) && RETURNED;
 
-  Tile<T, C, KP, NT, WHOLE> tk, tq;
-  Tile<T, C, NW * 32, NT, WHOLE> tv;
-  if (lo < hi) {
-    tk.load(k, P.ks[2], P.K, lo, hi, turn);
-    tv.load(v, P.vs[2], vw, lo, hi, turn);
-    if constexpr (!STATES) tq.load(q, P.qs[2], P.K, lo, hi, turn);
-  }
-  for (int p0 = lo; p0 < hi; p0 += C) {
+  // Tiles on their way: the next chunk's, and for STATES, which has the registers, the one after it too (two 32 KB loads
+  // to a workgroup keep a CU's share of HBM busy, one does not: 72 -> 51 us at B2 H32 T8192)
+  constexpr int AHEAD = STATES ? 2 : 1;
+  Tile<T, C, KP, NT, WHOLE> tk[AHEAD], tq;
+  Tile<T, C, NW * 32, NT, WHOLE> tv[AHEAD];
+  auto fetch = [&](auto& k1, auto& v1, int p) {
+    if (p >= hi) return;
+    k1.load(k, P.ks[2], P.K, p, hi, turn);
+    v1.load(v, P.vs[2], vw, p, hi, turn);
+    if constexpr (!STATES) tq.load(q, P.qs[2], P.K, p, hi, turn);
+  };
+  auto chunk = [&](auto& k1, auto& v1, int p0) {
     __syncthreads();  // the chunk before has been read
-    tk.template store<true>(sk);
-    tv.template store<false>(sv);
+    k1.template store<true>(sk);
+    v1.template store<false>(sv);
     if constexpr (!STATES) tq.template store<true>(sq);
     __syncthreads();
-    if (p0 + C < hi) {
-      tk.load(k, P.ks[2], P.K, p0 + C, hi, turn);
-      tv.load(v, P.vs[2], vw, p0 + C, hi, turn);
-      if constexpr (!STATES) tq.load(q, P.qs[2], P.K, p0 + C, hi, turn);
-    }
-    if (!mine) continue;
+    fetch(k1, v1, p0 + AHEAD * C);
+    if (!mine) return;
     const int cl = min(C, hi - p0), shift = C - cl;  // tokens of this chunk: its last rows
     const int early = P.rev && p0 == 0 ? 1 : 0;      // the entering state meets the first token without a decay
     // opaque, or the compiler forms every product of these weights before the loop, and spills
@@ -428,6 +437,13 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
         if (three) S[kb] = O::mma(kf, v3, S[kb]);
       }
     }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) fetch(tk[i], tv[i], lo + i * C);
+  for (int p0 = lo; p0 < hi; p0 += AHEAD * C) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i == 0 || p0 + i * C < hi) chunk(tk[i], tv[i], p0 + i * C);
   }
 
   // the final state of a head in one segment, or the segment's own
@@ -456,7 +472,7 @@ __global__ __launch_bounds__(NW * 64, KP <= 128 && sizeof(T) == 2 ? 2 : 1) void 
 template <typename T, int KP, int NW>
 void launch_dims(const Args& a, bool whole, bool states, hipStream_t st) {
   constexpr int C = chunk_tokens(sizeof(T), KP);
-  const dim3 grid((unsigned)a.nblk, 1, (unsigned)a.npass);
+  const dim3 grid((unsigned)a.nblk);
   const bool returned = __is_same(T, bf16) && a.returned;
   auto run = [&](auto kernel) { kernel<<<grid, NW * 64, 0, st>>>(a); };
   if (states) {

@@ -290,7 +290,7 @@ struct GroupedModuleFn : public Function<GroupedModuleFn> {
 struct LinearAttentionFn : public Function<LinearAttentionFn> {
   // o over token-major memory, and the final state if it is wanted
   static variable_list run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const Tensor& s0,
-                           const Tensor& lengths, double scale, bool want_state) {
+                           const Tensor& lengths, double scale, bool want_state, Tensor* states = nullptr) {
     const int64_t B = q.size(0), H = q.size(1), T = q.size(2), K = q.size(3), V = v.size(3);
     const int dt = dtype_code(q);
     Tensor o = at::empty({B, T, H, V}, q.options()).transpose(1, 2);
@@ -304,6 +304,7 @@ struct LinearAttentionFn : public Function<LinearAttentionFn> {
                                    static_cast<float*>(ptr(st)), ptr(ws), n, B, H, T, K, V, (float)scale, dt,
                                    stream_of(q)),
           "linear attention forward");
+    if (states) *states = ws;
     variable_list out{o};
     if (want_state) out.push_back(st);
     return out;
@@ -312,7 +313,9 @@ struct LinearAttentionFn : public Function<LinearAttentionFn> {
                                const std::optional<Tensor>& s0, const Tensor& lam, const std::optional<Tensor>& lengths,
                                double scale, bool want_state) {
     const Tensor s = s0.value_or(Tensor()), n = lengths.value_or(Tensor());
-    variable_list out = run(q, k, v, lam, s, n, scale, want_state);
+    Tensor states;  // before each segment: the backward starts from them (an internal buffer, a function of the inputs)
+    variable_list out = run(q, k, v, lam, s, n, scale, want_state, &states);
+    if (states.defined()) ctx->saved_data["states"] = states;
     ctx->save_for_backward({q, k, v, s, lam, n});
     ctx->saved_data["scale"] = scale;
     ctx->set_materialize_grads(false);
@@ -333,12 +336,14 @@ struct LinearAttentionFn : public Function<LinearAttentionFn> {
     const int64_t n = abi.linear_attention_ws_bytes(B, H, T, K, V, dt, 1);
     check(n, "linear attention backward workspace query");
     const Tensor ws = bytes_like(q, n);
+    const auto it = ctx->saved_data.find("states");
+    const Tensor states = it != ctx->saved_data.end() ? it->second.toTensor() : Tensor();
     check(abi.linear_attention_bwd(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(),
                                    static_cast<float*>(ptr(lam)), static_cast<float*>(ptr(s0)),
                                    static_cast<int32_t*>(ptr(lengths)), ptr(d), d.strides().data(),
                                    static_cast<float*>(ptr(ds)), ptr(dq), dq.strides().data(), ptr(dk),
                                    dk.strides().data(), ptr(dv), dv.strides().data(), static_cast<float*>(ptr(ds0)),
-                                   ptr(ws), n, B, H, T, K, V, (float)ctx->saved_data["scale"].toDouble(), dt,
+                                   ptr(states), ptr(ws), n, B, H, T, K, V, (float)ctx->saved_data["scale"].toDouble(), dt,
                                    stream_of(q)),
           "linear attention backward");
     return {dq, dk, dv, ds0, Tensor(), Tensor(), Tensor(), Tensor()};

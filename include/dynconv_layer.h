@@ -36,7 +36,8 @@ extern "C" {
  *   lengths [B] int32 or NULL: sequence b has lengths[b] (clamped to 0 .. T)
  *   tokens; rows past them are not used, whatever they hold, their outputs are
  *   zero and the state is the one after the last token.
- * T may be 0. */
+ * T may be 0.  Both calls need a workspace of dc_linear_attention_ws_bytes
+ * bytes (0: none), 16-byte aligned. */
 int64_t dc_linear_attention_ws_bytes(int64_t B, int64_t H, int64_t T, int64_t K, int64_t V, int dtype, int bwd);
 int dc_linear_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                             const void* v, const int64_t* v_strides, const float* log_decay,
@@ -46,14 +47,16 @@ int dc_linear_attention_fwd(const void* q, const int64_t* q_strides, const void*
 
 /* Gradients of dc_linear_attention_fwd: dq, dk, dv from d_o [B, H, T, V] and
  * d_final_state [B, H, K, V] (NULL: zero), and d_initial_state (NULL: not
- * wanted).  Rows past a sequence's length get zero. */
+ * wanted).  Rows past a sequence's length get zero.  fwd_workspace is NULL or the
+ * workspace of the forward of the same inputs, as that call left it: it holds
+ * the states that the backward would form again (trusted, not checked). */
 int dc_linear_attention_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                             const void* v, const int64_t* v_strides, const float* log_decay,
                             const float* initial_state, const int32_t* lengths, const void* d_o,
                             const int64_t* do_strides, const float* d_final_state, void* dq,
                             const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
-                            const int64_t* dv_strides, float* d_initial_state, void* workspace, int64_t ws_bytes,
-                            int64_t B, int64_t H, int64_t T, int64_t K, int64_t V, float scale, int dtype,
+                            const int64_t* dv_strides, float* d_initial_state, const void* fwd_workspace,
+                            void* workspace, int64_t ws_bytes, int64_t B, int64_t H, int64_t T, int64_t K, int64_t V, float scale, int dtype,
                             void* stream);
 
 /* One token of each of B sequences: q, k [B, H, K], v [B, H, V] with strides

@@ -37,9 +37,9 @@ def la_fwd(lib, B=1, H=2, T=8, K=16, V=16, q=P, o=P, lam=P, s=st(1, 1, 1), dt=0,
     return lib.dc_linear_attention_fwd(q, s, P, s, P, s, lam, None, None, o, s, None, ws, nws, B, H, T, K, V, 1.0, dt, None)
 
 
-def la_bwd(lib, B=1, H=2, T=8, K=16, V=16, dq=P, s=st(1, 1, 1), dt=0, ws=P, nws=1 << 40):
-    return lib.dc_linear_attention_bwd(P, s, P, s, P, s, P, None, None, P, s, None, dq, s, P, s, P, s, None, ws, nws, B, H,
-                                       T, K, V, 1.0, dt, None)
+def la_bwd(lib, B=1, H=2, T=8, K=16, V=16, dq=P, s=st(1, 1, 1), dt=0, ws=P, nws=1 << 40, states=None):
+    return lib.dc_linear_attention_bwd(P, s, P, s, P, s, P, None, None, P, s, None, dq, s, P, s, P, s, None, states, ws, nws,
+                                       B, H, T, K, V, 1.0, dt, None)
 
 
 @pytest.mark.parametrize("call", [la_fwd, la_bwd])
@@ -61,6 +61,7 @@ def test_linear_attention_forward_pointers(lib):
     assert la_fwd(lib, q=None) == E_NULL and la_fwd(lib, o=None) == E_NULL and la_fwd(lib, lam=None) == E_NULL
     assert la_fwd(lib, q=P + 1) == E_ALIGN and la_fwd(lib, q=P + 2, dt=2) == E_ALIGN
     assert la_fwd(lib, lam=P + 2) == E_ALIGN
+    assert la_bwd(lib, states=P + 8) == E_WS
     assert la_bwd(lib, dq=None) == E_NULL and la_bwd(lib, dq=P + 1) == E_ALIGN
     if NO_DEV:  # no rows: the activations' pointers do not matter
         assert la_fwd(lib, T=0, q=None, o=None) == E_DEV
