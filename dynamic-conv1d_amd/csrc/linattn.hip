@@ -120,20 +120,22 @@ hipError_t launch(const LaProblem& p, const Cut& c, float* const* states_of, boo
     a.p = p;
     a.seg = c.seg;
     a.nseg = c.nseg;
-    const int kp = cover(p.pass[i].K), nw = p.pass[i].V <= 64 ? 2 : 4;
+    const int kp = states ? la::kStateRows : cover(p.pass[i].K), nw = p.pass[i].V <= 64 ? 2 : 4;
     const bool w = whole(p.pass[i], es, states);
-    a.nvb = 1;
+    a.nvb = a.nkb = 1;
     for (int j = i; j < p.npass; ++j) {
       const LaPass& b = p.pass[j];
-      if (done[j] || cover(b.K) != kp || (b.V <= 64 ? 2 : 4) != nw || whole(b, es, states) != w) continue;
+      if (done[j] || (!states && cover(b.K) != kp) || (b.V <= 64 ? 2 : 4) != nw || whole(b, es, states) != w) continue;
       done[j] = true;
       a.p.pass[a.npass] = b;
       a.states[a.npass++] = c.nseg > 1 ? states_of[j] : nullptr;
       a.returned |= b.s_out && states == (c.nseg > 1);
       const int nvb = (b.V + nw * 32 - 1) / (nw * 32);
       if (nvb > a.nvb) a.nvb = nvb;
+      const int nkb = states ? (b.K + kp - 1) / kp : 1;
+      if (nkb > a.nkb) a.nkb = nkb;
     }
-    const int64_t nblk = p.B * p.H * c.nseg * a.nvb * a.npass;
+    const int64_t nblk = p.B * p.H * c.nseg * a.nvb * a.nkb * a.npass;
     if (nblk > 0x7fffffff) return hipErrorInvalidValue;
     a.nblk = (int)nblk;
     hipError_t e;

@@ -26,12 +26,11 @@
 // 8 (e/4) + 4 half + e%4 for element e), so scores and S go from results to
 // operands without leaving their lane: scores are formed as k q^T (column i in
 // lane i), S as k^T v (column n in lane n), o as (v^T scores^T + S^T q^T), whose
-// column i sits in lane i with four neighbouring channels to a store.  q and k
+// column i sits in lane i with four neighbouring channels to a store.  The blocks
+// of scores go round the wavefronts, through LDS, lane by lane as they are.  q and k
 // rows lie in LDS so that a lane's 8 values of that order are neighbours (16-byte
 // reads; two 8-byte reads took twice the LDS's time), v and k columns are read
-// through transposing reads.  The scores are formed by each of the NW
-// wavefronts: 24 of its 78 products at 128 channels, against an exchange
-// through LDS and a barrier.
+// through transposing reads.
 //
 // Precision.  Scores and S are rounded to the inputs' type as operands (relative
 // 2^-8 / 2^-11 of single terms, below the rounding of o); the products that make
@@ -54,7 +53,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // chunk), and the states before each segment, [B * H][nseg][K * V] per set.
 struct Args {
   LaProblem p;
-  int npass, seg, nseg, nvb;
+  int npass, seg, nseg, nvb, nkb;
   int nblk;
   bool returned;  // a state formed by this launch is the caller's result
   // what a pass starts its segments from / a state pass writes: one set of states (null: one segment, s_in / s_out)
@@ -63,6 +62,9 @@ struct Args {
 
 // Tokens of a chunk: 64, or 32 where three tiles of 64 float32 rows would pass the LDS.
 __host__ __device__ constexpr int chunk_tokens(int es, int kp) { return es == 4 && kp > 128 ? 32 : 64; }
+
+// Rows of a state that a workgroup forms in the states' launch: 64, so that three workgroups fit a CU whatever K is.
+constexpr int kStateRows = 64;
 
 // Where channel c of a row of q or k lies in LDS: of each 16 channels the second and third quads change places, so that
 // the 8 channels of a lane's half, 4 half .. + 3 and 8 + 4 half .. + 3, are neighbours.
@@ -221,11 +223,10 @@ __device__ __forceinline__ void scale(float* v, float by) {
 
 // Wavefronts on a SIMD that leave a kernel's registers unspilled.
 constexpr int waves_per_simd(int es, int kp, int nw, bool states) {
-  if (es == 4 || kp > 128) return 1;
-  return states ? (kp == 64 ? 3 : 2) : kp == 128 && nw == 2 ? 1 : 2;
+  return es == 4 || kp > 128 || (kp == 128 && nw == 2) ? 1 : states ? 3 : 2;
 }
 
-// STATES: only the state after each segment, from zero, for states[pass].  RETURNED: a state that is formed here is the
+// STATES: only the state after each segment, from zero, for states[pass], KP of its rows to a workgroup.  RETURNED: a state that is formed here is the
 // caller's result (three parts in bf16; in every kernel they cost the common one 10% by spilled registers).
 template <typename T, int KP, int NW, int C, bool WHOLE, bool STATES, bool RETURNED>
 __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES)) void la_chunks(Args A) {
@@ -235,11 +236,17 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   __shared__ __align__(16) T sk[C * RK];
   __shared__ __align__(16) T sv[C * RV];
   __shared__ __align__(16) T sq[STATES ? 8 : C * RK];
+  // scores as operands: blocks of 32 x 32 on and below the diagonal, two steps of a lane's 8, and what they are smaller by
+  constexpr int NP = NB * (NB + 1) / 2;
+  __shared__ __align__(16) Frag sp[STATES ? 1 : NP * 2 * 64];
+  __shared__ float sdown[NP];
 
   // the passes of one segment run side by side: what one reads, the others find in the last-level cache
   int blk = xcd_remap(blockIdx.x, A.nblk);
   const int vb = blk % A.nvb;
   blk /= A.nvb;
+  const int k0 = STATES ? blk % A.nkb * KP : 0;  // first row of the state
+  if (STATES) blk /= A.nkb;
   const int pass = blk % A.npass;
   blk /= A.npass;
   const LaPass& P = A.p.pass[pass];
@@ -247,7 +254,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   const int b = bh / (int)A.p.H, hd = bh % (int)A.p.H;
   const int lane = threadIdx.x % 64, half = lane / 32, col = lane % 32, wv = wave_id();
   const int n0 = vb * NW * 32 + wv * 32;  // first column of this wavefront
-  if (vb * NW * 32 >= P.V) return;
+  if (vb * NW * 32 >= P.V || k0 >= P.K) return;
   if (STATES && seg == A.nseg - 1 && !P.s_out) return;  // nothing reads the last segment's
   const bool mine = n0 < P.V;
   const float lam = A.p.log_decay[hd], lam2 = lam * 1.44269504088896f;
@@ -255,7 +262,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   const int len = A.p.lengths ? min(max(A.p.lengths[b], 0), T_) : T_;
   const int lo = seg * A.seg, top = min(T_, lo + A.seg), hi = min(len, top);
   const int turn = P.rev ? len - 1 : -1;
-  const T* k = (const T*)P.k + b * P.ks[0] + hd * P.ks[1];
+  const T* k = (const T*)P.k + b * P.ks[0] + hd * P.ks[1] + k0;
   const T* v = (const T*)P.v + b * P.vs[0] + hd * P.vs[1] + vb * NW * 32;
   const T* q = (const T*)P.q + b * P.qs[0] + hd * P.qs[1];
   T* o = (T*)P.o + b * P.os[0] + hd * P.os[1];
@@ -279,7 +286,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        S[kb][r] = __uint_as_float(bload32(rs, at(kb * 32 + 8 * (r / 4) + 4 * half + r % 4, n0 + col)));
+        S[kb][r] = __uint_as_float(bload32(rs, at(k0 + kb * 32 + 8 * (r / 4) + 4 * half + r % 4, n0 + col)));
   }
 
   // weights that every full chunk has, element e of a step (or register r of a result) at row(e): of the last 16
@@ -296,14 +303,13 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
 
   constexpr bool three = __is_same(T, bf16) && RETURNED;
 
-  // Tiles on their way: the next chunk's, and for STATES, which has the registers, the one after it too (two 32 KB loads
-  // to a workgroup keep a CU's share of HBM busy, one does not: 72 -> 51 us at B2 H32 T8192)
+  // Tiles on their way: the next chunk's, and for STATES, which has the registers, the one after it too.
   constexpr int AHEAD = STATES ? 2 : 1;
   Tile<T, C, KP, NT, WHOLE> tk[AHEAD], tq;
   Tile<T, C, NW * 32, NT, WHOLE> tv[AHEAD];
   auto fetch = [&](auto& k1, auto& v1, int p) {
     if (p >= hi) return;
-    k1.load(k, P.ks[2], P.K, p, hi, turn);
+    k1.load(k, P.ks[2], P.K - k0, p, hi, turn);
     v1.load(v, P.vs[2], vw, p, hi, turn);
     if constexpr (!STATES) tq.load(q, P.qs[2], P.K, p, hi, turn);
   };
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
     if constexpr (!STATES) tq.template store<true>(sq);
     __syncthreads();
     fetch(k1, v1, p0 + AHEAD * C);
-    if (!mine) return;
+    if (STATES && !mine) return;
     const int cl = min(C, hi - p0), shift = C - cl;  // tokens of this chunk: its last rows
     const int early = P.rev && p0 == 0 ? 1 : 0;      // the entering state meets the first token without a decay
     // opaque, or the compiler forms every product of these weights before the loop, and spills
@@ -323,68 +329,78 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
     float* const Sf = reinterpret_cast<float*>(S);
 
     if constexpr (!STATES) {
-      f32x16 acc[NB] = {};
-      bool small = false;
-      if constexpr (O::kNarrow) {
-        small = near_end(largest<KB * 16>(Sf));
-        if (small) scale<KB * 16>(Sf, kSmaller);
+      // the blocks of scores go round the wavefronts: 0 (0, 0), 1 (1, 0), 2 (1, 1); those of zero rows are not used
+      for (int blk = wv; blk < NP; blk += NW) {
+        const int ib = blk > 0, jb = blk > 1;
+        if (jb * 32 + 31 < shift) continue;
+        f32x16 sc = {};
+#pragma unroll
+        for (int s = 0; s < KP / 16; ++s)
+          sc = O::mma(O::rows(sk + (jb * 32 + col) * RK + s * 16, half), O::rows(sq + (ib * 32 + col) * RK + s * 16, half), sc);
+        float t[16];
+        if (blk == 1) {  // by way of the block's last token: g^{i-j} = g^{col+1} g^{31-j}, the first factor with o
+#pragma unroll
+          for (int r = 0; r < 16; ++r) t[r] = sc[r] * (r < 8 ? vlast[r] * g1 : vlast[r - 8]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) t[r] = sc[r] * diag[r];
+        }
+        if constexpr (O::kNarrow) {
+          const bool small = near_end(largest<16>(t));
+          if (small) scale<16>(t, kSmaller);
+          if (lane == 0) sdown[blk] = small ? kSmaller : 1.f;
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) sp[(blk * 2 + s) * 64 + lane] = O::pack(t + 8 * s);
       }
+
+      phase();
+      f32x16 acc[NB] = {};
+      // a state near the end of fp16 takes part smaller: scaled and back in place, or (128 registers of it: the branch
+      // spilled 165) as it is packed
+      constexpr bool ONCE = O::kNarrow && KP <= 128, PACKED = O::kNarrow && KP > 128;
+      bool small = false;
+      if constexpr (O::kNarrow) small = near_end(largest<KB * 16>(Sf));
+      if (ONCE && small) scale<KB * 16>(Sf, kSmaller);
+      const float by = PACKED && small ? kSmaller : 1.f;
 #pragma unroll
       for (int s = 0; s < KP / 16; ++s) {
-        const Frag sf = O::pack(Sf + s * 8);
+        float t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = PACKED ? Sf[s * 8 + e] * by : Sf[s * 8 + e];
+        const Frag sf = O::pack(t);
 #pragma unroll
         for (int ib = 0; ib < NB; ++ib) acc[ib] = O::mma(sf, O::rows(sq + (ib * 32 + col) * RK + s * 16, half), acc[ib]);
       }
-      if constexpr (O::kNarrow)
-        if (small) {
-          scale<KB * 16>(Sf, 1.f / kSmaller);
+      if (O::kNarrow && small) {
+        if constexpr (ONCE) scale<KB * 16>(Sf, 1.f / kSmaller);
 #pragma unroll
-          for (int ib = 0; ib < NB; ++ib) scale<16>(reinterpret_cast<float*>(&acc[ib]), 1.f / kSmaller);
-        }
+        for (int ib = 0; ib < NB; ++ib) scale<16>(reinterpret_cast<float*>(&acc[ib]), 1.f / kSmaller);
+      }
+      __syncthreads();  // the scores are there
+      if (!mine) return;
 #pragma unroll
       for (int ib = 0; ib < NB; ++ib) {
-        phase();
         if (ib * 32 + 31 < shift) continue;
-        const int jb0 = shift / 32;  // the first block with tokens
         float* const af = reinterpret_cast<float*>(&acc[ib]);
-        f32x16 sc[NB] = {};
-#pragma unroll
-        for (int s = 0; s < KP / 16; ++s) {
-          const Frag qf = O::rows(sq + (ib * 32 + col) * RK + s * 16, half);
-#pragma unroll
-          for (int jb = 0; jb <= ib; ++jb) sc[jb] = O::mma(O::rows(sk + (jb * 32 + col) * RK + s * 16, half), qf, sc[jb]);
-        }
-        bool tiny = false;  // acc is held smaller
-        auto add = [&](float* t, int jb) {
-          if constexpr (O::kNarrow) {
-            if (tiny) scale<16>(t, kSmaller);
-            else if (near_end(largest<16>(t))) {
-              tiny = true;
-              scale<16>(t, kSmaller);
-              scale<16>(af, kSmaller);
-            }
-          }
+        auto add = [&](int jb) {
+          const int blk = ib + jb;
+          const bool down = O::kNarrow && sdown[blk] != 1.f;
+          if (down) scale<16>(af, kSmaller);
 #pragma unroll
           for (int s = 0; s < 2; ++s)
-            acc[ib] = O::mma(O::template cols<false>(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane), O::pack(t + 8 * s), acc[ib]);
+            acc[ib] = O::mma(O::template cols<false>(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane),
+                             sp[(blk * 2 + s) * 64 + lane], acc[ib]);
+          if (down) scale<16>(af, 1.f / kSmaller);
         };
-        if (NB > 1 && ib > jb0) {
-          // the state and the block before by way of its last token: g^{i+1} = g^{32} g^{col+1}, g^{i-j} = g^{col+1} g^{31-j}
+        if (ib > 0 && shift < 32) {  // the state and the block before by way of its last token: g^{i+1} = g^{32} g^{col+1}
           scale<16>(af, power(lam2, 32 - early - shift));
-          float t[16];
-#pragma unroll
-          for (int r = 0; r < 16; ++r) t[r] = sc[0][r] * (r < 8 ? vlast[r] * g1 : vlast[r - 8]);
-          add(t, 0);
+          add(0);
           scale<16>(af, gcol);
         } else {
           scale<16>(af, P.so * power(lam2, max(ib * 32 + col + 1 - early - shift, 0)));
         }
-        float t[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) t[r] = sc[ib][r] * diag[r];
-        add(t, ib);
-        if constexpr (O::kNarrow)
-          if (tiny) scale<16>(af, 1.f / kSmaller);
+        add(ib);
         const int i = ib * 32 + col - shift;
         if (i >= 0) {
           T* to = o + (int64_t)(turn >= 0 ? turn - p0 - i : p0 + i) * P.os[2] + n0 + 4 * half;
@@ -459,7 +475,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        BufUnit<4>::template store<false>(__float_as_uint(S[kb][r] * g), rs, at(kb * 32 + 8 * (r / 4) + h4 + r % 4, c));
+        BufUnit<4>::template store<false>(__float_as_uint(S[kb][r] * g), rs, at(k0 + kb * 32 + 8 * (r / 4) + h4 + r % 4, c));
   }
   if constexpr (!STATES) {  // rows past the sequence's length
     const int z0 = max(len, lo), w = min(vw, NW * 32);
@@ -469,25 +485,20 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
 }
 
 // The kernel of a type for these sizes (instantiated in linattn_<type>.hip).
-template <typename T, int KP, int NW>
-void launch_dims(const Args& a, bool whole, bool states, hipStream_t st) {
+template <typename T, int KP, int NW, bool STATES>
+void launch_dims(const Args& a, bool whole, hipStream_t st) {
   constexpr int C = chunk_tokens(sizeof(T), KP);
-  const dim3 grid((unsigned)a.nblk);
-  const bool returned = __is_same(T, bf16) && a.returned;
-  auto run = [&](auto kernel) { kernel<<<grid, NW * 64, 0, st>>>(a); };
-  if (states) {
-    if (returned) run(whole ? la_chunks<T, KP, NW, C, true, true, __is_same(T, bf16)> : la_chunks<T, KP, NW, C, false, true, __is_same(T, bf16)>);
-    else run(whole ? la_chunks<T, KP, NW, C, true, true, false> : la_chunks<T, KP, NW, C, false, true, false>);
-  } else {
-    if (returned) run(whole ? la_chunks<T, KP, NW, C, true, false, __is_same(T, bf16)> : la_chunks<T, KP, NW, C, false, false, __is_same(T, bf16)>);
-    else run(whole ? la_chunks<T, KP, NW, C, true, false, false> : la_chunks<T, KP, NW, C, false, false, false>);
-  }
+  constexpr bool B16 = __is_same(T, bf16);
+  auto run = [&](auto kernel) { kernel<<<(unsigned)a.nblk, NW * 64, 0, st>>>(a); };
+  if (B16 && a.returned) run(whole ? la_chunks<T, KP, NW, C, true, STATES, B16> : la_chunks<T, KP, NW, C, false, STATES, B16>);
+  else run(whole ? la_chunks<T, KP, NW, C, true, STATES, false> : la_chunks<T, KP, NW, C, false, STATES, false>);
 }
 template <typename T>
 hipError_t launch(const Args& a, int kp, int nw, bool whole, bool states, hipStream_t st) {
-  if (kp == 64) nw == 2 ? launch_dims<T, 64, 2>(a, whole, states, st) : launch_dims<T, 64, 4>(a, whole, states, st);
-  else if (kp == 128) nw == 2 ? launch_dims<T, 128, 2>(a, whole, states, st) : launch_dims<T, 128, 4>(a, whole, states, st);
-  else nw == 2 ? launch_dims<T, 256, 2>(a, whole, states, st) : launch_dims<T, 256, 4>(a, whole, states, st);
+  if (states) nw == 2 ? launch_dims<T, kStateRows, 2, true>(a, whole, st) : launch_dims<T, kStateRows, 4, true>(a, whole, st);
+  else if (kp == 64) nw == 2 ? launch_dims<T, 64, 2, false>(a, whole, st) : launch_dims<T, 64, 4, false>(a, whole, st);
+  else if (kp == 128) nw == 2 ? launch_dims<T, 128, 2, false>(a, whole, st) : launch_dims<T, 128, 4, false>(a, whole, st);
+  else nw == 2 ? launch_dims<T, 256, 2, false>(a, whole, st) : launch_dims<T, 256, 4, false>(a, whole, st);
   return hipGetLastError();
 }
 extern template hipError_t launch<bf16>(const Args&, int, int, bool, bool, hipStream_t);
