@@ -10,7 +10,8 @@
 // and dx, dgate out, each once.  A group's channels stay in the registers of L
 // neighbouring lanes (NV pieces of VEC channels each; L a power of two up to 64,
 // so that 64 / L groups share a wavefront): mean, then the sum of squares of the
-// differences, both in float32 from the registers, so large means cost no digits.  A
+// differences, both in float32 from the registers, so large means cost no digits (a group of more than 128 pieces
+// takes the workgroup's 256 lanes).  A
 // wavefront keeps its channels and walks rows: weight and bias stay in registers, and
 // in the backward dw and db too.  Each workgroup writes them once, as partial sums
 // that reduce_partials adds in a fixed order.  The backward forms mean and rstd again
@@ -31,20 +32,39 @@ struct GnArgs {
   float *pw, *pb;  // partial sums of dw and db, [row blocks][D] each (null: not wanted)
   int64_t M, D;
   int size, lanes;  // channels of a group, lanes it takes (a power of two)
-  int pdtype;
+  bool wide_params;   // weight and bias are float32 (else of x's type)
+  bool param_pieces;  // and 16-byte aligned
   float eps;
   int act;
 };
 
-__device__ __forceinline__ float param(const void* p, int64_t i, int dtype, float none) {
-  if (!p) return none;
-  return dtype == kBF16 ? (float)((const bf16*)p)[i] : dtype == kFP16 ? (float)((const fp16*)p)[i] : ((const float*)p)[i];
+// Sum over the group's lanes: every lane gets it.  Up to 16 lanes by data moves within the registers' rows (each step's
+// partner holds the other half's sum), beyond through the exchange network.
+__device__ __forceinline__ float lane_sum(float v, int lanes) {
+  if (lanes > 1) v += dpp_f<0xB1>(v);   // pairs
+  if (lanes > 2) v += dpp_f<0x4E>(v);   // quads
+  if (lanes > 4) v += dpp_f<0x141>(v);  // the mirrored lane of 8
+  if (lanes > 8) v += dpp_f<0x140>(v);  // of 16
+  if (lanes > 16) v += __shfl_xor(v, 16);
+  if (lanes > 32) v += __shfl_xor(v, 32);
+  return v;
 }
 
-// Sum over the group's lanes: every lane gets it.
-__device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int m = 1; m < lanes; m *= 2) v += __shfl_xor(v, m);
-  return v;
+// N sums over a group at once.  WIDE: over the workgroup, the wavefronts' sums meeting in LDS (`slot` alternates, so one
+// barrier serves).
+template <bool WIDE, int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], int lanes, float (*red)[kWaves][2], int& slot) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = lane_sum(v[i], WIDE ? 64 : lanes);
+  if constexpr (WIDE) {
+    if (threadIdx.x % 64 == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) red[slot][threadIdx.x / 64][i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (red[slot][0][i] + red[slot][1][i]) + (red[slot][2][i] + red[slot][3][i]);
+    slot ^= 1;
+  }
 }
 
 __device__ __forceinline__ float sigmoid(float a) { return 1.f / (1.f + __expf(-a)); }
@@ -56,8 +76,9 @@ struct Lane {
   bool live[NV];    // piece i: channels ch + i * lanes * VEC ..
   int step;         // channels from a piece to the next
   __device__ __forceinline__ Lane(const GnArgs& A) {
-    const int lane = threadIdx.x % 64, gl = lane & (A.lanes - 1);
-    const int64_t group = (int64_t)blockIdx.x * (64 / A.lanes) + lane / A.lanes;
+    // a group of more lanes than a wavefront's has the workgroup
+    const int lane = A.lanes > 64 ? threadIdx.x : threadIdx.x % 64, gl = lane & (A.lanes - 1);
+    const int64_t group = (int64_t)blockIdx.x * (A.lanes > 64 ? 1 : 64 / A.lanes) + lane / A.lanes;
     step = A.lanes * VEC;
     ch = group * A.size + gl * VEC;
 #pragma unroll
@@ -65,39 +86,50 @@ struct Lane {
   }
 };
 
+// A row's pieces as they come from memory: on their way while the row before is computed.
 template <typename T, int VEC, int NV>
-__device__ __forceinline__ void load_row(const Lane<VEC, NV>& L, const void* p, int64_t row, float (&v)[NV][VEC]) {
+struct Row {
+  Raw<T, VEC> v[NV];
+  __device__ __forceinline__ void load(const Lane<VEC, NV>& L, const void* p, int64_t row) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (L.live[i]) load_vals<T, VEC>((const T*)p + row + L.ch + i * L.step, v[i]);
-    else zero_vals<VEC>(v[i]);
+    for (int i = 0; i < NV; ++i) {
+      if (L.live[i]) v[i].load((const T*)p + row + L.ch + i * L.step);
+      else v[i].zero();
+    }
   }
-}
+  __device__ __forceinline__ void get(float (&f)[NV][VEC]) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i].to_float(f[i]);
+  }
+};
 template <typename T, int VEC, int NV>
 __device__ __forceinline__ void store_row(const Lane<VEC, NV>& L, void* p, int64_t row, const float (&v)[NV][VEC]) {
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if (L.live[i]) store_vals<T, VEC>((T*)p + row + L.ch + i * L.step, v[i]);
+    if (L.live[i]) store_vals<T, VEC, VEC * sizeof(T) == 16>((T*)p + row + L.ch + i * L.step, v[i]);
 }
 
 // x -> xh in place; returns rstd.
-template <int VEC, int NV>
-__device__ __forceinline__ float normalise(const Lane<VEC, NV>& L, const GnArgs& A, float (&x)[NV][VEC]) {
+template <bool WIDE, int VEC, int NV>
+__device__ __forceinline__ float normalise(const Lane<VEC, NV>& L, const GnArgs& A, float (*red)[kWaves][2], int& slot,
+                                           float (&x)[NV][VEC]) {
   const float inv = 1.f / A.size;
-  float s = 0.f, s2 = 0.f;
+  float s[1] = {0.f}, s2[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) s += x[i][j];
-  const float mean = group_sum(s, A.lanes) * inv;
+    for (int j = 0; j < VEC; ++j) s[0] += x[i][j];
+  group_sum<WIDE>(s, A.lanes, red, slot);
+  const float mean = s[0] * inv;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       x[i][j] = L.live[i] ? x[i][j] - mean : 0.f;
-      s2 += x[i][j] * x[i][j];
+      s2[0] += x[i][j] * x[i][j];
     }
-  const float rstd = 1.f / sqrtf(group_sum(s2, A.lanes) * inv + A.eps);
+  group_sum<WIDE>(s2, A.lanes, red, slot);
+  const float rstd = 1.f / sqrtf(s2[0] * inv + A.eps);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -105,28 +137,59 @@ __device__ __forceinline__ float normalise(const Lane<VEC, NV>& L, const GnArgs&
   return rstd;
 }
 
-template <int VEC, int NV>
+// weight and bias of the lane's channels, of type P (T or float)
+template <typename P, int VEC, int NV>
+__device__ __forceinline__ void load_param(const Lane<VEC, NV>& L, const void* p, bool pieces, float none,
+                                           float (&v)[NV][VEC]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[i][j] = L.live[i] ? none : 0.f;
+    if (p && L.live[i]) {
+      const P* q = (const P*)p + L.ch + i * L.step;
+      if (pieces) {
+        load_vals<P, VEC>(q, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] = (float)q[j];
+      }
+    }
+  }
+}
+template <typename T, int VEC, int NV>
 __device__ __forceinline__ void load_params(const Lane<VEC, NV>& L, const GnArgs& A, float (&w)[NV][VEC],
                                             float (&b)[NV][VEC]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      w[i][j] = L.live[i] ? param(A.weight, L.ch + i * L.step + j, A.pdtype, 1.f) : 0.f;
-      b[i][j] = L.live[i] ? param(A.bias, L.ch + i * L.step + j, A.pdtype, 0.f) : 0.f;
-    }
+  if (A.wide_params) {
+    load_param<float, VEC, NV>(L, A.weight, A.param_pieces, 1.f, w);
+    load_param<float, VEC, NV>(L, A.bias, A.param_pieces, 0.f, b);
+  } else {
+    load_param<T, VEC, NV>(L, A.weight, A.param_pieces, 1.f, w);
+    load_param<T, VEC, NV>(L, A.bias, A.param_pieces, 0.f, b);
+  }
 }
 
-template <typename T, int VEC, int NV>
+template <typename T, int VEC, int NV, bool WIDE>
 __global__ __launch_bounds__(64 * kWaves) void gn_fwd_kernel(GnArgs A) {
+  __shared__ float red[2][kWaves][2];
+  int slot = 0;
   const Lane<VEC, NV> L(A);
+  const int64_t step = (int64_t)gridDim.y * (WIDE ? 1 : kWaves);
+  int64_t m = WIDE ? (int64_t)blockIdx.y : (int64_t)blockIdx.y * kWaves + wave_id();
+  if (m >= A.M) return;
+  Row<T, VEC, NV> xr, ar;
+  xr.load(L, A.x, m * A.D);
+  if (A.gate) ar.load(L, A.gate, m * A.D);
   float w[NV][VEC], b[NV][VEC];
-  load_params<VEC, NV>(L, A, w, b);
-  for (int64_t m = (int64_t)blockIdx.y * kWaves + wave_id(); m < A.M; m += (int64_t)gridDim.y * kWaves) {
+  load_params<T, VEC, NV>(L, A, w, b);
+  for (; m < A.M; m += step) {
     float x[NV][VEC], a[NV][VEC];
-    load_row<T, VEC, NV>(L, A.x, m * A.D, x);
-    if (A.gate) load_row<T, VEC, NV>(L, A.gate, m * A.D, a);
-    normalise<VEC, NV>(L, A, x);
+    xr.get(x);
+    if (A.gate) ar.get(a);
+    if (m + step < A.M) {
+      xr.load(L, A.x, (m + step) * A.D);
+      if (A.gate) ar.load(L, A.gate, (m + step) * A.D);
+    }
+    normalise<WIDE, VEC, NV>(L, A, red, slot, x);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -139,25 +202,37 @@ __global__ __launch_bounds__(64 * kWaves) void gn_fwd_kernel(GnArgs A) {
   }
 }
 
-template <typename T, int VEC, int NV>
+template <typename T, int VEC, int NV, bool WIDE>
 __global__ __launch_bounds__(64 * kWaves) void gn_bwd_kernel(GnArgs A) {
-  __shared__ float red[kWaves][64 * VEC];
+  __shared__ float red[2][kWaves][2], sum[WIDE ? 1 : kWaves][WIDE ? 1 : 64 * VEC];
+  int slot = 0;
   const Lane<VEC, NV> L(A);
+  const int64_t step = (int64_t)gridDim.y * (WIDE ? 1 : kWaves);
+  int64_t m = WIDE ? (int64_t)blockIdx.y : (int64_t)blockIdx.y * kWaves + wave_id();
+  Row<T, VEC, NV> xr, dr, ar;
+  auto fetch = [&](int64_t row) {
+    if (row >= A.M) return;
+    xr.load(L, A.x, row * A.D);
+    dr.load(L, A.dy, row * A.D);
+    if (A.gate) ar.load(L, A.gate, row * A.D);
+  };
+  fetch(m);
   float w[NV][VEC], b[NV][VEC], dw[NV][VEC], db[NV][VEC];
-  load_params<VEC, NV>(L, A, w, b);
+  load_params<T, VEC, NV>(L, A, w, b);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     zero_vals<VEC>(dw[i]);
     zero_vals<VEC>(db[i]);
   }
   const float inv = 1.f / A.size;
-  for (int64_t m = (int64_t)blockIdx.y * kWaves + wave_id(); m < A.M; m += (int64_t)gridDim.y * kWaves) {
+  for (; m < A.M; m += step) {
     float x[NV][VEC], du[NV][VEC], a[NV][VEC];
-    load_row<T, VEC, NV>(L, A.x, m * A.D, x);
-    load_row<T, VEC, NV>(L, A.dy, m * A.D, du);
-    if (A.gate) load_row<T, VEC, NV>(L, A.gate, m * A.D, a);
-    const float rstd = normalise<VEC, NV>(L, A, x);
-    float c1 = 0.f, c2 = 0.f;
+    xr.get(x);
+    dr.get(du);
+    if (A.gate) ar.get(a);
+    fetch(m + step);
+    const float rstd = normalise<WIDE, VEC, NV>(L, A, red, slot, x);
+    float c[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -174,11 +249,11 @@ __global__ __launch_bounds__(64 * kWaves) void gn_bwd_kernel(GnArgs A) {
         dw[i][j] += du[i][j] * x[i][j];
         db[i][j] += du[i][j];
         du[i][j] *= w[i][j];
-        c1 += du[i][j];
-        c2 += du[i][j] * x[i][j];
+        c[0] += du[i][j];
+        c[1] += du[i][j] * x[i][j];
       }
-    c1 = group_sum(c1, A.lanes) * inv;
-    c2 = group_sum(c2, A.lanes) * inv;
+    group_sum<WIDE>(c, A.lanes, red, slot);
+    const float c1 = c[0] * inv, c2 = c[1] * inv;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -186,25 +261,31 @@ __global__ __launch_bounds__(64 * kWaves) void gn_bwd_kernel(GnArgs A) {
     store_row<T, VEC, NV>(L, A.dx, m * A.D, du);
     if (A.gate) store_row<T, VEC, NV>(L, A.dgate, m * A.D, a);
   }
-  // the wavefronts' sums, piece by piece through LDS
   if (!A.pw && !A.pb) return;
-  const int lane = threadIdx.x % 64, wv = threadIdx.x / 64;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       float* out = t ? A.pb : A.pw;
       if (!out) continue;
-      __syncthreads();
+      out += (int64_t)blockIdx.y * A.D + L.ch + i * L.step;
+      if constexpr (WIDE) {  // a channel has one lane of the workgroup
+        if (L.live[i])
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) red[wv][j * 64 + lane] = t ? db[i][j] : dw[i][j];
-      __syncthreads();
-      if (wv == 0 && L.live[i])
+          for (int j = 0; j < VEC; ++j) out[j] = t ? db[i][j] : dw[i][j];
+      } else {  // the wavefronts' sums meet in LDS
+        const int lane = threadIdx.x % 64, wv = threadIdx.x / 64;
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const int c = j * 64 + lane;
-          out[(int64_t)blockIdx.y * A.D + L.ch + i * L.step + j] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
-        }
+        for (int j = 0; j < VEC; ++j) sum[wv][j * 64 + lane] = t ? db[i][j] : dw[i][j];
+        __syncthreads();
+        if (wv == 0 && L.live[i])
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const int c = j * 64 + lane;
+            out[j] = (sum[0][c] + sum[1][c]) + (sum[2][c] + sum[3][c]);
+          }
+      }
     }
 }
 
@@ -215,33 +296,32 @@ struct Plan {
   int64_t gy;
 };
 
-template <typename T, int VEC, int NV>
+template <typename T, int VEC, int NV, bool WIDE>
 void launch(bool bwd, const GnArgs& a, const Plan& pl, hipStream_t st) {
   const dim3 grid(pl.gx, (unsigned)pl.gy);
-  if (bwd) gn_bwd_kernel<T, VEC, NV><<<grid, 64 * kWaves, 0, st>>>(a);
-  else gn_fwd_kernel<T, VEC, NV><<<grid, 64 * kWaves, 0, st>>>(a);
+  if (bwd) gn_bwd_kernel<T, VEC, NV, WIDE><<<grid, 64 * kWaves, 0, st>>>(a);
+  else gn_fwd_kernel<T, VEC, NV, WIDE><<<grid, 64 * kWaves, 0, st>>>(a);
 }
 
-// Lanes hold at most 64 channels (a group of 4096 over 64 lanes).
+// A group of up to 128 pieces lies in one wavefront, a larger one (up to 4096 channels) in the workgroup.
 template <typename T, int VEC>
 hipError_t launch_nv(bool bwd, const GnArgs& a, const Plan& pl, hipStream_t st) {
+  if (pl.lanes <= 64) {
+    if (pl.nv == 1) launch<T, VEC, 1, false>(bwd, a, pl, st);
+    else launch<T, VEC, 2, false>(bwd, a, pl, st);
+    return hipGetLastError();
+  }
   switch (pl.nv) {
-    case 1: launch<T, VEC, 1>(bwd, a, pl, st); break;
-    case 2:
-      if constexpr (VEC > 1) launch<T, VEC, 2>(bwd, a, pl, st);
-      break;
+    case 1: launch<T, VEC, 1, true>(bwd, a, pl, st); break;
+    case 2: launch<T, VEC, 2, true>(bwd, a, pl, st); break;
     case 4:
-      if constexpr (VEC > 1) launch<T, VEC, 4>(bwd, a, pl, st);
+      if constexpr (VEC <= 4) launch<T, VEC, 4, true>(bwd, a, pl, st);
       break;
-    case 8: launch<T, VEC, 8>(bwd, a, pl, st); break;
-    case 16:
-      if constexpr (VEC == 2 || VEC == 4) launch<T, VEC, 16>(bwd, a, pl, st);
-      break;
-    case 32:
-      if constexpr (VEC == 2) launch<T, VEC, 32>(bwd, a, pl, st);
+    case 8:
+      if constexpr (VEC <= 2) launch<T, VEC, 8, true>(bwd, a, pl, st);
       break;
     default:
-      if constexpr (VEC == 1) launch<T, VEC, 64>(bwd, a, pl, st);
+      if constexpr (VEC == 1) launch<T, VEC, 16, true>(bwd, a, pl, st);
       break;
   }
   return hipGetLastError();

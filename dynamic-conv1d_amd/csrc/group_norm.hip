@@ -10,7 +10,7 @@ using gn::GnArgs;
 using gn::kWaves;
 using gn::Plan;
 
-constexpr int kMaxGroup = 4096;  // channels of a group: at most 64 to a lane
+constexpr int kMaxGroup = 4096;  // channels of a group: at most 16 to a lane
 
 // Alignment that every tensor has (0: none has been given).
 bool all_aligned(std::initializer_list<const void*> ts, int bytes) {
@@ -34,14 +34,17 @@ Plan plan_of(const GnProblem& p) {
   const int64_t pieces = (size + pl.vec - 1) / pl.vec;
   pl.lanes = 1;
   while (pl.lanes < 64 && pl.lanes < pieces) pl.lanes *= 2;
+  if (pieces > 128) pl.lanes = 256;
   const int64_t per = (pieces + pl.lanes - 1) / pl.lanes;
   pl.nv = 1;
-  while (pl.nv < per) pl.nv *= pl.vec == 1 ? 8 : 2;  // single channels: 1, 8 or 64 to a lane
-  pl.gx = (unsigned)((p.groups + 64 / pl.lanes - 1) / (64 / pl.lanes));
-  // row blocks: enough wavefronts for every SIMD of 256 CUs four times over, and no more than there are rows
-  const int64_t want = (4096 + pl.gx * kWaves - 1) / (pl.gx * kWaves), most = (p.M + kWaves - 1) / kWaves;
+  while (pl.nv < per) pl.nv *= 2;
+  const bool wide = pl.lanes > 64;
+  pl.gx = (unsigned)(wide ? p.groups : (p.groups + 64 / pl.lanes - 1) / (64 / pl.lanes));
+  // row blocks: enough wavefronts for every SIMD of 256 CUs eight times over in the forward, four times in the backward
+  // (its partial sums grow with them), and no more than there are rows
+  const int64_t waves = p.dy ? 4096 : 8192, rows = wide ? 1 : kWaves;
+  const int64_t want = (waves + pl.gx * kWaves - 1) / (pl.gx * kWaves), most = (p.M + rows - 1) / rows;
   pl.gy = want < most ? want : most;
-  if (pl.gy < 1) pl.gy = 1;
   return pl;
 }
 
@@ -58,7 +61,7 @@ GnArgs args_of(const GnProblem& p, const Plan& pl) {
   a.x = p.x; a.weight = p.weight; a.bias = p.bias; a.gate = p.gate; a.dy = p.dy;
   a.y = p.y; a.dx = p.dx; a.dgate = p.dgate;
   a.M = p.M; a.D = p.D; a.size = (int)(p.D / p.groups); a.lanes = pl.lanes;
-  a.pdtype = p.pdtype; a.eps = p.eps; a.act = p.act;
+  a.wide_params = p.pdtype == kFP32; a.param_pieces = all_aligned({p.weight, p.bias}, 16); a.eps = p.eps; a.act = p.act;
   return a;
 }
 
@@ -69,12 +72,14 @@ bool gn_shape_ok(const GnProblem& p) { return p.D / p.groups <= kMaxGroup; }
 // Partial sums of dw and db for every row block.  The plan of aligned tensors, or of
 // single channels where there are more row blocks of those.
 int64_t gn_bwd_ws_bytes(const GnProblem& p) {
+  static const char kAligned[16] __attribute__((aligned(256))) = {0};
   GnProblem q = p;
-  q.x = q.gate = q.dy = nullptr;
+  q.x = q.dy = kAligned;
+  q.gate = nullptr;
   q.y = q.dx = q.dgate = nullptr;
   int64_t gy = plan_of(q).gy;
   for (const int off : {8, 2}) {
-    q.x = (const char*)0 + off;
+    q.x = kAligned + off;
     const int64_t n = plan_of(q).gy;
     gy = n > gy ? n : gy;
   }

@@ -162,7 +162,7 @@ int dc_linear_attention_step(const void* q, const int64_t* q_strides, const void
 
 // Sizes of a group norm.
 static int check_gn(int64_t M, int64_t D, int64_t groups, int act, int dtype, int pdtype) {
-  if (!dtype_ok(dtype) || !dtype_ok(pdtype)) return DC_ERR_DTYPE;
+  if (!dtype_ok(dtype) || (pdtype != dtype && pdtype != DC_DTYPE_FP32)) return DC_ERR_DTYPE;
   if (M <= 0 || D <= 0 || groups <= 0 || M > kI32Max || D > kI32Max || D % groups != 0) return DC_ERR_SHAPE;
   if (act != DC_ACT_NONE && act != DC_ACT_SILU) return DC_ERR_UNSUPPORTED;
   dc::GnProblem p{};

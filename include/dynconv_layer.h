@@ -76,7 +76,8 @@ typedef enum dc_activation { DC_ACT_NONE = 0, DC_ACT_SILU = 1 } dc_activation;
  * `groups` groups of D / groups neighbouring channels,
  *     u = (x - mean) / sqrt(var + eps) * weight + bias,
  *     y = u * act(gate)  with a gate,   y = act(u)  without (gate NULL)
- * (biased variance).  weight, bias [D] or NULL (1, 0), both in param_dtype. */
+ * (biased variance).  weight, bias [D] or NULL (1, 0), both in param_dtype:
+ * dtype or float32. */
 int dc_group_norm_fwd(const void* x, const void* weight, const void* bias, const void* gate, void* y, int64_t M,
                       int64_t D, int64_t groups, float eps, int activation, int dtype, int param_dtype, void* stream);
 
