@@ -23,7 +23,10 @@ namespace {
 
 using la::Args;
 
+// Channels of q and k that a kernel holds, and wavefronts of 32 columns of v: two for up to 64 columns, but not at 256
+// channels, where four share the loads that two have no registers for.
 int cover(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : 256; }
+int waves(int V, int kp) { return V <= 64 && kp <= 128 ? 2 : 4; }
 
 struct Cut {
   int seg, nseg;
@@ -120,12 +123,12 @@ hipError_t launch(const LaProblem& p, const Cut& c, float* const* states_of, boo
     a.p = p;
     a.seg = c.seg;
     a.nseg = c.nseg;
-    const int kp = states ? la::kStateRows : cover(p.pass[i].K), nw = p.pass[i].V <= 64 ? 2 : 4;
+    const int kp = states ? la::kStateRows : cover(p.pass[i].K), nw = waves(p.pass[i].V, kp);
     const bool w = whole(p.pass[i], es, states);
     a.nvb = a.nkb = 1;
     for (int j = i; j < p.npass; ++j) {
       const LaPass& b = p.pass[j];
-      if (done[j] || (!states && cover(b.K) != kp) || (b.V <= 64 ? 2 : 4) != nw || whole(b, es, states) != w) continue;
+      if (done[j] || (!states && cover(b.K) != kp) || waves(b.V, kp) != nw || whole(b, es, states) != w) continue;
       done[j] = true;
       a.p.pass[a.npass] = b;
       a.states[a.npass++] = c.nseg > 1 ? states_of[j] : nullptr;

@@ -235,7 +235,10 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   constexpr int NT = NW * 64, NB = C / 32, KB = KP / 32, RK = row_elems<T, KP, true>(), RV = row_elems<T, NW * 32, false>();
   __shared__ __align__(16) T sk[C * RK];
   __shared__ __align__(16) T sv[C * RV];
-  __shared__ __align__(16) T sq[STATES ? 8 : C * RK];
+  // q, and once it has been read o
+  constexpr int RO = NW * 32 + 16 / (int)sizeof(T);
+  __shared__ __align__(16) T sq[STATES ? 8 : C * (RK > RO ? RK : RO)];
+  T* const so = sq;
   // scores as operands: blocks of 32 x 32 on and below the diagonal, two steps of a lane's 8, and what they are smaller by
   constexpr int NP = NB * (NB + 1) / 2;
   __shared__ __align__(16) Frag sp[STATES ? 1 : NP * 2 * 64];
@@ -307,19 +310,18 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   constexpr int AHEAD = STATES ? 2 : 1;
   Tile<T, C, KP, NT, WHOLE> tk[AHEAD], tq;
   Tile<T, C, NW * 32, NT, WHOLE> tv[AHEAD];
-  auto fetch = [&](auto& k1, auto& v1, int p) {
-    if (p >= hi) return;
-    k1.load(k, P.ks[2], P.K - k0, p, hi, turn);
-    v1.load(v, P.vs[2], vw, p, hi, turn);
-    if constexpr (!STATES) tq.load(q, P.qs[2], P.K, p, hi, turn);
-  };
+  auto fetch_k = [&](auto& t, int p) { if (p < hi) t.load(k, P.ks[2], P.K - k0, p, hi, turn); };
+  auto fetch_v = [&](auto& t, int p) { if (p < hi) t.load(v, P.vs[2], vw, p, hi, turn); };
+  auto fetch_q = [&](int p) { if (!STATES && p < hi) tq.load(q, P.qs[2], P.K, p, hi, turn); };
   auto chunk = [&](auto& k1, auto& v1, int p0) {
     __syncthreads();  // the chunk before has been read
     k1.template store<true>(sk);
     v1.template store<false>(sv);
     if constexpr (!STATES) tq.template store<true>(sq);
     __syncthreads();
-    fetch(k1, v1, p0 + AHEAD * C);
+    // the next loads go out a tile at a time between the phases: twelve at once hold a wavefront up for 1100 cycles
+    fetch_k(k1, p0 + AHEAD * C);
+    if (STATES) fetch_v(v1, p0 + AHEAD * C);
     if (STATES && !mine) return;
     const int cl = min(C, hi - p0), shift = C - cl;  // tokens of this chunk: its last rows
     const int early = P.rev && p0 == 0 ? 1 : 0;      // the entering state meets the first token without a decay
@@ -355,6 +357,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
       }
 
       phase();
+      fetch_v(v1, p0 + C);
       f32x16 acc[NB] = {};
       // a state near the end of fp16 takes part smaller: scaled and back in place, or (128 registers of it: the branch
       // spilled 165) as it is packed
@@ -377,7 +380,8 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
 #pragma unroll
         for (int ib = 0; ib < NB; ++ib) scale<16>(reinterpret_cast<float*>(&acc[ib]), 1.f / kSmaller);
       }
-      __syncthreads();  // the scores are there
+      __syncthreads();  // the scores are there, and q has been read
+      fetch_q(p0 + C);
       if (!mine) return;
 #pragma unroll
       for (int ib = 0; ib < NB; ++ib) {
@@ -401,20 +405,31 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
           scale<16>(af, P.so * power(lam2, max(ib * 32 + col + 1 - early - shift, 0)));
         }
         add(ib);
-        const int i = ib * 32 + col - shift;
-        if (i >= 0) {
-          T* to = o + (int64_t)(turn >= 0 ? turn - p0 - i : p0 + i) * P.os[2] + n0 + 4 * half;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int n = n0 + 8 * g + 4 * half;
-            if constexpr (WHOLE) {
-              if (n < P.V) store_vals<T, 4>(to + 8 * g, af + 4 * g);
-            } else {
+        for (int g = 0; g < 4; ++g) store_vals<T, 4>(so + (ib * 32 + col) * RO + wv * 32 + 8 * g + 4 * half, af + 4 * g);
+      }
+      // o leaves by way of LDS, in 16-byte pieces of a row (the pieces that the wavefront's 32 columns have)
+      constexpr int VE = 16 / (int)sizeof(T), PR = 32 / VE, RPI = 64 / PR;
+      const int r0 = lane / PR - shift, c = lane % PR * VE;
+      const T* from = so + lane / PR * RO + wv * 32 + c;
+      if constexpr (WHOLE) {
+        // rows in front of the chunk's tokens fall out of the range, as they do in Tile
+        const int64_t st = P.os[2];
+        const int sb = (int)st * (int)sizeof(T), step = turn >= 0 ? -RPI * sb : RPI * sb;
+        const T* first = o + (turn >= 0 ? turn - (p0 + cl - 1) : p0) * st + n0;
+        const rsrc_t rs = make_rsrc_wave(const_cast<T*>(first), ((cl - 1) * st + P.V - n0) * (int64_t)sizeof(T));
+        const int off = (turn >= 0 ? cl - 1 - r0 : r0) * sb + c * (int)sizeof(T);
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (n + j < P.V) to[8 * g + j] = (T)af[4 * g + j];
-            }
-          }
+        for (int it = 0; it < C / RPI; ++it)
+          bstore128<false>(*reinterpret_cast<const u32x4*>(from + it * RPI * RO), rs, n0 + c < P.V ? off + it * step : kOut);
+      } else {
+#pragma unroll
+        for (int it = 0; it < C / RPI; ++it) {
+          const int i = r0 + it * RPI;
+          T* to = o + (int64_t)(turn >= 0 ? turn - p0 - i : p0 + i) * P.os[2] + n0 + c;
+#pragma unroll
+          for (int j = 0; j < VE; ++j)
+            if (i >= 0 && n0 + c + j < P.V) to[j] = from[it * RPI * RO + j];
         }
       }
     }
@@ -455,7 +470,11 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
     }
   };
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) fetch(tk[i], tv[i], lo + i * C);
+  for (int i = 0; i < AHEAD; ++i) {
+    fetch_k(tk[i], lo + i * C);
+    fetch_v(tv[i], lo + i * C);
+  }
+  fetch_q(lo);
   for (int p0 = lo; p0 < hi; p0 += AHEAD * C) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
@@ -498,7 +517,7 @@ hipError_t launch(const Args& a, int kp, int nw, bool whole, bool states, hipStr
   if (states) nw == 2 ? launch_dims<T, kStateRows, 2, true>(a, whole, st) : launch_dims<T, kStateRows, 4, true>(a, whole, st);
   else if (kp == 64) nw == 2 ? launch_dims<T, 64, 2, false>(a, whole, st) : launch_dims<T, 64, 4, false>(a, whole, st);
   else if (kp == 128) nw == 2 ? launch_dims<T, 128, 2, false>(a, whole, st) : launch_dims<T, 128, 4, false>(a, whole, st);
-  else nw == 2 ? launch_dims<T, 256, 2, false>(a, whole, st) : launch_dims<T, 256, 4, false>(a, whole, st);
+  else launch_dims<T, 256, 4, false>(a, whole, st);
   return hipGetLastError();
 }
 extern template hipError_t launch<bf16>(const Args&, int, int, bool, bool, hipStream_t);

@@ -8,8 +8,13 @@ Beyond the reference's operators: lowrank_dynamic_convolution_grouped (the
 q / k / v convolutions of one layer in one launch per direction, README.md:57-110)
 and the README's LowRankDynamicShortConvolution module, plus its grouped form.
 
-Both are torch.autograd.Functions backed by hand-written gfx950 HIP kernels
-in libdynconv.so, reached through a C ABI (include/dynconv.h).
+Behind the convolutions of a layer: linear_attention with a decay for each head (whole
+sequences) and linear_attention_step (single tokens), group_norm with its gate, the
+convolutions' single-token form lowrank_dynamic_convolution_step(_grouped), and
+DynamicLinearAttention, a layer of all of them.
+
+The operators are torch.autograd.Functions backed by hand-written gfx950 HIP kernels
+in libdynconv.so, reached through a C ABI (include/dynconv.h, include/dynconv_layer.h).
 """
 
 from .headwise import headwise_dynamic_convolution, _HeadwiseDynamicConvolutionFn  # noqa: F401
@@ -19,6 +24,7 @@ from .lowrank import lowrank_dynamic_convolution_step, lowrank_dynamic_convoluti
 from .linattn import linear_attention, linear_attention_step  # noqa: F401
 from .norm import group_norm  # noqa: F401
 from .modules import LowRankDynamicShortConvolution, GroupedLowRankDynamicShortConvolution  # noqa: F401
+from .modules import DynamicLinearAttention, LayerState  # noqa: F401
 from ._capi import LIB_PATH, load as load_library  # noqa: F401
 
 __all__ = [
@@ -32,6 +38,8 @@ __all__ = [
     "group_norm",
     "LowRankDynamicShortConvolution",
     "GroupedLowRankDynamicShortConvolution",
+    "DynamicLinearAttention",
+    "LayerState",
     "load_library",
     "LIB_PATH",
 ]

@@ -9,6 +9,10 @@ convolutions of README.md:86-110) and runs them as one grouped operator: one
 proj_in GEMM for all groups, and one launch per direction that reads the fused
 [B, T, G*D] projection in place instead of three .contiguous() slices.
 
+DynamicLinearAttention is a layer around it: the q, k and v convolutions, linear
+attention with a decay for each head, the heads' gated group norm, and the
+projections, for training, for prompts in pieces and for single tokens.
+
 The proj_in GEMM (README.md:67, 75) runs on libdynconv.so's own matrix-core
 kernels (dc_proj_in_fwd / dc_proj_in_bwd): skinny products bound by streaming
 pre_z, which the library GEMM runs at about a quarter of HBM bandwidth in the
@@ -19,13 +23,17 @@ and calls under autocast run the layer itself, as the reference module does.
 """
 
 import math
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
 from torch import nn
 
 from . import _capi
-from .lowrank import lowrank_dynamic_convolution, lowrank_dynamic_convolution_grouped
+from .linattn import linear_attention, linear_attention_step
+from .lowrank import (lowrank_dynamic_convolution, lowrank_dynamic_convolution_grouped,
+                      lowrank_dynamic_convolution_step_grouped)
+from .norm import group_norm
 
 
 class _ProjInFn(torch.autograd.Function):
@@ -174,3 +182,100 @@ class GroupedLowRankDynamicShortConvolution(nn.Module):
         Us = [self.proj_out[g] for g in range(G)]
         sws = [self.proj_out_bias[g] for g in range(G)]
         return lowrank_dynamic_convolution_grouped(x, zs, Us, static_w=sws, residual=True, head_dim=self.head_dim)
+
+
+class LayerState(NamedTuple):
+    """What DynamicLinearAttention keeps of each sequence (a row each)."""
+
+    conv: torch.Tensor  # [rows, W - 1, 3 * d_model]: the last projected rows, oldest first
+    attn: torch.Tensor  # [rows, heads, head_dim, head_dim] float32: the heads' states
+
+
+class DynamicLinearAttention(nn.Module):
+    """A layer of linear attention over convolved q, k and v:
+
+        q, k, v = GroupedLowRankDynamicShortConvolution(c_attn(x), x), in heads
+        o       = linear_attention(q, k, v) with a fixed decay for each head
+        out     = c_proj(group_norm(o, heads, gate=c_gate(x)))
+
+    forward(x) takes whole sequences [B, T, d_model]; step(x, state) one token [N, d_model] of each sequence.
+    Decays run from 1 - 2^-5 to 1 - 2^-12 over the heads; they are not trained and stay float32.
+    """
+
+    def __init__(self, d_model: int, heads: int, R: int, W: int, eps: float = 1e-5):
+        super().__init__()
+        if heads <= 0 or d_model % heads != 0:
+            raise ValueError("heads must divide d_model")
+        self.d_model, self.heads, self.head_dim, self.W, self.eps = d_model, heads, d_model // heads, W, eps
+        self.c_attn = nn.Linear(d_model, 3 * d_model, bias=False)
+        self.conv = GroupedLowRankDynamicShortConvolution(d_model, R, W, groups=3, head_dim=self.head_dim)
+        self.norm_weight = nn.Parameter(torch.ones(d_model))
+        self.norm_bias = nn.Parameter(torch.zeros(d_model))
+        self.c_gate = nn.Linear(d_model, d_model, bias=False)
+        self.c_proj = nn.Linear(d_model, d_model, bias=False)
+        self.register_buffer("log_decay", self._log_decay(), persistent=False)
+
+    def _log_decay(self):
+        u = 5 + 7 * torch.arange(self.heads, dtype=torch.float64) / max(self.heads - 1, 1)
+        return torch.log1p(-torch.exp2(-u)).to(torch.float32)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        # .to(bfloat16) and its like leave the decays as they are
+        if self.log_decay.dtype != torch.float32:
+            self.log_decay = self._log_decay().to(self.log_decay.device)
+        return self
+
+    def new_state(self, rows: int) -> LayerState:
+        """States of sequences without a token yet."""
+        w = self.c_attn.weight
+        return LayerState(torch.zeros(rows, self.W - 1, 3 * self.d_model, dtype=w.dtype, device=w.device),
+                          torch.zeros(rows, self.heads, self.head_dim, self.head_dim, device=w.device))
+
+    def _norm(self, o, gate):
+        return group_norm(o, self.heads, weight=self.norm_weight, bias=self.norm_bias, gate=gate, eps=self.eps)
+
+    def forward(self, x: torch.Tensor, state: LayerState | None = None, lengths: torch.Tensor | None = None,
+                return_state: bool = False):
+        """x [B, T, d_model] -> out like x, or (out, the state after it).
+
+        state:    of the same B sequences, where x goes on from (None: their start).
+        lengths:  [B] int32 on the device: rows at and past lengths[b] are padding, which does not reach the others or
+                  the state; out is of no use there.
+        """
+        B, T, D = x.shape
+        qkv = self.c_attn(x)
+        if state is None:
+            q, k, v = self.conv(qkv, x)
+        else:
+            # the convolutions look back W - 1 rows; what they give for those rows themselves is dropped
+            past = self.W - 1
+            qkv = torch.cat([state.conv, qkv], 1)
+            q, k, v = (t[:, :, past:] for t in self.conv(qkv, F.pad(x, (0, 0, past, 0))))
+        o = linear_attention(q, k, v, self.log_decay, initial_state=None if state is None else state.attn, lengths=lengths,
+                             return_state=return_state)
+        o, attn = o if return_state else (o, None)
+        out = self.c_proj(self._norm(o.transpose(1, 2).reshape(B, T, D), self.c_gate(x)))
+        if not return_state:
+            return out
+        if state is None:
+            qkv = F.pad(qkv, (0, 0, self.W - 1, 0))
+        first = torch.full((B,), T, device=x.device) if lengths is None else lengths.long().clamp(0, T)
+        rows = first[:, None] + torch.arange(self.W - 1, device=x.device)
+        return out, LayerState(qkv[torch.arange(B, device=x.device)[:, None], rows], attn)
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, state: LayerState, slots: torch.Tensor | None = None) -> torch.Tensor:
+        """One token x [N, d_model] of each of N sequences -> out [N, d_model]; `state` is updated in place.
+
+        slots: [N] int32 on the device, the row of `state` of each sequence (None: row n); -1 marks a sequence that
+        takes no part, whose out is of no use."""
+        N, D = x.shape
+        z = _module_proj_in(self.conv.proj_in, x[:, None], 3, self.conv.R)
+        U, sw = self.conv.proj_out, self.conv.proj_out_bias
+        q, k, v = lowrank_dynamic_convolution_step_grouped(
+            self.c_attn(x), [t.view(N, -1) for t in z], list(U.unbind(0)), state.conv, static_w=list(sw.unbind(0)),
+            residual=True, slots=slots)
+        heads = (N, self.heads, self.head_dim)
+        o = linear_attention_step(q.view(heads), k.view(heads), v.view(heads), self.log_decay, state.attn, slots=slots)
+        return self.c_proj(self._norm(o.view(N, D), self.c_gate(x)))

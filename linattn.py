@@ -1,8 +1,8 @@
 """Import path of the operators behind the convolutions, beside headwise.py and lowrank.py.
 
-    from linattn import linear_attention, linear_attention_step, group_norm
+    from linattn import linear_attention, linear_attention_step, group_norm, DynamicLinearAttention
 
-resolves to dynamic-conv1d_amd/dynconv/linattn.py and norm.py.
+resolves to dynamic-conv1d_amd/dynconv/linattn.py, norm.py and modules.py.
 """
 
 import os as _os
@@ -14,3 +14,4 @@ if _PKG_DIR not in _sys.path:
 
 from dynconv.linattn import linear_attention, linear_attention_step  # noqa: E402,F401
 from dynconv.norm import group_norm  # noqa: E402,F401
+from dynconv.modules import DynamicLinearAttention, LayerState  # noqa: E402,F401
