@@ -32,32 +32,33 @@ struct Cut {
   int seg, nseg;
 };
 
-// Time of one chunk of a workgroup that has a CU to itself, in us (measured; only ratios matter).  Two workgroups on a CU
-// take nearly twice as long.
-double chunk_us(int K, int V, int dtype) {
+// Time of one chunk of a workgroup that has a CU to itself, in us, measured with one segment (float32's chunks have 32
+// tokens, the others' 64).  Two workgroups on a CU take nearly twice as long.
+double chunk_us(int K, int dtype) {
   const int kp = cover(K);
-  const double t = kp == 64 ? 2.5 : kp == 128 ? 3.5 : 7;
-  return dtype == kFP32 ? 5 * t : t;
+  const double t = kp == 64 ? 2.4 : kp == 128 ? 3.5 : 6.5;
+  return dtype == kFP32 ? 1.8 * t : t;
 }
 
 // Segments of a problem, the forward's and the backward's alike: the count with the least estimated time of the forward.
-// The chunks run in rounds of one workgroup to a CU; segments cost half a chunk's time to form each of their states, all
-// but the last one's, and the carrying of states of float32 at 4.5 TB/s.  B2 H32 T8192 hd128, forward and backward, us:
-// 4 segments 200 + 478, 8 208 + 510, 5 250 + 503, 1 455 + 550.  B8 H32 T4096 hd64: 1 segment 159 + 322, 2 195 + 446.
+// The chunks run in rounds of one workgroup to a CU; segments cost 0.6 of a chunk's time to form each of their states, all
+// but the last one's, the carrying of float32 states at 4.5 TB/s, two launches, and the start of their workgroups.
+// Measured, forward + backward, us (* is what the estimate takes): B2 H32 T8192 hd128 bf16, 4 segments 202 + 391 *,
+// 8 215 + 402, 3 243 + 456, 1 455 + 550; B1 H8 T700 hd128, 1 segment 40 + 42, 6 24 + 32, 11 24 + 33 *; B8 H32 T4096 hd64,
+// 1 segment 172 + 274 *, 2 195 + 446; B3 H10 T1537 hd100 float32, 7 segments 80 + 179 *, 17 85 + 185, 1 312 + 322.
 Cut cut_of(const LaProblem& p) {
   // dq's pass of a backward has K and V the other way round: the same cut
   const int K = p.npass == 3 ? p.pass[0].V : p.pass[0].K, V = p.npass == 3 ? p.pass[0].K : p.pass[0].V;
-  const int es = dtype_size(p.dtype);
-  const int C = max(la::chunk_tokens(es, cover(K)), la::chunk_tokens(es, cover(V)));
+  const int C = la::chunk_tokens(dtype_size(p.dtype));
   const int64_t chunks = (p.T + C - 1) / C;
-  const double heads = (double)p.B * p.H * ((V + 127) / 128), us = chunk_us(K, V, p.dtype);
+  const double heads = (double)p.B * p.H, wgs = heads * ((V + 127) / 128), us = chunk_us(K, p.dtype);
   double best = 0;
   int64_t seg = chunks < 1 ? 1 : chunks;
-  for (int64_t n = 1; n <= 128 && n <= (chunks + 1) / 2; ++n) {
+  for (int64_t n = 1; n <= 128 && n <= chunks; ++n) {
     const int64_t len = (chunks + n - 1) / n;
     if ((chunks + len - 1) / len != n) continue;  // the same segments as fewer
-    double t = us * len * __builtin_ceil(heads * n / 256);
-    if (n > 1) t += 5 + 0.5 * us * len * __builtin_ceil(heads * (n - 1) / 256) + heads * n * K * V * 8 / 4.5e6;
+    double t = (us * len + 3) * __builtin_ceil(wgs * n / 256);
+    if (n > 1) t += 5 + (0.6 * us * len + 2) * __builtin_ceil(wgs * (n - 1) / 256) + heads * n * K * V * 8 / 4.5e6;
     if (n == 1 || t < best) {
       best = t;
       seg = len;

@@ -37,8 +37,8 @@
 // S take v g^{C-1-j} in two parts of the type (16 or 22 bits), bf16 in three where
 // the state is returned, which so is a float32 result; fp16 operands that would come near that type's end
 // are made 2^-16 smaller (a wavefront's scores or S together, where one of them
-// passes 2^15).  float32 inputs take float32 matrix products throughout.  All
-// sums and S are float32.
+// passes 2^15).  float32 inputs are products of three bf16 parts throughout (Parts).
+// All sums and S are float32.
 #pragma once
 
 #include "lowrank_mfma.h"
@@ -60,8 +60,8 @@ struct Args {
   float* states[kLaMaxPasses];
 };
 
-// Tokens of a chunk: 64, or 32 where three tiles of 64 float32 rows would pass the LDS.
-__host__ __device__ constexpr int chunk_tokens(int es, int kp) { return es == 4 && kp > 128 ? 32 : 64; }
+// Tokens of a chunk: 64, or 32 in float32, whose tiles are three planes (64 would pass the LDS).
+__host__ __device__ constexpr int chunk_tokens(int es) { return es == 4 ? 32 : 64; }
 
 // Rows of a state that a workgroup forms in the states' launch: 64, so that three workgroups fit a CU whatever K is.
 constexpr int kStateRows = 64;
@@ -72,6 +72,8 @@ __host__ __device__ constexpr int quad(int c) { return (c & ~12) | ((c & 4) << 1
 
 template <typename T> struct Ops {  // 16-bit types
   typedef u32x4 Frag;
+  typedef T Lds;  // elements of the tiles in LDS, in one plane
+  static constexpr int kPlanes = 1;
   static constexpr bool kSplit = true, kNarrow = __is_same(T, fp16);  // two parts; float32 values may not fit
   __device__ static __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
     if constexpr (__is_same(T, bf16))
@@ -80,11 +82,11 @@ template <typename T> struct Ops {  // 16-bit types
       return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
   }
   // this lane's half of 16 channels of a row: p points at the first of them
-  __device__ static __forceinline__ Frag rows(const T* p, int half) { return *reinterpret_cast<const Frag*>(p + 8 * half); }
+  __device__ static __forceinline__ Frag rows(const T* p, int half, int = 0) { return *reinterpret_cast<const Frag*>(p + 8 * half); }
   // column lane%32 of 16 rows: p points at (row 0, column 0) of the 16 x 32 block, rows rs elements apart; TURNED: the
   // rows' channels lie in quad() order
   template <bool TURNED>
-  __device__ static __forceinline__ Frag cols(const T* p, int rs, int lane) {
+  __device__ static __forceinline__ Frag cols(const T* p, int rs, int lane, int = 0) {
     const int c = 4 * (lane % 4);
     const T* q = p + (4 * (lane / 32) + (lane % 16) / 4) * rs + 16 * ((lane / 16) % 2) + (TURNED ? quad(c) : c);
     const u32x2 a = lds_read_tr16(q), b = lds_read_tr16(q + 8 * rs);
@@ -97,26 +99,91 @@ template <typename T> struct Ops {  // 16-bit types
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = Mma16<T>::to_f(elem16(f, e));
   }
+  // a lane's operand in LDS, 64 lanes to a plane
+  __device__ static __forceinline__ void put(u32x4* p, int lane, Frag f) { p[lane] = f; }
+  __device__ static __forceinline__ Frag get(const u32x4* p, int lane) { return p[lane]; }
 };
+
+// float32 as a sum of three bf16 (8 bits each: all 24 of them, over bf16's range, which is float32's).  A product is the
+// six products of parts down to 2^-16 of it, so it is as good as float32's own, at 6 matrix instructions of 32 cycles for 8
+// of 64 (v_mfma_f32_32x32x2): float32 training of B3 T1537 H10 hd100 went from 315 to 260 us.
+struct Parts {
+  struct Frag { u32x4 p[3]; };
+  typedef bf16 Lds;
+  static constexpr int kPlanes = 3;
+  static constexpr bool kSplit = false, kNarrow = false;
+  __device__ static __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
+    typedef Ops<bf16> O;
+    c = O::mma(a.p[2], b.p[0], c);  // the smallest first
+    c = O::mma(a.p[0], b.p[2], c);
+    c = O::mma(a.p[1], b.p[1], c);
+    c = O::mma(a.p[1], b.p[0], c);
+    c = O::mma(a.p[0], b.p[1], c);
+    return O::mma(a.p[0], b.p[0], c);
+  }
+  // two floats into their parts, a word of two for each
+  __device__ static __forceinline__ void split(float a, float b, uint32_t (&w)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      w[i] = pack2<bf16>(a, b);
+      a -= __uint_as_float(w[i] << 16);
+      b -= __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+  __device__ static __forceinline__ Frag rows(const bf16* p, int half, int plane) {
+    return Frag{{Ops<bf16>::rows(p, half), Ops<bf16>::rows(p + plane, half), Ops<bf16>::rows(p + 2 * plane, half)}};
+  }
+  template <bool TURNED>
+  __device__ static __forceinline__ Frag cols(const bf16* p, int rs, int lane, int plane) {
+    return Frag{{Ops<bf16>::cols<TURNED>(p, rs, lane), Ops<bf16>::cols<TURNED>(p + plane, rs, lane),
+                 Ops<bf16>::cols<TURNED>(p + 2 * plane, rs, lane)}};
+  }
+  __device__ static __forceinline__ Frag pack(const float* v) {
+    Frag f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t w[3];
+      split(v[2 * e], v[2 * e + 1], w);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) f.p[i][e] = w[i];
+    }
+    return f;
+  }
+  __device__ static __forceinline__ void unpack(const Frag& f, float* v) {
+    float u[8];
+    Ops<bf16>::unpack(f.p[2], v);
+#pragma unroll
+    for (int i = 1; i >= 0; --i) {
+      Ops<bf16>::unpack(f.p[i], u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += u[e];
+    }
+  }
+  __device__ static __forceinline__ void put(u32x4* p, int lane, const Frag& f) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) p[i * 64 + lane] = f.p[i];
+  }
+  __device__ static __forceinline__ Frag get(const u32x4* p, int lane) {
+    return Frag{{p[lane], p[64 + lane], p[128 + lane]}};
+  }
+};
+template <typename T> struct OpsOf { typedef Ops<T> type; };
+template <> struct OpsOf<float> { typedef Parts type; };
+
+// float32 on float32 matrix instructions (the lowrank step, whose products are few).
 template <> struct Ops<float> {
   struct Frag { float v[8]; };
-  static constexpr bool kSplit = false, kNarrow = false;
   __device__ static __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
     return c;
   }
-  __device__ static __forceinline__ Frag rows(const float* p, int half) {
-    Frag f;
-    load_vals<float, 8>(p + 8 * half, f.v);
-    return f;
-  }
   template <bool TURNED>
   __device__ static __forceinline__ Frag cols(const float* p, int rs, int lane) {
+    static_assert(!TURNED, "plain order");
     Frag f;
-    const int c = TURNED ? quad(lane % 32) : lane % 32;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.v[e] = p[(8 * (e / 4) + 4 * (lane / 32) + e % 4) * rs + c];
+    for (int e = 0; e < 8; ++e) f.v[e] = p[(8 * (e / 4) + 4 * (lane / 32) + e % 4) * rs + lane % 32];
     return f;
   }
   __device__ static __forceinline__ Frag pack(const float* v) {
@@ -124,10 +191,6 @@ template <> struct Ops<float> {
 #pragma unroll
     for (int e = 0; e < 8; ++e) f.v[e] = v[e];
     return f;
-  }
-  __device__ static __forceinline__ void unpack(Frag f, float* v) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = f.v[e];
   }
 };
 
@@ -189,14 +252,21 @@ struct Tile {
       }
     }
   }
-  // TURNED: channels in quad() order
-  template <bool TURNED>
-  __device__ __forceinline__ void store(T* lds) const {
+  // TURNED: channels in quad() order; planes `plane` elements apart
+  template <typename O, bool TURNED>
+  __device__ __forceinline__ void store(typename O::Lds* lds, int plane) const {
+    typedef typename O::Lds L;
     const int c = ((int)threadIdx.x % PR) * VE;
-    T* to = lds + (int)threadIdx.x / PR * row_elems<T, N, TURNED>() + (TURNED ? quad(c) : c);
+    L* to = lds + (int)threadIdx.x / PR * row_elems<L, N, TURNED>() + (TURNED ? quad(c) : c);
 #pragma unroll
-    for (int i = 0; i < NV; ++i, to += RPI * row_elems<T, N, TURNED>()) {
-      if constexpr (TURNED && VE == 8) {  // two quads, which part
+    for (int i = 0; i < NV; ++i, to += RPI * row_elems<L, N, TURNED>()) {
+      if constexpr (O::kPlanes == 3) {
+        uint32_t a[3], b[3];
+        O::split(__uint_as_float(v[i][0]), __uint_as_float(v[i][1]), a);
+        O::split(__uint_as_float(v[i][2]), __uint_as_float(v[i][3]), b);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) *reinterpret_cast<u32x2*>(to + j * plane) = u32x2{a[j], b[j]};
+      } else if constexpr (TURNED) {  // two quads, which part
         *reinterpret_cast<u32x2*>(to) = u32x2{v[i][0], v[i][1]};
         *reinterpret_cast<u32x2*>(to + 8) = u32x2{v[i][2], v[i][3]};
       } else {
@@ -230,18 +300,21 @@ constexpr int waves_per_simd(int es, int kp, int nw, bool states) {
 // caller's result (three parts in bf16; in every kernel they cost the common one 10% by spilled registers).
 template <typename T, int KP, int NW, int C, bool WHOLE, bool STATES, bool RETURNED>
 __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES)) void la_chunks(Args A) {
-  typedef Ops<T> O;
+  typedef typename OpsOf<T>::type O;
   typedef typename O::Frag Frag;
-  constexpr int NT = NW * 64, NB = C / 32, KB = KP / 32, RK = row_elems<T, KP, true>(), RV = row_elems<T, NW * 32, false>();
-  __shared__ __align__(16) T sk[C * RK];
-  __shared__ __align__(16) T sv[C * RV];
+  typedef typename O::Lds L;
+  constexpr int NT = NW * 64, NB = C / 32, KB = KP / 32, RK = row_elems<L, KP, true>(), RV = row_elems<L, NW * 32, false>();
+  constexpr int PL = O::kPlanes, PK = C * RK, PV = C * RV;  // planes of a tile, elements from one to the next
+  __shared__ __align__(16) L sk[PL * PK];
+  __shared__ __align__(16) L sv[PL * PV];
   // q, and once it has been read o
-  constexpr int RO = NW * 32 + 16 / (int)sizeof(T);
-  __shared__ __align__(16) T sq[STATES ? 8 : C * (RK > RO ? RK : RO)];
-  T* const so = sq;
+  constexpr int RO = NW * 32 + 16 / (int)sizeof(T), QB = PL * PK * (int)sizeof(L), OB = C * RO * (int)sizeof(T);
+  __shared__ __align__(16) unsigned char sqo[STATES ? 16 : QB > OB ? QB : OB];
+  L* const sq = reinterpret_cast<L*>(sqo);
+  T* const so = reinterpret_cast<T*>(sqo);
   // scores as operands: blocks of 32 x 32 on and below the diagonal, two steps of a lane's 8, and what they are smaller by
   constexpr int NP = NB * (NB + 1) / 2;
-  __shared__ __align__(16) Frag sp[STATES ? 1 : NP * 2 * 64];
+  __shared__ u32x4 sp[STATES ? 1 : NP * 2 * PL * 64];
   __shared__ float sdown[NP];
 
   // the passes of one segment run side by side: what one reads, the others find in the last-level cache
@@ -315,9 +388,9 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   auto fetch_q = [&](int p) { if (!STATES && p < hi) tq.load(q, P.qs[2], P.K, p, hi, turn); };
   auto chunk = [&](auto& k1, auto& v1, int p0) {
     __syncthreads();  // the chunk before has been read
-    k1.template store<true>(sk);
-    v1.template store<false>(sv);
-    if constexpr (!STATES) tq.template store<true>(sq);
+    k1.template store<O, true>(sk, PK);
+    v1.template store<O, false>(sv, PV);
+    if constexpr (!STATES) tq.template store<O, true>(sq, PK);
     __syncthreads();
     // the next loads go out a tile at a time between the phases: twelve at once hold a wavefront up for 1100 cycles
     fetch_k(k1, p0 + AHEAD * C);
@@ -338,7 +411,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
         f32x16 sc = {};
 #pragma unroll
         for (int s = 0; s < KP / 16; ++s)
-          sc = O::mma(O::rows(sk + (jb * 32 + col) * RK + s * 16, half), O::rows(sq + (ib * 32 + col) * RK + s * 16, half), sc);
+          sc = O::mma(O::rows(sk + (jb * 32 + col) * RK + s * 16, half, PK), O::rows(sq + (ib * 32 + col) * RK + s * 16, half, PK), sc);
         float t[16];
         if (blk == 1) {  // by way of the block's last token: g^{i-j} = g^{col+1} g^{31-j}, the first factor with o
 #pragma unroll
@@ -353,7 +426,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
           if (lane == 0) sdown[blk] = small ? kSmaller : 1.f;
         }
 #pragma unroll
-        for (int s = 0; s < 2; ++s) sp[(blk * 2 + s) * 64 + lane] = O::pack(t + 8 * s);
+        for (int s = 0; s < 2; ++s) O::put(sp + (blk * 2 + s) * PL * 64, lane, O::pack(t + 8 * s));
       }
 
       phase();
@@ -373,7 +446,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
         for (int e = 0; e < 8; ++e) t[e] = PACKED ? Sf[s * 8 + e] * by : Sf[s * 8 + e];
         const Frag sf = O::pack(t);
 #pragma unroll
-        for (int ib = 0; ib < NB; ++ib) acc[ib] = O::mma(sf, O::rows(sq + (ib * 32 + col) * RK + s * 16, half), acc[ib]);
+        for (int ib = 0; ib < NB; ++ib) acc[ib] = O::mma(sf, O::rows(sq + (ib * 32 + col) * RK + s * 16, half, PK), acc[ib]);
       }
       if (O::kNarrow && small) {
         if constexpr (ONCE) scale<KB * 16>(Sf, 1.f / kSmaller);
@@ -393,8 +466,8 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
           if (down) scale<16>(af, kSmaller);
 #pragma unroll
           for (int s = 0; s < 2; ++s)
-            acc[ib] = O::mma(O::template cols<false>(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane),
-                             sp[(blk * 2 + s) * 64 + lane], acc[ib]);
+            acc[ib] = O::mma(O::template cols<false>(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane, PV),
+                             O::get(sp + (blk * 2 + s) * PL * 64, lane), acc[ib]);
           if (down) scale<16>(af, 1.f / kSmaller);
         };
         if (ib > 0 && shift < 32) {  // the state and the block before by way of its last token: g^{i+1} = g^{32} g^{col+1}
@@ -442,7 +515,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
       float t[8], g = 1.f;  // g^{C-16-16s}
 #pragma unroll
       for (int i = s + 1; i < C / 16; ++i) g *= g1;
-      O::unpack(O::template cols<false>(sv + s * 16 * RV + wv * 32, RV, lane), t);
+      O::unpack(O::template cols<false>(sv + s * 16 * RV + wv * 32, RV, lane, PV), t);
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[e] *= vlast[e] * g;
       const Frag v1 = O::pack(t);
@@ -462,7 +535,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
       }
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const Frag kf = O::template cols<true>(sk + s * 16 * RK + kb * 32, RK, lane);
+        const Frag kf = O::template cols<true>(sk + s * 16 * RK + kb * 32, RK, lane, PK);
         S[kb] = O::mma(kf, v1, S[kb]);
         if constexpr (O::kSplit) S[kb] = O::mma(kf, v2, S[kb]);
         if (three) S[kb] = O::mma(kf, v3, S[kb]);
@@ -506,7 +579,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
 // The kernel of a type for these sizes (instantiated in linattn_<type>.hip).
 template <typename T, int KP, int NW, bool STATES>
 void launch_dims(const Args& a, bool whole, hipStream_t st) {
-  constexpr int C = chunk_tokens(sizeof(T), KP);
+  constexpr int C = chunk_tokens(sizeof(T));
   constexpr bool B16 = __is_same(T, bf16);
   auto run = [&](auto kernel) { kernel<<<(unsigned)a.nblk, NW * 64, 0, st>>>(a); };
   if (B16 && a.returned) run(whole ? la_chunks<T, KP, NW, C, true, STATES, B16> : la_chunks<T, KP, NW, C, false, STATES, B16>);
