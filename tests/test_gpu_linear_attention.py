@@ -314,6 +314,45 @@ def test_graph():
             assert torch.equal(x, y), f"replay {seed}"
 
 
+def test_fp16_scores_and_states_past_the_type():
+    """Scores and states above 65504 whose outputs are within fp16: operands are held smaller, and none is lost."""
+    g = gen(15)
+    B, H, T, K, V = 1, 2, 200, 64, 64
+    lam = torch.tensor([0.0, -0.01])
+    k, v = (300 * randn(g, B, H, T, K)).to(HF), (300 * randn(g, B, H, T, V)).to(HF)
+    q = (1e-3 * randn(g, B, H, T, K)).to(HF)
+    o, S = linear_attention(q.to(DEV), k.to(DEV), v.to(DEV), lam.to(DEV), scale=0.01, return_state=True)
+    ro, rS = linear_attention_ref(q, k, v, lam, 0.01)
+    assert rS.abs().max() > 2 * 65504
+    tol, stol, f = _norms(q, k, v, lam, None, 0.01, 1.0, [T], False, HF)
+    _close(o, ro, tol, HF, f, "o")
+    _close(S, rS, stol, F32, f, "state")
+    # scores: q . k far above the type, values small
+    q2, v2 = (300 * randn(g, B, H, T, K)).to(HF), (1e-3 * randn(g, B, H, T, V)).to(HF)
+    o = linear_attention(q2.to(DEV), k.to(DEV), v2.to(DEV), lam.to(DEV), scale=1.0)
+    ro, _ = linear_attention_ref(q2, k, v2, lam, 1.0)
+    assert ((q2.double() @ k.double().transpose(2, 3)).abs().max() > 2 * 65504) and ro.abs().max() < 65504
+    tol, _, f = _norms(q2, k, v2, lam, None, 1.0, 1.0, [T], False, HF)
+    _close(o, ro, tol, HF, f, "o of large scores")
+
+
+def test_rows_past_32_bits():
+    """Tensors of more than 2^31 elements: their last rows, under a decay that forgets all before them."""
+    K, tail = 128, 300
+    T = (1 << 31) // K + 1000
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 20 GiB of GPU memory")
+    x = torch.randn(T, K, device=DEV, dtype=BF).view(1, 1, T, K)
+    lam = torch.tensor([-1.0], device=DEV)
+    with torch.no_grad():
+        o, S = linear_attention(x, x, x, lam, return_state=True)
+        end = x[:, :, -tail:].contiguous()
+        o2, S2 = linear_attention(end, end, end, lam, return_state=True)
+    # e^-200 of what came before; the chunks lie elsewhere, so scores are rounded in other places
+    assert (o[:, :, -100:].float() - o2[:, :, -100:].float()).abs().max() <= 2.0**-6 * o2.abs().max().float()
+    assert (S - S2).abs().max() <= 1e-4 * S2.abs().max()
+
+
 # ------------------------------------------------------------------- single tokens
 @pytest.mark.parametrize("dtype", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("B,H,K,V", [(3, 4, 128, 128), (1, 1, 1, 1), (2, 3, 100, 100), (5, 2, 33, 7), (2, 1, 256, 256),

@@ -33,7 +33,8 @@ def _dev(t):
 @pytest.mark.parametrize("G,N,D,R,W,static,residual", [
     (1, 1, 256, 16, 4, False, True), (3, 8, 256, 15, 4, True, True), (2, 9, 130, 7, 3, True, False),
     (4, 3, 65, 1, 1, True, True), (1, 21, 33, 8, 2, False, False), (3, 17, 512, 31, 4, True, True),
-    (1, 5, 200, 64, 16, False, True), (2, 40, 128, 127, 9, True, True), (1, 300, 64, 4, 5, False, True)])
+    (1, 5, 200, 64, 16, False, True), (2, 40, 128, 127, 9, True, True), (1, 300, 64, 4, 5, False, True),
+    (1, 33, 136, 256, 2, False, True), (2, 70, 128, 63, 3, True, True)])
 def test_step(G, N, D, R, W, static, residual, dtype):
     print(f"[step] G{G} N{N} D{D} R{R} W{W} static={static} {dtype}", flush=True)
     g = gen(G + N + D + W)
@@ -76,6 +77,20 @@ def test_steps_follow_the_whole_sequence():
         y = lowrank_dynamic_convolution_step(x[:, t].contiguous(), z[:, t].contiguous(), U, state, static_w=sw, residual=True)
         torch.testing.assert_close(y, whole[:, t], rtol=1e-5, atol=1e-5)
     assert torch.equal(state, x[:, T - W + 1:])
+
+
+def test_step_in_a_cache_past_32_bits():
+    rows, D, W = 70000, 4096, 4
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 6 GiB of GPU memory")
+    x, z, U, sw, first = (_dev(t) for t in _inputs(gen(36), 3, 3, D, 7, W, True, 3, BF))
+    state = torch.empty(rows, W - 1, 3 * D, dtype=BF, device=DEV)
+    ids = torch.tensor([rows - 1, 60000, 2], dtype=torch.int32, device=DEV)
+    state[ids.long()] = first
+    small = first.clone()
+    a = lowrank_dynamic_convolution_step_grouped(x, z, U, state, static_w=sw, slots=ids)
+    b = lowrank_dynamic_convolution_step_grouped(x, z, U, small, static_w=sw)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and torch.equal(state[ids.long()], small)
 
 
 def test_wide_rows_and_unaligned_tensors():
