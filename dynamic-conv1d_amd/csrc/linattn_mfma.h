@@ -379,23 +379,25 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
 
   constexpr bool three = __is_same(T, bf16) && RETURNED;
 
-  // Tiles on their way: the next chunk's, and for STATES, which has the registers, the one after it too.
-  constexpr int AHEAD = STATES ? 2 : 1;
-  Tile<T, C, KP, NT, WHOLE> tk[AHEAD], tq;
-  Tile<T, C, NW * 32, NT, WHOLE> tv[AHEAD];
-  auto fetch_k = [&](auto& t, int p) { if (p < hi) t.load(k, P.ks[2], P.K - k0, p, hi, turn); };
-  auto fetch_v = [&](auto& t, int p) { if (p < hi) t.load(v, P.vs[2], vw, p, hi, turn); };
+  // tiles on their way: the next chunk's (STATES with the one after it too: 62 -> 67 us at B2 H32 T8192 hd128)
+  Tile<T, C, KP, NT, WHOLE> tk, tq;
+  Tile<T, C, NW * 32, NT, WHOLE> tv;
+  auto fetch_k = [&](int p) { if (p < hi) tk.load(k, P.ks[2], P.K - k0, p, hi, turn); };
+  auto fetch_v = [&](int p) { if (p < hi) tv.load(v, P.vs[2], vw, p, hi, turn); };
   auto fetch_q = [&](int p) { if (!STATES && p < hi) tq.load(q, P.qs[2], P.K, p, hi, turn); };
-  auto chunk = [&](auto& k1, auto& v1, int p0) {
+  fetch_k(lo);
+  fetch_v(lo);
+  fetch_q(lo);
+  for (int p0 = lo; p0 < hi; p0 += C) {
     __syncthreads();  // the chunk before has been read
-    k1.template store<O, true>(sk, PK);
-    v1.template store<O, false>(sv, PV);
+    tk.template store<O, true>(sk, PK);
+    tv.template store<O, false>(sv, PV);
     if constexpr (!STATES) tq.template store<O, true>(sq, PK);
     __syncthreads();
     // the next loads go out a tile at a time between the phases: twelve at once hold a wavefront up for 1100 cycles
-    fetch_k(k1, p0 + AHEAD * C);
-    if (STATES) fetch_v(v1, p0 + AHEAD * C);
-    if (STATES && !mine) return;
+    fetch_k(p0 + C);
+    if (STATES) fetch_v(p0 + C);
+    if (STATES && !mine) continue;
     const int cl = min(C, hi - p0), shift = C - cl;  // tokens of this chunk: its last rows
     const int early = P.rev && p0 == 0 ? 1 : 0;      // the entering state meets the first token without a decay
     // opaque, or the compiler forms every product of these weights before the loop, and spills
@@ -430,7 +432,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
       }
 
       phase();
-      fetch_v(v1, p0 + C);
+      fetch_v(p0 + C);
       f32x16 acc[NB] = {};
       // a state near the end of fp16 takes part smaller: scaled and back in place, or (128 registers of it: the branch
       // spilled 165) as it is packed
@@ -455,7 +457,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
       }
       __syncthreads();  // the scores are there, and q has been read
       fetch_q(p0 + C);
-      if (!mine) return;
+      if (!mine) continue;
 #pragma unroll
       for (int ib = 0; ib < NB; ++ib) {
         if (ib * 32 + 31 < shift) continue;
@@ -541,17 +543,6 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
         if (three) S[kb] = O::mma(kf, v3, S[kb]);
       }
     }
-  };
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) {
-    fetch_k(tk[i], lo + i * C);
-    fetch_v(tv[i], lo + i * C);
-  }
-  fetch_q(lo);
-  for (int p0 = lo; p0 < hi; p0 += AHEAD * C) {
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-      if (i == 0 || p0 + i * C < hi) chunk(tk[i], tv[i], p0 + i * C);
   }
 
   // the final state of a head in one segment, or the segment's own
