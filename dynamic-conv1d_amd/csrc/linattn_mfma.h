@@ -39,6 +39,10 @@
 // are made 2^-16 smaller (a wavefront's scores or S together, where one of them
 // passes 2^15).  float32 inputs are products of three bf16 parts throughout (Parts).
 // All sums and S are float32.
+//
+// An infinity or a NaN stays out of the tokens before its own, also within a chunk: scores of later tokens are selected
+// away, not multiplied by zero, and v's elements that are not finite are taken out of the products of the diagonal blocks
+// and added token by token (a branch that finite values do not take).
 #pragma once
 
 #include "lowrank_mfma.h"
@@ -99,6 +103,19 @@ template <typename T> struct Ops {  // 16-bit types
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = Mma16<T>::to_f(elem16(f, e));
   }
+  // sign bits of the halves of a word that are infinite or NaN, and others that mean nothing
+  __device__ static __forceinline__ uint32_t odd_bits(uint32_t w) {
+    return __is_same(T, bf16) ? (w & 0x7F807F80u) + 0x00800080u : (w & 0x7C007C00u) + 0x04000400u;
+  }
+  __device__ static __forceinline__ bool odd(Frag f) {
+    return (odd_bits(f[0]) | odd_bits(f[1]) | odd_bits(f[2]) | odd_bits(f[3])) & 0x80008000u;
+  }
+  __device__ static __forceinline__ Frag keep_finite(Frag f, Frag by) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] &= ~(((odd_bits(by[i]) & 0x80008000u) >> 15) * 0xFFFFu);
+    return f;
+  }
+  __device__ static __forceinline__ Frag finite(Frag f) { return keep_finite(f, f); }
   // a lane's operand in LDS, 64 lanes to a plane
   __device__ static __forceinline__ void put(u32x4* p, int lane, Frag f) { p[lane] = f; }
   __device__ static __forceinline__ Frag get(const u32x4* p, int lane) { return p[lane]; }
@@ -158,6 +175,12 @@ struct Parts {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += u[e];
     }
+  }
+  // the first part of an infinity is one, and of a NaN
+  __device__ static __forceinline__ bool odd(const Frag& f) { return Ops<bf16>::odd(f.p[0]); }
+  __device__ static __forceinline__ Frag finite(const Frag& f) {
+    typedef Ops<bf16> O;
+    return Frag{{O::finite(f.p[0]), O::keep_finite(f.p[1], f.p[0]), O::keep_finite(f.p[2], f.p[0])}};
   }
   __device__ static __forceinline__ void put(u32x4* p, int lane, const Frag& f) {
 #pragma unroll
@@ -284,11 +307,37 @@ __device__ __forceinline__ float largest(const float* v, float m = 0.f) {
   for (int i = 0; i < N; i += 2) m = fmaxf(fmaxf(m, fabsf(v[i])), fabsf(v[i + 1]));
   return m;
 }
-__device__ __forceinline__ bool near_end(float m) { return __any(!(m <= 32768.f)); }
+__device__ __forceinline__ bool near_end(float m) { return __any(m > 32768.f); }
+template <int N>
+__device__ __forceinline__ bool near_end_of(const float* v) {
+  if (!near_end(largest<N>(v))) return false;
+  float m = 0.f;  // infinities have no part in it: the others would lose their digits to one
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]) < __builtin_inff() ? fabsf(v[i]) : 0.f);
+  return near_end(m);
+}
 template <int N>
 __device__ __forceinline__ void scale(float* v, float by) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] *= by;
+}
+
+// A diagonal block's products with the elements of v that are not finite, for the tokens from theirs on: v points at
+// (token 0, column 0), p at the block's scores.
+template <typename O, int PL>
+__device__ __forceinline__ void add_odd(float* acc, const typename O::Lds* v, int rs, const u32x4* p, int lane) {
+  typedef typename O::Lds L;
+  const int half = lane / 32, col = lane % 32;
+#pragma unroll 1
+  for (int j = 0; j < 32; ++j) {
+    const uint16_t* pj = reinterpret_cast<const uint16_t*>(p + j / 16 * PL * 64 + j / 4 % 2 * 32 + col);
+    const float pv = Mma16<L>::to_f(pj[j % 16 / 8 * 4 + j % 4]);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float x = Mma16<L>::to_f(reinterpret_cast<const uint16_t*>(v)[j * rs + 8 * (r / 4) + 4 * half + r % 4]);
+      acc[r] += j <= col && !(fabsf(x) < __builtin_inff()) ? pv * x : 0.f;
+    }
+  }
 }
 
 // Wavefronts on a SIMD that leave a kernel's registers unspilled.
@@ -373,7 +422,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   for (int e = 0; e < 8; ++e) vlast[e] = P.skv * power(lam2, 15 - row(e));
   if constexpr (!STATES)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) diag[r] = row(r) <= col ? P.skv * P.so * power(lam2, col - row(r)) : 0.f;
+    for (int r = 0; r < 16; ++r) diag[r] = P.skv * P.so * power(lam2, max(col - row(r), 0));
   const float g16 = power(lam2, 16), gcol = P.so * power(lam2, col + 1);
   const float gC = power(lam2, C);
 
@@ -420,10 +469,10 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
           for (int r = 0; r < 16; ++r) t[r] = sc[r] * (r < 8 ? vlast[r] * g1 : vlast[r - 8]);
         } else {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) t[r] = sc[r] * diag[r];
+          for (int r = 0; r < 16; ++r) t[r] = row(r) <= col ? sc[r] * diag[r] : 0.f;
         }
         if constexpr (O::kNarrow) {
-          const bool small = near_end(largest<16>(t));
+          const bool small = near_end_of<16>(t);
           if (small) scale<16>(t, kSmaller);
           if (lane == 0) sdown[blk] = small ? kSmaller : 1.f;
         }
@@ -438,7 +487,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
       // spilled 165) as it is packed
       constexpr bool ONCE = O::kNarrow && KP <= 128, PACKED = O::kNarrow && KP > 128;
       bool small = false;
-      if constexpr (O::kNarrow) small = near_end(largest<KB * 16>(Sf));
+      if constexpr (O::kNarrow) small = near_end_of<KB * 16>(Sf);
       if (ONCE && small) scale<KB * 16>(Sf, kSmaller);
       const float by = PACKED && small ? kSmaller : 1.f;
 #pragma unroll
@@ -466,10 +515,17 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
           const int blk = ib + jb;
           const bool down = O::kNarrow && sdown[blk] != 1.f;
           if (down) scale<16>(af, kSmaller);
+          Frag vf[2];
 #pragma unroll
-          for (int s = 0; s < 2; ++s)
-            acc[ib] = O::mma(O::template cols<false>(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane, PV),
-                             O::get(sp + (blk * 2 + s) * PL * 64, lane), acc[ib]);
+          for (int s = 0; s < 2; ++s) vf[s] = O::template cols<false>(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane, PV);
+          const bool late = jb == ib && __any(O::odd(vf[0]) | O::odd(vf[1]));
+          if (late) {
+            vf[0] = O::finite(vf[0]);
+            vf[1] = O::finite(vf[1]);
+          }
+#pragma unroll
+          for (int s = 0; s < 2; ++s) acc[ib] = O::mma(vf[s], O::get(sp + (blk * 2 + s) * PL * 64, lane), acc[ib]);
+          if (late) add_odd<O, PL>(af, sv + jb * 32 * RV + wv * 32, RV, sp + blk * 2 * PL * 64, lane);
           if (down) scale<16>(af, 1.f / kSmaller);
         };
         if (ib > 0 && shift < 32) {  // the state and the block before by way of its last token: g^{i+1} = g^{32} g^{col+1}
@@ -561,9 +617,15 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
         BufUnit<4>::template store<false>(__float_as_uint(S[kb][r] * g), rs, at(k0 + kb * 32 + 8 * (r / 4) + h4 + r % 4, c));
   }
   if constexpr (!STATES) {  // rows past the sequence's length
-    const int z0 = max(len, lo), w = min(vw, NW * 32);
-    for (int64_t i = threadIdx.x; i < (int64_t)(top - z0) * w; i += NT)
-      o[(z0 + i / w) * P.os[2] + vb * NW * 32 + i % w] = (T)0.f;
+    constexpr int VE = 16 / (int)sizeof(T), PR = NW * 32 / VE;
+    const int c = (int)threadIdx.x % PR * VE;
+    for (int t = max(len, lo) + (int)threadIdx.x / PR; t < top; t += NT / PR) {
+      T* to = o + t * P.os[2] + vb * NW * 32 + c;
+      if (WHOLE && c < vw) *reinterpret_cast<u32x4*>(to) = u32x4{0, 0, 0, 0};
+      if constexpr (!WHOLE)
+        for (int j = 0; j < VE; ++j)
+          if (c + j < vw) to[j] = (T)0.f;
+    }
   }
 }
 

@@ -314,6 +314,44 @@ def test_graph():
             assert torch.equal(x, y), f"replay {seed}"
 
 
+@pytest.mark.parametrize("K,V", [(64, 64), (100, 37), (128, 128), (256, 40)])
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,t", [(200, 77), (64, 0), (63, 62), (40, 20)])
+def test_not_finite_values_stay_behind_their_token(K, V, dtype, T, t):
+    """An infinity or a NaN in a row of k or v (or of o's gradient) reaches the tokens from its own on (up to its own), and
+    what it does not reach is what it is without it, to the bit."""
+    g = gen(16 + T + K)
+    B, H, h = 1, 3, 1
+    lam = torch.tensor([-0.02, -0.05, 0.0]).to(DEV)
+    clean = [randn(g, B, H, T, c).to(dtype).to(DEV) for c in (K, K, V, V)]  # q, k, v, do
+
+    def run(q, k, v, do):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        o = linear_attention(*leaves, lam)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    want = run(*clean)
+    rows = torch.arange(T, device=DEV)
+    for i, c, value in ((1, K - 1, float("nan")), (2, V // 2, float("nan")), (2, V - 1, float("inf")), (3, 3, float("nan")),
+                        (3, 0, -float("inf")), (0, 2, float("nan"))):
+        bad = [x.clone() for x in clean]
+        bad[i][:, h, t, c] = value
+        got = run(*bad)
+        # what it reaches: rows of o, dq, dk, dv
+        late, early, own = rows >= t, rows <= t, rows == t
+        none = rows < 0
+        reach = {0: (own, none, early, early), 1: (late, late, none, own), 2: (late, late, own, none),
+                 3: (none, own, early, early)}[i]
+        for x, w, r, name in zip(got, want, reach, ("o", "dq", "dk", "dv")):
+            what = f"{value} in input {i}: {name}"
+            assert torch.equal(x[:, [0, 2]], w[:, [0, 2]]), f"{what}, other heads"
+            assert torch.equal(x[:, h, ~r], w[:, h, ~r]), f"{what}, rows that it does not reach"
+            assert r.sum() == 0 or not x[:, h, r].isfinite().all(-1).any(), f"{what}, rows that it reaches"
+        if i == 2 and value != value:
+            others = torch.arange(V, device=DEV) != c
+            assert torch.equal(got[0][:, h][..., others], want[0][:, h][..., others]), "o's other columns"
+
+
 def test_fp16_scores_and_states_past_the_type():
     """Scores and states above 65504 whose outputs are within fp16: operands are held smaller, and none is lost."""
     g = gen(15)
