@@ -56,7 +56,9 @@ __global__ __launch_bounds__(256) void lr_step_mma(LrStep p) {
   }
   for (int i = tid; i < kSeqs * RP; i += 256) {
     const int n = i / RP, r = i % RP;
-    sz[n * RZ + r] = n0 + n >= p.N ? (T)0.f : r < R ? z[(n0 + n) * R + r] : r == R && sw ? (T)1.f : (T)0.f;
+    const int64_t slot = n0 + n >= p.N ? -1 : p.slot_ids ? (int64_t)p.slot_ids[n0 + n] : n0 + n;
+    const bool live = slot >= 0 && slot < p.slots;  // whatever the others' z holds, their y is zero
+    sz[n * RZ + r] = !live ? (T)0.f : r < R ? z[(n0 + n) * R + r] : r == R && sw ? (T)1.f : (T)0.f;
   }
 
   float y[16];

@@ -66,6 +66,16 @@ def test_step(G, N, D, R, W, static, residual, dtype):
         assert (got[out] == 0).all()
 
 
+@pytest.mark.parametrize("D", [128, 33])
+def test_sequences_that_take_no_part_may_hold_anything(D):
+    g = gen(30)
+    x, z, U, _, state = _inputs(g, 1, 5, D, 8, 3, False, 5, BF)
+    x[2], z[0][2], x[4], z[0][4] = float("nan"), float("nan"), float("inf"), float("inf")
+    ids = torch.tensor([0, 1, -1, 3, 5], dtype=torch.int32, device=DEV)
+    y, = lowrank_dynamic_convolution_step_grouped(_dev(x), _dev(z), _dev(U), _dev(state), slots=ids)
+    assert (y[[2, 4]] == 0).all() and y.isfinite().all()
+
+
 def test_steps_follow_the_whole_sequence():
     g = gen(31)
     N, T, D, R, W = 3, 11, 96, 7, 4
