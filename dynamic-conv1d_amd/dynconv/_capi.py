@@ -152,6 +152,13 @@ def int64_array(values):
     return (ctypes.c_int64 * len(values))(*values)
 
 
+def int32(t):
+    """Indexes as contiguous int32; what does not fit becomes the nearest that does, not its low bits."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-(2**31), 2**31 - 1)
+    return t.to(torch.int32).contiguous()
+
+
 # torch's current-stream handle without building a Stream object (2 us -> 0.1 us per call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _get_device = getattr(torch._C, "_cuda_getDevice", None)

@@ -99,7 +99,7 @@ def _index(t, n, device, name):
         return None
     assert t.device == device and t.dtype in (torch.int32, torch.int64), f"{name} must be int32, on q's device"
     assert tuple(t.shape) == (n,), f"{name} must have one entry a sequence"
-    return t.to(torch.int32).contiguous()
+    return _capi.int32(t)
 
 
 def linear_attention(

@@ -340,7 +340,7 @@ def lowrank_dynamic_convolution_step_grouped(
     else:
         assert slots.device == x.device and slots.dtype in (torch.int32, torch.int64) and tuple(slots.shape) == (N,), \
             "slots must be int32 [N], on x's device"
-        slots = slots.to(torch.int32).contiguous()
+        slots = _capi.int32(slots)
     return _step_grouped(x, z, U, state, static_w, residual, slots, W)
 
 

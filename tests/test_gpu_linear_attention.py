@@ -205,6 +205,19 @@ def test_lengths_outside_the_rows_are_clamped():
         assert torch.equal(a[0], b[0]) and (b[1] == 0).all()
 
 
+def test_indexes_past_32_bits():
+    """int64 lengths and slots whose low 32 bits would name other rows."""
+    q = torch.randn(2, 1, 40, 16, device=DEV)
+    lam = _decays(1, 0).to(DEV)
+    whole = linear_attention(q, q, q, lam)
+    far = linear_attention(q, q, q, lam, lengths=torch.tensor([1 << 32, 40 - (1 << 32)], device=DEV))
+    assert torch.equal(far[0], whole[0]) and (far[1] == 0).all()
+    state = torch.randn(2, 1, 16, 16, device=DEV)
+    before = state.clone()
+    o = linear_attention_step(q[:, :, 0], q[:, :, 0], q[:, :, 0], lam, state, slots=torch.tensor([1 << 32, 1], device=DEV))
+    assert (o[0] == 0).all() and torch.equal(state[0], before[0]) and not torch.equal(state[1], before[1])
+
+
 def test_shared_heads_and_partial_gradients():
     """Keys and values shared by the heads as expanded views; a loss of the state alone."""
     g = gen(11)
