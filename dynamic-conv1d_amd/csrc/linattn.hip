@@ -67,7 +67,8 @@ Cut cut_of(const LaProblem& p) {
   return {(int)(seg * C), (int)(chunks > 0 ? (chunks + seg - 1) / seg : 1)};
 }
 
-// States from segment to segment: states[s] <- the state before segment s.
+// States from segment to segment: states[s] <- the state before segment s.  A thread to an element, which it reads and
+// writes once per segment: bound by memory (64 heads, 4 segments, 128 x 128: 34 MB in 9 us).
 struct Carry {
   const float* log_decay;
   const int32_t* lengths;

@@ -16,6 +16,9 @@
 // holds them: taps go from the oldest on, so the row that x_w is written to has
 // been read by the same thread.
 //
+// Measured, q|k|v in one launch, W 4, static filter: 256 sequences, D 4096, rank 31, bf16 13.6 us (53 MB, 3.9 TB/s; 47.7
+// with lr_step_any), 8 sequences, D 2048, rank 15 6.4 us (7.9), of which the launch's own 5.5 are mostly one round trip.
+//
 // Other rows take lr_step_any, a thread to a channel.
 #include "linattn_mfma.h"
 
