@@ -69,6 +69,7 @@ Cut cut_of(const LaProblem& p) {
 
 // States from segment to segment: states[s] <- the state before segment s.  A thread to an element, which it reads and
 // writes once per segment: bound by memory (64 heads, 4 segments, 128 x 128: 34 MB in 9 us).
+constexpr int kAhead = 8;  // segments' states on their way at once: one by one, 45 segments of 4 heads took 15 us
 struct Carry {
   const float* log_decay;
   const int32_t* lengths;
@@ -91,13 +92,22 @@ __global__ __launch_bounds__(256) void la_carry(Carry A) {
   float* st = A.states[set] + bh * A.nseg * A.n + e;
   float run = A.s_in[set] ? A.s_in[set][bh * A.n + e] : 0.f;
   const float full = (float)exp(lam * A.seg);
-  for (int s = 0; s < A.nseg; ++s) {
-    const bool last = s == A.nseg - 1;
-    const float own = last && !A.s_out[set] ? 0.f : st[s * A.n];
-    st[s * A.n] = run;
-    const int cnt = min(max(len - s * A.seg, 0), A.seg) - (rev && s == 0 && len > 0 ? 1 : 0);
-    const float g = cnt == 0 ? 1.f : cnt == A.seg ? full : (float)exp(lam * cnt);
-    run = g * run + own;
+  for (int s0 = 0; s0 < A.nseg; s0 += kAhead) {
+    float own[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int s = s0 + i, end = A.s_out[set] ? A.nseg : A.nseg - 1;
+      own[i] = s < end ? st[s * A.n] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int s = s0 + i;
+      if (s == A.nseg) break;
+      st[s * A.n] = run;
+      const int cnt = min(max(len - s * A.seg, 0), A.seg) - (rev && s == 0 && len > 0 ? 1 : 0);
+      const float g = cnt == 0 ? 1.f : cnt == A.seg ? full : (float)exp(lam * cnt);
+      run = g * run + own[i];
+    }
   }
   if (A.s_out[set]) A.s_out[set][bh * A.n + e] = rev && len > 0 ? (float)(run * exp(lam)) : run;
 }

@@ -47,8 +47,7 @@
 //
 // An infinity or a NaN stays out of the tokens before its own, also within a chunk: scores of later tokens are selected
 // away, not multiplied by zero, and v's elements that are not finite are taken out of the products of the diagonal blocks
-// and added token by token (a branch that finite values do not take).  The select and the test for it cost 2% of the
-// chunks' launches in bf16 (5% in fp16).
+// and added token by token (a branch that finite values do not take).
 #pragma once
 
 #include "lowrank_mfma.h"
@@ -313,15 +312,9 @@ __device__ __forceinline__ float largest(const float* v, float m = 0.f) {
   for (int i = 0; i < N; i += 2) m = fmaxf(fmaxf(m, fabsf(v[i])), fabsf(v[i + 1]));
   return m;
 }
-__device__ __forceinline__ bool near_end(float m) { return __any(m > 32768.f); }
-template <int N>
-__device__ __forceinline__ bool near_end_of(const float* v) {
-  if (!near_end(largest<N>(v))) return false;
-  float m = 0.f;  // infinities have no part in it: the others would lose their digits to one
-#pragma unroll
-  for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]) < __builtin_inff() ? fabsf(v[i]) : 0.f);
-  return near_end(m);
-}
+// A lane with an infinity does not ask for it: its token's (or column's) o is not finite either way, and the other lanes
+// would lose digits.
+__device__ __forceinline__ bool near_end(float m) { return __any(m > 32768.f && m < __builtin_inff()); }
 template <int N>
 __device__ __forceinline__ void scale(float* v, float by) {
 #pragma unroll
@@ -474,11 +467,15 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
 #pragma unroll
           for (int r = 0; r < 16; ++r) t[r] = sc[r] * (r < 8 ? vlast[r] * g1 : vlast[r - 8]);
         } else {
+          // opaque in fp16, or the sixteen conditions wait in spilled scalar registers (H16 T32768 hd128 156 -> 145
+          // us; in bf16 it costs 1%)
+          int later = col - 4 * half;
+          if constexpr (O::kNarrow) asm volatile("" : "+v"(later));
 #pragma unroll
-          for (int r = 0; r < 16; ++r) t[r] = row(r) <= col ? sc[r] * diag[r] : 0.f;
+          for (int r = 0; r < 16; ++r) t[r] = 8 * (r / 4) + r % 4 <= later ? sc[r] * diag[r] : 0.f;
         }
         if constexpr (O::kNarrow) {
-          const bool small = near_end_of<16>(t);
+          const bool small = near_end(largest<16>(t));
           if (small) scale<16>(t, kSmaller);
           if (lane == 0) sdown[blk] = small ? kSmaller : 1.f;
         }
@@ -493,7 +490,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
       // spilled 165) as it is packed
       constexpr bool ONCE = O::kNarrow && KP <= 128, PACKED = O::kNarrow && KP > 128;
       bool small = false;
-      if constexpr (O::kNarrow) small = near_end_of<KB * 16>(Sf);
+      if constexpr (O::kNarrow) small = near_end(largest<KB * 16>(Sf));
       if (ONCE && small) scale<KB * 16>(Sf, kSmaller);
       const float by = PACKED && small ? kSmaller : 1.f;
 #pragma unroll
