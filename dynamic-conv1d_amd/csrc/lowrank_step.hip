@@ -17,9 +17,10 @@
 // been read by the same thread.
 //
 // Measured, q|k|v in one launch, W 4, static filter: 256 sequences, D 4096, rank 31, bf16 13.6 us (53 MB, 3.9 TB/s; 47.7
-// with lr_step_any), 8 sequences, D 2048, rank 15 6.4 us (7.9), of which the launch's own 5.5 are mostly one round trip.
+// with lr_step_any), 8 sequences, D 2048, rank 15 (lr_step_taps) 4.4 us behind one another, one round trip of loads and
+// the launch (lr_step_mma 5.1).
 //
-// Other rows take lr_step_any, a thread to a channel.
+// Few workgroups of those take lr_step_taps; other rows take lr_step_any, a thread to a channel.
 #include "linattn_mfma.h"
 
 namespace dc {
@@ -130,6 +131,111 @@ __global__ __launch_bounds__(256) void lr_step_mma(LrStep p) {
   }
 }
 
+// lr_step_mma for few workgroups: 32 channels to one, and the taps go round its wavefronts, so four times the workgroups
+// and a quarter of the chain.  A thread has TAPS taps of U and x in flight; four of them at a time lie in LDS.  The
+// wavefronts' sums of y meet in a fixed order.
+template <typename T, int RP, int TAPS>
+__global__ __launch_bounds__(256) void lr_step_taps(LrStep p) {
+  typedef la::Ops<T> O;
+  constexpr int CH = 32, VE = 16 / (int)sizeof(T), PR = CH / VE, ROWS = 256 / PR, UP = RP > ROWS ? RP / ROWS : 1;
+  constexpr int RU = la::row_elems<T, CH, false>(), RX = CH + VE, RZ = RP + VE, RY = CH + 1;
+  constexpr int UB = kWaves * RP * RU * (int)sizeof(T), YB = kWaves * kSeqs * RY * (int)sizeof(float);
+  __shared__ __align__(16) unsigned char buf[UB > YB ? UB : YB];  // U's taps, then the sums of y
+  __shared__ __align__(16) T sx[kWaves * kSeqs * RX];
+  __shared__ __align__(16) T sz[kSeqs * RZ];
+  T* const su = reinterpret_cast<T*>(buf);
+  float* const sy = reinterpret_cast<float*>(buf);
+  const int R = (int)p.R, W = (int)p.W, g = blockIdx.z, tid = threadIdx.x;
+  const int64_t D = p.D, C = p.G * D, d0 = (int64_t)blockIdx.x * CH, n0 = (int64_t)blockIdx.y * kSeqs;
+  const int lane = tid % 64, half = lane / 32, col = lane % 32, wv = wave_id();
+  const T* z = (const T*)p.z[g];
+  const T* U = (const T*)p.U[g] + d0;
+  const T* sw = p.static_w[g] ? (const T*)p.static_w[g] + d0 : nullptr;
+
+  const int c = tid % PR * VE, row = tid / PR;
+  const bool in = d0 + c < D;
+  const int64_t n = n0 + row;
+  const int64_t slot = row >= kSeqs || n >= p.N ? -1 : p.slot_ids ? (int64_t)p.slot_ids[n] : n;
+  const bool live = in && slot >= 0 && slot < p.slots;
+  const T* xr = live ? (const T*)p.x + n * p.x_ld + g * D + d0 + c : nullptr;
+  T* sr = (T*)p.state + slot * (W - 1) * C + g * D + d0 + c;
+
+  float y[16];
+  zero_vals<16>(y);
+  for (int w1 = W; w1 > 0; w1 -= TAPS) {  // taps w1 - 1 .. w1 - TAPS, the oldest first
+    u32x4 u[TAPS][UP], x[TAPS];
+#pragma unroll
+    for (int k = 0; k < TAPS; ++k) {
+      const int w = w1 - 1 - k;
+      x[k] = u32x4{0, 0, 0, 0};
+      if (w >= 0 && xr) x[k] = *reinterpret_cast<const u32x4*>(w == 0 ? xr : sr + (W - 1 - w) * C);
+#pragma unroll
+      for (int i = 0; i < UP; ++i) {
+        const int r = row + i * ROWS;
+        u[k][i] = u32x4{0, 0, 0, 0};
+        if (w >= 0 && in && r < R) u[k][i] = *reinterpret_cast<const u32x4*>(U + ((int64_t)r * W + w) * D + c);
+        else if (w >= 0 && in && r == R && sw) u[k][i] = *reinterpret_cast<const u32x4*>(sw + w * D + c);
+      }
+    }
+    if (w1 == W)  // behind the loads
+      for (int i = tid; i < kSeqs * RP; i += 256) {
+        const int m = i / RP, r = i % RP;
+        const int64_t of = n0 + m >= p.N ? -1 : p.slot_ids ? (int64_t)p.slot_ids[n0 + m] : n0 + m;
+        const bool part = of >= 0 && of < p.slots;  // whatever the others' z holds, their y is zero
+        sz[m * RZ + r] = !part ? (T)0.f : r < R ? z[(n0 + m) * R + r] : r == R && sw ? (T)1.f : (T)0.f;
+      }
+#pragma unroll
+    for (int k0 = 0; k0 < TAPS; k0 += kWaves) {
+      if (w1 - 1 - k0 < 0) break;
+      __syncthreads();  // the taps before have been read
+#pragma unroll
+      for (int k = k0; k < k0 + kWaves; ++k) {
+        const int w = w1 - 1 - k;
+        if (w < 0) break;
+        if (row < kSeqs) *reinterpret_cast<u32x4*>(sx + ((k - k0) * kSeqs + row) * RX + c) = x[k];
+        if (xr && w < W - 1) *reinterpret_cast<u32x4*>(sr + (W - 2 - w) * C) = x[k];
+#pragma unroll
+        for (int i = 0; i < UP; ++i)
+          if (row + i * ROWS < RP) *reinterpret_cast<u32x4*>(su + ((k - k0) * RP + row + i * ROWS) * RU + c) = u[k][i];
+      }
+      __syncthreads();
+      const int w = w1 - 1 - k0 - wv;
+      if (w < 0) continue;
+      la::f32x16 acc = {};
+#pragma unroll
+      for (int s = 0; s < RP / 16; ++s) {
+        const T* zr = sz + col * RZ + s * 16 + 4 * half;
+        float t[8];
+        load_vals<T, 4>(zr, t);
+        load_vals<T, 4>(zr + 8, t + 4);
+        acc = O::mma(O::template cols<false>(su + (wv * RP + s * 16) * RU, RU, lane), O::pack(t), acc);
+      }
+      const float one = w == 0 && p.residual ? 1.f : 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float xv[4];
+        load_vals<T, 4>(sx + (wv * kSeqs + col) * RX + 8 * q + 4 * half, xv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[4 * q + j] += (acc[4 * q + j] + one) * xv[j];
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 16; ++q) sy[(wv * kSeqs + col) * RY + 8 * (q / 4) + 4 * half + q % 4] = y[q];
+  __syncthreads();
+  if (row < kSeqs && in && n < p.N) {
+    float v[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+      const float* t = sy + row * RY + c + j;
+      constexpr int next = kSeqs * RY;
+      v[j] = (t[0] + t[next]) + (t[2 * next] + t[3 * next]);
+    }
+    store_vals<T, VE>((T*)p.y[g] + n * D + d0 + c, v);
+  }
+}
+
 // A wavefront takes 64 channels, kN sequences and every fourth tap; the wavefronts' sums of y meet in LDS in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves) void lr_step_any(LrStep p) {
@@ -207,6 +313,16 @@ bool mma_ok(const LrStep& p) {
   return ok;
 }
 
+// Whether lr_step_taps takes a problem: its workgroups, four for each of lr_step_mma's, then have a CU each in 16 bits
+// (float32's, of half the channels to a piece, gain to three rounds).  Measured, lr_step_taps against lr_step_mma, us, 32
+// sequences, W 4 rank 16 / W 8 rank 32 / W 16 rank 64, bf16: D 2048 4.3 / 6.6 / 11.3 against 5.3 / 8.7 / 19.6, D 8192 (64
+// workgroups) 5.0 / 7.9 / 18.6 against 5.6 / 9.2 / 20.3, D 12288 5.6 / 9.3 / 21.9 against 5.7 / 9.6 / 30.2 but W 16 rank 32
+// 17.9 against 15.3, D 16384 6.0 against 5.9; float32, 64 sequences, D 12288 (192) 7.3 / 15.3 / 52 against 9.0 / 21.5 / 65,
+// D 32768 19.2 against 16.3.
+bool few(const LrStep& p) {
+  return (p.D + kChans - 1) / kChans * ((p.N + kSeqs - 1) / kSeqs) * p.G <= (p.dtype == kFP32 ? 192 : 64);
+}
+
 // Sequences in parts of what the grid's second axis holds.
 template <typename T, typename F>
 hipError_t in_parts(const LrStep& p, int per, F launch) {
@@ -234,6 +350,18 @@ hipError_t launch(const LrStep& p) {
       lr_step_any<T><<<dim3((unsigned)((p.D + 63) / 64), ny, G), 64 * kWaves, lds, p.stream>>>(q);
     });
   const int64_t rank = p.R + (p.static_w[0] ? 1 : 0);
+  if (few(p))
+    return in_parts<T>(p, kSeqs, [&](const LrStep& q, unsigned ny) {
+      const dim3 grid((unsigned)((p.D + 31) / 32), ny, G);
+      // taps in flight: eight, or as many as there are or registers hold
+      const bool four = p.W <= 4;
+      auto run = [&](auto kernel) { kernel<<<grid, 256, 0, p.stream>>>(q); };
+      if (rank <= 16) run(four ? lr_step_taps<T, 16, 4> : lr_step_taps<T, 16, 8>);
+      else if (rank <= 32) run(four ? lr_step_taps<T, 32, 4> : lr_step_taps<T, 32, 8>);
+      else if (rank <= 64) run(four ? lr_step_taps<T, 64, 4> : lr_step_taps<T, 64, 8>);
+      else if (rank <= 128) run(lr_step_taps<T, 128, 4>);
+      else if constexpr (sizeof(T) == 2) run(lr_step_taps<T, 256, 4>);
+    });
   return in_parts<T>(p, kSeqs, [&](const LrStep& q, unsigned ny) {
     const dim3 grid((unsigned)((p.D + kChans - 1) / kChans), ny, G);
     // taps in flight: what 64 registers hold of U

@@ -66,7 +66,16 @@ def test_step(G, N, D, R, W, static, residual, dtype):
         assert (got[out] == 0).all()
 
 
-@pytest.mark.parametrize("D", [128, 33])
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("R,W,static", [(15, 4, True), (8, 1, False), (31, 5, True), (63, 9, True), (128, 3, False),
+                                        (256, 2, False)])
+def test_many_workgroups(R, W, static, dtype):
+    """Sizes past those that split the taps over a workgroup's wavefronts."""
+    N, D = (300, 2568) if dtype == F32 else (70, 2824)
+    test_step(1, N, D, R, W, static, True, dtype)
+
+
+@pytest.mark.parametrize("D", [128, 33, 8448])
 def test_sequences_that_take_no_part_may_hold_anything(D):
     g = gen(30)
     x, z, U, _, state = _inputs(g, 1, 5, D, 8, 3, False, 5, BF)
