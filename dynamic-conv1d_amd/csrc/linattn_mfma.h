@@ -39,9 +39,9 @@
 // smaller (a wavefront's scores or S together, where one of them passes 2^15).  float32 inputs are products of three bf16 parts throughout (Parts).
 // All sums and S are float32.
 //
-// Measured at B2 H32 T8192, 128 x 128, bf16 (134 MB a tensor), four segments: the states' launch 66 us (4.1 TB/s of k and
-// v), the carry 9, the forward's chunks 133 (4.0 TB/s), the backward's three passes 311 (3.0 TB/s: what they read again
-// comes from the last-level cache), with the backward's own states 589 in all.  Loads alone take 42, 73 and 163, stores
+// Measured at B2 H32 T8192, 128 x 128, bf16 (134 MB a tensor), four segments: the states' launch 64 us (4.2 TB/s of k and
+// v), the carry 8, the forward's chunks 133 (4.0 TB/s), the backward's three passes 313 (3.0 TB/s: what they read again
+// comes from the last-level cache), with the backward's own states 580 in all.  Loads alone take 42, 73 and 163, stores
 // 20 and 60-78 more.  Matrix instructions fill 28% of the SIMDs' cycles in the chunks' launches and vector instructions
 // 35%; the rest is the chain of one chunk's phases, which two workgroups on a CU hide from each other in part.
 //
