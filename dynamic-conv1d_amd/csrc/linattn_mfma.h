@@ -35,8 +35,9 @@
 // Precision.  Scores and S are rounded to the inputs' type as operands (relative
 // 2^-8 / 2^-11 of single terms, below the rounding of o); the products that make
 // S take v g^{C-1-j} in two parts of the type (16 or 22 bits), bf16 in three where
-// the state is returned, which so is a float32 result; fp16 operands that would come near that type's end are made 2^-16
-// smaller (a wavefront's scores or S together, where one of them passes 2^15).  float32 inputs are products of three bf16 parts throughout (Parts).
+// the state is returned, which so is a float32 result.  fp16 scores are lifted to the upper end of the type, each token's
+// by a power of two of its own, which its float32 sums leave again; an S that would pass the type's end is made 2^-16
+// smaller (a wavefront's together, where one of them passes 2^15).  float32 inputs are products of three bf16 parts throughout (Parts).
 // All sums and S are float32.
 //
 // Measured at B2 H32 T8192, 128 x 128, bf16 (134 MB a tensor), four segments: the states' launch 64 us (4.2 TB/s of k and
@@ -312,13 +313,24 @@ __device__ __forceinline__ float largest(const float* v, float m = 0.f) {
   for (int i = 0; i < N; i += 2) m = fmaxf(fmaxf(m, fabsf(v[i])), fabsf(v[i + 1]));
   return m;
 }
-// A lane with an infinity does not ask for it: its token's (or column's) o is not finite either way, and the other lanes
-// would lose digits.
+// A lane with an infinity does not ask for it: its column's o is not finite either way, and the other lanes would lose
+// digits.
 __device__ __forceinline__ bool near_end(float m) { return __any(m > 32768.f && m < __builtin_inff()); }
 template <int N>
 __device__ __forceinline__ void scale(float* v, float by) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] *= by;
+}
+
+// fp16 operands whose largest value (m, of a token) may lie anywhere in float32's range: the power of two that brings it
+// between 2^14 and 2^15, so that what is down to 2^-28 of it keeps all of the type's bits.  (An infinity or a NaN gives
+// any: its products are not finite either way.)
+__device__ __forceinline__ int lift_of(float m) { return min(15 - __builtin_amdgcn_frexp_expf(m), 120); }
+__device__ __forceinline__ float two_to(int n) { return __builtin_ldexpf(1.f, n); }
+// The larger of a lane's value and its partner's, 32 lanes on.
+__device__ __forceinline__ float pair_max(float m) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
 }
 
 // A diagonal block's products with the elements of v that are not finite, for the tokens from theirs on: v points at
@@ -360,10 +372,11 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   __shared__ __align__(16) unsigned char sqo[STATES ? 16 : QB > OB ? QB : OB];
   L* const sq = reinterpret_cast<L*>(sqo);
   T* const so = reinterpret_cast<T*>(sqo);
-  // scores as operands: blocks of 32 x 32 on and below the diagonal, two steps of a lane's 8, and what they are smaller by
+  // scores as operands: blocks of 32 x 32 on and below the diagonal, two steps of a lane's 8; in fp16 each token's are
+  // lifted (lift_of), and sback brings them back
   constexpr int NP = NB * (NB + 1) / 2;
   __shared__ u32x4 sp[STATES ? 1 : NP * 2 * PL * 64];
-  __shared__ float sdown[NP];
+  __shared__ float sback[O::kNarrow && !STATES ? NP * 32 : 1];
 
   // the passes of one segment run side by side: what one reads, the others find in the last-level cache
   int blk = xcd_remap(blockIdx.x, A.nblk);
@@ -475,9 +488,9 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
           for (int r = 0; r < 16; ++r) t[r] = 8 * (r / 4) + r % 4 <= later ? sc[r] * diag[r] : 0.f;
         }
         if constexpr (O::kNarrow) {
-          const bool small = near_end(largest<16>(t));
-          if (small) scale<16>(t, kSmaller);
-          if (lane == 0) sdown[blk] = small ? kSmaller : 1.f;
+          const int n = lift_of(pair_max(largest<16>(t)));
+          scale<16>(t, two_to(n));
+          sback[blk * 32 + col] = two_to(-n);
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) O::put(sp + (blk * 2 + s) * PL * 64, lane, O::pack(t + 8 * s));
@@ -514,10 +527,9 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
       for (int ib = 0; ib < NB; ++ib) {
         if (ib * 32 + 31 < shift) continue;
         float* const af = reinterpret_cast<float*>(&acc[ib]);
-        auto add = [&](int jb) {
+        // by: what the sum is multiplied with later on, and these products with it
+        auto add = [&](int jb, float by) {
           const int blk = ib + jb;
-          const bool down = O::kNarrow && sdown[blk] != 1.f;
-          if (down) scale<16>(af, kSmaller);
           Frag vf[2];
 #pragma unroll
           for (int s = 0; s < 2; ++s) vf[s] = O::template cols<false>(sv + (jb * 2 + s) * 16 * RV + wv * 32, RV, lane, PV);
@@ -526,19 +538,32 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
             vf[0] = O::finite(vf[0]);
             vf[1] = O::finite(vf[1]);
           }
+          // lifted scores: sums of their own, brought back by token
+          f32x16 own = {};
+          f32x16& sum = O::kNarrow ? own : acc[ib];
+          float* const sf = reinterpret_cast<float*>(&sum);
 #pragma unroll
-          for (int s = 0; s < 2; ++s) acc[ib] = O::mma(vf[s], O::get(sp + (blk * 2 + s) * PL * 64, lane), acc[ib]);
-          if (late) add_odd<O, PL>(af, sv + jb * 32 * RV + wv * 32, RV, sp + blk * 2 * PL * 64, lane);
-          if (down) scale<16>(af, 1.f / kSmaller);
+          for (int s = 0; s < 2; ++s) sum = O::mma(vf[s], O::get(sp + (blk * 2 + s) * PL * 64, lane), sum);
+          if (late) add_odd<O, PL>(sf, sv + jb * 32 * RV + wv * 32, RV, sp + blk * 2 * PL * 64, lane);
+          if constexpr (O::kNarrow) {
+            const float back = sback[blk * 32 + col] * by;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) af[r] = fmaf(sf[r], back, af[r]);
+          }
         };
         if (ib > 0 && shift < 32) {  // the state and the block before by way of its last token: g^{i+1} = g^{32} g^{col+1}
-          scale<16>(af, power(lam2, 32 - early - shift));
-          add(0);
-          scale<16>(af, gcol);
+          if constexpr (O::kNarrow) {
+            scale<16>(af, power(lam2, 32 - early - shift) * gcol);
+            add(0, gcol);
+          } else {
+            scale<16>(af, power(lam2, 32 - early - shift));
+            add(0, 1.f);
+            scale<16>(af, gcol);
+          }
         } else {
           scale<16>(af, P.so * power(lam2, max(ib * 32 + col + 1 - early - shift, 0)));
         }
-        add(ib);
+        add(ib, 1.f);
 #pragma unroll
         for (int g = 0; g < 4; ++g) store_vals<T, 4>(so + (ib * 32 + col) * RO + wv * 32 + 8 * g + 4 * half, af + 4 * g);
       }
