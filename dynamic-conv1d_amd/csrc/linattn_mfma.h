@@ -35,9 +35,11 @@
 // Precision.  Scores and S are rounded to the inputs' type as operands (relative
 // 2^-8 / 2^-11 of single terms, below the rounding of o); the products that make
 // S take v g^{C-1-j} in two parts of the type (16 or 22 bits), bf16 in three where
-// the state is returned, which so is a float32 result.  fp16 scores are lifted to the upper end of the type, each token's
-// by a power of two of its own, which its float32 sums leave again; an S that would pass the type's end is made 2^-16
-// smaller (a wavefront's together, where one of them passes 2^15).  float32 inputs are products of three bf16 parts throughout (Parts).
+// the state is returned, which so is a float32 result.  fp16 operands are lifted to
+// the upper end of the type by powers of two that the float32 sums leave again:
+// each token's scores and each column's v g^{C-1-j} by its own, the 32 columns of S
+// of a wavefront by one (what is below 2^-28 of their largest value loses digits in
+// q S, not in S).  float32 inputs are products of three bf16 parts throughout (Parts).
 // All sums and S are float32.
 //
 // Measured at B2 H32 T8192, 128 x 128, bf16 (134 MB a tensor), four segments: the states' launch 64 us (4.2 TB/s of k and
@@ -50,6 +52,8 @@
 // away, not multiplied by zero, and v's elements that are not finite are taken out of the products of the diagonal blocks
 // and added token by token (a branch that finite values do not take).
 #pragma once
+
+#include <type_traits>
 
 #include "lowrank_mfma.h"
 #include "layer_launch.h"
@@ -305,32 +309,51 @@ struct Tile {
   }
 };
 
-// Whether one of a wavefront's N values comes near the end of fp16: they then take part 2^-16 smaller.
-constexpr float kSmaller = 1.f / 65536;
+// The largest of N values.
 template <int N>
 __device__ __forceinline__ float largest(const float* v, float m = 0.f) {
 #pragma unroll
   for (int i = 0; i < N; i += 2) m = fmaxf(fmaxf(m, fabsf(v[i])), fabsf(v[i + 1]));
   return m;
 }
-// A lane with an infinity does not ask for it: its column's o is not finite either way, and the other lanes would lose
-// digits.
-__device__ __forceinline__ bool near_end(float m) { return __any(m > 32768.f && m < __builtin_inff()); }
 template <int N>
 __device__ __forceinline__ void scale(float* v, float by) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] *= by;
 }
 
-// fp16 operands whose largest value (m, of a token) may lie anywhere in float32's range: the power of two that brings it
-// between 2^14 and 2^15, so that what is down to 2^-28 of it keeps all of the type's bits.  (An infinity or a NaN gives
-// any: its products are not finite either way.)
+// fp16 operands whose largest value m may lie anywhere in float32's range: the exponent that brings it between 2^14 and
+// 2^15, so that what is down to 2^-28 of it keeps all of the type's bits.  (An infinity or a NaN gives any: its products
+// are not finite either way.)
 __device__ __forceinline__ int lift_of(float m) { return min(15 - __builtin_amdgcn_frexp_expf(m), 120); }
 __device__ __forceinline__ float two_to(int n) { return __builtin_ldexpf(1.f, n); }
 // The larger of a lane's value and its partner's, 32 lanes on.
 __device__ __forceinline__ float pair_max(float m) {
   const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
   return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+
+// The exponent of a lane's largest value m, far below all others where m is zero or not finite, and its largest over the
+// wavefront.
+__device__ __forceinline__ int exponent_of(float m) {
+  return m > 0.f && m < __builtin_inff() ? __builtin_amdgcn_frexp_expf(m) : -1000;
+}
+__device__ __forceinline__ int wave_max(int e) {
+  auto dpp = [&](auto ctrl) { return max(e, __builtin_amdgcn_update_dpp(0, e, decltype(ctrl)::value, 0xF, 0xF, false)); };
+  e = dpp(std::integral_constant<int, 0xB1>());   // pairs
+  e = dpp(std::integral_constant<int, 0x4E>());   // quads
+  e = dpp(std::integral_constant<int, 0x141>());  // the mirrored lane of 8
+  e = dpp(std::integral_constant<int, 0x140>());  // of 16
+  return max(max(__builtin_amdgcn_readlane(e, 0), __builtin_amdgcn_readlane(e, 16)),
+             max(__builtin_amdgcn_readlane(e, 32), __builtin_amdgcn_readlane(e, 48)));
+}
+// The largest magnitude of a lane's 16 fp16 values of two steps' halves, as bits of fp16 (a NaN's are the largest).
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float largest16(u32x4 f) {
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, f[i] & 0x7FFF7FFFu));
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)max(m[0], m[1]));
 }
 
 // A diagonal block's products with the elements of v that are not finite, for the tokens from theirs on: v points at
@@ -439,6 +462,9 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   const float gC = power(lam2, C);
 
   constexpr bool three = __is_same(T, bf16) && RETURNED;
+  // fp16: S is held times 2^ex; smax: the exponent of a column's largest value; skv_top: v's largest weight in its 16 tokens
+  int ex = 0, smax = -1000;
+  const float skv_top = fabsf(P.skv) * fmaxf(1.f, power(lam2, 15));
 
   // tiles on their way: the next chunk's (STATES with the one after it too: 62 -> 67 us at B2 H32 T8192 hd128)
   Tile<T, C, KP, NT, WHOLE> tk, tq;
@@ -499,26 +525,23 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
       phase();
       fetch_v(p0 + C);
       f32x16 acc[NB] = {};
-      // a state near the end of fp16 takes part smaller: scaled and back in place, or (128 registers of it: the branch
-      // spilled 165) as it is packed
-      constexpr bool ONCE = O::kNarrow && KP <= 128, PACKED = O::kNarrow && KP > 128;
-      bool small = false;
-      if constexpr (O::kNarrow) small = near_end(largest<KB * 16>(Sf));
-      if (ONCE && small) scale<KB * 16>(Sf, kSmaller);
-      const float by = PACKED && small ? kSmaller : 1.f;
+      // fp16: the wavefront's columns of S lifted together, by one power of two, which leaves again with o's factors (one of
+      // each column's own would stand in the rows of o: 16 registers and 32 products more, 8% of the launch)
+      float up = 1.f, back = 1.f;
+      if constexpr (O::kNarrow) {
+        smax = exponent_of(largest<KB * 16>(Sf)) - ex;
+        const int n = min(15 - wave_max(smax), 120);
+        up = two_to(min(n - ex, 120));
+        back = two_to(-n);
+      }
 #pragma unroll
       for (int s = 0; s < KP / 16; ++s) {
         float t[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = PACKED ? Sf[s * 8 + e] * by : Sf[s * 8 + e];
+        for (int e = 0; e < 8; ++e) t[e] = O::kNarrow ? Sf[s * 8 + e] * up : Sf[s * 8 + e];
         const Frag sf = O::pack(t);
 #pragma unroll
         for (int ib = 0; ib < NB; ++ib) acc[ib] = O::mma(sf, O::rows(sq + (ib * 32 + col) * RK + s * 16, half, PK), acc[ib]);
-      }
-      if (O::kNarrow && small) {
-        if constexpr (ONCE) scale<KB * 16>(Sf, 1.f / kSmaller);
-#pragma unroll
-        for (int ib = 0; ib < NB; ++ib) scale<16>(reinterpret_cast<float*>(&acc[ib]), 1.f / kSmaller);
       }
       __syncthreads();  // the scores are there, and q has been read
       fetch_q(p0 + C);
@@ -553,7 +576,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
         };
         if (ib > 0 && shift < 32) {  // the state and the block before by way of its last token: g^{i+1} = g^{32} g^{col+1}
           if constexpr (O::kNarrow) {
-            scale<16>(af, power(lam2, 32 - early - shift) * gcol);
+            scale<16>(af, power(lam2, 32 - early - shift) * gcol * back);
             add(0, gcol);
           } else {
             scale<16>(af, power(lam2, 32 - early - shift));
@@ -561,7 +584,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
             scale<16>(af, gcol);
           }
         } else {
-          scale<16>(af, P.so * power(lam2, max(ib * 32 + col + 1 - early - shift, 0)));
+          scale<16>(af, P.so * power(lam2, max(ib * 32 + col + 1 - early - shift, 0)) * back);
         }
         add(ib, 1.f);
 #pragma unroll
@@ -594,11 +617,25 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
     }
 
     phase();
-    // S <- g^cl S + k^T (skv g^{C-1-row} v)
-    scale<KB * 16>(Sf, cl == C && !early ? gC : power(lam2, cl - early));
+    // S <- g^cl S + k^T (skv g^{C-1-row} v).  In fp16 S is held times 2^ex, each column by itself, so that the chunk's
+    // weighted v come between 2^14 and 2^15 (by a bound of each 16 tokens, which weights below it only lower by g^15)
+    float lift = 1.f;
+    if constexpr (O::kNarrow) {
+      float m = 0.f, g = skv_top;
+#pragma unroll
+      for (int s = C / 16 - 1; s >= 0; --s, g *= g1)
+        m = fmaxf(m, largest16(O::template cols<false>(sv + s * 16 * RV + wv * 32, RV, lane, PV)) * g);
+      // S itself stays within float32: a large one asks for no more of v
+      const int n = min(min(lift_of(pair_max(m)), 64), 100 - smax);
+      scale<KB * 16>(Sf, power(lam2, cl - early) * two_to(n - ex));
+      lift = two_to(n);
+      ex = n;
+    } else {
+      scale<KB * 16>(Sf, cl == C && !early ? gC : power(lam2, cl - early));
+    }
 #pragma unroll
     for (int s = 0; s < C / 16; ++s) {
-      float t[8], g = 1.f;  // g^{C-16-16s}
+      float t[8], g = lift;  // g^{C-16-16s}
 #pragma unroll
       for (int i = s + 1; i < C / 16; ++i) g *= g1;
       O::unpack(O::template cols<false>(sv + s * 16 * RV + wv * 32, RV, lane, PV), t);
@@ -632,7 +669,8 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   // the final state of a head in one segment, or the segment's own
   float* to = STATES ? states : states ? nullptr : P.s_out ? P.s_out + sbase : nullptr;
   if (to) {
-    const float g = !STATES && P.rev && len > 0 ? power(lam2, 1) : 1.f;
+    float g = !STATES && P.rev && len > 0 ? power(lam2, 1) : 1.f;
+    if constexpr (O::kNarrow) g *= two_to(-ex);
     const rsrc_t rs = make_rsrc_wave(to, srange);
     // opaque to the compiler, which would otherwise keep the offsets of the first
     // state's loads in registers through the whole segment (100 spilled registers)

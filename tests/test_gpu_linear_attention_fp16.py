@@ -108,6 +108,91 @@ def test_small_scores(size):
         _compare(got[name], want[name], E[name], f, f"{name}, by token", c=2, dim=-1)
 
 
+# ------------------------------------------------------------------- states
+@pytest.mark.parametrize("q_size,lo,hi", [(1e3, -6, 0), (3e-3, -0.5, 5.5)], ids=["small", "large"])
+@pytest.mark.parametrize("K,V", [(64, 64), (128, 128), (200, 72), (33, 31)])
+def test_columns_of_the_state_of_many_sizes(K, V, q_size, lo, hi):
+    """o = q S for a state whose columns lie anywhere from below fp16's bits to past its end, 2^20 apart."""
+    g = gen(42 + K)
+    B, H, T = 1, 3, 64
+    sizes = 10.0 ** torch.linspace(lo, hi, V)[torch.randperm(V, generator=g)]
+    S0 = randn(g, B, H, K, V) * sizes
+    q, k, v, do = q_size * randn(g, B, H, T, K), randn(g, B, H, T, K), torch.zeros(B, H, T, V), randn(g, B, H, T, V)
+    got, want, E, f = _run(*(t.to(HF) for t in (q, k, v, do)), LAM, K**-0.5, S0, torch.zeros_like(S0))
+    assert want["o"].abs().max() < 65504
+    _compare(got["o"], want["o"], E["o"], f, "o, by column", c=2, dim=-2)
+    # dk = dS v: dS of all sizes by its rows, which are dk's channels
+    rows = 10.0 ** torch.linspace(lo, hi, K)[:, None]
+    got, want, E, f = _run(*(t.to(HF) for t in (q, k, q_size * do, 0 * do)), LAM, K**-0.5, torch.zeros_like(S0),
+                           randn(g, B, H, K, V) * rows)
+    assert want["dk"].abs().max() < 65504
+    _compare(got["dk"], want["dk"], E["dk"], f, "dk, by column", c=2, dim=-2)
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("T", [40, 300, 1500])
+@pytest.mark.parametrize("K,V", [(64, 64), (128, 128), (200, 40), (100, 100)])
+def test_small_gradients(K, V, T, size):
+    """o's gradient as it is without a loss scale: every gradient, and the initial state's in float32."""
+    g = gen(43 + K)
+    B, H = 1, 3
+    q, k, v, do = (randn(g, B, H, T, c) for c in (K, K, V, V))
+    S0, dS = randn(g, B, H, K, V), size * randn(g, B, H, K, V)
+    got, want, E, f = _run(*(t.to(HF) for t in (q, k, v, size * do)), LAM, K**-0.5, S0, dS)
+    for name in ("o", "dq", "dk", "dv"):
+        _compare(got[name], want[name], E[name], f, name)
+    _compare_state(got["state"], want["state"], E["state"], f, "state")
+    _compare_state(got["dinitial"], want["dinitial"], E["dinitial"], f, "dinitial")
+
+
+@pytest.mark.parametrize("size", [1e-3, 1e-5])
+@pytest.mark.parametrize("T", [40, 300, 1500])
+def test_small_values(T, size):
+    """v small, and some of its columns smaller still: o, and the state by column, which is float32."""
+    g = gen(44)
+    B, H, K, V = 2, 3, 64, 96
+    q, k, v, do = (randn(g, B, H, T, c) for c in (K, K, V, V))
+    sizes = torch.where(torch.arange(V) % 3 == 0, size, 1.0)
+    got, want, E, f = _run(*(t.to(HF) for t in (q, k, v * size, do)), LAM, K**-0.5)
+    _compare(got["o"], want["o"], E["o"], f, "o")
+    _compare(got["dq"], want["dq"], E["dq"], f, "dq")
+    _compare_state(got["state"], want["state"], E["state"], f, "state")
+    got, want, E, f = _run(*(t.to(HF) for t in (q, k, v * sizes, do)), LAM, K**-0.5)
+    _compare(got["o"], want["o"], E["o"], f, "o, by column", c=2, dim=-2)
+    for n in range(0, V, 7):
+        _compare_state(got["state"][..., n], want["state"][..., n], E["state"][..., n], f, f"state, column {n}")
+
+
+@pytest.mark.parametrize("T", [40, 300, 1500])
+@pytest.mark.parametrize("scale", [4.0, 300.0, -4.0])
+def test_scaled_values_past_the_type(T, scale):
+    """A scale above one and a loss-scaled gradient: their product passes the type, the gradients do not."""
+    g = gen(45)
+    B, H, K = 1, 3, 64
+    q, k, v, do = (randn(g, B, H, T, K) for _ in range(4))
+    small = 0.02 * abs(4.0 / scale) ** 0.5 * min(1.0, (300 / T) ** 0.5)
+    q, k, v, do = (t.to(HF) for t in (small * q, small * k, small * 1e-2 * v, (2e4 * do).clamp(-6e4, 6e4)))
+    assert do.double().abs().max() * abs(scale) > 2 * 65504
+    got, want, E, f = _run(q, k, v, do, LAM, scale, torch.zeros(B, H, K, K), torch.zeros(B, H, K, K))
+    for name in ("o", "dq", "dk", "dv"):
+        assert want[name].abs().max() < 65504
+        _compare(got[name], want[name], E[name], f, name)
+    _compare_state(got["dinitial"], want["dinitial"], E["dinitial"], f, "dinitial")
+
+
+def test_values_and_decays_far_apart():
+    """Chunks whose values are far larger or smaller than those before, under decays that leave either, and zeros."""
+    g = gen(46)
+    B, H, T, K = 1, 4, 512, 64
+    lam = torch.tensor([0.0, -0.01, -0.7, -float("inf")])
+    q, k, v, do = (randn(g, B, H, T, K) for _ in range(4))
+    sizes = torch.tensor([1e-4, 1e3, 0.0, 1e-2, 1.0, 3e-5, 1e2, 0.0]).repeat_interleave(64)[:, None]
+    got, want, E, f = _run(*(t.to(HF) for t in (q, k, v * sizes, do)), lam, K**-0.5)
+    _compare(got["o"], want["o"], E["o"], f, "o, by token", c=2, dim=-1)
+    for h in range(H):
+        _compare_state(got["state"][:, h], want["state"][:, h], E["state"][:, h], f, f"state of head {h}")
+
+
 @pytest.mark.parametrize("T", [1, 2, 31, 32, 33, 63, 64, 65, 127, 130, 300])
 def test_lengths(T):
     _check(2, 3, T, 64, 64, HF)
