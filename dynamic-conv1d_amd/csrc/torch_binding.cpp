@@ -90,6 +90,11 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor bytes_like(const Tensor& t, int64_t n) {
   return n > 0 ? at::empty({n}, t.options().dtype(at::kByte)) : Tensor();
 }
+// A kernel has written t through its pointer: what autograd has saved of it is stale, as after torch's in-place operations
+// (tensors of inference mode have no version, and are not saved).
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 // A gradient as the kernels read it: contiguous, in x's dtype.
 Tensor grad_in(const Tensor& dy, at::ScalarType dtype) { return dy.contiguous().to(dtype); }
 
@@ -627,6 +632,7 @@ PyObject* py_linear_attention_step(PyObject*, PyObject* const* args, Py_ssize_t 
                                     static_cast<int32_t*>(ptr(slots)), ptr(o), B, H, K, V, state.size(0), (float)scale,
                                     dtype_code(q), stream_of(q)),
           "linear attention step");
+    written(state);
   }
   return THPVariable_Wrap(std::move(o));
   END_HANDLE_TH_ERRORS
@@ -710,6 +716,7 @@ PyObject* py_lowrank_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                    static_cast<int32_t*>(ptr(slots)), yp, N, D, R, W, state.size(0), dtype_code(x),
                                    residual != 0, stream_of(x)),
           "lowrank step");
+    written(state);
   }
   return wrap_all(std::move(ys));
   END_HANDLE_TH_ERRORS

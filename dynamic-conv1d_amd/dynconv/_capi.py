@@ -147,6 +147,13 @@ def ptr_array(ts):
     return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
 
 
+def written(t):
+    """A kernel has written t through its pointer: what autograd has saved of it is stale, as after torch's in-place
+    operations (tensors of inference mode have no version, and are not saved)."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def int64_array(values):
     """A host array of int64 (a `const int64_t*` argument)."""
     return (ctypes.c_int64 * len(values))(*values)

@@ -176,7 +176,8 @@ def linear_attention_step(
                    the cache (-1) mark sequences that take no part: their outputs are zero.  None: row b.
 
     Returns:
-        o [B, H, V] in q's dtype.  Serving only: no gradients.
+        o [B, H, V] in q's dtype.  Serving only: no gradients; a backward that has saved `state` from before raises, as
+        after torch's own in-place operations.
     """
     if _capi.binding is not None:
         o = _capi.binding.linear_attention_step(q, k, v, log_decay, state, scale, slots)
@@ -213,4 +214,5 @@ def _step(q, k, v, log_decay, state, slots, scale, dtype):
         _capi.ptr(log_decay), _capi.ptr(state), _capi.ptr(slots), _capi.ptr(o), B, H, K, V, state.shape[0], scale,
         dtype, _capi.stream_of(q))
     _capi.check(status, "linear attention step")
+    _capi.written(state)
     return o

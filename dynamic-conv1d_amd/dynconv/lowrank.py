@@ -281,6 +281,7 @@ def _step_grouped(x, z, U, state, static_w, residual, slots, W):
         _capi.ptr(state), _capi.ptr(slots), _capi.ptr_array(ys), N, D, z[0].shape[-1], W, state.shape[0],
         _capi.dtype_code(x.dtype), int(bool(residual)), _capi.stream_of(x))
     _capi.check(status, "lowrank step")
+    _capi.written(state)
     return ys
 
 
@@ -306,7 +307,8 @@ def lowrank_dynamic_convolution_step_grouped(
 
     Returns:
         a tuple of G tensors [N, D]: row t of what the whole-sequence operator gives for the sequence so far.
-        Serving only: no gradients.
+        Serving only: no gradients; a backward that has saved `state` from before raises, as after torch's own in-place
+        operations.
     """
     z, U = list(z), list(U)
     static_w = None if static_w is None else list(static_w)
