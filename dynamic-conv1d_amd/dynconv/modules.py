@@ -230,7 +230,8 @@ class DynamicLinearAttention(nn.Module):
         """States of sequences without a token yet."""
         w = self.c_attn.weight
         return LayerState(torch.zeros(rows, self.W - 1, 3 * self.d_model, dtype=w.dtype, device=w.device),
-                          torch.zeros(rows, self.heads, self.head_dim, self.head_dim, device=w.device))
+                          torch.zeros(rows, self.heads, self.head_dim, self.head_dim, dtype=torch.float32,
+                                      device=w.device))
 
     def _norm(self, o, gate):
         return group_norm(o, self.heads, weight=self.norm_weight, bias=self.norm_bias, gate=gate, eps=self.eps)
