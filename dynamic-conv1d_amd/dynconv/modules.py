@@ -213,17 +213,18 @@ class DynamicLinearAttention(nn.Module):
         self.norm_bias = nn.Parameter(torch.zeros(d_model))
         self.c_gate = nn.Linear(d_model, d_model, bias=False)
         self.c_proj = nn.Linear(d_model, d_model, bias=False)
-        self.register_buffer("log_decay", self._log_decay(), persistent=False)
+        self.register_buffer("log_decay", self._log_decay(self.c_attn.weight.device), persistent=False)
 
-    def _log_decay(self):
-        u = 5 + 7 * torch.arange(self.heads, dtype=torch.float64) / max(self.heads - 1, 1)
-        return torch.log1p(-torch.exp2(-u)).to(torch.float32)
+    def _log_decay(self, device):
+        u = 5 + 7 * torch.arange(self.heads, dtype=torch.float64, device="cpu") / max(self.heads - 1, 1)
+        return torch.log1p(-torch.exp2(-u)).to(device=device, dtype=torch.float32)
 
     def _apply(self, fn, recurse=True):
+        old = self.log_decay
         super()._apply(fn, recurse)
-        # .to(bfloat16) and its like leave the decays as they are
-        if self.log_decay.dtype != torch.float32:
-            self.log_decay = self._log_decay().to(self.log_decay.device)
+        # .to(bfloat16) and its like leave the decays as they are, and so does to_empty, whose memory holds anything
+        device = self.log_decay.device
+        self.log_decay = self._log_decay(device) if old.is_meta else old.to(device)
         return self
 
     def new_state(self, rows: int) -> LayerState:
