@@ -147,6 +147,12 @@ def ptr_array(ts):
     return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
 
 
+def differentiated(ts) -> bool:
+    """Whether a gradient or a tangent (forward mode) is asked for through any of ts."""
+    return ((torch.is_grad_enabled() and any(t.requires_grad for t in ts))
+            or any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in ts))
+
+
 def written(t):
     """A kernel has written t through its pointer: what autograd has saved of it is stale, as after torch's in-place
     operations (tensors of inference mode have no version, and are not saved)."""

@@ -191,8 +191,8 @@ def linear_attention_step(
     dtype = _capi.dtype_code(q.dtype)
     V = v.shape[-1]
     assert B > 0 and H > 0 and 0 < K <= MAX_DIM and 0 < V <= MAX_DIM, "head dims must be between 1 and 256"
-    assert not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state))), \
-        "linear_attention_step has no gradient: call it under torch.no_grad()"
+    assert not _capi.differentiated((q, k, v, log_decay, state)), \
+        "linear_attention_step has no gradient and no tangent: call it under torch.no_grad(), without dual tensors"
     _check_decay(log_decay, H, q.device)
     assert state.device == q.device and state.dtype == torch.float32 and state.is_contiguous(), \
         "state must be contiguous float32 on q's device"

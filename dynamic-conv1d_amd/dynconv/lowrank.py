@@ -330,8 +330,8 @@ def lowrank_dynamic_convolution_step_grouped(
     tensors = [*z, *U, state] + ([] if static_w is None else static_w)
     assert all(t.device == x.device and t.is_contiguous() for t in tensors), "contiguous tensors on x's device"
     assert all(t.dtype == x.dtype for t in tensors), "x, z, U, static_w and state must share one dtype"
-    assert not (torch.is_grad_enabled() and any(t.requires_grad for t in [x, *tensors])), \
-        "the step has no gradient: call it under torch.no_grad()"
+    assert not _capi.differentiated([x, *tensors]), \
+        "the step has no gradient and no tangent: call it under torch.no_grad(), without dual tensors"
     for g in range(G):
         assert tuple(z[g].shape) == (N, R), "every z must be [N, R]"
         assert U[g].dim() == 2 and tuple(U[g].shape) == (R, W * D) and W > 0, "every U must be [R, W*D]"

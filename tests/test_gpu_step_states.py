@@ -75,3 +75,27 @@ def test_states_of_inference_mode_are_taken(path):
         assert torch.equal(S, S2)
         linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], lam, S)
         lowrank_dynamic_convolution_step(x, z, U, state)
+
+
+def test_a_forward_mode_tangent_is_refused(path):
+    """The steps have none: taken for a plain tensor, a dual tensor would lose it."""
+    fw = torch.autograd.forward_ad
+    q, k, v, lam, S = _attention(gen(6))
+    args = [q[:, :, 0], k[:, :, 0], v[:, :, 0], lam, S]
+    before = S.clone()
+    x, z, U, state = _conv(gen(7))
+    conv, past = [x, z, U, state], state.clone()
+    with torch.no_grad(), fw.dual_level():
+        for i in range(5):
+            dual = [fw.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(args)]
+            with pytest.raises(AssertionError):
+                linear_attention_step(*dual)
+        for i in range(4):
+            dual = [fw.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(conv)]
+            with pytest.raises(AssertionError):
+                lowrank_dynamic_convolution_step(*dual)
+        assert torch.equal(S, before) and torch.equal(state, past)
+        linear_attention_step(*args)
+        lowrank_dynamic_convolution_step(*conv)
+    with torch.no_grad(), pytest.raises((AssertionError, RuntimeError)):
+        torch.func.jvp(lambda t: linear_attention_step(t, *args[1:]), (args[0],), (torch.ones_like(args[0]),))
