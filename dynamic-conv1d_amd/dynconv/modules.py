@@ -30,7 +30,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import _capi
-from .linattn import linear_attention, linear_attention_step
+from .linattn import MAX_DIM, linear_attention, linear_attention_step
 from .lowrank import (lowrank_dynamic_convolution, lowrank_dynamic_convolution_grouped,
                       lowrank_dynamic_convolution_step_grouped)
 from .norm import group_norm
@@ -206,6 +206,8 @@ class DynamicLinearAttention(nn.Module):
         super().__init__()
         if heads <= 0 or d_model % heads != 0:
             raise ValueError("heads must divide d_model")
+        if d_model // heads > MAX_DIM:
+            raise ValueError(f"linear attention's heads have at most {MAX_DIM} channels")
         self.d_model, self.heads, self.head_dim, self.W, self.eps = d_model, heads, d_model // heads, W, eps
         self.c_attn = nn.Linear(d_model, 3 * d_model, bias=False)
         self.conv = GroupedLowRankDynamicShortConvolution(d_model, R, W, groups=3, head_dim=self.head_dim)

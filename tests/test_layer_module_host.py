@@ -45,3 +45,9 @@ def test_decays_follow_the_module():
         m = move(m)
         assert m.log_decay.dtype == torch.float32 and torch.equal(m.log_decay, want)
     assert m.to("meta").log_decay.is_meta
+
+
+def test_head_dims_past_the_operator_are_refused_when_built():
+    with pytest.raises(ValueError):
+        DynamicLinearAttention(1024, 2, 7, 4)  # 512 channels a head
+    assert DynamicLinearAttention(512, 2, 7, 4).head_dim == 256
