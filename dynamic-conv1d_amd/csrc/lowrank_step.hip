@@ -126,8 +126,10 @@ __global__ __launch_bounds__(256) void lr_step_mma(LrStep p) {
 #pragma unroll
   for (int i = 0; i < XP; ++i) {
     const int n = tid / PR + i * (256 / PR);
+    // zeros where a sequence takes no part: of its zeros, infinities and NaN in the filters make NaN
     if (in && n0 + n < p.N)
-      *reinterpret_cast<u32x4*>((T*)p.y[g] + (n0 + n) * D + d0 + c) = *reinterpret_cast<const u32x4*>(sx + n * RX + c);
+      *reinterpret_cast<u32x4*>((T*)p.y[g] + (n0 + n) * D + d0 + c) =
+          xr[i] ? *reinterpret_cast<const u32x4*>(sx + n * RX + c) : u32x4{0, 0, 0, 0};
   }
 }
 
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(256) void lr_step_taps(LrStep p) {
     for (int j = 0; j < VE; ++j) {
       const float* t = sy + row * RY + c + j;
       constexpr int next = kSeqs * RY;
-      v[j] = (t[0] + t[next]) + (t[2 * next] + t[3 * next]);
+      v[j] = xr ? (t[0] + t[next]) + (t[2 * next] + t[3 * next]) : 0.f;  // as in lr_step_mma
     }
     store_vals<T, VE>((T*)p.y[g] + n * D + d0 + c, v);
   }

@@ -189,3 +189,18 @@ def test_refusals():
         with pytest.raises(AssertionError):
             f()
             pytest.fail(f"call {i} was taken")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("D", [128, 33, 25088])
+def test_sequences_that_take_no_part_are_zero_whatever_the_filters_hold(D, dtype):
+    x, z, U, sw, state = _inputs(gen(37), 1, 5, D, 7, 3, True, 5, dtype)
+    U[0][3] = float("inf")
+    U[0][5, ::2] = float("nan")
+    sw[0][1] = float("-inf")
+    before = state.clone()
+    ids = torch.tensor([0, 1, -1, 3, 5], dtype=torch.int32, device=DEV)
+    dstate = _dev(state)
+    y, = lowrank_dynamic_convolution_step_grouped(_dev(x), _dev(z), _dev(U), dstate, static_w=_dev(sw), slots=ids)
+    assert (y[[2, 4]] == 0).all() and not y[[0, 1, 3]].isfinite().any()
+    assert torch.equal(dstate[[2, 4]].cpu(), before[[2, 4]])
