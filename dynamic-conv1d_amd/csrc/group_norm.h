@@ -36,6 +36,7 @@ struct GnArgs {
   float *pw, *pb;  // partial sums of dw and db, [row blocks][D] each (null: not wanted)
   int64_t M, D;
   int size, lanes;  // channels of a group, lanes it takes (a power of two)
+  int64_t gx0;      // first block of groups of a launch
   bool wide_params;   // weight and bias are float32 (else of x's type)
   bool param_pieces;  // and 16-byte aligned
   float eps;
@@ -90,7 +91,7 @@ struct Lane {
   __device__ __forceinline__ Lane(const GnArgs& A) {
     // a group of more lanes than a wavefront's has the workgroup
     const int lane = A.lanes > 64 ? threadIdx.x : threadIdx.x % 64, gl = lane & (A.lanes - 1);
-    const int64_t group = (int64_t)blockIdx.x * (A.lanes > 64 ? 1 : 64 / A.lanes) + lane / A.lanes;
+    const int64_t group = (A.gx0 + blockIdx.x) * (A.lanes > 64 ? 1 : 64 / A.lanes) + lane / A.lanes;
     step = A.lanes * VEC;
     ch = group * A.size + gl * VEC;
 #pragma unroll
@@ -309,10 +310,14 @@ struct Plan {
 };
 
 template <typename T, int VEC, int NV, bool WIDE>
-void launch(bool bwd, const GnArgs& a, const Plan& pl, hipStream_t st) {
-  const dim3 grid(pl.gx, (unsigned)pl.gy);
-  if (bwd) gn_bwd_kernel<T, VEC, NV, WIDE><<<grid, 64 * kWaves, 0, st>>>(a);
-  else gn_fwd_kernel<T, VEC, NV, WIDE><<<grid, 64 * kWaves, 0, st>>>(a);
+void launch(bool bwd, const GnArgs& args, const Plan& pl, hipStream_t st) {
+  constexpr int64_t most = most_workgroups(64 * kWaves);
+  GnArgs a = args;
+  for (a.gx0 = 0; a.gx0 < pl.gx; a.gx0 += most) {
+    const dim3 grid((unsigned)(pl.gx - a.gx0 < most ? pl.gx - a.gx0 : most), (unsigned)pl.gy);
+    if (bwd) gn_bwd_kernel<T, VEC, NV, WIDE><<<grid, 64 * kWaves, 0, st>>>(a);
+    else gn_fwd_kernel<T, VEC, NV, WIDE><<<grid, 64 * kWaves, 0, st>>>(a);
+  }
 }
 
 // A group of up to 128 pieces lies in one wavefront, a larger one (up to 4096 channels) in the workgroup.

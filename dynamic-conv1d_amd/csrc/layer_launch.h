@@ -9,6 +9,9 @@
 
 namespace dc {
 
+// Workgroups of one launch: a grid's work-items along an axis are counted in 32 bits.
+constexpr int64_t most_workgroups(int threads) { return 0xFFFFFFFFll / threads; }
+
 // ------------------------------------------------------- linear attention
 // One pass of the chunked operator over B x H sequences of one head each:
 //     S_t = g S_{t-1} + skv k_t^T v_t,    o_t = so q_t S_t
@@ -51,6 +54,7 @@ struct LaStep {
   const int32_t* slot_ids;
   void* o;
   int64_t B, H, K, V, slots;
+  int64_t bh0;  // first head of a launch (all of them: as many launches as it takes)
   float scale;
   int dtype;
   hipStream_t stream;

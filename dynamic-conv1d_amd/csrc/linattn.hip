@@ -152,14 +152,17 @@ hipError_t launch(const LaProblem& p, const Cut& c, float* const* states_of, boo
     }
     const int64_t nblk = p.B * p.H * c.nseg * a.nvb * a.nkb * a.npass;
     if (nblk > 0x7fffffff) return hipErrorInvalidValue;
-    a.nblk = (int)nblk;
-    hipError_t e;
-    switch (p.dtype) {
-      case kBF16: e = la::launch<bf16>(a, kp, nw, w, states, p.stream); break;
-      case kFP16: e = la::launch<fp16>(a, kp, nw, w, states, p.stream); break;
-      default: e = la::launch<float>(a, kp, nw, w, states, p.stream); break;
+    for (int64_t b0 = 0; b0 < nblk; b0 += most_workgroups(nw * 64)) {
+      a.blk0 = (int)b0;
+      a.nblk = (int)(nblk - b0 < most_workgroups(nw * 64) ? nblk - b0 : most_workgroups(nw * 64));
+      hipError_t e;
+      switch (p.dtype) {
+        case kBF16: e = la::launch<bf16>(a, kp, nw, w, states, p.stream); break;
+        case kFP16: e = la::launch<fp16>(a, kp, nw, w, states, p.stream); break;
+        default: e = la::launch<float>(a, kp, nw, w, states, p.stream); break;
+      }
+      if (e != hipSuccess) return e;
     }
-    if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }

@@ -68,7 +68,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 struct Args {
   LaProblem p;
   int npass, seg, nseg, nvb, nkb;
-  int nblk;
+  int blk0, nblk;  // workgroups of this launch, of all
   bool returned;  // a state formed by this launch is the caller's result
   // what a pass starts its segments from / a state pass writes: one set of states (null: one segment, s_in / s_out)
   float* states[kLaMaxPasses];
@@ -347,7 +347,7 @@ __device__ __forceinline__ int wave_max(int e) {
   return max(max(__builtin_amdgcn_readlane(e, 0), __builtin_amdgcn_readlane(e, 16)),
              max(__builtin_amdgcn_readlane(e, 32), __builtin_amdgcn_readlane(e, 48)));
 }
-// The largest magnitude of a lane's 16 fp16 values of two steps' halves, as bits of fp16 (a NaN's are the largest).
+// The largest magnitude of a lane's 8 fp16 values (NaN where one is).
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float largest16(u32x4 f) {
   u16x2 m = {0, 0};
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
   __shared__ float sback[O::kNarrow && !STATES ? NP * 32 : 1];
 
   // the passes of one segment run side by side: what one reads, the others find in the last-level cache
-  int blk = xcd_remap(blockIdx.x, A.nblk);
+  int blk = A.blk0 + xcd_remap(blockIdx.x, A.nblk);
   const int vb = blk % A.nvb;
   blk /= A.nvb;
   const int k0 = STATES ? blk % A.nkb * KP : 0;  // first row of the state

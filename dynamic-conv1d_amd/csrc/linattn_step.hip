@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStep p) {
   typedef float vec __attribute__((ext_vector_type(VEC)));
   __shared__ vec red[4][kLanes];
   const int nv = (int)((p.V + kLanes * VEC - 1) / (kLanes * VEC));
-  const int64_t bh = blockIdx.x / nv;
+  const int64_t bh = p.bh0 + blockIdx.x / nv;
   const int64_t b = bh / p.H, h = bh % p.H;
   const int lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
   const int64_t col = ((int64_t)(blockIdx.x % nv) * kLanes + lane) * VEC;
@@ -77,14 +77,15 @@ __global__ __launch_bounds__(256) void la_step_kernel(LaStep p) {
 
 template <typename T, int VEC>
 hipError_t launch(const LaStep& p) {
-  const int64_t nv = (p.V + kLanes * VEC - 1) / (kLanes * VEC);
-  const int64_t blocks = p.B * p.H * nv;  // within 2^31: the ABI bounds B * H, and nv is at most 32
-  const dim3 grid((unsigned)blocks);
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  if (p.K <= 32) la_step_kernel<T, VEC, 1><<<grid, 256, 0, p.stream>>>(p);
-  else if (p.K <= 64) la_step_kernel<T, VEC, 2><<<grid, 256, 0, p.stream>>>(p);
-  else if (p.K <= 128) la_step_kernel<T, VEC, 4><<<grid, 256, 0, p.stream>>>(p);
-  else la_step_kernel<T, VEC, 8><<<grid, 256, 0, p.stream>>>(p);
+  const int64_t nv = (p.V + kLanes * VEC - 1) / (kLanes * VEC), heads = p.B * p.H, per = most_workgroups(256) / nv;
+  LaStep q = p;
+  for (q.bh0 = 0; q.bh0 < heads; q.bh0 += per) {
+    const dim3 grid((unsigned)((heads - q.bh0 < per ? heads - q.bh0 : per) * nv));
+    if (p.K <= 32) la_step_kernel<T, VEC, 1><<<grid, 256, 0, p.stream>>>(q);
+    else if (p.K <= 64) la_step_kernel<T, VEC, 2><<<grid, 256, 0, p.stream>>>(q);
+    else if (p.K <= 128) la_step_kernel<T, VEC, 4><<<grid, 256, 0, p.stream>>>(q);
+    else la_step_kernel<T, VEC, 8><<<grid, 256, 0, p.stream>>>(q);
+  }
   return hipGetLastError();
 }
 
