@@ -318,17 +318,17 @@ struct LinearAttentionFn : public Function<LinearAttentionFn> {
                                const std::optional<Tensor>& s0, const Tensor& lam, const std::optional<Tensor>& lengths,
                                double scale, bool want_state) {
     const Tensor s = s0.value_or(Tensor()), n = lengths.value_or(Tensor());
-    Tensor states;  // before each segment: the backward starts from them (an internal buffer, a function of the inputs)
+    Tensor states;  // before each segment, a function of the inputs: the backward starts from them
     variable_list out = run(q, k, v, lam, s, n, scale, want_state, &states);
-    if (states.defined()) ctx->saved_data["states"] = states;
-    ctx->save_for_backward({q, k, v, s, lam, n});
+    ctx->save_for_backward({q, k, v, s, lam, n, states});
     ctx->saved_data["scale"] = scale;
     ctx->set_materialize_grads(false);
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &s0 = saved[3], &lam = saved[4], &lengths = saved[5];
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &s0 = saved[3], &lam = saved[4], &lengths = saved[5],
+                 &states = saved[6];
     const c10::DeviceGuard guard(q.device());
     const int64_t B = q.size(0), H = q.size(1), T = q.size(2), K = q.size(3), V = v.size(3);
     const int dt = dtype_code(q);
@@ -341,8 +341,6 @@ struct LinearAttentionFn : public Function<LinearAttentionFn> {
     const int64_t n = abi.linear_attention_ws_bytes(B, H, T, K, V, dt, 1);
     check(n, "linear attention backward workspace query");
     const Tensor ws = bytes_like(q, n);
-    const auto it = ctx->saved_data.find("states");
-    const Tensor states = it != ctx->saved_data.end() ? it->second.toTensor() : Tensor();
     check(abi.linear_attention_bwd(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(),
                                    static_cast<float*>(ptr(lam)), static_cast<float*>(ptr(s0)),
                                    static_cast<int32_t*>(ptr(lengths)), ptr(d), d.strides().data(),

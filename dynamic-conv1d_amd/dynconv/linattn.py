@@ -54,16 +54,16 @@ class _LinearAttentionFn(torch.autograd.Function):
             _capi.ptr(log_decay), _capi.ptr(initial), _capi.ptr(lengths), _capi.ptr(o), _strides(o, 3),
             _capi.ptr(state), _capi.ptr(ws), nws, B, H, T, K, V, scale, dtype, _capi.stream_of(q))
         _capi.check(status, "linear attention forward")
-        ctx.save_for_backward(q, k, v, initial, log_decay, lengths)
+        # ws: the states before each segment, a function of the inputs, which the backward starts from
+        ctx.save_for_backward(q, k, v, initial, log_decay, lengths, ws)
         ctx.scale = scale
-        ctx.states = ws  # the states before each segment, a function of the inputs: the backward starts from them
         ctx.set_materialize_grads(False)
         return (o, state) if return_state else o
 
     @staticmethod
     @_capi.on_tensor_device
     def backward(ctx, do, dstate=None):
-        q, k, v, initial, log_decay, lengths = ctx.saved_tensors
+        q, k, v, initial, log_decay, lengths, states = ctx.saved_tensors
         B, H, T, K = q.shape
         V = v.shape[-1]
         # an output that did not reach the loss has no gradient
@@ -80,7 +80,7 @@ class _LinearAttentionFn(torch.autograd.Function):
             _capi.ptr(q), _strides(q, 3), _capi.ptr(k), _strides(k, 3), _capi.ptr(v), _strides(v, 3),
             _capi.ptr(log_decay), _capi.ptr(initial), _capi.ptr(lengths), _capi.ptr(do), _strides(do, 3),
             _capi.ptr(dstate), _capi.ptr(dq), _strides(dq, 3), _capi.ptr(dk), _strides(dk, 3), _capi.ptr(dv),
-            _strides(dv, 3), _capi.ptr(dinitial), _capi.ptr(ctx.states), _capi.ptr(ws), nws, B, H, T, K, V, ctx.scale, dtype,
+            _strides(dv, 3), _capi.ptr(dinitial), _capi.ptr(states), _capi.ptr(ws), nws, B, H, T, K, V, ctx.scale, dtype,
             _capi.stream_of(q))
         _capi.check(status, "linear attention backward")
         return dq, dk, dv, dinitial, None, None, None, None
