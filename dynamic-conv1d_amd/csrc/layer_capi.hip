@@ -49,7 +49,7 @@ int64_t dc_linear_attention_ws_bytes(int64_t B, int64_t H, int64_t T, int64_t K,
     p.pass[i].K = (int)(turned ? V : K);
     p.pass[i].V = (int)(turned ? K : V);
   }
-  return dc::la_ws_bytes(p);
+  return dc::la_ws_bytes(p, bwd == 2);
 }
 
 int dc_linear_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -78,7 +78,7 @@ int dc_linear_attention_fwd(const void* q, const int64_t* q_strides, const void*
   p.npass = 1;
   p.log_decay = log_decay; p.lengths = lengths;
   p.B = B; p.H = H; p.T = T; p.dtype = dtype;
-  p.ws = workspace; p.ws_bytes = ws_bytes; p.stream = (hipStream_t)stream;
+  p.ws = workspace; p.stream = (hipStream_t)stream;
   return launch_status(dc::la_run(p));
 }
 
@@ -90,7 +90,7 @@ int dc_linear_attention_bwd(const void* q, const int64_t* q_strides, const void*
                             const int64_t* dv_strides, float* d_initial_state, const void* fwd_workspace,
                             void* workspace, int64_t ws_bytes, int64_t B, int64_t H, int64_t T, int64_t K, int64_t V, float scale, int dtype,
                             void* stream) {
-  const int64_t need = dc_linear_attention_ws_bytes(B, H, T, K, V, dtype, 1);
+  const int64_t need = dc_linear_attention_ws_bytes(B, H, T, K, V, dtype, fwd_workspace ? 2 : 1);
   if (need < 0) return (int)need;
   if (!log_decay || (T > 0 && (!q || !k || !v || !d_o || !dq || !dk || !dv))) return DC_ERR_NULL;
   const int es = dc::dtype_size(dtype);
@@ -128,7 +128,7 @@ int dc_linear_attention_bwd(const void* q, const int64_t* q_strides, const void*
   p.fwd_states = static_cast<const float*>(fwd_workspace);
   p.log_decay = log_decay; p.lengths = lengths;
   p.B = B; p.H = H; p.T = T; p.dtype = dtype;
-  p.ws = workspace; p.ws_bytes = ws_bytes; p.stream = (hipStream_t)stream;
+  p.ws = workspace; p.stream = (hipStream_t)stream;
   return launch_status(dc::la_run(p));
 }
 

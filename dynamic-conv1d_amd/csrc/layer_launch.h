@@ -39,11 +39,10 @@ struct LaProblem {
   int64_t B, H, T;
   int dtype;
   void* ws;
-  int64_t ws_bytes;
   const float* fwd_states;  // backward: the states before each segment that the forward left in its workspace (null: none)
   hipStream_t stream;
 };
-int64_t la_ws_bytes(const LaProblem& p);
+int64_t la_ws_bytes(const LaProblem& p, bool fwd_states);  // fwd_states: whether the backward will be given them
 hipError_t la_run(const LaProblem& p);
 
 struct LaStep {

@@ -170,11 +170,11 @@ hipError_t launch(const LaProblem& p, const Cut& c, float* const* states_of, boo
 }  // namespace
 
 // Sets of states before each segment: the forward's one, and for the backward dv's, that dk shares, behind dq's, which is
-// the forward's where the caller has kept it.
-int64_t la_ws_bytes(const LaProblem& p) {
+// the forward's, in its workspace, where the caller has kept it.
+int64_t la_ws_bytes(const LaProblem& p, bool fwd_states) {
   const Cut c = cut_of(p);
   if (c.nseg == 1) return 0;
-  return (p.npass == 3 ? 2 : 1) * p.B * p.H * c.nseg * (int64_t)p.pass[0].K * p.pass[0].V * (int64_t)sizeof(float);
+  return (p.npass == 3 && !fwd_states ? 2 : 1) * p.B * p.H * c.nseg * (int64_t)p.pass[0].K * p.pass[0].V * (int64_t)sizeof(float);
 }
 
 hipError_t la_run(const LaProblem& p) {
@@ -185,7 +185,7 @@ hipError_t la_run(const LaProblem& p) {
     float* ws = static_cast<float*>(p.ws);
     of[0] = ws;
     if (p.npass == 3) {
-      of[1] = of[2] = ws + p.B * p.H * c.nseg * n;
+      of[1] = of[2] = p.fwd_states ? ws : ws + p.B * p.H * c.nseg * n;
       if (p.fwd_states) of[0] = const_cast<float*>(p.fwd_states);
     }
     // the passes that form states, and where

@@ -338,7 +338,7 @@ struct LinearAttentionFn : public Function<LinearAttentionFn> {
     const Tensor ds = grads.size() > 1 && grads[1].defined() ? grad_in(grads[1], at::kFloat) : Tensor();
     Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
     Tensor ds0 = s0.defined() && ctx->needs_input_grad(3) ? at::empty_like(s0) : Tensor();
-    const int64_t n = abi.linear_attention_ws_bytes(B, H, T, K, V, dt, 1);
+    const int64_t n = abi.linear_attention_ws_bytes(B, H, T, K, V, dt, states.defined() ? 2 : 1);
     check(n, "linear attention backward workspace query");
     const Tensor ws = bytes_like(q, n);
     check(abi.linear_attention_bwd(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(),

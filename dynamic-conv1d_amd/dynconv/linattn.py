@@ -73,7 +73,7 @@ class _LinearAttentionFn(torch.autograd.Function):
         dinitial = torch.empty_like(initial) if initial is not None and ctx.needs_input_grad[3] else None
         lib = _capi.load()
         dtype = _capi.dtype_code(q.dtype)
-        nws = lib.dc_linear_attention_ws_bytes(B, H, T, K, V, dtype, 1)
+        nws = lib.dc_linear_attention_ws_bytes(B, H, T, K, V, dtype, 1 if states is None else 2)
         _capi.check(int(nws) if nws < 0 else 0, "linear attention backward workspace query")
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws > 0 else None
         status = lib.dc_linear_attention_bwd(

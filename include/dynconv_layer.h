@@ -37,7 +37,8 @@ extern "C" {
  *   tokens; rows past them are not used, whatever they hold, their outputs are
  *   zero and the state is the one after the last token.
  * T may be 0.  Both calls need a workspace of dc_linear_attention_ws_bytes
- * bytes (0: none), 16-byte aligned. */
+ * bytes (0: none), 16-byte aligned; bwd: 0 the forward, 1 the backward, 2 the
+ * backward that is given the forward's workspace. */
 int64_t dc_linear_attention_ws_bytes(int64_t B, int64_t H, int64_t T, int64_t K, int64_t V, int dtype, int bwd);
 int dc_linear_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                             const void* v, const int64_t* v_strides, const float* log_decay,

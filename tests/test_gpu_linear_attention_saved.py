@@ -66,3 +66,36 @@ def test_saved_tensor_hooks_see_them(path):
     assert _states_bytes() in sizes
     for a, b in zip(torch.autograd.grad(o, leaves, do), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("given", [True, False], ids=["forward's workspace", "own states"])
+def test_the_backward_stays_within_its_workspace(given):
+    """The C entry with and without the forward's workspace: equal gradients, and nothing written past either size."""
+    from dynconv import _capi
+
+    lib = _capi.load()
+    q, k, v = (t.detach() for t in _leaves(4))
+    do = randn(gen(5), B, H, T, K).to(torch.bfloat16).to(DEV)
+    lam = torch.full((H,), -0.01, device=DEV)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(linear_attention(*leaves, lam), leaves, do)
+    o, grads = torch.empty_like(q), [torch.empty_like(t) for t in (q, k, v)]
+    dtype, st = _capi.dtype_code(q.dtype), _capi.int64_array(q.stride()[:3])
+
+    def room(which):
+        n = lib.dc_linear_attention_ws_bytes(B, H, T, K, K, dtype, which)
+        return torch.full((n + 4096,), 77, dtype=torch.uint8, device=DEV), n
+
+    ws, n = room(0)
+    args = [x for t in (q, k, v) for x in (_capi.ptr(t), st)]
+    _capi.check(lib.dc_linear_attention_fwd(*args, _capi.ptr(lam), None, None, _capi.ptr(o), st, None, _capi.ptr(ws), n, B,
+                                            H, T, K, K, K**-0.5, dtype, _capi.stream_of(q)), "forward")
+    kept = ws.clone()
+    bws, m = room(2 if given else 1)
+    out = [x for t in grads for x in (_capi.ptr(t), st)]
+    _capi.check(lib.dc_linear_attention_bwd(*args, _capi.ptr(lam), None, None, _capi.ptr(do), st, None, *out, None,
+                                            _capi.ptr(ws) if given else None, _capi.ptr(bws), m, B, H, T, K, K, K**-0.5,
+                                            dtype, _capi.stream_of(q)), "backward")
+    assert (ws[n:] == 77).all() and (bws[m:] == 77).all() and torch.equal(ws, kept)
+    for a, b in zip(grads, want):
+        assert torch.equal(a, b)

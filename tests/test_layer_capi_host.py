@@ -116,3 +116,15 @@ def test_lowrank_step_refusals(lib):
     assert step(x=P + 1) == E_ALIGN and step(z=P + 2, dt=2) == E_ALIGN and step(ids=P + 1, N=4) == E_ALIGN
     if NO_DEV:
         assert step() == E_DEV and step(W=1, state=None) == E_DEV and step(N=4, ids=P) == E_DEV
+
+
+def test_linear_attention_backward_workspace_with_the_forwards(lib):
+    """Given the forward's workspace, the backward needs room for one set of states instead of two."""
+    size = (1, 2, 1 << 16, 16, 16, 0)
+    fwd, alone, given = (lib.dc_linear_attention_ws_bytes(*size, which) for which in (0, 1, 2))
+    assert fwd > 0 and given == fwd and alone == 2 * fwd
+    assert la_bwd(lib, T=1 << 16, states=P, nws=given - 1) == E_WS
+    assert la_bwd(lib, T=1 << 16, nws=given) == E_WS and la_bwd(lib, T=1 << 16, nws=alone - 1) == E_WS
+    assert lib.dc_linear_attention_ws_bytes(1, 2, 8, 16, 16, 0, 2) == 0
+    if NO_DEV:
+        assert la_bwd(lib, T=1 << 16, states=P, nws=given) == E_DEV and la_bwd(lib, T=1 << 16, nws=alone) == E_DEV
