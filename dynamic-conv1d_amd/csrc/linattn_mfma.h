@@ -506,10 +506,7 @@ __global__ __launch_bounds__(NW * 64, waves_per_simd(sizeof(T), KP, NW, STATES))
 #pragma unroll
           for (int r = 0; r < 16; ++r) t[r] = sc[r] * (r < 8 ? vlast[r] * g1 : vlast[r - 8]);
         } else {
-          // opaque in fp16, or the sixteen conditions wait in spilled scalar registers (H16 T32768 hd128 156 -> 145
-          // us; in bf16 it costs 1%)
-          int later = col - 4 * half;
-          if constexpr (O::kNarrow) asm volatile("" : "+v"(later));
+          const int later = col - 4 * half;
 #pragma unroll
           for (int r = 0; r < 16; ++r) t[r] = 8 * (r / 4) + r % 4 <= later ? sc[r] * diag[r] : 0.f;
         }
