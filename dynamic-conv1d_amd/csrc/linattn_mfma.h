@@ -42,11 +42,14 @@
 // q S, not in S).  float32 inputs are products of three bf16 parts throughout (Parts).
 // All sums and S are float32.
 //
-// Measured at B2 H32 T8192, 128 x 128, bf16 (134 MB a tensor), four segments: the states' launch 64 us (4.2 TB/s of k and
-// v), the carry 8, the forward's chunks 133 (4.0 TB/s), the backward's three passes 313 (3.0 TB/s: what they read again
-// comes from the last-level cache), with the backward's own states 580 in all.  Loads alone take 42, 73 and 163, stores
-// 20 and 60-78 more.  Matrix instructions fill 28% of the SIMDs' cycles in the chunks' launches and vector instructions
-// 35%; the rest is the chain of one chunk's phases, which two workgroups on a CU hide from each other in part.
+// Measured at B2 H32 T8192, 128 x 128, bf16 (134 MB a tensor), four segments: the states' launch 63 us (3.2 TB/s of the
+// k and v of three segments), the carry 8, the forward's chunks 133 (0.55 GB past the L2, 4.2 TB/s), the backward's three
+// passes 308 (1.40 GB, 4.5 TB/s), with the backward's own states 590 in all.  The backward is near the rate of the memory
+// path for what it moves: dk's and dv's passes walk a segment side by side and share their loads, dq's walks it the other
+// way round and meets them in the middle only, so seven tensors are read past the L2 where four exist.  Loads alone take
+// 42, 73 and 163, stores 20 and 60-78 more.  Matrix instructions fill 22% of the SIMDs' cycles in the forward's chunks and
+// 31% in the backward's, vector instructions 28% and 38%.  In fp16 the lifts take 5-6% (B1 H16 T32768: chunks 146 ->
+// 153 us, states 68 -> 74).
 //
 // An infinity or a NaN stays out of the tokens before its own, also within a chunk: scores of later tokens are selected
 // away, not multiplied by zero, and v's elements that are not finite are taken out of the products of the diagonal blocks

@@ -131,7 +131,9 @@ def linear_attention(
         o [B, H, T, V] in q's dtype, over token-major memory (o.transpose(1, 2).reshape(B, T, H * V) is a view), or
         (o, state [B, H, K, V] float32).
 
-    Products of 16-bit inputs run on matrix cores with float32 sums; the state is float32 throughout.
+    Products of 16-bit inputs run on matrix cores with float32 sums; the state is float32 throughout.  As operands of such
+    products the decayed scores, and the state where a token's q meets it, are rounded to the inputs' type; a caller who
+    wants neither rounded passes q, k and v in float32.
     """
     if _capi.binding is not None:
         out = _capi.binding.linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_state)
