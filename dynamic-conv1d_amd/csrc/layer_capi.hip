@@ -253,3 +253,201 @@ int dc_lowrank_step_grouped(int64_t G, const void* x, int64_t x_ld, const void* 
 }
 
 }  // extern "C"
+
+// Sizes of the gated delta rule.
+static int check_dr(int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int64_t V, int dtype, int gdtype, int flags) {
+  const int s = check_la(B, H, T, K, V, dtype);
+  if (s != DC_OK) return s;
+  if (gdtype != dtype && gdtype != DC_DTYPE_FP32) return DC_ERR_DTYPE;
+  if (Hk <= 0 || H % Hk != 0) return DC_ERR_SHAPE;
+  return (flags & ~(DC_DELTA_NORMALIZE | DC_DELTA_PRECISE)) ? DC_ERR_UNSUPPORTED : DC_OK;
+}
+
+static dc::DrProblem dr_sizes(int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int64_t V, int dtype, int gdtype,
+                              int flags) {
+  dc::DrProblem p{};
+  p.B = B; p.Hk = Hk; p.H = H; p.T = T; p.K = K; p.V = V;
+  p.dtype = dtype; p.gdtype = gdtype;
+  p.normalize = (flags & DC_DELTA_NORMALIZE) != 0;
+  p.precise = (flags & DC_DELTA_PRECISE) != 0;
+  return p;
+}
+
+extern "C" {
+
+int64_t dc_delta_rule_ws_bytes(int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int64_t V, int dtype, int flags,
+                               int bwd) {
+  const int s = check_dr(B, Hk, H, T, K, V, dtype, dtype, flags);
+  if (s != DC_OK) return s;
+  return dc::dr_ws_bytes(dr_sizes(B, Hk, H, T, K, V, dtype, dtype, flags), bwd);
+}
+
+int dc_delta_rule_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                      const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                      const void* beta, const int64_t* beta_strides, const float* initial_state, const int32_t* lengths,
+                      void* o, const int64_t* o_strides, float* final_state, void* workspace, int64_t ws_bytes,
+                      int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int64_t V, float scale, float eps,
+                      int dtype, int gate_dtype, int flags, void* stream) {
+  int s = check_dr(B, Hk, H, T, K, V, dtype, gate_dtype, flags);
+  if (s != DC_OK) return s;
+  if (T > 0 && (!q || !k || !v || !log_decay || !beta || !o)) return DC_ERR_NULL;
+  const int es = dc::dtype_size(dtype), gs = dc::dtype_size(gate_dtype);
+  if (!aligned_to(q, es) || !aligned_to(k, es) || !aligned_to(v, es) || !aligned_to(o, es) ||
+      !aligned_to(log_decay, gs) || !aligned_to(beta, gs) || !aligned_to(initial_state, 4) ||
+      !aligned_to(final_state, 4) || !aligned_to(lengths, 4))
+    return DC_ERR_ALIGN;
+  dc::DrProblem p = dr_sizes(B, Hk, H, T, K, V, dtype, gate_dtype, flags);
+  const int64_t need = dc::dr_ws_bytes(p, 0);
+  if (need > 0 && (!workspace || ws_bytes < need || !aligned_to(workspace, 16))) return DC_ERR_WORKSPACE;
+  if (!copy3(p.qs, q_strides) || !copy3(p.ks, k_strides) || !copy3(p.vs, v_strides) || !copy3(p.os, o_strides) ||
+      !copy3(p.gs, log_decay_strides) || !copy3(p.bs, beta_strides))
+    return DC_ERR_NULL;
+  if ((s = device_status()) != DC_OK) return s;
+  p.q = q; p.k = k; p.v = v; p.g = log_decay; p.b = beta; p.o = o;
+  p.s_in = initial_state; p.s_out = final_state; p.lengths = lengths;
+  p.ws = workspace; p.scale = scale; p.eps = eps; p.stream = (hipStream_t)stream;
+  return launch_status(dc::dr_fwd(p));
+}
+
+int dc_delta_rule_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                      const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                      const void* beta, const int64_t* beta_strides, const float* initial_state, const int32_t* lengths,
+                      const void* d_o, const int64_t* do_strides, const float* d_final_state, void* dq,
+                      const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                      const int64_t* dv_strides, void* dlog_decay, const int64_t* dlog_decay_strides, void* dbeta,
+                      const int64_t* dbeta_strides, float* d_initial_state, const void* fwd_workspace, void* workspace,
+                      int64_t ws_bytes, int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int64_t V, float scale,
+                      float eps, int dtype, int gate_dtype, int flags, void* stream) {
+  int s = check_dr(B, Hk, H, T, K, V, dtype, gate_dtype, flags);
+  if (s != DC_OK) return s;
+  if (T > 0 && (!q || !k || !v || !log_decay || !beta || !d_o || !dq || !dk || !dv || !dlog_decay || !dbeta))
+    return DC_ERR_NULL;
+  const int es = dc::dtype_size(dtype), gs = dc::dtype_size(gate_dtype);
+  for (const void* t : {q, k, v, d_o, (const void*)dq, (const void*)dk, (const void*)dv})
+    if (!aligned_to(t, es)) return DC_ERR_ALIGN;
+  for (const void* t : {log_decay, beta, (const void*)dlog_decay, (const void*)dbeta})
+    if (!aligned_to(t, gs)) return DC_ERR_ALIGN;
+  for (const void* t : {(const void*)initial_state, (const void*)d_final_state, (const void*)d_initial_state,
+                        (const void*)lengths})
+    if (!aligned_to(t, 4)) return DC_ERR_ALIGN;
+  dc::DrProblem p = dr_sizes(B, Hk, H, T, K, V, dtype, gate_dtype, flags);
+  const int64_t need = dc::dr_ws_bytes(p, fwd_workspace ? 2 : 1);
+  if (need > 0 && (!workspace || ws_bytes < need || !aligned_to(workspace, 16))) return DC_ERR_WORKSPACE;
+  if (!aligned_to(fwd_workspace, 16)) return DC_ERR_WORKSPACE;
+  if (!copy3(p.qs, q_strides) || !copy3(p.ks, k_strides) || !copy3(p.vs, v_strides) || !copy3(p.dos, do_strides) ||
+      !copy3(p.gs, log_decay_strides) || !copy3(p.bs, beta_strides) || !copy3(p.dqs, dq_strides) ||
+      !copy3(p.dks, dk_strides) || !copy3(p.dvs, dv_strides) || !copy3(p.dgs, dlog_decay_strides) ||
+      !copy3(p.dbs, dbeta_strides))
+    return DC_ERR_NULL;
+  if ((s = device_status()) != DC_OK) return s;
+  p.q = q; p.k = k; p.v = v; p.g = log_decay; p.b = beta; p.d_o = d_o;
+  p.dq = dq; p.dk = dk; p.dv = dv; p.dg = dlog_decay; p.db = dbeta;
+  p.s_in = initial_state; p.ds_in = d_final_state; p.ds_out = d_initial_state; p.lengths = lengths;
+  p.fwd_ws = fwd_workspace; p.ws = workspace; p.scale = scale; p.eps = eps; p.stream = (hipStream_t)stream;
+  return launch_status(dc::dr_bwd(p));
+}
+
+int dc_delta_rule_step(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                       const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                       const void* beta, const int64_t* beta_strides, float* state, const int32_t* slot_ids, void* o,
+                       int64_t B, int64_t Hk, int64_t H, int64_t K, int64_t V, int64_t slots, float scale, float eps,
+                       int dtype, int gate_dtype, int flags, void* stream) {
+  int s = check_dr(B, Hk, H, 1, K, V, dtype, gate_dtype, flags);
+  if (s != DC_OK) return s;
+  if (slots <= 0 || slots > kI32Max || (!slot_ids && B > slots)) return DC_ERR_SHAPE;
+  if (!q || !k || !v || !o || !log_decay || !beta || !state || !q_strides || !k_strides || !v_strides ||
+      !log_decay_strides || !beta_strides)
+    return DC_ERR_NULL;
+  const int es = dc::dtype_size(dtype), gs = dc::dtype_size(gate_dtype);
+  if (!aligned_to(q, es) || !aligned_to(k, es) || !aligned_to(v, es) || !aligned_to(o, es) ||
+      !aligned_to(log_decay, gs) || !aligned_to(beta, gs) || !aligned_to(state, 4) || !aligned_to(slot_ids, 4))
+    return DC_ERR_ALIGN;
+  if ((s = device_status()) != DC_OK) return s;
+  dc::DrStep p{};
+  p.q = q; p.k = k; p.v = v; p.g = log_decay; p.b = beta;
+  for (int i = 0; i < 2; ++i) {
+    p.qs[i] = q_strides[i];
+    p.ks[i] = k_strides[i];
+    p.vs[i] = v_strides[i];
+    p.gs[i] = log_decay_strides[i];
+    p.bs[i] = beta_strides[i];
+  }
+  p.state = state; p.slot_ids = slot_ids; p.o = o;
+  p.B = B; p.Hk = Hk; p.H = H; p.K = K; p.V = V; p.slots = slots;
+  p.scale = scale; p.eps = eps; p.dtype = dtype; p.gdtype = gate_dtype;
+  p.normalize = (flags & DC_DELTA_NORMALIZE) != 0; p.stream = (hipStream_t)stream;
+  return launch_status(dc::dr_step(p));
+}
+
+}  // extern "C"
+
+// Sizes and types of a residual norm.
+static int check_rn(int64_t M, int64_t D, int act, int dtype, int xdtype, int pdtype) {
+  if (!dtype_ok(dtype) || (xdtype != dtype && xdtype != DC_DTYPE_FP32) || (pdtype != dtype && pdtype != DC_DTYPE_FP32))
+    return DC_ERR_DTYPE;
+  if (M <= 0 || D <= 0 || M > kI32Max) return DC_ERR_SHAPE;
+  if (act != DC_ACT_NONE && act != DC_ACT_SILU && act != DC_ACT_SIGMOID) return DC_ERR_UNSUPPORTED;
+  return D <= DC_RN_MAX_DIM ? DC_OK : DC_ERR_UNSUPPORTED;
+}
+
+extern "C" {
+
+int dc_residual_norm_fwd(const void* x, const void* branch, const void* weight, const void* branch_weight,
+                         const void* gate, const void* scale, void* y, void* h, int64_t M, int64_t D, float constant,
+                         float eps, int activation, int dtype, int x_dtype, int param_dtype, void* stream) {
+  int s = check_rn(M, D, activation, dtype, x_dtype, param_dtype);
+  if (s != DC_OK) return s;
+  if (!x || !branch || !y || !h) return DC_ERR_NULL;
+  const int es = dc::dtype_size(dtype), xs = dc::dtype_size(x_dtype), ps = dc::dtype_size(param_dtype);
+  if (!aligned_to(x, xs) || !aligned_to(h, xs) || !aligned_to(branch, es) || !aligned_to(gate, es) ||
+      !aligned_to(y, es) || !aligned_to(weight, ps) || !aligned_to(branch_weight, ps) || !aligned_to(scale, ps))
+    return DC_ERR_ALIGN;
+  if ((s = device_status()) != DC_OK) return s;
+  dc::RnProblem p{};
+  p.x = x; p.branch = branch; p.weight = weight; p.branch_weight = branch_weight; p.gate = gate; p.scale = scale;
+  p.y = y; p.h = h;
+  p.M = M; p.D = D; p.constant = constant; p.eps = eps; p.act = activation;
+  p.dtype = dtype; p.xdtype = x_dtype; p.pdtype = param_dtype; p.stream = (hipStream_t)stream;
+  return launch_status(dc::rn_fwd(p));
+}
+
+int64_t dc_residual_norm_bwd_ws_bytes(int64_t M, int64_t D, int dtype) {
+  const int s = check_rn(M, D, DC_ACT_NONE, dtype, dtype, dtype);
+  if (s != DC_OK) return s;
+  dc::RnProblem p{};
+  p.M = M; p.D = D; p.dtype = p.xdtype = dtype;
+  return dc::rn_bwd_ws_bytes(p);
+}
+
+int dc_residual_norm_bwd(const void* h, const void* branch, const void* weight, const void* branch_weight,
+                         const void* gate, const void* scale, const void* dy, const void* dh, void* dx, void* dbranch,
+                         void* dgate, void* dweight, void* dbranch_weight, void* dscale, void* workspace,
+                         int64_t ws_bytes, int64_t M, int64_t D, float constant, float eps, int activation, int dtype,
+                         int x_dtype, int param_dtype, void* stream) {
+  int s = check_rn(M, D, activation, dtype, x_dtype, param_dtype);
+  if (s != DC_OK) return s;
+  if (!h || !branch || !dx || !dbranch || (gate == nullptr) != (dgate == nullptr)) return DC_ERR_NULL;
+  const int es = dc::dtype_size(dtype), xs = dc::dtype_size(x_dtype), ps = dc::dtype_size(param_dtype);
+  for (const void* t : {branch, gate, dy, (const void*)dbranch, (const void*)dgate})
+    if (!aligned_to(t, es)) return DC_ERR_ALIGN;
+  for (const void* t : {h, dh, (const void*)dx})
+    if (!aligned_to(t, xs)) return DC_ERR_ALIGN;
+  for (const void* t : {weight, branch_weight, scale, (const void*)dweight, (const void*)dbranch_weight,
+                        (const void*)dscale})
+    if (!aligned_to(t, ps)) return DC_ERR_ALIGN;
+  if (dweight || dbranch_weight || dscale) {
+    const int64_t need = dc_residual_norm_bwd_ws_bytes(M, D, dtype);
+    if (!workspace || ws_bytes < need || !aligned_to(workspace, 16)) return DC_ERR_WORKSPACE;
+  }
+  if ((s = device_status()) != DC_OK) return s;
+  dc::RnProblem p{};
+  p.h = const_cast<void*>(h); p.branch = branch; p.weight = weight; p.branch_weight = branch_weight; p.gate = gate;
+  p.scale = scale; p.dy = dy; p.dh = dh;
+  p.dx = dx; p.dbranch = dbranch; p.dgate = dgate; p.dweight = dweight; p.dbranch_weight = dbranch_weight;
+  p.dscale = dscale; p.ws = (float*)workspace;
+  p.M = M; p.D = D; p.constant = constant; p.eps = eps; p.act = activation;
+  p.dtype = dtype; p.xdtype = x_dtype; p.pdtype = param_dtype; p.stream = (hipStream_t)stream;
+  return launch_status(dc::rn_bwd(p));
+}
+
+}  // extern "C"

@@ -60,6 +60,47 @@ struct LaStep {
 };
 hipError_t la_step(const LaStep& p);
 
+// ------------------------------------------------------- gated delta rule
+struct DrProblem {
+  const void *q, *k, *v, *g, *b;  // g: log_decay, b: beta
+  int64_t qs[3], ks[3], vs[3], gs[3], bs[3];  // strides (batch, head, row), elements
+  const float* s_in;
+  const int32_t* lengths;
+  void* o;
+  int64_t os[3];
+  float* s_out;
+  // backward
+  const void* d_o;
+  int64_t dos[3];
+  const float* ds_in;  // the final state's gradient
+  void *dq, *dk, *dv, *dg, *db;
+  int64_t dqs[3], dks[3], dvs[3], dgs[3], dbs[3];
+  float* ds_out;  // the initial state's
+  const void* fwd_ws;
+  void* ws;
+  int64_t B, Hk, H, T, K, V;
+  float scale, eps;
+  int dtype, gdtype, normalize, precise;
+  hipStream_t stream;
+};
+int64_t dr_ws_bytes(const DrProblem& p, int bwd);
+hipError_t dr_fwd(const DrProblem& p);
+hipError_t dr_bwd(const DrProblem& p);
+
+struct DrStep {
+  const void *q, *k, *v, *g, *b;
+  int64_t qs[2], ks[2], vs[2], gs[2], bs[2];
+  float* state;
+  const int32_t* slot_ids;
+  void* o;
+  int64_t B, Hk, H, K, V, slots;
+  int64_t bh0;  // first head of a launch
+  float scale, eps;
+  int dtype, gdtype, normalize;
+  hipStream_t stream;
+};
+hipError_t dr_step(const DrStep& p);
+
 // ------------------------------------------------------------- group norm
 struct GnProblem {
   const void *x, *weight, *bias, *gate, *dy;
@@ -75,6 +116,21 @@ bool gn_shape_ok(const GnProblem& p);
 int64_t gn_bwd_ws_bytes(const GnProblem& p);
 hipError_t gn_fwd(const GnProblem& p);
 hipError_t gn_bwd(const GnProblem& p);
+
+// ---------------------------------------------------------- residual norm
+struct RnProblem {
+  const void *x, *branch, *weight, *branch_weight, *gate, *scale, *dy, *dh;
+  void *y, *h, *dx, *dbranch, *dgate, *dweight, *dbranch_weight, *dscale;  // h: the backward reads it
+  float* ws;
+  int64_t M, D;
+  float constant, eps;
+  int act;
+  int dtype, xdtype, pdtype;
+  hipStream_t stream;
+};
+int64_t rn_bwd_ws_bytes(const RnProblem& p);
+hipError_t rn_fwd(const RnProblem& p);
+hipError_t rn_bwd(const RnProblem& p);
 
 // ------------------------------------------------------- convolution step
 struct LrStep {

@@ -1,0 +1,4 @@
+// The fp16 residual norm kernels (residual_norm.h).
+#include "residual_norm.h"
+
+template hipError_t dc::rn::launch_vec<dc::fp16>(bool, const dc::rn::Args&, const dc::rn::Plan&, bool, hipStream_t);

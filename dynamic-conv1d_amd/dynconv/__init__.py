@@ -9,7 +9,8 @@ q / k / v convolutions of one layer in one launch per direction, README.md:57-11
 and the README's LowRankDynamicShortConvolution module, plus its grouped form.
 
 Behind the convolutions of a layer: linear_attention with a decay for each head (whole
-sequences) and linear_attention_step (single tokens), group_norm with its gate, the
+sequences) and linear_attention_step (single tokens), gated_delta_rule and
+gated_delta_rule_step, group_norm with its gate, residual_norm around a block, the
 convolutions' single-token form lowrank_dynamic_convolution_step(_grouped), and
 DynamicLinearAttention, a layer of all of them.
 
@@ -22,7 +23,8 @@ from .lowrank import lowrank_dynamic_convolution, _LowrankDynamicConvolutionFn  
 from .lowrank import lowrank_dynamic_convolution_grouped  # noqa: F401
 from .lowrank import lowrank_dynamic_convolution_step, lowrank_dynamic_convolution_step_grouped  # noqa: F401
 from .linattn import linear_attention, linear_attention_step  # noqa: F401
-from .norm import group_norm  # noqa: F401
+from .delta import gated_delta_rule, gated_delta_rule_step  # noqa: F401
+from .norm import group_norm, residual_norm  # noqa: F401
 from .modules import LowRankDynamicShortConvolution, GroupedLowRankDynamicShortConvolution  # noqa: F401
 from .modules import DynamicLinearAttention, LayerState  # noqa: F401
 from ._capi import LIB_PATH, load as load_library  # noqa: F401
@@ -35,7 +37,10 @@ __all__ = [
     "lowrank_dynamic_convolution_step_grouped",
     "linear_attention",
     "linear_attention_step",
+    "gated_delta_rule",
+    "gated_delta_rule_step",
     "group_norm",
+    "residual_norm",
     "LowRankDynamicShortConvolution",
     "GroupedLowRankDynamicShortConvolution",
     "DynamicLinearAttention",

@@ -62,6 +62,15 @@ LAYER_SIGNATURES = {
     "dc_linear_attention_bwd": (_c_int, [_c_vp, _c_st] * 3 + [_c_vp] * 4 + [_c_st] + [_c_vp] + [_c_vp, _c_st] * 3
                                 + [_c_vp] * 3 + [_c_i64] * 6 + [_c_f, _c_int, _c_vp]),
     "dc_linear_attention_step": (_c_int, [_c_vp, _c_st] * 3 + [_c_vp] * 4 + [_c_i64] * 5 + [_c_f, _c_int, _c_vp]),
+    "dc_delta_rule_ws_bytes": (_c_i64, [_c_i64] * 6 + [_c_int] * 3),
+    "dc_delta_rule_fwd": (_c_int, [_c_vp, _c_st] * 5 + [_c_vp] * 3 + [_c_st] + [_c_vp] * 2 + [_c_i64] * 7 + [_c_f] * 2
+                          + [_c_int] * 3 + [_c_vp]),
+    "dc_delta_rule_bwd": (_c_int, [_c_vp, _c_st] * 5 + [_c_vp] * 3 + [_c_st] + [_c_vp] + [_c_vp, _c_st] * 5 + [_c_vp] * 3
+                          + [_c_i64] * 7 + [_c_f] * 2 + [_c_int] * 3 + [_c_vp]),
+    "dc_delta_rule_step": (_c_int, [_c_vp, _c_st] * 5 + [_c_vp] * 3 + [_c_i64] * 6 + [_c_f] * 2 + [_c_int] * 3 + [_c_vp]),
+    "dc_residual_norm_fwd": (_c_int, [_c_vp] * 8 + [_c_i64] * 2 + [_c_f] * 2 + [_c_int] * 4 + [_c_vp]),
+    "dc_residual_norm_bwd_ws_bytes": (_c_i64, [_c_i64] * 2 + [_c_int]),
+    "dc_residual_norm_bwd": (_c_int, [_c_vp] * 15 + [_c_i64] * 3 + [_c_f] * 2 + [_c_int] * 4 + [_c_vp]),
     "dc_group_norm_fwd": (_c_int, [_c_vp] * 5 + [_c_i64] * 3 + [_c_f] + [_c_int] * 3 + [_c_vp]),
     "dc_group_norm_bwd_ws_bytes": (_c_i64, [_c_i64] * 3 + [_c_int]),
     "dc_group_norm_bwd": (_c_int, [_c_vp] * 10 + [_c_i64] * 4 + [_c_f] + [_c_int] * 3 + [_c_vp]),

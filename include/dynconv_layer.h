@@ -2,9 +2,10 @@
  * dynconv_layer.h -- C ABI of the operators that stand behind the short
  * convolutions in a layer (libdynconv.so, with dynconv.h): linear attention
  * with a decay for each head, in its form for whole sequences and its form for
- * single tokens; the group norm of its heads with an activation or a gate; and
- * the lowrank convolutions' form for single tokens.  The reference has none of
- * these.
+ * single tokens; the gated delta rule in both forms; the group norm of their
+ * heads with an activation or a gate; the norms around a block with its gate,
+ * its residual scale and the residual sum; and the lowrank convolutions' form
+ * for single tokens.  The reference has none of these.
  *
  * Conventions are those of dynconv.h (device pointers, int64 sizes, a status
  * of DC_OK or below, no allocation, no synchronisation, kernels only, on
@@ -70,8 +71,53 @@ int dc_linear_attention_step(const void* q, const int64_t* q_strides, const void
                              const int32_t* slot_ids, void* o, int64_t B, int64_t H, int64_t K, int64_t V,
                              int64_t slots, float scale, int dtype, void* stream);
 
-/* Activations of dc_group_norm_fwd / _bwd. */
-typedef enum dc_activation { DC_ACT_NONE = 0, DC_ACT_SILU = 1 } dc_activation;
+/* Flags of the gated delta rule. */
+typedef enum dc_delta_flags {
+  DC_DELTA_NORMALIZE = 1, /* the rows of q and k are divided by sqrt(|row|^2 + eps) */
+  DC_DELTA_PRECISE = 2    /* bf16: every product's operands in two parts of the type (16 bits), for float32 results */
+} dc_delta_flags;
+
+/* The gated delta rule: with a = exp(log_decay_t), b = beta_t, for each sequence and head,
+ *     S' = a S_{t-1},   u = b (v_t - k_t S'),   S_t = S' + k_t^T u,   o_t = scale * q_t S_t
+ * from S_{-1} = initial_state (NULL: zero).
+ *   q, k [B, Hk, T, K], v, o [B, H, T, V], log_decay, beta [B, H, T], with strides (batch, head, row) each, those of
+ *   log_decay and beta for the whole of their axes; Hk divides H, and head h reads q and k of head h / (H / Hk);
+ *   log_decay <= 0 (-inf forgets at once), beta and log_decay in gate_dtype: dtype or float32;
+ *   initial_state, final_state, lengths as in dc_linear_attention_fwd.
+ * T may be 0.  Both calls need a workspace of dc_delta_rule_ws_bytes bytes (0: none), 16-byte aligned; bwd: 0 the
+ * forward, 1 the backward, 2 the backward that is given the forward's workspace (of the same flags). */
+int64_t dc_delta_rule_ws_bytes(int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int64_t V, int dtype, int flags,
+                               int bwd);
+int dc_delta_rule_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                      const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                      const void* beta, const int64_t* beta_strides, const float* initial_state, const int32_t* lengths,
+                      void* o, const int64_t* o_strides, float* final_state, void* workspace, int64_t ws_bytes,
+                      int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int64_t V, float scale, float eps,
+                      int dtype, int gate_dtype, int flags, void* stream);
+
+/* Gradients of dc_delta_rule_fwd: dq, dk, dv, dlog_decay, dbeta from d_o and d_final_state (NULL: zero), and
+ * d_initial_state (NULL: not wanted).  Rows past a sequence's length get zero.  fwd_workspace is NULL or the
+ * workspace of the forward of the same inputs, as that call left it (trusted, not checked). */
+int dc_delta_rule_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                      const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                      const void* beta, const int64_t* beta_strides, const float* initial_state, const int32_t* lengths,
+                      const void* d_o, const int64_t* do_strides, const float* d_final_state, void* dq,
+                      const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                      const int64_t* dv_strides, void* dlog_decay, const int64_t* dlog_decay_strides, void* dbeta,
+                      const int64_t* dbeta_strides, float* d_initial_state, const void* fwd_workspace, void* workspace,
+                      int64_t ws_bytes, int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int64_t V, float scale,
+                      float eps, int dtype, int gate_dtype, int flags, void* stream);
+
+/* One token of each of B sequences: q, k [B, Hk, K], v [B, H, V], log_decay, beta [B, H] with strides (batch, head),
+ * o [B, H, V] contiguous; state and slot_ids as in dc_linear_attention_step. */
+int dc_delta_rule_step(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                       const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
+                       const void* beta, const int64_t* beta_strides, float* state, const int32_t* slot_ids, void* o,
+                       int64_t B, int64_t Hk, int64_t H, int64_t K, int64_t V, int64_t slots, float scale, float eps,
+                       int dtype, int gate_dtype, int flags, void* stream);
+
+/* Activations of dc_group_norm_fwd / _bwd (the first two) and of dc_residual_norm_fwd / _bwd. */
+typedef enum dc_activation { DC_ACT_NONE = 0, DC_ACT_SILU = 1, DC_ACT_SIGMOID = 2 } dc_activation;
 
 /* Group norm over the channels of each row: x, y, gate [M, D] contiguous, in
  * `groups` groups of D / groups neighbouring channels,
@@ -87,6 +133,27 @@ int64_t dc_group_norm_bwd_ws_bytes(int64_t M, int64_t D, int64_t groups, int dty
 int dc_group_norm_bwd(const void* x, const void* weight, const void* bias, const void* gate, const void* dy, void* dx,
                       void* dgate, void* dweight, void* dbias, void* workspace, int64_t ws_bytes, int64_t M, int64_t D,
                       int64_t groups, float eps, int activation, int dtype, int param_dtype, void* stream);
+
+/* Largest rows of the residual norm. */
+#define DC_RN_MAX_DIM 8192
+
+/* The norms around a block, its gate, its residual scale and the residual sum, row by row of [M, D]:
+ *     u = branch / sqrt(mean(branch^2) + eps) * branch_weight,    h = x + constant * scale * act(gate) * u,
+ *     y = h / sqrt(mean(h^2) + eps) * weight
+ * x, h contiguous in x_dtype: dtype or float32 (h is rounded to it before its norm); branch, gate (or NULL: no factor),
+ * y contiguous in dtype; weight, branch_weight, scale [D] or NULL (1), all in param_dtype: dtype or float32. */
+int dc_residual_norm_fwd(const void* x, const void* branch, const void* weight, const void* branch_weight,
+                         const void* gate, const void* scale, void* y, void* h, int64_t M, int64_t D, float constant,
+                         float eps, int activation, int dtype, int x_dtype, int param_dtype, void* stream);
+
+/* dx (in x_dtype), dbranch, dgate (with a gate), dweight, dbranch_weight, dscale (NULL: not wanted) from dy and dh
+ * (either NULL: zero) and the forward's h. */
+int64_t dc_residual_norm_bwd_ws_bytes(int64_t M, int64_t D, int dtype);
+int dc_residual_norm_bwd(const void* h, const void* branch, const void* weight, const void* branch_weight,
+                         const void* gate, const void* scale, const void* dy, const void* dh, void* dx, void* dbranch,
+                         void* dgate, void* dweight, void* dbranch_weight, void* dscale, void* workspace,
+                         int64_t ws_bytes, int64_t M, int64_t D, float constant, float eps, int activation, int dtype,
+                         int x_dtype, int param_dtype, void* stream);
 
 /* One token of each of N sequences through G lowrank convolutions of one shape
  * (the single-token form of dc_lowrank_fwd_grouped): with x_0 = x[n] and x_w
