@@ -1,0 +1,1127 @@
+// The gated delta rule in chunks of tokens on matrix cores (formulas: delta.hip).
+//
+// Operands and results.  v_mfma_f32_16x16x32 leaves element (row, col) of its result in lane col + 16 (row/4), register
+// row%4; an operand wants 8 values of the summed index in a lane.  Products sum in the order that two results of 16 rows
+// come in (step s: 32 s + 16 (e/4) + 4 (lane/16) + e%4 for element e), so that the chain from the state to the next one,
+// k S, Tb X, k^T U, goes from results to operands without leaving the lane: a wavefront keeps 16 columns of S.  Rows of
+// tiles lie in LDS so that a lane's 8 values of that order are neighbours (spot()); columns are read through transposing
+// reads.
+//
+// Precision.  Operands are bf16: q, k, v and dO as one part (bf16), two (fp16: all of its bits) or three (float32), what is
+// computed (S, X, U, Tb, P and their gradients) in NP parts: one in bf16 (2^-9 of each, below the rounding of the results),
+// two where a result is float32 and in fp16 (2^-17), three in float32 (2^-25).  A product of parts keeps those down to the
+// last part's size.  Sums, S and dS, decays and norms are float32; sums of logarithms of decays are float64.
+#pragma once
+
+#include <type_traits>
+
+#include "layer_launch.h"
+#include "lowrank_mfma.h"
+
+namespace dc {
+namespace dr {
+
+constexpr float kTiny = 0x1p-60f;  // stands for a b of zero
+// What a token's chunk keeps of it, floats: c in two parts, b, 1/|k|, 1/|q|, G/|k|, D/|k|, scale G/|q|.
+constexpr int kC = 0, kB = 2, kRk = 3, kRq = 4, kGk = 5, kDk = 6, kGq = 7, kVecs = 8;
+constexpr int kPiece = 128;  // columns of v that the gradients' launch holds at once
+
+template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __is_same(T, fp16) ? 2 : 1; }
+// Tokens of a chunk: 64, or 32 where tiles of 64 would pass the LDS.
+__host__ __device__ constexpr int chunk_of(int parts, int kp) { return parts == 3 || parts * kp > 256 ? 32 : 64; }
+__host__ __device__ constexpr int cover(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : 256; }
+
+struct Args {
+  DrProblem p;
+  float* vec;          // [chunks][kVecs][C]
+  bf16 *tb, *pp;       // [chunks][NP][C][C], spot() order
+  bf16 *u, *x, *s, *ds;  // [chunks][NP][C][VP] U and dX, [chunks][NP][KP][VP] states before and their gradients after
+  int64_t n;           // chunks of a head
+  int vp;              // V in whole 32 columns
+  int64_t blk0;
+  int nblk;
+};
+
+// Where column c of a row lies: of each 32 the quads of both halves side by side.
+__host__ __device__ constexpr int spot(int c) { return (c & ~31) | ((c & 12) << 1) | ((c & 16) >> 2) | (c & 3); }
+
+constexpr int kOut = 0x7FFFFFF0;  // a byte offset past every buffer's range
+
+template <int N> struct Frag { u32x4 p[N]; };
+
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4 c) {
+  constexpr int N = NA > NB ? NA : NB;
+#pragma unroll
+  for (int t = N - 1; t >= 0; --t)  // the smallest first
+#pragma unroll
+    for (int i = t; i >= 0; --i)
+      if (i < NA && t - i < NB) c = Mma32<bf16>::run(a.p[i], b.p[t - i], c);
+  return c;
+}
+
+// Two floats in N parts, a word of two for each.
+template <int N>
+__device__ __forceinline__ void split(float a, float b, uint32_t (&w)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    w[i] = pack2<bf16>(a, b);
+    if (i + 1 < N) {
+      a -= __uint_as_float(w[i] << 16);
+      b -= __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+// The operand of two results of 16 rows each.
+template <int N>
+__device__ __forceinline__ Frag<N> pack(f32x4 a, f32x4 b) {
+  Frag<N> f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t w[N];
+    if (e < 2) split<N>(a[2 * e], a[2 * e + 1], w);
+    else split<N>(b[2 * e - 4], b[2 * e - 3], w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f.p[i][e] = w[i];
+  }
+  return f;
+}
+
+// A tile in LDS: R elements from a row to the next, PL from a part to the next.
+template <int N, int R, int PL>
+struct Tile {
+  bf16* t;
+  // row row0 + lane%16, step s of 32 columns
+  __device__ __forceinline__ Frag<N> rows(int row0, int s) const {
+    const int lane = threadIdx.x % 64;
+    const bf16* p = t + (row0 + lane % 16) * R + 32 * s + 8 * (lane / 16);
+    Frag<N> f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) f.p[i] = *reinterpret_cast<const u32x4*>(p + i * PL);
+    return f;
+  }
+  // column 16 cb + lane%16, step s of 32 rows (columns in spot() order)
+  __device__ __forceinline__ Frag<N> cols(int cb, int s) const {
+    const int lane = threadIdx.x % 64;
+    const bf16* p = t + (32 * s + 4 * (lane / 16) + (lane % 16) / 4) * R + 32 * (cb / 2) + 8 * (lane % 4) + 4 * (cb % 2);
+    Frag<N> f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const u32x2 a = lds_read_tr16(p + i * PL), b = lds_read_tr16(p + i * PL + 16 * R);
+      f.p[i] = u32x4{a[0], a[1], b[0], b[1]};
+    }
+    return f;
+  }
+  // element (row, c) of spot() order
+  __device__ __forceinline__ float at(int row, int c) const {
+    float v = 0.f;
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) v += (float)t[row * R + spot(c) + i * PL];
+    return v;
+  }
+};
+
+// C rows of W channels on their way from memory to a tile: 16-byte pieces that wait in registers.  WHOLE: rows are whole
+// 16-byte pieces, no shorter apart than they are long and within 32-bit offsets: buffer loads, whose range drops the rows
+// that are not there (loads under branches wait for one another).  Else they are gathered element by element.
+template <typename T, int C, int W, int NT, bool WHOLE>
+struct Rows {
+  static constexpr int VE = 16 / (int)sizeof(T), PR = W / VE, NV = C * PR / NT, RPI = NT / PR;
+  static_assert(C * PR % NT == 0 && NT % PR == 0, "whole pieces and rows to every thread");
+  u32x4 v[NV];
+  // rows 0 .. cnt-1 of base, `width` of the channels exist; the others are zero
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int width, int cnt) {
+    const int r0 = (int)threadIdx.x / PR, c = (int)threadIdx.x % PR * VE;
+    if constexpr (WHOLE) {  // the range ends behind the last row
+      const rsrc_t rs = make_rsrc_wave(base, ((int64_t)(cnt - 1) * stride + width) * (int64_t)sizeof(T));
+      const int sb = (int)stride * (int)sizeof(T), off = r0 * sb + c * (int)sizeof(T);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] = bload128(rs, c < width ? off + i * RPI * sb : kOut);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int r = r0 + i * RPI;
+        T e[VE];
+#pragma unroll
+        for (int j = 0; j < VE; ++j) e[j] = r < cnt && c + j < width ? base[(int64_t)r * stride + c + j] : (T)0.f;
+        __builtin_memcpy(&v[i], e, 16);
+      }
+    }
+  }
+  // into a tile of R elements a row, in spot() order or as they are
+  template <int R, int PL, bool SPOT>
+  __device__ __forceinline__ void store(bf16* lds) const {
+    const int c = (int)threadIdx.x % PR * VE;
+    bf16* to = lds + (int)threadIdx.x / PR * R;
+#pragma unroll
+    for (int i = 0; i < NV; ++i, to += RPI * R) {
+      if constexpr (sizeof(T) == 4) {
+        uint32_t a[3], b[3];
+        split<3>(__uint_as_float(v[i][0]), __uint_as_float(v[i][1]), a);
+        split<3>(__uint_as_float(v[i][2]), __uint_as_float(v[i][3]), b);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) *reinterpret_cast<u32x2*>(to + (SPOT ? spot(c) : c) + j * PL) = u32x2{a[j], b[j]};
+      } else {
+        constexpr int N = parts_of<T>();
+        u32x4 w[N];
+        if constexpr (N == 1) {
+          w[0] = v[i];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t ab[2];
+            split<2>(Mma16<T>::to_f(v[i][e] & 0xFFFFu), Mma16<T>::to_f(v[i][e] >> 16), ab);
+            w[0][e] = ab[0];
+            w[1][e] = ab[1];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if constexpr (SPOT) {
+            *reinterpret_cast<u32x2*>(to + spot(c) + j * PL) = u32x2{w[j][0], w[j][1]};
+            *reinterpret_cast<u32x2*>(to + spot(c + 4) + j * PL) = u32x2{w[j][2], w[j][3]};
+          } else {
+            *reinterpret_cast<u32x4*>(to + c + j * PL) = w[j];
+          }
+        }
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ int length_of(const DrProblem& p, int64_t b) {
+  const int T = (int)p.T;
+  return p.lengths ? min(max(p.lengths[b], 0), T) : T;
+}
+__device__ __forceinline__ float gate_at(const void* t, int gdtype, int64_t i) {
+  return gdtype == kBF16 ? (float)((const bf16*)t)[i] : gdtype == kFP16 ? (float)((const fp16*)t)[i] : ((const float*)t)[i];
+}
+__device__ __forceinline__ void put_gate(void* t, int gdtype, int64_t i, float v) {
+  if (gdtype == kBF16) ((bf16*)t)[i] = (bf16)v;
+  else if (gdtype == kFP16) ((fp16*)t)[i] = (fp16)v;
+  else ((float*)t)[i] = v;
+}
+
+
+
+// What each chunk needs of its own keys: a workgroup of four wavefronts to a chunk of one head.
+template <typename T, int NP, int KP, bool WHOLE>
+__global__ __launch_bounds__(256) void dr_prep(Args a) {
+  constexpr int NI = parts_of<T>(), C = chunk_of(NI, KP), NB = C / 16, R = KP + 8, PL = C * R, RA = C + 4;
+  constexpr int TILES = 2 * NI * PL * 2, MATS = 2 * C * RA * 4;
+  __shared__ __align__(16) unsigned char mem[TILES > MATS ? TILES : MATS];
+  __shared__ float chi[C], clo[C], be[C], rk[C], rq[C];
+  bf16 *lk = reinterpret_cast<bf16*>(mem), *lq = lk + NI * PL;
+  float (*A)[RA] = reinterpret_cast<float (*)[RA]>(mem), (*X)[RA] = A + C;
+  const DrProblem& p = a.p;
+  const int64_t blk = a.blk0 + blockIdx.x, n = blk % a.n, bh = blk / a.n, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
+  const int t0 = (int)n * C, len = length_of(p, b), t = threadIdx.x, lane = t % 64, g = lane / 16, col = lane % 16, wv = wave_id();
+  if (t0 >= len) return;
+  const int cnt = min(C, len - t0);
+  {
+    Rows<T, C, KP, 256, WHOLE> k, q;
+    k.load((const T*)p.k + b * p.ks[0] + hk * p.ks[1] + (int64_t)t0 * p.ks[2], p.ks[2], (int)p.K, cnt);
+    q.load((const T*)p.q + b * p.qs[0] + hk * p.qs[1] + (int64_t)t0 * p.qs[2], p.qs[2], (int)p.K, cnt);
+    k.template store<R, PL, false>(lk);
+    q.template store<R, PL, false>(lq);
+  }
+  if (wv == 0) {
+    // a token to a lane; the sums in float64: their differences count to the last place
+    const bool live = lane < cnt;
+    float lam = live ? gate_at(p.g, p.gdtype, b * p.gs[0] + h * p.gs[1] + (t0 + lane) * p.gs[2]) : 0.f;
+    lam = lam < -128.f ? -128.f : lam;  // e^-128 is nothing to float32, and differences stay finite
+    double c = lam;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+      const double o = __shfl_up(c, m);
+      if (lane >= m) c += o;
+    }
+    const float bt = live ? gate_at(p.b, p.gdtype, b * p.bs[0] + h * p.bs[1] + (t0 + lane) * p.bs[2]) : 0.f;
+    if (lane < C) {
+      chi[lane] = (float)c;
+      clo[lane] = (float)(c - (double)(float)c);
+      be[lane] = fabsf(bt) < kTiny ? kTiny : bt;
+    }
+  }
+  __syncthreads();
+  const Tile<NI, R, PL> tk{lk}, tq{lq};
+  {
+    constexpr int TPR = 256 / C, CH = KP / TPR;  // threads to a row, channels to a thread
+    const int row = t / TPR, c0 = t % TPR * CH;
+    float s[2] = {0.f, 0.f};
+    if (p.normalize)
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll 4
+        for (int c = 0; c < CH; c += 2) {
+          float x = 0.f, y = 0.f;
+#pragma unroll
+          for (int i = NI - 1; i >= 0; --i) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>((m ? lq : lk) + row * R + c0 + c + i * PL);
+            x += __uint_as_float(w << 16);
+            y += __uint_as_float(w & 0xFFFF0000u);
+          }
+          s[m] += x * x + y * y;
+        }
+#pragma unroll
+    for (int m = 1; m < TPR; m *= 2) {
+      s[0] += __shfl_xor(s[0], m);
+      s[1] += __shfl_xor(s[1], m);
+    }
+    if (t % TPR == 0) {
+      rk[row] = p.normalize ? 1.f / sqrtf(s[0] + p.eps) : 1.f;
+      rq[row] = p.normalize ? 1.f / sqrtf(s[1] + p.eps) : 1.f;
+    }
+  }
+  // blocks on and below the diagonal, k k^T and q k^T, round the wavefronts
+  constexpr int NBL = NB * (NB + 1) / 2, NU = (2 * NBL + 3) / 4;
+  f32x4 acc[NU];
+  auto unit = [&](int i, int& m, int& rb, int& cb) {  // of this wavefront
+    const int u = wv + 4 * i;
+    m = u / NBL;
+    int e = u % NBL;
+    rb = 0;
+    while (e > rb) e -= ++rb;
+    cb = e;
+    return u < 2 * NBL;
+  };
+#pragma unroll
+  for (int i = 0; i < NU; ++i) {
+    int m, rb, cb;
+    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!unit(i, m, rb, cb)) continue;
+#pragma unroll
+    for (int s = 0; s < KP / 32; ++s) acc[i] = mma((m ? tq : tk).rows(16 * rb, s), tk.rows(16 * cb, s), acc[i]);
+  }
+  __syncthreads();  // the tiles have been read; rk and rq are there
+  if (t < C) {
+    float* vec = a.vec + blk * kVecs * C + t;
+    const float G = expf(chi[t]) * (1.f + clo[t]), D = expf((chi[C - 1] - chi[t]) + (clo[C - 1] - clo[t]));
+    vec[0] = chi[t];
+    vec[C] = clo[t];
+    vec[kB * C] = be[t];
+    vec[kRk * C] = rk[t];
+    vec[kRq * C] = rq[t];
+    vec[kGk * C] = G * rk[t];
+    vec[kDk * C] = D * rk[t];
+    vec[kGq * C] = p.scale * G * rq[t];
+  }
+#pragma unroll
+  for (int i = 0; i < NU; ++i) {
+    int m, rb, cb;
+    if (!unit(i, m, rb, cb)) continue;
+    const int j = 16 * cb + col;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int x = 16 * rb + 4 * g + r;
+      const float E = expf((chi[x] - chi[j]) + (clo[x] - clo[j]));
+      acc[i][r] = j < x + m ? acc[i][r] * E * (m ? p.scale * rq[x] : be[x] * rk[x]) * rk[j] : 0.f;
+      if (!m) A[x][j] = acc[i][r];
+    }
+  }
+  __syncthreads();
+  // (1 + A)^-1: the blocks on the diagonal column by column, those below from the diagonal outwards,
+  // X_ij = -X_ii sum_{j<=l<i} A_il X_lj, on float32 matrix instructions
+  if (wv < NB) {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == col ? 1.f : 0.f;
+#pragma unroll
+      for (int l = 0; l < i; ++l) s -= A[16 * wv + i][16 * wv + l] * x[l];
+      x[i] = s;
+    }
+    if (g == 0)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) X[16 * wv + i][16 * wv + col] = x[i];
+  }
+#pragma unroll
+  for (int d = 1; d < NB; ++d) {
+    __syncthreads();
+    if (wv < NB - d) {
+      const int i = wv + d, j = wv;
+      f32x4 m = {0.f, 0.f, 0.f, 0.f}, x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int l = 0; l < d; ++l)
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          m = __builtin_amdgcn_mfma_f32_16x16x4f32(A[16 * i + col][16 * (j + l) + 4 * s + g], X[16 * (j + l) + 4 * s + g][16 * j + col],
+                                                   m, 0, 0, 0);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) x = __builtin_amdgcn_mfma_f32_16x16x4f32(X[16 * i + col][16 * i + 4 * g + s], m[s], x, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) X[16 * i + 4 * g + r][16 * j + col] = -x[r];
+    }
+  }
+  __syncthreads();
+  // P takes A's place, and both leave in parts and in spot() order
+#pragma unroll
+  for (int i = 0; i < NU; ++i) {
+    int m, rb, cb;
+    if (!unit(i, m, rb, cb) || !m) continue;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) A[16 * rb + 4 * g + r][16 * cb + col] = acc[i][r];
+  }
+  __syncthreads();
+  for (int e = t; e < 2 * C * C / 8; e += 256) {
+    const int m = e / (C * C / 8), x = e % (C * C / 8) / (C / 8), c = e % (C / 8) * 8;  // places c .. c+7 of row x
+    const int j0 = (c & ~31) | ((c & 24) >> 1);                                       // columns j0 .. j0+3 and 16 on
+    f32x4 v[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = j0 + 16 * w + r;
+        v[w][r] = j > x ? 0.f : m ? A[x][j] : X[x][j] * be[j];
+      }
+    const Frag<NP> f = pack<NP>(v[0], v[1]);
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      *reinterpret_cast<u32x4*>((m ? a.pp : a.tb) + ((blk * NP + i) * C + x) * C + c) = f.p[i];
+  }
+}
+
+// A chunk's Tb or P on its way to LDS.
+template <int NP, int C, int NT>
+struct Square {
+  static constexpr int NV = NP * C * C / 8 / NT;
+  static_assert(NP * C * C / 8 % NT == 0, "whole pieces to every thread");
+  u32x4 v[NV];
+  __device__ __forceinline__ void load(const bf16* from) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const u32x4*>(from + (threadIdx.x + i * NT) * 8);
+  }
+  __device__ __forceinline__ void store(bf16* lds) const {  // C + 8 elements a row
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (threadIdx.x + i * NT) * 8;
+      *reinterpret_cast<u32x4*>(lds + e / C * (C + 8) + e % C) = v[i];
+    }
+  }
+};
+
+// 16 columns of C rows as results lie: element r of v[rb] is row 16 rb + 4 (lane/16) + r, column lane%16.
+template <typename T, int C, bool WHOLE>
+struct Columns {
+  typedef typename Unit<sizeof(T)>::type U;
+  U v[C / 16][4];
+  // base: row 0 of this lane's column; cnt rows, `left` columns from the wavefront's first on
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int left, int cnt) {
+    const int g = threadIdx.x % 64 / 16, col = threadIdx.x % 16;
+    if constexpr (WHOLE) {
+      const rsrc_t rs = make_rsrc_wave(base - col, ((int64_t)(cnt - 1) * stride + left) * (int64_t)sizeof(T));
+      const int sb = (int)stride * (int)sizeof(T), off = col < left ? 4 * g * sb + col * (int)sizeof(T) : kOut - 64 * sb;
+#pragma unroll
+      for (int rb = 0; rb < C / 16; ++rb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[rb][r] = BufUnit<sizeof(T)>::template load<>(rs, off + (16 * rb + r) * sb);
+    } else {
+#pragma unroll
+      for (int rb = 0; rb < C / 16; ++rb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * rb + 4 * g + r;
+          const T e = col < left && row < cnt ? base[row * stride] : (T)0.f;
+          __builtin_memcpy(&v[rb][r], &e, sizeof(T));
+        }
+    }
+  }
+  __device__ __forceinline__ f32x4 get(int rb) const {
+    f32x4 f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = (float)__builtin_bit_cast(T, v[rb][r]);
+    return f;
+  }
+};
+// Results of 16 rows (row0 ..) into such columns, rows below cnt.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void put_columns(T* base, int64_t stride, int left, int cnt, int row0, f32x4 y) {
+  const int g = threadIdx.x % 64 / 16, col = threadIdx.x % 16;
+  if constexpr (WHOLE) {
+    const rsrc_t rs = make_rsrc_wave(base - col, ((int64_t)(cnt - 1) * stride + left) * (int64_t)sizeof(T));
+    const int sb = (int)stride * (int)sizeof(T), off = col < left ? (row0 + 4 * g) * sb + col * (int)sizeof(T) : kOut - 4 * sb;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      BufUnit<sizeof(T)>::template store<false>(__builtin_bit_cast(typename Unit<sizeof(T)>::type, (T)y[r]), rs, off + r * sb);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (col < left && row0 + 4 * g + r < cnt) base[(row0 + 4 * g + r) * stride] = (T)y[r];
+  }
+}
+
+// An operand of 32 rows (row0 ..) and this wavefront's 16 columns into [NP][rows][vp], `plane` elements a part.
+template <int NP>
+__device__ __forceinline__ void keep(bf16* to, int vp, int64_t plane, int row0, const Frag<NP>& f) {
+  const int g = threadIdx.x % 64 / 16;
+  uint16_t* q = reinterpret_cast<uint16_t*>(to) + (row0 + 4 * g) * vp + threadIdx.x % 16;
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      q[i * plane + (16 * (e / 4) + e % 4) * vp] = (uint16_t)(f.p[i][e / 2] >> (16 * (e % 2)));
+}
+
+constexpr int kNW = 2, kNT = kNW * 64;  // wavefronts of the chains, 16 columns each
+
+// Nothing moves across the end of a phase where registers hold two phases' operands (DEEP).
+template <bool DEEP>
+__device__ __forceinline__ void phase() {
+  if constexpr (DEEP) __builtin_amdgcn_sched_barrier(0);
+}
+
+// The states from chunk to chunk, and o.  KEEP: U and the state before each chunk for the backward instead of o.
+template <typename T, int NP, int KP, bool WHOLE, bool KEEP>
+__global__ __launch_bounds__(kNT) void dr_chain(Args a) {
+  constexpr int NI = parts_of<T>(), C = chunk_of(NI, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
+  constexpr bool DEEP = NP == 1 && KP <= 128;
+  __shared__ __align__(16) bf16 lk[NI * PL], lq[KEEP ? 8 : NI * PL], lt[NP * PC], lp[KEEP ? 8 : NP * PC];
+  __shared__ __align__(16) float lv[3][C];
+  __shared__ float last;
+  const DrProblem& p = a.p;
+  const int nvb = (a.vp + kNW * 16 - 1) / (kNW * 16);
+  const int64_t blk = a.blk0 + xcd_remap(blockIdx.x, a.nblk), bh = blk / nvb, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
+  const int lane = threadIdx.x % 64, g = lane / 16, col = lane % 16;
+  const int n0 = (int)(blk % nvb) * kNW * 16 + wave_id() * 16, nn = n0 + col, K = (int)p.K, V = (int)p.V;
+  const bool live = nn < V;
+  const int len = length_of(p, b);
+  const T* q = (const T*)p.q + b * p.qs[0] + hk * p.qs[1];
+  const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[1];
+  const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1] + nn;
+  T* o = (T*)p.o + b * p.os[0] + h * p.os[1] + n0;
+  const int64_t sb = bh * K * V + nn;
+  const Tile<NI, R, PL> tk{lk}, tq{lq};
+  const Tile<NP, RC, PC> tt{lt}, tp{lp};
+  f32x4 S[KP / 16];
+#pragma unroll
+  for (int kb = 0; kb < KP / 16; ++kb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 16 * kb + 4 * g + r;
+      S[kb][r] = live && d < K && p.s_in ? p.s_in[sb + d * V] : 0.f;
+    }
+  Rows<T, C, KP, kNT, WHOLE> rk, rq;
+  Square<NP, C, kNT> rt, rp;
+  Columns<T, C, WHOLE> cv;
+  float vec[3 * C / kNT + 1], top = 0.f;
+  auto fetch = [&](int t0) {
+    if (t0 >= len) return;
+    const int cnt = min(C, len - t0);
+    const int64_t ch = bh * a.n + t0 / C;
+    rk.load(k + (int64_t)t0 * p.ks[2], p.ks[2], K, cnt);
+    rt.load(a.tb + ch * NP * C * C);
+    cv.load(v + (int64_t)t0 * p.vs[2], p.vs[2], V - n0, cnt);
+    if (!KEEP) {
+      rq.load(q + (int64_t)t0 * p.qs[2], p.qs[2], K, cnt);
+      rp.load(a.pp + ch * NP * C * C);
+    }
+    const float* w = a.vec + ch * kVecs * C;
+#pragma unroll
+    for (int i = 0; i * kNT < 3 * C; ++i)
+      if (i * kNT + (int)threadIdx.x < 3 * C) vec[i] = w[kGk * C + i * kNT + threadIdx.x];
+    top = w[C - 1];
+  };
+  fetch(0);
+  for (int t0 = 0; t0 < len; t0 += C) {
+    const int cnt = min(C, len - t0);
+    const int64_t ch = bh * a.n + t0 / C;
+    __syncthreads();  // the chunk before has been read
+    rk.template store<R, PL, true>(lk);
+    rt.store(lt);
+    if constexpr (!KEEP) {
+      rq.template store<R, PL, true>(lq);
+      rp.store(lp);
+    }
+#pragma unroll
+    for (int i = 0; i * kNT < 3 * C; ++i)
+      if (i * kNT + (int)threadIdx.x < 3 * C) lv[0][i * kNT + threadIdx.x] = vec[i];
+    if (threadIdx.x == 0) last = top;
+    f32x4 x[NB];
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) x[rb] = cv.get(rb);
+    __syncthreads();
+    fetch(t0 + C);
+    if (n0 >= a.vp) continue;
+    // each phase's operands are on their way from LDS while the phase before computes
+    Frag<NI> kr[NB][KP / 32];
+    Frag<NP> tr[NB][NB / 2];
+#pragma unroll
+    for (int s = 0; s < KP / 32; ++s)
+#pragma unroll
+      for (int rb = 0; rb < NB; ++rb) kr[rb][s] = tk.rows(16 * rb, s);
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+      for (int s = 0; s <= rb / 2; ++s) tr[rb][s] = tt.rows(16 * rb, s);
+    phase<DEEP>();
+    Frag<NP> sf[KP / 32];
+#pragma unroll
+    for (int s = 0; s < KP / 32; ++s) {
+      sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
+      if (KEEP) keep<NP>(a.s + ch * NP * KP * a.vp + n0, a.vp, (int64_t)KP * a.vp, 32 * s, sf[s]);
+    }
+    // X = V - G k S
+    f32x4 y[NB];
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) y[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < KP / 32; ++s)
+#pragma unroll
+      for (int rb = 0; rb < NB; ++rb) y[rb] = mma(kr[rb][s], sf[s], y[rb]);
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) x[rb] -= *reinterpret_cast<const f32x4*>(&lv[0][16 * rb + 4 * g]) * y[rb];
+    Frag<NP> f[C / 32], d[C / 32];
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s) f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
+    phase<DEEP>();
+    Frag<NI> kc[KP / 16][C / 32];
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s)
+#pragma unroll
+      for (int kb = 0; kb < KP / 16; ++kb) kc[kb][s] = tk.cols(kb, s);
+    phase<DEEP>();
+    // U = Tb X
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) x[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < NB / 2; ++s)
+#pragma unroll
+      for (int rb = 2 * s; rb < NB; ++rb) x[rb] = mma(tr[rb][s], f[s], x[rb]);
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s) {
+      f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
+      if (KEEP) keep<NP>(a.u + ch * NP * C * a.vp + n0, a.vp, (int64_t)C * a.vp, 32 * s, f[s]);
+      d[s] = pack<NP>(x[2 * s] * *reinterpret_cast<const f32x4*>(&lv[1][32 * s + 4 * g]),
+                      x[2 * s + 1] * *reinterpret_cast<const f32x4*>(&lv[1][32 * s + 16 + 4 * g]));
+    }
+    // S <- G_C S + k^T D U
+    const float gc = expf(last);
+#pragma unroll
+    for (int kb = 0; kb < KP / 16; ++kb) S[kb] *= gc;
+    phase<DEEP>();
+    Frag<NI> qr[KEEP ? 1 : NB][KEEP ? 1 : KP / 32];
+    if constexpr (!KEEP) {
+#pragma unroll
+      for (int s = 0; s < KP / 32; ++s)
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) qr[rb][s] = tq.rows(16 * rb, s);
+#pragma unroll
+      for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+        for (int s = 0; s <= rb / 2; ++s) tr[rb][s] = tp.rows(16 * rb, s);
+    }
+    phase<DEEP>();
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s)
+#pragma unroll
+      for (int kb = 0; kb < KP / 16; ++kb) S[kb] = mma(kc[kb][s], d[s], S[kb]);
+    // O^T = G S^T q^T + U^T P^T: four neighbouring channels of a token in a lane
+    if constexpr (!KEEP) {
+#pragma unroll
+      for (int rb = 0; rb < NB; ++rb) y[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KP / 32; ++s)
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) y[rb] = mma(sf[s], qr[rb][s], y[rb]);
+#pragma unroll
+      for (int rb = 0; rb < NB; ++rb) y[rb] *= lv[2][16 * rb + col];
+#pragma unroll
+      for (int s = 0; s < NB / 2; ++s)
+#pragma unroll
+        for (int rb = 2 * s; rb < NB; ++rb) y[rb] = mma(f[s], tr[rb][s], y[rb]);
+      if constexpr (WHOLE) {
+        const int sb = (int)p.os[2] * (int)sizeof(T);
+        const rsrc_t rs = make_rsrc_wave(o + (int64_t)t0 * p.os[2], ((int64_t)(cnt - 1) * p.os[2] + V - n0) * (int64_t)sizeof(T));
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) {
+          const float e[4] = {y[rb][0], y[rb][1], y[rb][2], y[rb][3]};
+          bstore_vals<T, 4>(rs, 4 * g < V - n0 ? (16 * rb + col) * sb + 4 * g * (int)sizeof(T) : kOut, e);
+        }
+      } else {
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * rb + col < cnt && n0 + 4 * g + r < V) o[(int64_t)(t0 + 16 * rb + col) * p.os[2] + 4 * g + r] = (T)y[rb][r];
+      }
+    }
+  }
+  if (!live || KEEP) return;
+  if (p.s_out)
+#pragma unroll
+    for (int kb = 0; kb < KP / 16; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * kb + 4 * g + r;
+        if (d < K) p.s_out[sb + d * V] = S[kb][r];
+      }
+  for (int64_t t = len + g; t < p.T; t += 4) o[t * p.os[2] + col] = (T)0.f;
+}
+
+// The states' gradients from the last chunk on, and dv.
+template <typename T, int NP, int KP, bool WHOLE>
+__global__ __launch_bounds__(kNT) void dr_chain_bwd(Args a) {
+  constexpr int NI = parts_of<T>(), C = chunk_of(NI, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
+  constexpr bool DEEP = NP == 1 && KP <= 128;
+  __shared__ __align__(16) bf16 lk[NI * PL], lq[NI * PL], lt[NP * PC], lp[NP * PC];
+  __shared__ __align__(16) float lv[3][C];
+  __shared__ float last;
+  const DrProblem& p = a.p;
+  const int nvb = (a.vp + kNW * 16 - 1) / (kNW * 16);
+  const int64_t blk = a.blk0 + xcd_remap(blockIdx.x, a.nblk), bh = blk / nvb, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
+  const int lane = threadIdx.x % 64, g = lane / 16, col = lane % 16;
+  const int n0 = (int)(blk % nvb) * kNW * 16 + wave_id() * 16, nn = n0 + col, K = (int)p.K, V = (int)p.V;
+  const bool live = nn < V;
+  const int len = length_of(p, b);
+  const T* q = (const T*)p.q + b * p.qs[0] + hk * p.qs[1];
+  const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[1];
+  const T* d_o = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + nn;
+  T* dv = (T*)p.dv + b * p.dvs[0] + h * p.dvs[1] + nn;
+  const int64_t sb = bh * K * V + nn;
+  const Tile<NI, R, PL> tk{lk}, tq{lq};
+  const Tile<NP, RC, PC> tt{lt}, tp{lp};
+  f32x4 S[KP / 16];
+#pragma unroll
+  for (int kb = 0; kb < KP / 16; ++kb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 16 * kb + 4 * g + r;
+      S[kb][r] = live && d < K && p.ds_in ? p.ds_in[sb + d * V] : 0.f;
+    }
+  Rows<T, C, KP, kNT, WHOLE> rk, rq;
+  Square<NP, C, kNT> rt, rp;
+  Columns<T, C, WHOLE> cd;
+  float vec[3 * C / kNT + 1], top = 0.f;
+  auto fetch = [&](int t0) {
+    if (t0 < 0) return;
+    const int cnt = min(C, len - t0);
+    const int64_t ch = bh * a.n + t0 / C;
+    rk.load(k + (int64_t)t0 * p.ks[2], p.ks[2], K, cnt);
+    rq.load(q + (int64_t)t0 * p.qs[2], p.qs[2], K, cnt);
+    rt.load(a.tb + ch * NP * C * C);
+    rp.load(a.pp + ch * NP * C * C);
+    cd.load(d_o + (int64_t)t0 * p.dos[2], p.dos[2], V - n0, cnt);
+    const float* w = a.vec + ch * kVecs * C;
+#pragma unroll
+    for (int i = 0; i * kNT < 3 * C; ++i)
+      if (i * kNT + (int)threadIdx.x < 3 * C) vec[i] = w[kGk * C + i * kNT + threadIdx.x];
+    top = w[C - 1];
+  };
+  const int first = (len + C - 1) / C * C - C;
+  fetch(first);
+  for (int t0 = first; t0 >= 0; t0 -= C) {
+    const int cnt = min(C, len - t0);
+    const int64_t ch = bh * a.n + t0 / C;
+    __syncthreads();  // the chunk before has been read
+    rk.template store<R, PL, true>(lk);
+    rq.template store<R, PL, true>(lq);
+    rt.store(lt);
+    rp.store(lp);
+#pragma unroll
+    for (int i = 0; i * kNT < 3 * C; ++i)
+      if (i * kNT + (int)threadIdx.x < 3 * C) lv[0][i * kNT + threadIdx.x] = vec[i];
+    if (threadIdx.x == 0) last = top;
+    f32x4 x[NB];
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) x[rb] = cd.get(rb);
+    __syncthreads();
+    fetch(t0 - C);
+    if (n0 >= a.vp) continue;
+    // each phase's operands are on their way from LDS while the phase before computes
+    Frag<NI> kr[NB][KP / 32];
+    Frag<NP> tc[NB][NB / 2];
+#pragma unroll
+    for (int s = 0; s < KP / 32; ++s)
+#pragma unroll
+      for (int rb = 0; rb < NB; ++rb) kr[rb][s] = tk.rows(16 * rb, s);
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+      for (int s = rb / 2; s < NB / 2; ++s) tc[rb][s] = tp.cols(rb, s);
+    phase<DEEP>();
+    Frag<NP> sf[KP / 32], gd[C / 32], f[C / 32];
+    Frag<NI> df[C / 32];
+#pragma unroll
+    for (int s = 0; s < KP / 32; ++s) {
+      sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
+      keep<NP>(a.ds + ch * NP * KP * a.vp + n0, a.vp, (int64_t)KP * a.vp, 32 * s, sf[s]);
+    }
+    auto at = [&](int m, int row) { return *reinterpret_cast<const f32x4*>(&lv[m][row + 4 * g]); };
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s) {
+      df[s] = pack<NI>(x[2 * s], x[2 * s + 1]);
+      gd[s] = pack<NP>(x[2 * s] * at(2, 32 * s), x[2 * s + 1] * at(2, 32 * s + 16));
+    }
+    // dU = P^T dO + D k dS
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) x[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < KP / 32; ++s)
+#pragma unroll
+      for (int rb = 0; rb < NB; ++rb) x[rb] = mma(kr[rb][s], sf[s], x[rb]);
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) x[rb] *= at(1, 16 * rb);
+#pragma unroll
+    for (int s = 0; s < NB / 2; ++s)
+#pragma unroll
+      for (int rb = 0; rb < 2 * s + 2; ++rb) x[rb] = mma(tc[rb][s], df[s], x[rb]);
+    phase<DEEP>();
+    Frag<NI> qc[KP / 16][C / 32], kc[KP / 16][C / 32];
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+      for (int s = rb / 2; s < NB / 2; ++s) tc[rb][s] = tt.cols(rb, s);
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s)
+#pragma unroll
+      for (int kb = 0; kb < KP / 16; ++kb) qc[kb][s] = tq.cols(kb, s);
+    phase<DEEP>();
+    // dS <- G_C dS + q^T G dO - k^T G dX: its first part, beside dX = Tb^T dU
+    const float gc = expf(last);
+#pragma unroll
+    for (int kb = 0; kb < KP / 16; ++kb) S[kb] *= gc;
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s) f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) x[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < NB / 2; ++s)
+#pragma unroll
+      for (int rb = 0; rb < 2 * s + 2; ++rb) x[rb] = mma(tc[rb][s], f[s], x[rb]);
+    phase<DEEP>();
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s)
+#pragma unroll
+      for (int kb = 0; kb < KP / 16; ++kb) kc[kb][s] = tk.cols(kb, s);
+    phase<DEEP>();
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s)
+#pragma unroll
+      for (int kb = 0; kb < KP / 16; ++kb) S[kb] = mma(qc[kb][s], gd[s], S[kb]);
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) put_columns<T, WHOLE>(dv + (int64_t)t0 * p.dvs[2], p.dvs[2], V - n0, cnt, 16 * rb, x[rb]);
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s) {
+      keep<NP>(a.x + ch * NP * C * a.vp + n0, a.vp, (int64_t)C * a.vp, 32 * s, pack<NP>(x[2 * s], x[2 * s + 1]));
+      f[s] = pack<NP>(-x[2 * s] * at(0, 32 * s), -x[2 * s + 1] * at(0, 32 * s + 16));
+    }
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s)
+#pragma unroll
+      for (int kb = 0; kb < KP / 16; ++kb) S[kb] = mma(kc[kb][s], f[s], S[kb]);
+  }
+  if (!live) return;
+  if (p.ds_out)
+#pragma unroll
+    for (int kb = 0; kb < KP / 16; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * kb + 4 * g + r;
+        if (d < K) p.ds_out[sb + d * V] = S[kb][r];
+      }
+  for (int64_t t = len + g; t < p.T; t += 4) dv[t * p.dvs[2]] = (T)0.f;
+}
+
+// The sum of a value over the 16 lanes of a result's row: every lane gets it.
+__device__ __forceinline__ float sum16(float v) {
+  v += dpp_f<0xB1>(v);
+  v += dpp_f<0x4E>(v);
+  v += dpp_f<0x141>(v);
+  return v + dpp_f<0x140>(v);
+}
+
+// Gradients of q, k and the gates, chunk by chunk: the value heads of one key head to a workgroup, a quarter of the
+// channels to a wavefront.  With the rows' norms in E's place (rq_i rk_j for P, rk_i rk_j for N) the sums are those of q and
+// k themselves, before their part along the row is taken out.  ONE: one value head to a key head, whose sums need no registers
+// of their own.
+template <typename T, int NP, int KP, bool WHOLE, bool ONE>
+__global__ __launch_bounds__(256, ONE && NP == 1 && KP <= 128 ? 2 : 1) void dr_grads(Args a) {
+  constexpr int NI = parts_of<T>(), C = chunk_of(NI, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
+  constexpr int NCB = KP / 64, RV = kPiece + 8, PV = C * RV;
+  constexpr int ROWS = (NI + 2 * NP) * PV, KEYS = 2 * NI * PL;
+  __shared__ __align__(16) bf16 mem[ROWS > KEYS ? ROWS : KEYS], lm[2 * NP * PC];
+  __shared__ __align__(16) float lv[kVecs][C];
+  __shared__ float diag[C], red[3][4][C], total[4], along[2][C];
+  const Tile<NI, RV, PV> to{mem};
+  const Tile<NP, RV, PV> tu{mem + NI * PV}, tx{mem + (NI + NP) * PV};
+  const Tile<NI, R, PL> tk{mem}, tq{mem + NI * PL};
+  const Tile<NP, RC, PC> pe{lm}, ne{lm + NP * PC};
+  const DrProblem& p = a.p;
+  const int64_t blk = a.blk0 + blockIdx.x, n = blk % a.n, bhk = blk / a.n, b = bhk / p.Hk, hk = bhk % p.Hk;
+  const int t0 = (int)n * C, len = length_of(p, b), cnt = min(C, max(len - t0, 0)), rows = min(C, (int)p.T - t0), t = threadIdx.x;
+  const int K = (int)p.K, V = (int)p.V, group = ONE ? 1 : (int)(p.H / p.Hk), lane = t % 64, g = lane / 16, col = lane % 16, wv = wave_id();
+  T* dq_ = (T*)p.dq + b * p.dqs[0] + hk * p.dqs[1] + (int64_t)t0 * p.dqs[2];
+  T* dk_ = (T*)p.dk + b * p.dks[0] + hk * p.dks[1] + (int64_t)t0 * p.dks[2];
+  f32x4 sq[NB][NCB], sk[NB][NCB];
+#pragma unroll
+  for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) sq[rb][cb] = sk[rb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (t < C) along[0][t] = along[1][t] = 0.f;
+  if (cnt == 0) {  // no token of the sequence: zeros
+    for (int hd = 0; hd < group; ++hd)
+      if (t < rows) {
+        const int64_t h = hk * group + hd;
+        put_gate(p.dg, p.gdtype, b * p.dgs[0] + h * p.dgs[1] + (t0 + t) * p.dgs[2], 0.f);
+        put_gate(p.db, p.gdtype, b * p.dbs[0] + h * p.dbs[1] + (t0 + t) * p.dbs[2], 0.f);
+      }
+    for (int e = t; e < rows * K; e += 256) {
+      dq_[(int64_t)(e / K) * p.dqs[2] + e % K] = (T)0.f;
+      dk_[(int64_t)(e / K) * p.dks[2] + e % K] = (T)0.f;
+    }
+    return;
+  }
+  for (int hd = 0; hd < group; ++hd) {
+    const int64_t h = hk * group + hd, bh = b * p.H + h, ch = bh * a.n + n;
+    const T* d_o = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + (int64_t)t0 * p.dos[2];
+    __syncthreads();  // the head before has been read
+    for (int e = t; e < kVecs * C; e += 256) lv[0][e] = a.vec[ch * kVecs * C + e];
+    f32x4 dq[NB][NCB], dr[NB][NCB], dw[NB][NCB];
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) dq[rb][cb] = dr[rb][cb] = dw[rb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // dO U^T and dX U^T: each wavefront has one of them, and of its blocks of rows a small and a large one
+    const int m = wv % 2;
+    f32x4 acc[NB / 2][NB];
+    int rbs[NB / 2];
+#pragma unroll
+    for (int i = 0; i < NB / 2; ++i) {
+      rbs[i] = i ? NB - 1 - wv / 2 : wv / 2;
+#pragma unroll
+      for (int cb = 0; cb < NB; ++cb) acc[i][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float dot = 0.f;
+    for (int v0 = 0; v0 < a.vp; v0 += kPiece) {
+      const int width = min(kPiece, a.vp - v0);
+      if (v0 > 0) __syncthreads();
+      Frag<NP> fs[NCB], fd[NCB];  // the states' operands of a step, the next step's on their way
+      auto states = [&](int s) {
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+          const int64_t at = ch * NP * KP * a.vp + (int64_t)(wv * NCB * 16 + 16 * cb + col) * a.vp + v0 + 32 * s + 8 * g;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            fs[cb].p[i] = *reinterpret_cast<const u32x4*>(a.s + at + (int64_t)i * KP * a.vp);
+            fd[cb].p[i] = *reinterpret_cast<const u32x4*>(a.ds + at + (int64_t)i * KP * a.vp);
+          }
+        }
+      };
+      {
+        Rows<T, C, kPiece, 256, WHOLE> ro;
+        Rows<bf16, C, kPiece, 256, true> ru[2 * NP];
+        ro.load(d_o + v0, p.dos[2], V - v0, cnt);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          ru[i].load(a.u + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
+          ru[NP + i].load(a.x + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
+        }
+        states(0);
+        ro.template store<RV, PV, false>(mem);
+#pragma unroll
+        for (int i = 0; i < 2 * NP; ++i) ru[i].template store<RV, PV, false>(mem + (NI + i) * PV);
+      }
+      __syncthreads();
+      for (int s = 0; s < width / 32; ++s) {
+        Frag<NP> gs[NCB], gd[NCB];
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+          gs[cb] = fs[cb];
+          gd[cb] = fd[cb];
+        }
+        if (s + 1 < width / 32) states(s + 1);
+#pragma unroll
+        for (int i = 0; i < NB / 2; ++i) {
+          auto row = [&](auto f) {
+#pragma unroll
+            for (int cb = 0; cb < NB; ++cb)
+              if (cb <= rbs[i]) acc[i][cb] = mma(f, tu.rows(16 * cb, s), acc[i][cb]);
+          };
+          if (m) row(tx.rows(16 * rbs[i], s));
+          else row(to.rows(16 * rbs[i], s));
+        }
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x[2] = {0.f, 0.f}, y[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = NP - 1; i >= 0; --i) {
+              x[0] += __uint_as_float(gs[cb].p[i][e] << 16);
+              x[1] += __uint_as_float(gs[cb].p[i][e] & 0xFFFF0000u);
+              y[0] += __uint_as_float(gd[cb].p[i][e] << 16);
+              y[1] += __uint_as_float(gd[cb].p[i][e] & 0xFFFF0000u);
+            }
+            dot += x[0] * y[0] + x[1] * y[1];
+          }
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) {
+          const Frag<NI> ro = to.rows(16 * rb, s);
+          const Frag<NP> rx = tx.rows(16 * rb, s), ru = tu.rows(16 * rb, s);
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb) {
+            dq[rb][cb] = mma(ro, gs[cb], dq[rb][cb]);
+            dr[rb][cb] = mma(rx, gs[cb], dr[rb][cb]);
+            dw[rb][cb] = mma(ru, gd[cb], dw[rb][cb]);
+          }
+        }
+      }
+    }
+    // the pairs' gradients with their decays and norms, as operands
+#pragma unroll
+    for (int i = 0; i < NB / 2; ++i)
+#pragma unroll
+      for (int cb = 0; cb < NB; ++cb) {
+        if (cb / 2 > rbs[i] / 2) continue;  // above the diagonal by whole steps: not read
+        const int j = 16 * cb + col;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int x = 16 * rbs[i] + 4 * g + r;
+          const float E = expf((lv[0][x] - lv[0][j]) + (lv[1][x] - lv[1][j]));
+          const float v = m ? -lv[kRk][x] * lv[kRk][j] * E * acc[i][cb][r] : p.scale * lv[kRq][x] * lv[kRk][j] * E * acc[i][cb][r];
+          if (m && x == j) diag[x] = acc[i][cb][r];
+          uint32_t w[NP];
+          split<NP>(j < x + 1 - m ? v : 0.f, 0.f, w);
+#pragma unroll
+          for (int l = 0; l < NP; ++l)
+            reinterpret_cast<uint16_t*>(lm)[(m * NP + l) * PC + x * RC + spot(j)] = (uint16_t)w[l];
+        }
+      }
+    Rows<T, C, KP, 256, WHOLE> rk, rq;
+    rk.load((const T*)p.k + b * p.ks[0] + hk * p.ks[1] + (int64_t)t0 * p.ks[2], p.ks[2], K, cnt);
+    rq.load((const T*)p.q + b * p.qs[0] + hk * p.qs[1] + (int64_t)t0 * p.qs[2], p.qs[2], K, cnt);
+    __syncthreads();  // the rows have been read, the pairs are there
+    rk.template store<R, PL, true>(mem);
+    rq.template store<R, PL, true>(mem + NI * PL);
+    __syncthreads();
+    const float gc = expf(lv[0][C - 1]);
+    float kept = gc * dot;
+    f32x4 sums[3][NB];
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) {
+      auto at = [&](int m, int row) { return *reinterpret_cast<const f32x4*>(&lv[m][row + 4 * g]); };
+      sums[0][rb] = sums[1][rb] = sums[2][rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const f32x4 gq = at(kGq, 16 * rb), gk = at(kGk, 16 * rb), dk = at(kDk, 16 * rb);
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        const int kb = wv * NCB + cb;
+        f32x4 kv, qv;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          kv[r] = tk.at(16 * rb + 4 * g + r, 16 * kb + col);
+          qv[r] = tq.at(16 * rb + 4 * g + r, 16 * kb + col);
+        }
+        f32x4 x = dq[rb][cb] * gq, y = -dr[rb][cb] * gk, z = dw[rb][cb] * dk;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) kept += kv[r] * z[r];
+#pragma unroll
+        for (int s = 0; s < C / 32; ++s) {
+          const Frag<NI> fk = tk.cols(kb, s), fq = tq.cols(kb, s);
+          if (s <= rb / 2) {
+            x = mma(pe.rows(16 * rb, s), fk, x);
+            y = mma(ne.rows(16 * rb, s), fk, y);
+          }
+          if (s >= rb / 2) {
+            z = mma(pe.cols(rb, s), fq, z);
+            z = mma(ne.cols(rb, s), fk, z);
+          }
+        }
+        sums[0][rb] += qv * x;
+        sums[1][rb] += kv * y;
+        sums[2][rb] += kv * z;
+        sq[rb][cb] += x;
+        sk[rb][cb] += y + z;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float s = sum16(sums[i][rb][r]);
+          if (col == 0) red[i][wv][16 * rb + 4 * g + r] = s;
+        }
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) kept += __shfl_xor(kept, i);
+    if (lane == 0) total[wv] = kept;
+    __syncthreads();
+    if (wv == 0) {
+      const int i = lane < C ? lane : 0;
+      float s[3];
+#pragma unroll
+      for (int j = 0; j < 3; ++j) s[j] = (red[j][0][i] + red[j][1][i]) + (red[j][2][i] + red[j][3][i]);
+      if (lane < C) {
+        along[0][i] += s[0];
+        along[1][i] += s[1] + s[2];
+      }
+      float c = lane < C ? s[0] + (s[1] - s[2]) : 0.f;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {  // sums over the tokens from this one on
+        const float o = __shfl_down(c, d);
+        if (lane + d < 64) c += o;
+      }
+      if (lane < rows) {
+        const bool in = lane < cnt;
+        c += (total[0] + total[1]) + (total[2] + total[3]);
+        const float be = lv[kB][i];
+        put_gate(p.dg, p.gdtype, b * p.dgs[0] + h * p.dgs[1] + (t0 + lane) * p.dgs[2], in ? c : 0.f);
+        put_gate(p.db, p.gdtype, b * p.dbs[0] + h * p.dbs[1] + (t0 + lane) * p.dbs[2], in ? diag[i] / be / be : 0.f);
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * rb + 4 * g + r;
+      if (i >= rows) continue;
+      const float rki = lv[kRk][i], rqi = lv[kRq][i];
+      const float ak = p.normalize ? rki * rki * along[1][i] : 0.f, aq = p.normalize ? rqi * rqi * along[0][i] : 0.f;
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        const int c = 16 * (wv * NCB + cb) + col;
+        if (c >= K) continue;
+        dq_[(int64_t)i * p.dqs[2] + c] = (T)(i < cnt ? sq[rb][cb][r] - tq.at(i, c) * aq : 0.f);
+        dk_[(int64_t)i * p.dks[2] + c] = (T)(i < cnt ? sk[rb][cb][r] - tk.at(i, c) * ak : 0.f);
+      }
+    }
+}
+
+// The four launches of a type and a number of parts (instantiated in delta_<type>.hip).
+enum Stage { kPrep, kChain, kKeep, kChainBwd, kGrads };
+template <typename T, int NP>
+hipError_t launch(Stage st, const Args& a, bool whole, hipStream_t stream) {
+  auto run = [&](auto kernel, int threads) {
+    kernel<<<(unsigned)a.nblk, threads, 0, stream>>>(a);
+    return hipGetLastError();
+  };
+  auto pick = [&](auto kp, auto w) {
+    constexpr int KP = decltype(kp)::value;
+    constexpr bool W = decltype(w)::value;
+    switch (st) {
+      case kPrep: return run(dr_prep<T, NP, KP, W>, 256);
+      case kChain: return run(dr_chain<T, NP, KP, W, false>, kNT);
+      case kKeep: return run(dr_chain<T, NP, KP, W, true>, kNT);
+      case kChainBwd: return run(dr_chain_bwd<T, NP, KP, W>, kNT);
+      default:
+        return a.p.H == a.p.Hk ? run(dr_grads<T, NP, KP, W, true>, 256) : run(dr_grads<T, NP, KP, W, false>, 256);
+    }
+  };
+  auto size = [&](auto w) {
+    switch (cover((int)a.p.K)) {
+      case 64: return pick(std::integral_constant<int, 64>(), w);
+      case 128: return pick(std::integral_constant<int, 128>(), w);
+      default: return pick(std::integral_constant<int, 256>(), w);
+    }
+  };
+  return whole ? size(std::true_type()) : size(std::false_type());
+}
+extern template hipError_t launch<bf16, 1>(Stage, const Args&, bool, hipStream_t);
+extern template hipError_t launch<bf16, 2>(Stage, const Args&, bool, hipStream_t);
+extern template hipError_t launch<fp16, 2>(Stage, const Args&, bool, hipStream_t);
+extern template hipError_t launch<float, 3>(Stage, const Args&, bool, hipStream_t);
+
+}  // namespace dr
+}  // namespace dc
