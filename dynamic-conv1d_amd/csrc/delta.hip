@@ -80,15 +80,17 @@ bool whole16(const void* t, const int64_t (&st)[3], int64_t width, int es) {
          slim(st, width, es);
 }
 
+// whole: rows are whole pieces; then the chains' loads write LDS themselves where they can.
 hipError_t run(Stage st, Args a, bool whole, int64_t blocks) {
+  const int mode = whole ? dr::kDirect : dr::kGather;
   const DrProblem& p = a.p;
   constexpr int64_t most = most_workgroups(256);
   for (a.blk0 = 0; a.blk0 < blocks; a.blk0 += most) {
     a.nblk = (int)(blocks - a.blk0 < most ? blocks - a.blk0 : most);
-    const hipError_t e = p.dtype == kFP32 ? dr::launch<float, 3>(st, a, whole, p.stream)
-                         : p.dtype == kFP16 ? dr::launch<fp16, 2>(st, a, whole, p.stream)
-                         : p.precise ? dr::launch<bf16, 2>(st, a, whole, p.stream)
-                                     : dr::launch<bf16, 1>(st, a, whole, p.stream);
+    const hipError_t e = p.dtype == kFP32 ? dr::launch<float, 3>(st, a, mode, p.stream)
+                         : p.dtype == kFP16 ? dr::launch<fp16, 2>(st, a, mode, p.stream)
+                         : p.precise ? dr::launch<bf16, 2>(st, a, mode, p.stream)
+                                     : dr::launch<bf16, 1>(st, a, mode, p.stream);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;

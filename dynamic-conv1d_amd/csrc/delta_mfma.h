@@ -87,23 +87,32 @@ __device__ __forceinline__ Frag<N> pack(f32x4 a, f32x4 b) {
   return f;
 }
 
-// A tile in LDS: R elements from a row to the next, PL from a part to the next.
-template <int N, int R, int PL>
+// Tiles that loads write themselves have no padding: of a row's 16-byte pieces, piece i lies at i ^ turn<W>(row), so that
+// neither 16 rows of one piece nor 4 rows of 4 pieces meet in a bank.
+template <int W>
+__device__ __forceinline__ int turn(int row) {
+  return W == 64 ? (row << 1 & 4) | (row >> 2 & 3) : (row << 2 & 12) | (row >> 2 & 3);
+}
+
+// A tile in LDS: R elements from a row to the next, PL from a part to the next; TURN: its pieces turned, R of them whole.
+template <int N, int R, int PL, bool TURN = false>
 struct Tile {
   bf16* t;
   // row row0 + lane%16, step s of 32 columns
   __device__ __forceinline__ Frag<N> rows(int row0, int s) const {
     const int lane = threadIdx.x % 64;
-    const bf16* p = t + (row0 + lane % 16) * R + 32 * s + 8 * (lane / 16);
+    const bf16* p = t + (row0 + lane % 16) * R + (TURN ? 8 * ((4 * s + lane / 16) ^ turn<R>(lane % 16)) : 32 * s + 8 * (lane / 16));
     Frag<N> f;
 #pragma unroll
     for (int i = 0; i < N; ++i) f.p[i] = *reinterpret_cast<const u32x4*>(p + i * PL);
     return f;
   }
-  // column 16 cb + lane%16, step s of 32 rows (columns in spot() order)
+  // column 16 cb + lane%16 of a tile in spot() order, step s of 32 rows; of one that lies as it is, column
+  // 32 (cb/2) + 8 (lane%16/4) + 4 (cb%2) + lane%4
   __device__ __forceinline__ Frag<N> cols(int cb, int s) const {
-    const int lane = threadIdx.x % 64;
-    const bf16* p = t + (32 * s + 4 * (lane / 16) + (lane % 16) / 4) * R + 32 * (cb / 2) + 8 * (lane % 4) + 4 * (cb % 2);
+    const int lane = threadIdx.x % 64, row = 4 * (lane / 16) + (lane % 16) / 4;
+    const bf16* p = t + (32 * s + row) * R + 4 * (cb % 2) +
+                    (TURN ? 8 * ((4 * (cb / 2) + lane % 4) ^ turn<R>(row)) : 32 * (cb / 2) + 8 * (lane % 4));
     Frag<N> f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -450,34 +459,127 @@ __device__ __forceinline__ void put_columns(T* base, int64_t stride, int left, i
   }
 }
 
-// An operand of 32 rows (row0 ..) and this wavefront's 16 columns into [NP][rows][vp], `plane` elements a part.
-template <int NP>
-__device__ __forceinline__ void keep(bf16* to, int vp, int64_t plane, int row0, const Frag<NP>& f) {
-  const int g = threadIdx.x % 64 / 16;
-  uint16_t* q = reinterpret_cast<uint16_t*>(to) + (row0 + 4 * g) * vp + threadIdx.x % 16;
+// An operand of 32 rows and this wavefront's 16 columns into [NP][rows][vp], `plane` elements a part; element e of a lane is
+// row 8 g + e (states) or 16 (e/4) + 4 g + e%4 (tokens).  Neighbouring lanes trade halves, so that a store has two columns of
+// a row (48 two-byte stores a chunk took 20% of the chain that keeps).
+template <int NP, bool STATE>
+__device__ __forceinline__ void keep(bf16* to, int vp, int64_t plane, const Frag<NP>& f) {
+  const int g = threadIdx.x % 64 / 16, col = threadIdx.x % 16, odd = col % 2;
+  uint32_t* q = reinterpret_cast<uint32_t*>(to + ((STATE ? 8 : 4) * g + odd) * vp + col - odd);
+  const uint32_t sel = odd ? 0x03020706u : 0x05040100u;  // (the neighbour's, own) high halves, or (own, its) low halves
 #pragma unroll
   for (int i = 0; i < NP; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      q[i * plane + (16 * (e / 4) + e % 4) * vp] = (uint16_t)(f.p[i][e / 2] >> (16 * (e % 2)));
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t own = f.p[i][e], its = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)own, 0xB1, 0xF, 0xF, false);
+      q[(i * plane + (STATE ? 2 * e : 16 * (e / 2) + 2 * (e % 2)) * vp) / 2] = __builtin_amdgcn_perm(its, own, sel);
+    }
 }
 
 constexpr int kNW = 2, kNT = kNW * 64;  // wavefronts of the chains, 16 columns each
 
-// Nothing moves across the end of a phase where registers hold two phases' operands (DEEP).
-template <bool DEEP>
-__device__ __forceinline__ void phase() {
-  if constexpr (DEEP) __builtin_amdgcn_sched_barrier(0);
+// Nothing moves across the end of a phase: without it the compiler sinks a batch of operands to its use, which then waits.
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
+
+// A lane's part of a state: element r of S[kb] is channel 32 (kb/2) + 8 g + 4 (kb%2) + r of q and k, so that an operand of
+// two results holds 8 neighbouring channels, as they lie in a row of a tile.
+template <int KP>
+__device__ __forceinline__ void load_state(f32x4 (&S)[KP / 16], const float* from, bool live, int K, int V) {
+  const int g = threadIdx.x % 64 / 16;
+#pragma unroll
+  for (int kb = 0; kb < KP / 16; ++kb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 32 * (kb / 2) + 8 * g + 4 * (kb % 2) + r;
+      S[kb][r] = from && live && d < K ? from[d * V] : 0.f;
+    }
+}
+template <int KP>
+__device__ __forceinline__ void store_state(const f32x4 (&S)[KP / 16], float* to, int K, int V) {
+  const int g = threadIdx.x % 64 / 16;
+#pragma unroll
+  for (int kb = 0; kb < KP / 16; ++kb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 32 * (kb / 2) + 8 * g + 4 * (kb % 2) + r;
+      if (d < K) to[d * V] = S[kb][r];
+    }
 }
 
+// The chains' scales of a chunk on their way to LDS: G/|k|, D/|k|, scale G/|q|; top: the whole chunk's decay's logarithm.
+template <int C>
+struct Scales {
+  float v[(3 * C + kNT - 1) / kNT], top = 0.f;
+  __device__ __forceinline__ void load(const float* vec) {
+#pragma unroll
+    for (int i = 0; i * kNT < 3 * C; ++i) {
+      const int e = i * kNT + (int)threadIdx.x;
+      v[i] = vec[kGk * C + (e < 3 * C ? e : 0)];
+    }
+    top = vec[C - 1];
+  }
+  __device__ __forceinline__ void store(float* lds) const {
+#pragma unroll
+    for (int i = 0; i * kNT < 3 * C; ++i) {
+      const int e = i * kNT + (int)threadIdx.x;
+      if (e < 3 * C) lds[e] = v[i];
+    }
+  }
+};
+
+// C rows of W channels from memory into a turned tile, by loads that write LDS themselves (16 bytes a lane, 1 KB of the tile
+// a wavefront): no registers hold them, and nothing but settle() waits for them.  Rows from cnt on repeat the last one.
+template <int C, int W>
+__device__ __forceinline__ void load_direct(const bf16* base, int64_t stride, int cnt, bf16* lds) {
+  constexpr int PR = W / 8, N = C * PR / kNT;  // pieces of a row, loads
+  static_assert(C * PR % kNT == 0, "whole loads");
+  const rsrc_t rs = make_rsrc_wave(base, ((int64_t)(cnt - 1) * stride + W) * 2);
+  const int wv = wave_id(), lane = threadIdx.x % 64, sb = (int)stride * 2;
+  const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) bf16*)lds;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int row = ((i * kNW + wv) * 64 + lane) / PR, off = min(row, cnt - 1) * sb + 16 * ((lane % PR) ^ turn<W>(row));
+    const uint32_t at = to + (i * kNW + wv) * 1024;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rs)
+                 : "m0", "memory");
+  }
+}
+// This wavefront's direct loads have arrived (and all its other loads and stores).
+__device__ __forceinline__ void settle() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// How rows reach the chains' tiles.
+enum Mode { kGather, kWhole, kDirect };
+
+// What the chains share: the sizes of their tiles in LDS, k, q, Tb, P and the scales, twice where loads write them directly.
+// The memory is asked for at the launch: with its size in sight the compiler takes one wavefront to a SIMD for granted, and
+// 512 registers, of which half are accumulation registers, whose moves were 300 of 490 vector instructions a chunk.
+template <typename T, int NP, int KP, int MODE>
+struct ChainSize {
+  static constexpr bool DIRECT = MODE == kDirect;
+  static constexpr int NI = parts_of<T>(), C = chunk_of(NI, KP), NB = C / 16, R = KP + (DIRECT ? 0 : 24), PL = C * R,
+                       RC = C + (DIRECT ? 0 : 8), PC = C * RC;
+  static constexpr int BUF = DIRECT ? 2 : 1, KEYS = NI * PL, SQUARE = NP * PC;
+  static constexpr int bytes(bool both) { return BUF * ((both ? 2 : 1) * (KEYS + SQUARE) * 2 + 3 * C * 4); }
+  static_assert(bytes(true) <= 160 * 1024, "the LDS");
+  static constexpr int WAVES = DIRECT && NP == 1 ? 2 : 1;
+};
+
+// bf16 rows of whole tiles, where two buffers fit.
+template <typename T, int NP, int KP>
+constexpr bool kHasDirect = __is_same(T, bf16) && 2 * (4 * 64 * KP + NP * 4 * 64 * 64 + 768) <= 160 * 1024;
+
 // The states from chunk to chunk, and o.  KEEP: U and the state before each chunk for the backward instead of o.
-template <typename T, int NP, int KP, bool WHOLE, bool KEEP>
-__global__ __launch_bounds__(kNT) void dr_chain(Args a) {
-  constexpr int NI = parts_of<T>(), C = chunk_of(NI, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
-  constexpr bool DEEP = NP == 1 && KP <= 128;
-  __shared__ __align__(16) bf16 lk[NI * PL], lq[KEEP ? 8 : NI * PL], lt[NP * PC], lp[KEEP ? 8 : NP * PC];
-  __shared__ __align__(16) float lv[3][C];
-  __shared__ float last;
+template <typename T, int NP, int KP, int MODE, bool KEEP>
+__global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain(Args a) {
+  typedef ChainSize<T, NP, KP, MODE> Z;
+  constexpr int NI = Z::NI, C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
+  constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
+  extern __shared__ __align__(16) unsigned char chain_lds[];
+  float (*lv)[3][C] = reinterpret_cast<float (*)[3][C]>(chain_lds);
+  bf16 (*lk)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lv + Z::BUF);
+  bf16 (*lt)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lk + Z::BUF);
+  bf16 (*lq)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lt + Z::BUF);  // not there if KEEP
+  bf16 (*lp)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lq + Z::BUF);
   const DrProblem& p = a.p;
   const int nvb = (a.vp + kNW * 16 - 1) / (kNW * 16);
   const int64_t blk = a.blk0 + xcd_remap(blockIdx.x, a.nblk), bh = blk / nvb, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
@@ -490,96 +592,135 @@ __global__ __launch_bounds__(kNT) void dr_chain(Args a) {
   const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1] + nn;
   T* o = (T*)p.o + b * p.os[0] + h * p.os[1] + n0;
   const int64_t sb = bh * K * V + nn;
-  const Tile<NI, R, PL> tk{lk}, tq{lq};
-  const Tile<NP, RC, PC> tt{lt}, tp{lp};
   f32x4 S[KP / 16];
-#pragma unroll
-  for (int kb = 0; kb < KP / 16; ++kb)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = 16 * kb + 4 * g + r;
-      S[kb][r] = live && d < K && p.s_in ? p.s_in[sb + d * V] : 0.f;
-    }
+  load_state<KP>(S, p.s_in ? p.s_in + sb : nullptr, live, K, V);
   Rows<T, C, KP, kNT, WHOLE> rk, rq;
   Square<NP, C, kNT> rt, rp;
   Columns<T, C, WHOLE> cv;
-  float vec[3 * C / kNT + 1], top = 0.f;
-  auto fetch = [&](int t0) {
+  Scales<C> vec;
+  auto fetch = [&](int t0, int buf) {
     if (t0 >= len) return;
     const int cnt = min(C, len - t0);
     const int64_t ch = bh * a.n + t0 / C;
-    rk.load(k + (int64_t)t0 * p.ks[2], p.ks[2], K, cnt);
-    rt.load(a.tb + ch * NP * C * C);
+    const T *kt = k + (int64_t)t0 * p.ks[2], *qt = q + (int64_t)t0 * p.qs[2];
+    const bf16 *tt = a.tb + ch * NP * C * C, *pt = a.pp + ch * NP * C * C;
+    if constexpr (DIRECT) {
+      load_direct<C, KP>(kt, p.ks[2], cnt, lk[buf]);
+      load_direct<NP * C, C>(tt, C, NP * C, lt[buf]);
+      if (!KEEP) {
+        load_direct<C, KP>(qt, p.qs[2], cnt, lq[buf]);
+        load_direct<NP * C, C>(pt, C, NP * C, lp[buf]);
+      }
+    } else {
+      rk.load(kt, p.ks[2], K, cnt);
+      rt.load(tt);
+      if (!KEEP) {
+        rq.load(qt, p.qs[2], K, cnt);
+        rp.load(pt);
+      }
+    }
     cv.load(v + (int64_t)t0 * p.vs[2], p.vs[2], V - n0, cnt);
-    if (!KEEP) {
-      rq.load(q + (int64_t)t0 * p.qs[2], p.qs[2], K, cnt);
-      rp.load(a.pp + ch * NP * C * C);
-    }
-    const float* w = a.vec + ch * kVecs * C;
-#pragma unroll
-    for (int i = 0; i * kNT < 3 * C; ++i)
-      if (i * kNT + (int)threadIdx.x < 3 * C) vec[i] = w[kGk * C + i * kNT + threadIdx.x];
-    top = w[C - 1];
+    vec.load(a.vec + ch * kVecs * C);
   };
-  fetch(0);
-  for (int t0 = 0; t0 < len; t0 += C) {
-    const int cnt = min(C, len - t0);
-    const int64_t ch = bh * a.n + t0 / C;
-    __syncthreads();  // the chunk before has been read
-    rk.template store<R, PL, true>(lk);
-    rt.store(lt);
-    if constexpr (!KEEP) {
-      rq.template store<R, PL, true>(lq);
-      rp.store(lp);
+  auto arrive = [&](int buf) {  // what fetch() left in registers
+    if constexpr (!DIRECT) {
+      rk.template store<R, PL, false>(lk[buf]);
+      rt.store(lt[buf]);
+      if (!KEEP) {
+        rq.template store<R, PL, false>(lq[buf]);
+        rp.store(lp[buf]);
+      }
     }
+    vec.store(lv[buf][0]);
+  };
+  f32x4 y[NB];
+  // the outputs of the chunk at t0; those of a chunk leave during the next one, whose loads then do not wait for them
+  auto leave = [&](int t0) {
+    const int cnt = min(C, len - t0);
+    if constexpr (WHOLE) {
+      const int st = (int)p.os[2] * (int)sizeof(T);
+      const rsrc_t rs = make_rsrc_wave(o + (int64_t)t0 * p.os[2], ((int64_t)(cnt - 1) * p.os[2] + V - n0) * (int64_t)sizeof(T));
 #pragma unroll
-    for (int i = 0; i * kNT < 3 * C; ++i)
-      if (i * kNT + (int)threadIdx.x < 3 * C) lv[0][i * kNT + threadIdx.x] = vec[i];
-    if (threadIdx.x == 0) last = top;
+      for (int rb = 0; rb < NB; ++rb) {
+        const float e[4] = {y[rb][0], y[rb][1], y[rb][2], y[rb][3]};
+        bstore_vals<T, 4>(rs, 4 * g < V - n0 ? (16 * rb + col) * st + 4 * g * (int)sizeof(T) : kOut, e);
+      }
+    } else {
+#pragma unroll
+      for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * rb + col < cnt && n0 + 4 * g + r < V) o[(int64_t)(t0 + 16 * rb + col) * p.os[2] + 4 * g + r] = (T)y[rb][r];
+    }
+  };
+  fetch(0, 0);
+  int buf = 0;
+  for (int t0 = 0; t0 < len; t0 += C, buf ^= DIRECT) {
+    const int64_t ch = bh * a.n + t0 / C;
+    if (!DIRECT) __syncthreads();  // the chunk before has been read
+    arrive(buf);
+    if (DIRECT) settle();
+    __syncthreads();  // this chunk is there (and the other buffer has been read)
+    const Tile<NI, R, PL, DIRECT> tk{lk[buf]}, tq{lq[buf]};
+    const Tile<NP, RC, PC, DIRECT> tt{lt[buf]}, tp{lp[buf]};
+    const float (*sc)[C] = lv[buf];
     f32x4 x[NB];
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] = cv.get(rb);
-    __syncthreads();
-    fetch(t0 + C);
-    if (n0 >= a.vp) continue;
-    // each phase's operands are on their way from LDS while the phase before computes
-    Frag<NI> kr[NB][KP / 32];
-    Frag<NP> tr[NB][NB / 2];
+    const float gc = expf(vec.top);
+    fetch(t0 + C, buf ^ DIRECT);
+    if (!KEEP && t0 > 0) leave(t0 - C);
+    // X = V - G k S
+    Frag<NI> even[2][NB], odd[2][NB];
+    auto rows = [&](const Tile<NI, R, PL, DIRECT>& t, Frag<NI> (&f)[2][NB], int s) {
 #pragma unroll
-    for (int s = 0; s < KP / 32; ++s)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int rb = 0; rb < NB; ++rb) kr[rb][s] = tk.rows(16 * rb, s);
-#pragma unroll
-    for (int rb = 0; rb < NB; ++rb)
-#pragma unroll
-      for (int s = 0; s <= rb / 2; ++s) tr[rb][s] = tt.rows(16 * rb, s);
-    phase<DEEP>();
+        for (int rb = 0; rb < NB; ++rb) f[i][rb] = t.rows(16 * rb, s + i);
+      phase();
+    };
+    rows(tk, even, 0);
     Frag<NP> sf[KP / 32];
 #pragma unroll
     for (int s = 0; s < KP / 32; ++s) {
       sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
-      if (KEEP) keep<NP>(a.s + ch * NP * KP * a.vp + n0, a.vp, (int64_t)KP * a.vp, 32 * s, sf[s]);
+      if (KEEP) keep<NP, true>(a.s + (ch * NP * KP + 32 * s) * a.vp + n0, a.vp, (int64_t)KP * a.vp, sf[s]);
     }
-    // X = V - G k S
-    f32x4 y[NB];
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) y[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Frag<NP> tr[NB][NB / 2];
+    auto square = [&](const Tile<NP, RC, PC, DIRECT>& t) {
 #pragma unroll
-    for (int s = 0; s < KP / 32; ++s)
+      for (int rb = 0; rb < NB; ++rb)
 #pragma unroll
-      for (int rb = 0; rb < NB; ++rb) y[rb] = mma(kr[rb][s], sf[s], y[rb]);
+        for (int s = 0; s <= rb / 2; ++s) tr[rb][s] = t.rows(16 * rb, s);
+      phase();
+    };
 #pragma unroll
-    for (int rb = 0; rb < NB; ++rb) x[rb] -= *reinterpret_cast<const f32x4*>(&lv[0][16 * rb + 4 * g]) * y[rb];
+    for (int s = 0; s < KP / 32; s += 2) {
+      Frag<NI> (&now)[2][NB] = s % 4 ? odd : even, (&then)[2][NB] = s % 4 ? even : odd;
+      if (s + 2 < KP / 32) rows(tk, then, s + 2);
+      else square(tt);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) y[rb] = mma(now[i][rb], sf[s + i], y[rb]);
+      phase();
+    }
+    // operands of k^T: batches of 8, the step of 32 tokens first
+    constexpr int KN = KP / 16, NK = KN * (C / 32);
+    Frag<NI> kc[2][NK < 8 ? NK : 8];
+    auto keys = [&](int e0) {
+#pragma unroll
+      for (int e = 0; e < 8 && e < NK; ++e) kc[e0 / 8 % 2][e] = tk.cols((e0 + e) % KN, (e0 + e) / KN);
+      phase();
+    };
+    keys(0);
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) x[rb] -= *reinterpret_cast<const f32x4*>(&sc[0][16 * rb + 4 * g]) * y[rb];
     Frag<NP> f[C / 32], d[C / 32];
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
-    phase<DEEP>();
-    Frag<NI> kc[KP / 16][C / 32];
-#pragma unroll
-    for (int s = 0; s < C / 32; ++s)
-#pragma unroll
-      for (int kb = 0; kb < KP / 16; ++kb) kc[kb][s] = tk.cols(kb, s);
-    phase<DEEP>();
     // U = Tb X
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -588,84 +729,68 @@ __global__ __launch_bounds__(kNT) void dr_chain(Args a) {
 #pragma unroll
       for (int rb = 2 * s; rb < NB; ++rb) x[rb] = mma(tr[rb][s], f[s], x[rb]);
 #pragma unroll
+    for (int kb = 0; kb < KN; ++kb) S[kb] *= gc;
+#pragma unroll
     for (int s = 0; s < C / 32; ++s) {
       f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
-      if (KEEP) keep<NP>(a.u + ch * NP * C * a.vp + n0, a.vp, (int64_t)C * a.vp, 32 * s, f[s]);
-      d[s] = pack<NP>(x[2 * s] * *reinterpret_cast<const f32x4*>(&lv[1][32 * s + 4 * g]),
-                      x[2 * s + 1] * *reinterpret_cast<const f32x4*>(&lv[1][32 * s + 16 + 4 * g]));
+      if (KEEP) keep<NP, false>(a.u + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, f[s]);
+      d[s] = pack<NP>(x[2 * s] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 4 * g]),
+                      x[2 * s + 1] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 16 + 4 * g]));
     }
+    phase();
     // S <- G_C S + k^T D U
-    const float gc = expf(last);
 #pragma unroll
-    for (int kb = 0; kb < KP / 16; ++kb) S[kb] *= gc;
-    phase<DEEP>();
-    Frag<NI> qr[KEEP ? 1 : NB][KEEP ? 1 : KP / 32];
-    if constexpr (!KEEP) {
+    for (int e0 = 0; e0 < NK; e0 += 8) {
+      if (e0 + 8 < NK) keys(e0 + 8);
+      else if (!KEEP) rows(tq, even, 0);
 #pragma unroll
-      for (int s = 0; s < KP / 32; ++s)
-#pragma unroll
-        for (int rb = 0; rb < NB; ++rb) qr[rb][s] = tq.rows(16 * rb, s);
-#pragma unroll
-      for (int rb = 0; rb < NB; ++rb)
-#pragma unroll
-        for (int s = 0; s <= rb / 2; ++s) tr[rb][s] = tp.rows(16 * rb, s);
+      for (int e = 0; e < 8 && e < NK; ++e) {
+        const int kb = (e0 + e) % KN, s = (e0 + e) / KN;
+        S[kb] = mma(kc[e0 / 8 % 2][e], d[s], S[kb]);
+      }
+      phase();
     }
-    phase<DEEP>();
-#pragma unroll
-    for (int s = 0; s < C / 32; ++s)
-#pragma unroll
-      for (int kb = 0; kb < KP / 16; ++kb) S[kb] = mma(kc[kb][s], d[s], S[kb]);
     // O^T = G S^T q^T + U^T P^T: four neighbouring channels of a token in a lane
     if constexpr (!KEEP) {
 #pragma unroll
       for (int rb = 0; rb < NB; ++rb) y[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < KP / 32; ++s)
+      for (int s = 0; s < KP / 32; s += 2) {
+        Frag<NI> (&now)[2][NB] = s % 4 ? odd : even, (&then)[2][NB] = s % 4 ? even : odd;
+        if (s + 2 < KP / 32) rows(tq, then, s + 2);
+        else square(tp);
 #pragma unroll
-        for (int rb = 0; rb < NB; ++rb) y[rb] = mma(sf[s], qr[rb][s], y[rb]);
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int rb = 0; rb < NB; ++rb) y[rb] *= lv[2][16 * rb + col];
+          for (int rb = 0; rb < NB; ++rb) y[rb] = mma(sf[s + i], now[i][rb], y[rb]);
+        phase();
+      }
+#pragma unroll
+      for (int rb = 0; rb < NB; ++rb) y[rb] *= sc[2][16 * rb + col];
 #pragma unroll
       for (int s = 0; s < NB / 2; ++s)
 #pragma unroll
         for (int rb = 2 * s; rb < NB; ++rb) y[rb] = mma(f[s], tr[rb][s], y[rb]);
-      if constexpr (WHOLE) {
-        const int sb = (int)p.os[2] * (int)sizeof(T);
-        const rsrc_t rs = make_rsrc_wave(o + (int64_t)t0 * p.os[2], ((int64_t)(cnt - 1) * p.os[2] + V - n0) * (int64_t)sizeof(T));
-#pragma unroll
-        for (int rb = 0; rb < NB; ++rb) {
-          const float e[4] = {y[rb][0], y[rb][1], y[rb][2], y[rb][3]};
-          bstore_vals<T, 4>(rs, 4 * g < V - n0 ? (16 * rb + col) * sb + 4 * g * (int)sizeof(T) : kOut, e);
-        }
-      } else {
-#pragma unroll
-        for (int rb = 0; rb < NB; ++rb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (16 * rb + col < cnt && n0 + 4 * g + r < V) o[(int64_t)(t0 + 16 * rb + col) * p.os[2] + 4 * g + r] = (T)y[rb][r];
-      }
     }
   }
+  if (!KEEP && len > 0) leave((len - 1) / C * C);
   if (!live || KEEP) return;
-  if (p.s_out)
-#pragma unroll
-    for (int kb = 0; kb < KP / 16; ++kb)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * kb + 4 * g + r;
-        if (d < K) p.s_out[sb + d * V] = S[kb][r];
-      }
+  if (p.s_out) store_state<KP>(S, p.s_out + sb, K, V);
   for (int64_t t = len + g; t < p.T; t += 4) o[t * p.os[2] + col] = (T)0.f;
 }
 
 // The states' gradients from the last chunk on, and dv.
-template <typename T, int NP, int KP, bool WHOLE>
-__global__ __launch_bounds__(kNT) void dr_chain_bwd(Args a) {
-  constexpr int NI = parts_of<T>(), C = chunk_of(NI, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
-  constexpr bool DEEP = NP == 1 && KP <= 128;
-  __shared__ __align__(16) bf16 lk[NI * PL], lq[NI * PL], lt[NP * PC], lp[NP * PC];
-  __shared__ __align__(16) float lv[3][C];
-  __shared__ float last;
+template <typename T, int NP, int KP, int MODE>
+__global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain_bwd(Args a) {
+  typedef ChainSize<T, NP, KP, MODE> Z;
+  constexpr int NI = Z::NI, C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
+  constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
+  extern __shared__ __align__(16) unsigned char chain_lds[];
+  float (*lv)[3][C] = reinterpret_cast<float (*)[3][C]>(chain_lds);
+  bf16 (*lk)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lv + Z::BUF);
+  bf16 (*lt)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lk + Z::BUF);
+  bf16 (*lq)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lt + Z::BUF);
+  bf16 (*lp)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lq + Z::BUF);
   const DrProblem& p = a.p;
   const int nvb = (a.vp + kNW * 16 - 1) / (kNW * 16);
   const int64_t blk = a.blk0 + xcd_remap(blockIdx.x, a.nblk), bh = blk / nvb, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
@@ -678,75 +803,76 @@ __global__ __launch_bounds__(kNT) void dr_chain_bwd(Args a) {
   const T* d_o = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + nn;
   T* dv = (T*)p.dv + b * p.dvs[0] + h * p.dvs[1] + nn;
   const int64_t sb = bh * K * V + nn;
-  const Tile<NI, R, PL> tk{lk}, tq{lq};
-  const Tile<NP, RC, PC> tt{lt}, tp{lp};
   f32x4 S[KP / 16];
-#pragma unroll
-  for (int kb = 0; kb < KP / 16; ++kb)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = 16 * kb + 4 * g + r;
-      S[kb][r] = live && d < K && p.ds_in ? p.ds_in[sb + d * V] : 0.f;
-    }
+  load_state<KP>(S, p.ds_in ? p.ds_in + sb : nullptr, live, K, V);
   Rows<T, C, KP, kNT, WHOLE> rk, rq;
   Square<NP, C, kNT> rt, rp;
   Columns<T, C, WHOLE> cd;
-  float vec[3 * C / kNT + 1], top = 0.f;
-  auto fetch = [&](int t0) {
+  Scales<C> vec;
+  auto fetch = [&](int t0, int buf) {
     if (t0 < 0) return;
     const int cnt = min(C, len - t0);
     const int64_t ch = bh * a.n + t0 / C;
-    rk.load(k + (int64_t)t0 * p.ks[2], p.ks[2], K, cnt);
-    rq.load(q + (int64_t)t0 * p.qs[2], p.qs[2], K, cnt);
-    rt.load(a.tb + ch * NP * C * C);
-    rp.load(a.pp + ch * NP * C * C);
+    const T *kt = k + (int64_t)t0 * p.ks[2], *qt = q + (int64_t)t0 * p.qs[2];
+    const bf16 *tt = a.tb + ch * NP * C * C, *pt = a.pp + ch * NP * C * C;
+    if constexpr (DIRECT) {
+      load_direct<C, KP>(kt, p.ks[2], cnt, lk[buf]);
+      load_direct<NP * C, C>(tt, C, NP * C, lt[buf]);
+      load_direct<C, KP>(qt, p.qs[2], cnt, lq[buf]);
+      load_direct<NP * C, C>(pt, C, NP * C, lp[buf]);
+    } else {
+      rk.load(kt, p.ks[2], K, cnt);
+      rt.load(tt);
+      rq.load(qt, p.qs[2], K, cnt);
+      rp.load(pt);
+    }
     cd.load(d_o + (int64_t)t0 * p.dos[2], p.dos[2], V - n0, cnt);
-    const float* w = a.vec + ch * kVecs * C;
-#pragma unroll
-    for (int i = 0; i * kNT < 3 * C; ++i)
-      if (i * kNT + (int)threadIdx.x < 3 * C) vec[i] = w[kGk * C + i * kNT + threadIdx.x];
-    top = w[C - 1];
+    vec.load(a.vec + ch * kVecs * C);
+  };
+  auto arrive = [&](int buf) {  // what fetch() left in registers
+    if constexpr (!DIRECT) {
+      rk.template store<R, PL, false>(lk[buf]);
+      rt.store(lt[buf]);
+      rq.template store<R, PL, false>(lq[buf]);
+      rp.store(lp[buf]);
+    }
+    vec.store(lv[buf][0]);
   };
   const int first = (len + C - 1) / C * C - C;
-  fetch(first);
-  for (int t0 = first; t0 >= 0; t0 -= C) {
+  fetch(first, 0);
+  int buf = 0;
+  for (int t0 = first; t0 >= 0; t0 -= C, buf ^= DIRECT) {
     const int cnt = min(C, len - t0);
     const int64_t ch = bh * a.n + t0 / C;
-    __syncthreads();  // the chunk before has been read
-    rk.template store<R, PL, true>(lk);
-    rq.template store<R, PL, true>(lq);
-    rt.store(lt);
-    rp.store(lp);
-#pragma unroll
-    for (int i = 0; i * kNT < 3 * C; ++i)
-      if (i * kNT + (int)threadIdx.x < 3 * C) lv[0][i * kNT + threadIdx.x] = vec[i];
-    if (threadIdx.x == 0) last = top;
+    if (!DIRECT) __syncthreads();  // the chunk before has been read
+    arrive(buf);
+    if (DIRECT) settle();
+    __syncthreads();  // this chunk is there (and the other buffer has been read)
+    const Tile<NI, R, PL, DIRECT> tk{lk[buf]}, tq{lq[buf]};
+    const Tile<NP, RC, PC, DIRECT> tt{lt[buf]}, tp{lp[buf]};
+    const float (*sc)[C] = lv[buf];
     f32x4 x[NB];
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] = cd.get(rb);
-    __syncthreads();
-    fetch(t0 - C);
-    if (n0 >= a.vp) continue;
-    // each phase's operands are on their way from LDS while the phase before computes
-    Frag<NI> kr[NB][KP / 32];
-    Frag<NP> tc[NB][NB / 2];
+    const float gc = expf(vec.top);
+    fetch(t0 - C, buf ^ DIRECT);
+    auto at = [&](int m, int row) { return *reinterpret_cast<const f32x4*>(&sc[m][row + 4 * g]); };
+    Frag<NI> even[2][NB], odd[2][NB];
+    auto rows = [&](Frag<NI> (&f)[2][NB], int s) {
 #pragma unroll
-    for (int s = 0; s < KP / 32; ++s)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int rb = 0; rb < NB; ++rb) kr[rb][s] = tk.rows(16 * rb, s);
-#pragma unroll
-    for (int rb = 0; rb < NB; ++rb)
-#pragma unroll
-      for (int s = rb / 2; s < NB / 2; ++s) tc[rb][s] = tp.cols(rb, s);
-    phase<DEEP>();
+        for (int rb = 0; rb < NB; ++rb) f[i][rb] = tk.rows(16 * rb, s + i);
+      phase();
+    };
+    rows(even, 0);
     Frag<NP> sf[KP / 32], gd[C / 32], f[C / 32];
     Frag<NI> df[C / 32];
 #pragma unroll
     for (int s = 0; s < KP / 32; ++s) {
       sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
-      keep<NP>(a.ds + ch * NP * KP * a.vp + n0, a.vp, (int64_t)KP * a.vp, 32 * s, sf[s]);
+      keep<NP, true>(a.ds + (ch * NP * KP + 32 * s) * a.vp + n0, a.vp, (int64_t)KP * a.vp, sf[s]);
     }
-    auto at = [&](int m, int row) { return *reinterpret_cast<const f32x4*>(&lv[m][row + 4 * g]); };
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) {
       df[s] = pack<NI>(x[2 * s], x[2 * s + 1]);
@@ -755,70 +881,83 @@ __global__ __launch_bounds__(kNT) void dr_chain_bwd(Args a) {
     // dU = P^T dO + D k dS
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Frag<NP> tc[NB][NB / 2];
+    auto square = [&](const Tile<NP, RC, PC, DIRECT>& t) {
 #pragma unroll
-    for (int s = 0; s < KP / 32; ++s)
+      for (int rb = 0; rb < NB; ++rb)
 #pragma unroll
-      for (int rb = 0; rb < NB; ++rb) x[rb] = mma(kr[rb][s], sf[s], x[rb]);
+        for (int s = rb / 2; s < NB / 2; ++s) tc[rb][s] = t.cols(rb, s);
+      phase();
+    };
+#pragma unroll
+    for (int s = 0; s < KP / 32; s += 2) {
+      Frag<NI> (&now)[2][NB] = s % 4 ? odd : even, (&then)[2][NB] = s % 4 ? even : odd;
+      if (s + 2 < KP / 32) rows(then, s + 2);
+      else square(tp);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) x[rb] = mma(now[i][rb], sf[s + i], x[rb]);
+      phase();
+    }
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] *= at(1, 16 * rb);
 #pragma unroll
     for (int s = 0; s < NB / 2; ++s)
 #pragma unroll
       for (int rb = 0; rb < 2 * s + 2; ++rb) x[rb] = mma(tc[rb][s], df[s], x[rb]);
-    phase<DEEP>();
-    Frag<NI> qc[KP / 16][C / 32], kc[KP / 16][C / 32];
-#pragma unroll
-    for (int rb = 0; rb < NB; ++rb)
-#pragma unroll
-      for (int s = rb / 2; s < NB / 2; ++s) tc[rb][s] = tt.cols(rb, s);
-#pragma unroll
-    for (int s = 0; s < C / 32; ++s)
-#pragma unroll
-      for (int kb = 0; kb < KP / 16; ++kb) qc[kb][s] = tq.cols(kb, s);
-    phase<DEEP>();
+    phase();
     // dS <- G_C dS + q^T G dO - k^T G dX: its first part, beside dX = Tb^T dU
-    const float gc = expf(last);
+    square(tt);
+    constexpr int KN = KP / 16, NK = KN * (C / 32);
+    Frag<NI> kc[2][NK < 8 ? NK : 8];
+    auto keys = [&](const Tile<NI, R, PL, DIRECT>& t, int e0) {
 #pragma unroll
-    for (int kb = 0; kb < KP / 16; ++kb) S[kb] *= gc;
+      for (int e = 0; e < 8 && e < NK; ++e) kc[e0 / 8 % 2][e] = t.cols((e0 + e) % KN, (e0 + e) / KN);
+      phase();
+    };
+    keys(tq, 0);
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
+#pragma unroll
+    for (int kb = 0; kb < KN; ++kb) S[kb] *= gc;
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < NB / 2; ++s)
 #pragma unroll
       for (int rb = 0; rb < 2 * s + 2; ++rb) x[rb] = mma(tc[rb][s], f[s], x[rb]);
-    phase<DEEP>();
+    phase();
+    constexpr int NBATCH = (NK + 7) / 8;
 #pragma unroll
-    for (int s = 0; s < C / 32; ++s)
+    for (int i = 0; i < 2 * NBATCH; ++i) {  // q's batches, then k's
+      const int e0 = i % NBATCH * 8, slot = i % 2;
+      auto load = [&](int j) {
 #pragma unroll
-      for (int kb = 0; kb < KP / 16; ++kb) kc[kb][s] = tk.cols(kb, s);
-    phase<DEEP>();
+        for (int e = 0; e < 8 && e < NK; ++e)
+          kc[j % 2][e] = (j < NBATCH ? tq : tk).cols((j % NBATCH * 8 + e) % KN, (j % NBATCH * 8 + e) / KN);
+        phase();
+      };
+      if (i + 1 < 2 * NBATCH) load(i + 1);
 #pragma unroll
-    for (int s = 0; s < C / 32; ++s)
+      for (int e = 0; e < 8 && e < NK; ++e) {
+        const int kb = (e0 + e) % KN, s = (e0 + e) / KN;
+        S[kb] = mma(kc[slot][e], i < NBATCH ? gd[s] : f[s], S[kb]);
+      }
+      if (i == 0) {
 #pragma unroll
-      for (int kb = 0; kb < KP / 16; ++kb) S[kb] = mma(qc[kb][s], gd[s], S[kb]);
+        for (int rb = 0; rb < NB; ++rb) put_columns<T, WHOLE>(dv + (int64_t)t0 * p.dvs[2], p.dvs[2], V - n0, cnt, 16 * rb, x[rb]);
 #pragma unroll
-    for (int rb = 0; rb < NB; ++rb) put_columns<T, WHOLE>(dv + (int64_t)t0 * p.dvs[2], p.dvs[2], V - n0, cnt, 16 * rb, x[rb]);
-#pragma unroll
-    for (int s = 0; s < C / 32; ++s) {
-      keep<NP>(a.x + ch * NP * C * a.vp + n0, a.vp, (int64_t)C * a.vp, 32 * s, pack<NP>(x[2 * s], x[2 * s + 1]));
-      f[s] = pack<NP>(-x[2 * s] * at(0, 32 * s), -x[2 * s + 1] * at(0, 32 * s + 16));
+        for (int s = 0; s < C / 32; ++s) {
+          keep<NP, false>(a.x + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, pack<NP>(x[2 * s], x[2 * s + 1]));
+          f[s] = pack<NP>(-x[2 * s] * at(0, 32 * s), -x[2 * s + 1] * at(0, 32 * s + 16));
+        }
+      }
+      phase();
     }
-#pragma unroll
-    for (int s = 0; s < C / 32; ++s)
-#pragma unroll
-      for (int kb = 0; kb < KP / 16; ++kb) S[kb] = mma(kc[kb][s], f[s], S[kb]);
   }
   if (!live) return;
-  if (p.ds_out)
-#pragma unroll
-    for (int kb = 0; kb < KP / 16; ++kb)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * kb + 4 * g + r;
-        if (d < K) p.ds_out[sb + d * V] = S[kb][r];
-      }
+  if (p.ds_out) store_state<KP>(S, p.ds_out + sb, K, V);
   for (int64_t t = len + g; t < p.T; t += 4) dv[t * p.dvs[2]] = (T)0.f;
 }
 
@@ -1089,25 +1228,30 @@ __global__ __launch_bounds__(256, ONE && NP == 1 && KP <= 128 ? 2 : 1) void dr_g
     }
 }
 
-// The four launches of a type and a number of parts (instantiated in delta_<type>.hip).
+// The launches of a type and a number of parts (instantiated in delta_<type>.hip).
 enum Stage { kPrep, kChain, kKeep, kChainBwd, kGrads };
 template <typename T, int NP>
-hipError_t launch(Stage st, const Args& a, bool whole, hipStream_t stream) {
-  auto run = [&](auto kernel, int threads) {
-    kernel<<<(unsigned)a.nblk, threads, 0, stream>>>(a);
+hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
+  auto run = [&](auto kernel, int threads, int lds) {
+    kernel<<<(unsigned)a.nblk, threads, lds, stream>>>(a);
     return hipGetLastError();
+  };
+  auto chain = [&](auto kp, auto m) {
+    constexpr int KP = decltype(kp)::value, M = decltype(m)::value;
+    typedef ChainSize<T, NP, KP, M> Z;
+    if (st == kChain) return run(dr_chain<T, NP, KP, M, false>, kNT, Z::bytes(true));
+    if (st == kKeep) return run(dr_chain<T, NP, KP, M, true>, kNT, Z::bytes(false));
+    return run(dr_chain_bwd<T, NP, KP, M>, kNT, Z::bytes(true));
   };
   auto pick = [&](auto kp, auto w) {
     constexpr int KP = decltype(kp)::value;
     constexpr bool W = decltype(w)::value;
-    switch (st) {
-      case kPrep: return run(dr_prep<T, NP, KP, W>, 256);
-      case kChain: return run(dr_chain<T, NP, KP, W, false>, kNT);
-      case kKeep: return run(dr_chain<T, NP, KP, W, true>, kNT);
-      case kChainBwd: return run(dr_chain_bwd<T, NP, KP, W>, kNT);
-      default:
-        return a.p.H == a.p.Hk ? run(dr_grads<T, NP, KP, W, true>, 256) : run(dr_grads<T, NP, KP, W, false>, 256);
-    }
+    if (st == kPrep) return run(dr_prep<T, NP, KP, W>, 256, 0);
+    if (st == kGrads)
+      return a.p.H == a.p.Hk ? run(dr_grads<T, NP, KP, W, true>, 256, 0) : run(dr_grads<T, NP, KP, W, false>, 256, 0);
+    if constexpr (W && kHasDirect<T, NP, KP>)
+      if (mode == kDirect && a.p.K == KP) return chain(kp, std::integral_constant<int, kDirect>());
+    return chain(kp, std::integral_constant<int, W ? kWhole : kGather>());
   };
   auto size = [&](auto w) {
     switch (cover((int)a.p.K)) {
@@ -1116,12 +1260,12 @@ hipError_t launch(Stage st, const Args& a, bool whole, hipStream_t stream) {
       default: return pick(std::integral_constant<int, 256>(), w);
     }
   };
-  return whole ? size(std::true_type()) : size(std::false_type());
+  return mode != kGather ? size(std::true_type()) : size(std::false_type());
 }
-extern template hipError_t launch<bf16, 1>(Stage, const Args&, bool, hipStream_t);
-extern template hipError_t launch<bf16, 2>(Stage, const Args&, bool, hipStream_t);
-extern template hipError_t launch<fp16, 2>(Stage, const Args&, bool, hipStream_t);
-extern template hipError_t launch<float, 3>(Stage, const Args&, bool, hipStream_t);
+extern template hipError_t launch<bf16, 1>(Stage, const Args&, int, hipStream_t);
+extern template hipError_t launch<bf16, 2>(Stage, const Args&, int, hipStream_t);
+extern template hipError_t launch<fp16, 2>(Stage, const Args&, int, hipStream_t);
+extern template hipError_t launch<float, 3>(Stage, const Args&, int, hipStream_t);
 
 }  // namespace dr
 }  // namespace dc
