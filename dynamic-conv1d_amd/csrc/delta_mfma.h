@@ -414,16 +414,27 @@ template <typename T, int C, bool WHOLE>
 struct Columns {
   typedef typename Unit<sizeof(T)>::type U;
   U v[C / 16][4];
+  __device__ static __forceinline__ U load1(rsrc_t rs, int off, int more) {
+    if constexpr (sizeof(T) == 2) return (U)__builtin_amdgcn_raw_buffer_load_b16(rs, off, more, 0);
+    else return (U)__builtin_amdgcn_raw_buffer_load_b32(rs, off, more, 0);
+  }
   // base: row 0 of this lane's column; cnt rows, `left` columns from the wavefront's first on
   __device__ __forceinline__ void load(const T* base, int64_t stride, int left, int cnt) {
     const int g = threadIdx.x % 64 / 16, col = threadIdx.x % 16;
     if constexpr (WHOLE) {
       const rsrc_t rs = make_rsrc_wave(base - col, ((int64_t)(cnt - 1) * stride + left) * (int64_t)sizeof(T));
       const int sb = (int)stride * (int)sizeof(T), off = col < left ? 4 * g * sb + col * (int)sizeof(T) : kOut - 64 * sb;
+      if (cnt == C) {  // every row is there: the range need only drop columns, which it does without the scalar offset
 #pragma unroll
-      for (int rb = 0; rb < C / 16; ++rb)
+        for (int rb = 0; rb < C / 16; ++rb)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[rb][r] = BufUnit<sizeof(T)>::template load<>(rs, off + (16 * rb + r) * sb);
+          for (int r = 0; r < 4; ++r) v[rb][r] = load1(rs, off, (16 * rb + r) * sb);
+      } else {
+#pragma unroll
+        for (int rb = 0; rb < C / 16; ++rb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[rb][r] = load1(rs, off + (16 * rb + r) * sb, 0);
+      }
     } else {
 #pragma unroll
       for (int rb = 0; rb < C / 16; ++rb)
@@ -528,24 +539,34 @@ struct Scales {
 };
 
 // C rows of W channels from memory into a turned tile, by loads that write LDS themselves (16 bytes a lane, 1 KB of the tile
-// a wavefront): no registers hold them, and nothing but settle() waits for them.  Rows from cnt on repeat the last one.
+// a wavefront): no registers hold them.  Rows from cnt on repeat the last one.  Memory operations complete in order: a
+// wavefront that has waited for a later load of its own (the scales, which it stores to LDS) has these in LDS too, and the
+// barrier after that makes them everybody's.  Waiting for all, stores among them, took half of the time of the chains that
+// keep states.
 template <int C, int W>
 __device__ __forceinline__ void load_direct(const bf16* base, int64_t stride, int cnt, bf16* lds) {
-  constexpr int PR = W / 8, N = C * PR / kNT;  // pieces of a row, loads
-  static_assert(C * PR % kNT == 0, "whole loads");
+  constexpr int PR = W / 8, N = C * PR / kNT, VAR = W / 64;  // pieces of a row, loads, loads to 16 rows
+  static_assert(C * PR % kNT == 0 && N % VAR == 0, "whole loads");
   const rsrc_t rs = make_rsrc_wave(base, ((int64_t)(cnt - 1) * stride + W) * 2);
   const int wv = wave_id(), lane = threadIdx.x % 64, sb = (int)stride * 2;
-  const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) bf16*)lds;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int row = ((i * kNW + wv) * 64 + lane) / PR, off = min(row, cnt - 1) * sb + 16 * ((lane % PR) ^ turn<W>(row));
-    const uint32_t at = to + (i * kNW + wv) * 1024;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rs)
+  const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) bf16*)lds + wv * 1024;
+  auto place = [&](int i, int last) {
+    const int row = ((i * kNW + wv) * 64 + lane) / PR;
+    return min(row, last) * sb + 16 * ((lane % PR) ^ turn<W>(row));
+  };
+  auto load = [&](int i, int off, int more) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to + i * kNW * 1024), "v"(off),
+                 "s"(rs), "s"(more)
                  : "m0", "memory");
+  };
+  if (cnt == C) {  // the turns repeat after 16 rows
+#pragma unroll
+    for (int i = 0; i < N; ++i) load(i, place(i % VAR, C), i / VAR * 16 * sb);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) load(i, place(i, cnt - 1), 0);
   }
 }
-// This wavefront's direct loads have arrived (and all its other loads and stores).
-__device__ __forceinline__ void settle() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // How rows reach the chains' tiles.
 enum Mode { kGather, kWhole, kDirect };
@@ -633,43 +654,25 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
     }
     vec.store(lv[buf][0]);
   };
-  f32x4 y[NB];
-  // the outputs of the chunk at t0; those of a chunk leave during the next one, whose loads then do not wait for them
-  auto leave = [&](int t0) {
-    const int cnt = min(C, len - t0);
-    if constexpr (WHOLE) {
-      const int st = (int)p.os[2] * (int)sizeof(T);
-      const rsrc_t rs = make_rsrc_wave(o + (int64_t)t0 * p.os[2], ((int64_t)(cnt - 1) * p.os[2] + V - n0) * (int64_t)sizeof(T));
-#pragma unroll
-      for (int rb = 0; rb < NB; ++rb) {
-        const float e[4] = {y[rb][0], y[rb][1], y[rb][2], y[rb][3]};
-        bstore_vals<T, 4>(rs, 4 * g < V - n0 ? (16 * rb + col) * st + 4 * g * (int)sizeof(T) : kOut, e);
-      }
-    } else {
-#pragma unroll
-      for (int rb = 0; rb < NB; ++rb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (16 * rb + col < cnt && n0 + 4 * g + r < V) o[(int64_t)(t0 + 16 * rb + col) * p.os[2] + 4 * g + r] = (T)y[rb][r];
-    }
-  };
   fetch(0, 0);
+  f32x4 x[NB];
+  auto arrived = [&](int buf) {
+    arrive(buf);
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) x[rb] = cv.get(rb);
+  };
+  arrived(0);
   int buf = 0;
   for (int t0 = 0; t0 < len; t0 += C, buf ^= DIRECT) {
+    const int cnt = min(C, len - t0);
     const int64_t ch = bh * a.n + t0 / C;
-    if (!DIRECT) __syncthreads();  // the chunk before has been read
-    arrive(buf);
-    if (DIRECT) settle();
     __syncthreads();  // this chunk is there (and the other buffer has been read)
     const Tile<NI, R, PL, DIRECT> tk{lk[buf]}, tq{lq[buf]};
     const Tile<NP, RC, PC, DIRECT> tt{lt[buf]}, tp{lp[buf]};
     const float (*sc)[C] = lv[buf];
-    f32x4 x[NB];
-#pragma unroll
-    for (int rb = 0; rb < NB; ++rb) x[rb] = cv.get(rb);
     const float gc = expf(vec.top);
     fetch(t0 + C, buf ^ DIRECT);
-    if (!KEEP && t0 > 0) leave(t0 - C);
+    f32x4 y[NB];
     // X = V - G k S
     Frag<NI> even[2][NB], odd[2][NB];
     auto rows = [&](const Tile<NI, R, PL, DIRECT>& t, Frag<NI> (&f)[2][NB], int s) {
@@ -771,9 +774,28 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
       for (int s = 0; s < NB / 2; ++s)
 #pragma unroll
         for (int rb = 2 * s; rb < NB; ++rb) y[rb] = mma(f[s], tr[rb][s], y[rb]);
+      if constexpr (WHOLE) {
+        const int st = (int)p.os[2] * (int)sizeof(T);
+        const rsrc_t rs = make_rsrc_wave(o + (int64_t)t0 * p.os[2], ((int64_t)(cnt - 1) * p.os[2] + V - n0) * (int64_t)sizeof(T));
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) {
+          const float e[4] = {y[rb][0], y[rb][1], y[rb][2], y[rb][3]};
+          bstore_vals<T, 4>(rs, 4 * g < V - n0 ? (16 * rb + col) * st + 4 * g * (int)sizeof(T) : kOut, e);
+        }
+      } else {
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * rb + col < cnt && n0 + 4 * g + r < V) o[(int64_t)(t0 + 16 * rb + col) * p.os[2] + 4 * g + r] = (T)y[rb][r];
+      }
+    }
+    // waited for where its loads were issued, in one iteration: stores since then need not have ended
+    if (t0 + C < len) {
+      if (!DIRECT) __syncthreads();  // this chunk has been read
+      arrived(buf ^ DIRECT);
     }
   }
-  if (!KEEP && len > 0) leave((len - 1) / C * C);
   if (!live || KEEP) return;
   if (p.s_out) store_state<KP>(S, p.s_out + sb, K, V);
   for (int64_t t = len + g; t < p.T; t += 4) o[t * p.os[2] + col] = (T)0.f;
@@ -839,21 +861,22 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
     vec.store(lv[buf][0]);
   };
   const int first = (len + C - 1) / C * C - C;
-  fetch(first, 0);
+  if (first >= 0) fetch(first, 0);
+  f32x4 x[NB];
+  auto arrived = [&](int buf) {
+    arrive(buf);
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) x[rb] = cd.get(rb);
+  };
+  arrived(0);
   int buf = 0;
   for (int t0 = first; t0 >= 0; t0 -= C, buf ^= DIRECT) {
     const int cnt = min(C, len - t0);
     const int64_t ch = bh * a.n + t0 / C;
-    if (!DIRECT) __syncthreads();  // the chunk before has been read
-    arrive(buf);
-    if (DIRECT) settle();
     __syncthreads();  // this chunk is there (and the other buffer has been read)
     const Tile<NI, R, PL, DIRECT> tk{lk[buf]}, tq{lq[buf]};
     const Tile<NP, RC, PC, DIRECT> tt{lt[buf]}, tp{lp[buf]};
     const float (*sc)[C] = lv[buf];
-    f32x4 x[NB];
-#pragma unroll
-    for (int rb = 0; rb < NB; ++rb) x[rb] = cd.get(rb);
     const float gc = expf(vec.top);
     fetch(t0 - C, buf ^ DIRECT);
     auto at = [&](int m, int row) { return *reinterpret_cast<const f32x4*>(&sc[m][row + 4 * g]); };
@@ -954,6 +977,10 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
         }
       }
       phase();
+    }
+    if (t0 >= C) {  // as in the forward
+      if (!DIRECT) __syncthreads();
+      arrived(buf ^ DIRECT);
     }
   }
   if (!live) return;
