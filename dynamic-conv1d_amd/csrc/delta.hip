@@ -28,9 +28,10 @@ namespace {
 using dr::Args;
 using dr::Stage;
 
-int np_of(const DrProblem& p) { return p.dtype == kFP32 ? 3 : p.dtype == kFP16 || p.precise ? 2 : 1; }
+// Parts of what is computed (delta_mfma.h).
+int np_of(const DrProblem& p) { return p.dtype == kFP32 || p.precise ? 3 : p.dtype == kFP16 ? 2 : 1; }
 int chunk(const DrProblem& p) {
-  return dr::chunk_of(p.dtype == kFP32 ? 3 : p.dtype == kFP16 ? 2 : 1, dr::cover((int)p.K));
+  return dr::chunk_of(p.dtype == kFP32 ? 3 : p.dtype == kFP16 ? 2 : 1, np_of(p), dr::cover((int)p.K));
 }
 
 // The workspace: of the forward vec, Tb and P, of the backward U, dX, the states and their gradients.
@@ -88,9 +89,10 @@ hipError_t run(Stage st, Args a, bool whole, int64_t blocks) {
   for (a.blk0 = 0; a.blk0 < blocks; a.blk0 += most) {
     a.nblk = (int)(blocks - a.blk0 < most ? blocks - a.blk0 : most);
     const hipError_t e = p.dtype == kFP32 ? dr::launch<float, 3>(st, a, mode, p.stream)
-                         : p.dtype == kFP16 ? dr::launch<fp16, 2>(st, a, mode, p.stream)
-                         : p.precise ? dr::launch<bf16, 2>(st, a, mode, p.stream)
-                                     : dr::launch<bf16, 1>(st, a, mode, p.stream);
+                         : p.dtype == kFP16 && p.precise ? dr::launch<fp16, 3>(st, a, mode, p.stream)
+                         : p.dtype == kFP16              ? dr::launch<fp16, 2>(st, a, mode, p.stream)
+                         : p.precise                     ? dr::launch<bf16, 3>(st, a, mode, p.stream)
+                                                         : dr::launch<bf16, 1>(st, a, mode, p.stream);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;

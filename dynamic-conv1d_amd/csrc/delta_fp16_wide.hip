@@ -1,0 +1,4 @@
+// The fp16 gated delta rule kernels for float32 results (delta_mfma.h).
+#include "delta_mfma.h"
+
+template hipError_t dc::dr::launch<dc::fp16, 3>(dc::dr::Stage, const dc::dr::Args&, int, hipStream_t);

@@ -7,10 +7,12 @@
 // tiles lie in LDS so that a lane's 8 values of that order are neighbours (spot()); columns are read through transposing
 // reads.
 //
-// Precision.  Operands are bf16: q, k, v and dO as one part (bf16), two (fp16: all of its bits) or three (float32), what is
-// computed (S, X, U, Tb, P and their gradients) in NP parts: one in bf16 (2^-9 of each, below the rounding of the results),
-// two where a result is float32 and in fp16 (2^-17), three in float32 (2^-25).  A product of parts keeps those down to the
-// last part's size.  Sums, S and dS, decays and norms are float32; sums of logarithms of decays are float64.
+// Precision.  Operands are bf16 parts: q, k, v and dO one part (bf16), two (fp16: all of its bits) or three (float32); what is
+// computed NP parts: three where a result is float32 (24 bits), two in fp16 (16 bits, results have 11), one in bf16 (8 bits)
+// of what goes through memory (Tb, P, S, dS, U, dX) and two of what does not (X, U, dU and their scaled forms: NR).  Were
+// those one part too, a dozen roundings of a result's own size would add up to 2-3 of its roundings (o 3.2e-3 of its norm,
+// dlog_decay 4.5-8e-3; two parts cost the chains 10%).  A product of parts keeps those down to the last part's size.
+// Sums, S and dS, decays and norms are float32; sums of logarithms of decays are float64.
 #pragma once
 
 #include <type_traits>
@@ -27,8 +29,9 @@ constexpr int kC = 0, kB = 2, kRk = 3, kRq = 4, kGk = 5, kDk = 6, kGq = 7, kVecs
 constexpr int kPiece = 128;  // columns of v that the gradients' launch holds at once
 
 template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __is_same(T, fp16) ? 2 : 1; }
-// Tokens of a chunk: 64, or 32 where tiles of 64 would pass the LDS.
-__host__ __device__ constexpr int chunk_of(int parts, int kp) { return parts == 3 || parts * kp > 256 ? 32 : 64; }
+constexpr int held(int np) { return np == 1 ? 2 : np; }  // parts of operands that stay in registers
+// Tokens of a chunk: 64, or 32 where tiles of 64 would pass the LDS (np: parts of what is computed, ni: of q and k).
+__host__ __device__ constexpr int chunk_of(int ni, int np, int kp) { return np == 3 || ni * kp > 256 ? 32 : 64; }
 __host__ __device__ constexpr int cover(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : 256; }
 
 struct Args {
@@ -91,7 +94,16 @@ __device__ __forceinline__ Frag<N> pack(f32x4 a, f32x4 b) {
 // neither 16 rows of one piece nor 4 rows of 4 pieces meet in a bank.
 template <int W>
 __device__ __forceinline__ int turn(int row) {
-  return W == 64 ? (row << 1 & 4) | (row >> 2 & 3) : (row << 2 & 12) | (row >> 2 & 3);
+  return W == 32 ? row >> 2 & 3 : W == 64 ? (row << 1 & 4) | (row >> 2 & 3) : (row << 2 & 12) | (row >> 2 & 3);
+}
+
+// The first parts of an operand.
+template <int N, int M>
+__device__ __forceinline__ Frag<N> first(const Frag<M>& f) {
+  Frag<N> t;
+#pragma unroll
+  for (int i = 0; i < N; ++i) t.p[i] = f.p[i];
+  return t;
 }
 
 // A tile in LDS: R elements from a row to the next, PL from a part to the next; TURN: its pieces turned, R of them whole.
@@ -216,7 +228,7 @@ __device__ __forceinline__ void put_gate(void* t, int gdtype, int64_t i, float v
 // What each chunk needs of its own keys: a workgroup of four wavefronts to a chunk of one head.
 template <typename T, int NP, int KP, bool WHOLE>
 __global__ __launch_bounds__(256) void dr_prep(Args a) {
-  constexpr int NI = parts_of<T>(), C = chunk_of(NI, KP), NB = C / 16, R = KP + 8, PL = C * R, RA = C + 4;
+  constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RA = C + 4;
   constexpr int TILES = 2 * NI * PL * 2, MATS = 2 * C * RA * 4;
   __shared__ __align__(16) unsigned char mem[TILES > MATS ? TILES : MATS];
   __shared__ float chi[C], clo[C], be[C], rk[C], rq[C];
@@ -545,7 +557,8 @@ struct Scales {
 // keep states.
 template <int C, int W>
 __device__ __forceinline__ void load_direct(const bf16* base, int64_t stride, int cnt, bf16* lds) {
-  constexpr int PR = W / 8, N = C * PR / kNT, VAR = W / 64;  // pieces of a row, loads, loads to 16 rows
+  constexpr int PR = W / 8, N = C * PR / kNT, RPL = kNT / PR;  // pieces of a row, loads, rows of a load
+  constexpr int VAR = RPL < 16 ? 16 / RPL : 1;                 // loads after which the rows' turns repeat
   static_assert(C * PR % kNT == 0 && N % VAR == 0, "whole loads");
   const rsrc_t rs = make_rsrc_wave(base, ((int64_t)(cnt - 1) * stride + W) * 2);
   const int wv = wave_id(), lane = threadIdx.x % 64, sb = (int)stride * 2;
@@ -559,9 +572,9 @@ __device__ __forceinline__ void load_direct(const bf16* base, int64_t stride, in
                  "s"(rs), "s"(more)
                  : "m0", "memory");
   };
-  if (cnt == C) {  // the turns repeat after 16 rows
+  if (cnt == C) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) load(i, place(i % VAR, C), i / VAR * 16 * sb);
+    for (int i = 0; i < N; ++i) load(i, place(i % VAR, C), i / VAR * VAR * RPL * sb);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) load(i, place(i, cnt - 1), 0);
@@ -577,23 +590,22 @@ enum Mode { kGather, kWhole, kDirect };
 template <typename T, int NP, int KP, int MODE>
 struct ChainSize {
   static constexpr bool DIRECT = MODE == kDirect;
-  static constexpr int NI = parts_of<T>(), C = chunk_of(NI, KP), NB = C / 16, R = KP + (DIRECT ? 0 : 24), PL = C * R,
+  static constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + (DIRECT ? 0 : 24), PL = C * R,
                        RC = C + (DIRECT ? 0 : 8), PC = C * RC;
   static constexpr int BUF = DIRECT ? 2 : 1, KEYS = NI * PL, SQUARE = NP * PC;
   static constexpr int bytes(bool both) { return BUF * ((both ? 2 : 1) * (KEYS + SQUARE) * 2 + 3 * C * 4); }
-  static_assert(bytes(true) <= 160 * 1024, "the LDS");
   static constexpr int WAVES = DIRECT && NP == 1 ? 2 : 1;
 };
 
 // bf16 rows of whole tiles, where two buffers fit.
 template <typename T, int NP, int KP>
-constexpr bool kHasDirect = __is_same(T, bf16) && 2 * (4 * 64 * KP + NP * 4 * 64 * 64 + 768) <= 160 * 1024;
+constexpr bool kHasDirect = __is_same(T, bf16) && ChainSize<T, NP, KP, kDirect>::bytes(true) <= 160 * 1024;
 
 // The states from chunk to chunk, and o.  KEEP: U and the state before each chunk for the backward instead of o.
 template <typename T, int NP, int KP, int MODE, bool KEEP>
 __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
-  constexpr int NI = Z::NI, C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
+  constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
   constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
   extern __shared__ __align__(16) unsigned char chain_lds[];
   float (*lv)[3][C] = reinterpret_cast<float (*)[3][C]>(chain_lds);
@@ -721,9 +733,9 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
     keys(0);
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] -= *reinterpret_cast<const f32x4*>(&sc[0][16 * rb + 4 * g]) * y[rb];
-    Frag<NP> f[C / 32], d[C / 32];
+    Frag<NR> f[C / 32], d[C / 32];
 #pragma unroll
-    for (int s = 0; s < C / 32; ++s) f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
+    for (int s = 0; s < C / 32; ++s) f[s] = pack<NR>(x[2 * s], x[2 * s + 1]);
     // U = Tb X
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -735,9 +747,9 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
     for (int kb = 0; kb < KN; ++kb) S[kb] *= gc;
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) {
-      f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
-      if (KEEP) keep<NP, false>(a.u + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, f[s]);
-      d[s] = pack<NP>(x[2 * s] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 4 * g]),
+      f[s] = pack<NR>(x[2 * s], x[2 * s + 1]);
+      if (KEEP) keep<NP, false>(a.u + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, first<NP>(f[s]));
+      d[s] = pack<NR>(x[2 * s] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 4 * g]),
                       x[2 * s + 1] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 16 + 4 * g]));
     }
     phase();
@@ -805,7 +817,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
 template <typename T, int NP, int KP, int MODE>
 __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain_bwd(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
-  constexpr int NI = Z::NI, C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
+  constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
   constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
   extern __shared__ __align__(16) unsigned char chain_lds[];
   float (*lv)[3][C] = reinterpret_cast<float (*)[3][C]>(chain_lds);
@@ -889,7 +901,8 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
       phase();
     };
     rows(even, 0);
-    Frag<NP> sf[KP / 32], gd[C / 32], f[C / 32];
+    Frag<NP> sf[KP / 32];
+    Frag<NR> gd[C / 32], f[C / 32];
     Frag<NI> df[C / 32];
 #pragma unroll
     for (int s = 0; s < KP / 32; ++s) {
@@ -899,7 +912,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) {
       df[s] = pack<NI>(x[2 * s], x[2 * s + 1]);
-      gd[s] = pack<NP>(x[2 * s] * at(2, 32 * s), x[2 * s + 1] * at(2, 32 * s + 16));
+      gd[s] = pack<NR>(x[2 * s] * at(2, 32 * s), x[2 * s + 1] * at(2, 32 * s + 16));
     }
     // dU = P^T dO + D k dS
 #pragma unroll
@@ -941,7 +954,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
     };
     keys(tq, 0);
 #pragma unroll
-    for (int s = 0; s < C / 32; ++s) f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
+    for (int s = 0; s < C / 32; ++s) f[s] = pack<NR>(x[2 * s], x[2 * s + 1]);
 #pragma unroll
     for (int kb = 0; kb < KN; ++kb) S[kb] *= gc;
 #pragma unroll
@@ -973,7 +986,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
           keep<NP, false>(a.x + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, pack<NP>(x[2 * s], x[2 * s + 1]));
-          f[s] = pack<NP>(-x[2 * s] * at(0, 32 * s), -x[2 * s + 1] * at(0, 32 * s + 16));
+          f[s] = pack<NR>(-x[2 * s] * at(0, 32 * s), -x[2 * s + 1] * at(0, 32 * s + 16));
         }
       }
       phase();
@@ -1001,8 +1014,8 @@ __device__ __forceinline__ float sum16(float v) {
 // k themselves, before their part along the row is taken out.  ONE: one value head to a key head, whose sums need no registers
 // of their own.
 template <typename T, int NP, int KP, bool WHOLE, bool ONE>
-__global__ __launch_bounds__(256, ONE && NP == 1 && KP <= 128 ? 2 : 1) void dr_grads(Args a) {
-  constexpr int NI = parts_of<T>(), C = chunk_of(NI, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
+__global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && parts_of<T>() == 1) ? 2 : 1) void dr_grads(Args a) {
+  constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
   constexpr int NCB = KP / 64, RV = kPiece + 8, PV = C * RV;
   constexpr int ROWS = (NI + 2 * NP) * PV, KEYS = 2 * NI * PL;
   __shared__ __align__(16) bf16 mem[ROWS > KEYS ? ROWS : KEYS], lm[2 * NP * PC];
@@ -1290,8 +1303,9 @@ hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
   return mode != kGather ? size(std::true_type()) : size(std::false_type());
 }
 extern template hipError_t launch<bf16, 1>(Stage, const Args&, int, hipStream_t);
-extern template hipError_t launch<bf16, 2>(Stage, const Args&, int, hipStream_t);
+extern template hipError_t launch<bf16, 3>(Stage, const Args&, int, hipStream_t);
 extern template hipError_t launch<fp16, 2>(Stage, const Args&, int, hipStream_t);
+extern template hipError_t launch<fp16, 3>(Stage, const Args&, int, hipStream_t);
 extern template hipError_t launch<float, 3>(Stage, const Args&, int, hipStream_t);
 
 }  // namespace dr

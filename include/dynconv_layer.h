@@ -74,7 +74,7 @@ int dc_linear_attention_step(const void* q, const int64_t* q_strides, const void
 /* Flags of the gated delta rule. */
 typedef enum dc_delta_flags {
   DC_DELTA_NORMALIZE = 1, /* the rows of q and k are divided by sqrt(|row|^2 + eps) */
-  DC_DELTA_PRECISE = 2    /* bf16: every product's operands in two parts of the type (16 bits), for float32 results */
+  DC_DELTA_PRECISE = 2    /* bf16, fp16: products as good as float32's, for the results that are float32 */
 } dc_delta_flags;
 
 /* The gated delta rule: with a = exp(log_decay_t), b = beta_t, for each sequence and head,

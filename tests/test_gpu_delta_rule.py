@@ -1,7 +1,8 @@
 """gated_delta_rule and gated_delta_rule_step against float64 (oracle/layer.py).
 
-Bounds.  The operands of the kernels' products are rounded: bf16 once (u_r = 2^-8 of each), bf16 with float32 results and
-fp16 in two bf16 parts (2^-16), float32 as float32 (2^-24, and float32 sums of up to 256 + 64 terms in chains of chunks).
+Bounds.  The operands of the kernels' products are rounded: bf16 once (u_r = 2^-8 of each, or better), fp16 in two bf16 parts
+(2^-16), float32 and 16 bits with float32 results as float32 (2^-24, and float32 sums of up to 256 + 64 terms in chains of
+chunks).
 What these roundings take a result away from its float64 value depends on how far its terms cancel, so it is computed: err_r is
 the error of gated_delta_rule_chunked in float32 with the same operands rounded the same way.  The kernel's roundings are
 others of the same kind and number (other sums, other orders), independent and many, so their norm comes out alike: within a
@@ -37,9 +38,9 @@ def _two_parts(t):
 
 
 def _rounding(dtype, wide):
-    if dtype == F32:
+    if dtype == F32 or wide:
         return (lambda t: t), 2.0**-24
-    return (_two_parts, 2.0**-16) if dtype == HF or wide else ((lambda t: t.to(BF).to(t.dtype)), 2.0**-8)
+    return (_two_parts, 2.0**-16) if dtype == HF else ((lambda t: t.to(BF).to(t.dtype)), 2.0**-8)
 
 
 @pytest.fixture(params=["native", "python"])
