@@ -17,9 +17,9 @@
 //   db_i = (dX_i . U_i) / b_i^2
 //   dc_i = q_i.dq_i + k_i.(R_i - W_i),   dc_C += <S after the chunk, dS>;   dlog_decay_i = sum_{l >= i} dc_l
 //
-// Four launches: what each chunk needs of its own keys (Tb, P and the decays), the states from chunk to chunk with the
-// outputs, the same against time for the states' gradients, and the gradients chunk by chunk.  A b of zero counts as
-// 2^-60, so that db has its quotient.
+// Launches: what each chunk needs of its own keys (Tb, P and the decays); the states from chunk to chunk with the outputs, and
+// in the backward with U and the states themselves; the same against time for the states' gradients; and the gradients chunk
+// by chunk.  A b of zero counts as 2^-60, so that db has its quotient.
 #include "delta_mfma.h"
 
 namespace dc {
@@ -34,10 +34,34 @@ int chunk(const DrProblem& p) {
   return dr::chunk_of(p.dtype == kFP32 ? 3 : p.dtype == kFP16 ? 2 : 1, np_of(p), dr::cover((int)p.K));
 }
 
-// The workspace: of the forward vec, Tb and P, of the backward U, dX, the states and their gradients.
+// Segments of the tokens, where heads and columns leave CUs idle: one launch finds what each makes of the state before it, a
+// second carries the states across, and the chains run side by side.  The count with the least estimated time, per chunk of
+// a workgroup in units of the forward's chain: 1 for a chain, 0.8 for one without outputs (twice, with the unit vectors'
+// columns, where K is V), rounds of `fit` workgroups, and the launches.
+int segments(const DrProblem& p, int C, int np) {
+  const int kp = dr::cover((int)p.K), vp = ((int)p.V + 31) / 32 * 32, cols = 2 * 16;
+  const int64_t chunks = (p.T + C - 1) / C, heads = p.B * p.H;
+  // workgroups side by side on 256 CUs, by their LDS
+  const double fit = 256 * (np == 1 && kp > 64 ? 1 : 2), us = np == 1 ? 2.5 : 2.8;
+  double best = 0;
+  int n = 1;
+  for (int s = 1; s <= 64 && s <= chunks; ++s) {
+    const int64_t len = (chunks + s - 1) / s;
+    if ((chunks + len - 1) / len != s) continue;  // the same segments as fewer
+    double t = us * len * __builtin_ceil(heads * s * (vp / cols) / fit);
+    if (s > 1) t += 0.8 * us * len * __builtin_ceil(heads * (s - 1) * ((vp + kp) / cols) / 512.) + 15 + 4 * s;
+    if (s == 1 || t < best) {
+      best = t;
+      n = s;
+    }
+  }
+  return n;
+}
+
+// The workspace: of the forward vec, Tb, P and the segments' states, of the backward U, dX, the states and their gradients.
 struct Plan {
-  int64_t n, vec, sq, rows, st;  // chunks of a head; bytes of each array
-  int vp;
+  int64_t n, vec, sq, rows, st, cut, trans;  // chunks of a head; bytes of each array
+  int vp, seg, nseg;
   explicit Plan(const DrProblem& p) {
     const int C = chunk(p), np = np_of(p);
     n = (p.T + C - 1) / C;
@@ -46,10 +70,15 @@ struct Plan {
     vec = chunks * dr::kVecs * C * 4;
     sq = chunks * np * C * C * 2;
     rows = chunks * np * C * vp * 2;
-    st = chunks * np * dr::cover((int)p.K) * vp * 2;
+    const int kp = dr::cover((int)p.K);
+    st = chunks * np * kp * vp * 2;
+    nseg = segments(p, C, np);
+    seg = (int)((n + nseg - 1) / nseg) * C;
+    cut = nseg > 1 ? (p.B * p.H * nseg * p.K * p.V * 4 + 15) / 16 * 16 : 0;
+    trans = nseg > 1 ? p.B * p.H * nseg * kp * kp * 4 : 0;
   }
-  int64_t fwd() const { return vec + 2 * sq; }
-  int64_t bwd() const { return 2 * rows + 2 * st; }
+  int64_t fwd() const { return vec + 2 * sq + trans + cut; }
+  int64_t bwd() const { return 2 * rows + 2 * st + cut; }
 };
 
 Args args_of(const DrProblem& p, bool bwd) {
@@ -58,16 +87,21 @@ Args args_of(const DrProblem& p, bool bwd) {
   a.p = p;
   a.n = pl.n;
   a.vp = pl.vp;
+  a.seg = pl.seg;
+  a.nseg = pl.nseg;
   char* f = static_cast<char*>(bwd && p.fwd_ws ? const_cast<void*>(p.fwd_ws) : p.ws);
   a.vec = reinterpret_cast<float*>(f);
   a.tb = reinterpret_cast<bf16*>(f + pl.vec);
   a.pp = reinterpret_cast<bf16*>(f + pl.vec + pl.sq);
+  a.trans = reinterpret_cast<float*>(f + pl.vec + 2 * pl.sq);
+  a.start = reinterpret_cast<float*>(f + pl.vec + 2 * pl.sq + pl.trans);
   if (bwd) {
     char* w = static_cast<char*>(p.ws) + (p.fwd_ws ? 0 : pl.fwd());
     a.u = reinterpret_cast<bf16*>(w);
     a.x = reinterpret_cast<bf16*>(w + pl.rows);
     a.s = reinterpret_cast<bf16*>(w + 2 * pl.rows);
     a.ds = reinterpret_cast<bf16*>(w + 2 * pl.rows + pl.st);
+    a.dstart = reinterpret_cast<float*>(w + 2 * pl.rows + 2 * pl.st);
   }
   return a;
 }
@@ -98,8 +132,17 @@ hipError_t run(Stage st, Args a, bool whole, int64_t blocks) {
   return hipSuccess;
 }
 
-// Workgroups of the chains.
-int64_t columns(const Args& a) { return a.p.B * a.p.H * ((a.vp + dr::kNW * 16 - 1) / (dr::kNW * 16)); }
+// Workgroups of the chains over `seg` segments, and `more` columns beside V's.
+int64_t columns(const Args& a, int seg, int more = 0) { return a.p.B * a.p.H * seg * ((a.vp + more) / (dr::kNW * 16)); }
+
+// What the chunks need of their own keys, and the states before the segments.
+hipError_t ahead(const Args& a, bool keys, bool values) {
+  const DrProblem& p = a.p;
+  hipError_t e = run(dr::kPrep, a, keys, p.B * p.H * a.n);
+  if (a.nseg == 1 || e != hipSuccess) return e;
+  e = run(dr::kAhead, a, keys && values, columns(a, a.nseg - 1, dr::cover((int)p.K)));
+  return e != hipSuccess || a.nseg == 2 ? e : run(dr::kCarry, a, true, p.B * p.H * (a.vp / 16));
+}
 
 }  // namespace
 
@@ -111,18 +154,21 @@ int64_t dr_ws_bytes(const DrProblem& p, int bwd) {
 hipError_t dr_fwd(const DrProblem& p) {
   const Args a = args_of(p, false);
   const int es = dtype_size(p.dtype);
-  const bool w = whole16(p.q, p.qs, p.K, es) && whole16(p.k, p.ks, p.K, es);
-  const hipError_t e = run(dr::kPrep, a, w, p.B * p.H * a.n);
-  return e != hipSuccess ? e : run(dr::kChain, a, w && slim(p.vs, p.V, es) && whole16(p.o, p.os, p.V, es), columns(a));
+  const bool w = whole16(p.q, p.qs, p.K, es) && whole16(p.k, p.ks, p.K, es), v = slim(p.vs, p.V, es);
+  const hipError_t e = ahead(a, w, v);
+  return e != hipSuccess ? e : run(dr::kChain, a, w && v && whole16(p.o, p.os, p.V, es), columns(a, a.nseg));
 }
 
 hipError_t dr_bwd(const DrProblem& p) {
   const Args a = args_of(p, true);
   const int es = dtype_size(p.dtype);
-  const bool w = whole16(p.q, p.qs, p.K, es) && whole16(p.k, p.ks, p.K, es);
-  hipError_t e = p.fwd_ws ? hipSuccess : run(dr::kPrep, a, w, p.B * p.H * a.n);
-  if (e == hipSuccess) e = run(dr::kKeep, a, w && slim(p.vs, p.V, es), columns(a));
-  if (e == hipSuccess) e = run(dr::kChainBwd, a, w && slim(p.dos, p.V, es) && slim(p.dvs, p.V, es), columns(a));
+  const bool w = whole16(p.q, p.qs, p.K, es) && whole16(p.k, p.ks, p.K, es), v = slim(p.vs, p.V, es);
+  hipError_t e = p.fwd_ws ? hipSuccess : ahead(a, w, v);
+  if (e == hipSuccess) e = run(dr::kKeepStates, a, w && v, columns(a, a.nseg));
+  const bool d = w && slim(p.dos, p.V, es) && slim(p.dvs, p.V, es);
+  if (e == hipSuccess && a.nseg > 1) e = run(dr::kAheadBwd, a, d, columns(a, a.nseg - 1));
+  if (e == hipSuccess && a.nseg > 2) e = run(dr::kCarryBwd, a, true, p.B * p.H * (a.vp / 16));
+  if (e == hipSuccess) e = run(dr::kChainBwd, a, d, columns(a, a.nseg));
   return e != hipSuccess ? e : run(dr::kGrads, a, w && whole16(p.d_o, p.dos, p.V, es), p.B * p.Hk * a.n);
 }
 

@@ -39,6 +39,10 @@ struct Args {
   float* vec;          // [chunks][kVecs][C]
   bf16 *tb, *pp;       // [chunks][NP][C][C], spot() order
   bf16 *u, *x, *s, *ds;  // [chunks][NP][C][VP] U and dX, [chunks][NP][KP][VP] states before and their gradients after
+  // tokens cut into nseg segments of seg (whole chunks): the states before each but the first [heads][nseg][K][V], the
+  // gradients after each but the last, and what a segment makes of the state before it, [heads][nseg][KP][KP]
+  float *start, *dstart, *trans;
+  int seg, nseg;
   int64_t n;           // chunks of a head
   int vp;              // V in whole 32 columns
   int64_t blk0;
@@ -601,12 +605,15 @@ struct ChainSize {
 template <typename T, int NP, int KP>
 constexpr bool kHasDirect = __is_same(T, bf16) && ChainSize<T, NP, KP, kDirect>::bytes(true) <= 160 * 1024;
 
-// The states from chunk to chunk, and o.  KEEP: U and the state before each chunk for the backward instead of o.
-template <typename T, int NP, int KP, int MODE, bool KEEP>
+// The states from chunk to chunk, and o (kOutputs); or U and the state before each chunk for the backward (kKeep); or what each
+// segment but the last makes of the state before it (kAcross): its end from zero, and behind those columns its end from each
+// unit vector without values.
+enum What { kOutputs, kKeep, kAcross };
+template <typename T, int NP, int KP, int MODE, int WHAT>
 __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
   constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
-  constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
+  constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather, KEEP = WHAT != kOutputs;  // KEEP: no q and no o
   extern __shared__ __align__(16) unsigned char chain_lds[];
   float (*lv)[3][C] = reinterpret_cast<float (*)[3][C]>(chain_lds);
   bf16 (*lk)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lv + Z::BUF);
@@ -614,19 +621,34 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
   bf16 (*lq)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lt + Z::BUF);  // not there if KEEP
   bf16 (*lp)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lq + Z::BUF);
   const DrProblem& p = a.p;
-  const int nvb = (a.vp + kNW * 16 - 1) / (kNW * 16);
-  const int64_t blk = a.blk0 + xcd_remap(blockIdx.x, a.nblk), bh = blk / nvb, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
+  // columns: V's, and behind them those of the unit vectors
+  const int nvb = (a.vp + (WHAT == kAcross ? KP : 0)) / (kNW * 16), nseg = WHAT == kAcross ? a.nseg - 1 : a.nseg;
+  int64_t blk = a.blk0 + xcd_remap(blockIdx.x, a.nblk);
+  const int vb = (int)(blk % nvb);
+  blk /= nvb;
+  const int seg = (int)(blk % nseg);
+  const int64_t bh = blk / nseg, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
   const int lane = threadIdx.x % 64, g = lane / 16, col = lane % 16;
-  const int n0 = (int)(blk % nvb) * kNW * 16 + wave_id() * 16, nn = n0 + col, K = (int)p.K, V = (int)p.V;
-  const bool live = nn < V;
-  const int len = length_of(p, b);
+  const int n0 = vb * kNW * 16 + wave_id() * 16, nn = n0 + col, K = (int)p.K, V = (int)p.V;
+  const bool live = nn < V, unit = WHAT == kAcross && vb * kNW * 16 >= a.vp;
+  if (unit && seg == 0) return;  // the state before the first segment is known
+  const int lo = seg * a.seg, len = min(length_of(p, b), lo + a.seg), whole = length_of(p, b);
   const T* q = (const T*)p.q + b * p.qs[0] + hk * p.qs[1];
   const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[1];
   const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1] + nn;
   T* o = (T*)p.o + b * p.os[0] + h * p.os[1] + n0;
   const int64_t sb = bh * K * V + nn;
   f32x4 S[KP / 16];
-  load_state<KP>(S, p.s_in ? p.s_in + sb : nullptr, live, K, V);
+  const int64_t at0 = (bh * a.nseg + seg) * K * V + nn;
+  if (unit) {
+#pragma unroll
+    for (int kb = 0; kb < KP / 16; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[kb][r] = 32 * (kb / 2) + 8 * g + 4 * (kb % 2) + r == nn - a.vp ? 1.f : 0.f;
+  } else {
+    const float* from = seg == 0 ? (p.s_in ? p.s_in + sb : nullptr) : WHAT == kAcross ? nullptr : a.start + at0;
+    load_state<KP>(S, from, live, K, V);
+  }
   Rows<T, C, KP, kNT, WHOLE> rk, rq;
   Square<NP, C, kNT> rt, rp;
   Columns<T, C, WHOLE> cv;
@@ -652,7 +674,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
         rp.load(pt);
       }
     }
-    cv.load(v + (int64_t)t0 * p.vs[2], p.vs[2], V - n0, cnt);
+    cv.load(v + (int64_t)t0 * p.vs[2], p.vs[2], unit ? 0 : V - n0, cnt);
     vec.load(a.vec + ch * kVecs * C);
   };
   auto arrive = [&](int buf) {  // what fetch() left in registers
@@ -666,7 +688,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
     }
     vec.store(lv[buf][0]);
   };
-  fetch(0, 0);
+  fetch(lo, 0);
   f32x4 x[NB];
   auto arrived = [&](int buf) {
     arrive(buf);
@@ -675,7 +697,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
   };
   arrived(0);
   int buf = 0;
-  for (int t0 = 0; t0 < len; t0 += C, buf ^= DIRECT) {
+  for (int t0 = lo; t0 < len; t0 += C, buf ^= DIRECT) {
     const int cnt = min(C, len - t0);
     const int64_t ch = bh * a.n + t0 / C;
     __syncthreads();  // this chunk is there (and the other buffer has been read)
@@ -699,7 +721,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
 #pragma unroll
     for (int s = 0; s < KP / 32; ++s) {
       sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
-      if (KEEP) keep<NP, true>(a.s + (ch * NP * KP + 32 * s) * a.vp + n0, a.vp, (int64_t)KP * a.vp, sf[s]);
+      if (WHAT == kKeep) keep<NP, true>(a.s + (ch * NP * KP + 32 * s) * a.vp + n0, a.vp, (int64_t)KP * a.vp, sf[s]);
     }
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) y[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -748,7 +770,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) {
       f[s] = pack<NR>(x[2 * s], x[2 * s + 1]);
-      if (KEEP) keep<NP, false>(a.u + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, first<NP>(f[s]));
+      if (WHAT == kKeep) keep<NP, false>(a.u + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, first<NP>(f[s]));
       d[s] = pack<NR>(x[2 * s] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 4 * g]),
                       x[2 * s + 1] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 16 + 4 * g]));
     }
@@ -808,13 +830,17 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
       arrived(buf ^ DIRECT);
     }
   }
-  if (!live || KEEP) return;
-  if (p.s_out) store_state<KP>(S, p.s_out + sb, K, V);
-  for (int64_t t = len + g; t < p.T; t += 4) o[t * p.os[2] + col] = (T)0.f;
+  if (unit) store_state<KP>(S, a.trans + (bh * a.nseg + seg) * KP * KP + nn - a.vp, KP, KP);
+  if (!live) return;
+  if (WHAT == kAcross) store_state<KP>(S, a.start + at0 + K * V, K, V);
+  if (WHAT != kOutputs) return;
+  if (p.s_out && (lo < whole ? whole <= lo + a.seg : seg == 0 && whole == 0)) store_state<KP>(S, p.s_out + sb, K, V);
+  for (int64_t t = max(whole, lo) + g; t < min(p.T, (int64_t)lo + a.seg); t += 4) o[t * p.os[2] + col] = (T)0.f;
 }
 
-// The states' gradients from the last chunk on, and dv.
-template <typename T, int NP, int KP, int MODE>
+// The states' gradients from the last chunk on, and dv; ACROSS: only what each segment but the first makes of them from zero
+// (from the state after it they come by the transpose of what the forward found).
+template <typename T, int NP, int KP, int MODE, bool ACROSS>
 __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain_bwd(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
   constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
@@ -826,25 +852,31 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
   bf16 (*lq)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lt + Z::BUF);
   bf16 (*lp)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lq + Z::BUF);
   const DrProblem& p = a.p;
-  const int nvb = (a.vp + kNW * 16 - 1) / (kNW * 16);
-  const int64_t blk = a.blk0 + xcd_remap(blockIdx.x, a.nblk), bh = blk / nvb, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
+  const int nvb = a.vp / (kNW * 16), nseg = ACROSS ? a.nseg - 1 : a.nseg;
+  int64_t blk = a.blk0 + xcd_remap(blockIdx.x, a.nblk);
+  const int vb = (int)(blk % nvb);
+  blk /= nvb;
+  const int seg = (int)(blk % nseg) + ACROSS;
+  const int64_t bh = blk / nseg, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
   const int lane = threadIdx.x % 64, g = lane / 16, col = lane % 16;
-  const int n0 = (int)(blk % nvb) * kNW * 16 + wave_id() * 16, nn = n0 + col, K = (int)p.K, V = (int)p.V;
+  const int n0 = vb * kNW * 16 + wave_id() * 16, nn = n0 + col, K = (int)p.K, V = (int)p.V;
   const bool live = nn < V;
-  const int len = length_of(p, b);
+  const int lo = seg * a.seg, len = min(length_of(p, b), lo + a.seg), whole = length_of(p, b);
   const T* q = (const T*)p.q + b * p.qs[0] + hk * p.qs[1];
   const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[1];
   const T* d_o = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + nn;
   T* dv = (T*)p.dv + b * p.dvs[0] + h * p.dvs[1] + nn;
   const int64_t sb = bh * K * V + nn;
   f32x4 S[KP / 16];
-  load_state<KP>(S, p.ds_in ? p.ds_in + sb : nullptr, live, K, V);
+  const int64_t at0 = (bh * a.nseg + seg) * K * V + nn;
+  const float* from = seg == a.nseg - 1 ? (p.ds_in ? p.ds_in + sb : nullptr) : ACROSS ? nullptr : a.dstart + at0;
+  load_state<KP>(S, from, live, K, V);
   Rows<T, C, KP, kNT, WHOLE> rk, rq;
   Square<NP, C, kNT> rt, rp;
   Columns<T, C, WHOLE> cd;
   Scales<C> vec;
   auto fetch = [&](int t0, int buf) {
-    if (t0 < 0) return;
+    if (t0 < lo) return;
     const int cnt = min(C, len - t0);
     const int64_t ch = bh * a.n + t0 / C;
     const T *kt = k + (int64_t)t0 * p.ks[2], *qt = q + (int64_t)t0 * p.qs[2];
@@ -872,8 +904,8 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
     }
     vec.store(lv[buf][0]);
   };
-  const int first = (len + C - 1) / C * C - C;
-  if (first >= 0) fetch(first, 0);
+  const int first = (len + C - 1) / C * C - C;  // lo is whole chunks: below it where no token is
+  fetch(first, 0);
   f32x4 x[NB];
   auto arrived = [&](int buf) {
     arrive(buf);
@@ -882,7 +914,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
   };
   arrived(0);
   int buf = 0;
-  for (int t0 = first; t0 >= 0; t0 -= C, buf ^= DIRECT) {
+  for (int t0 = first; t0 >= lo; t0 -= C, buf ^= DIRECT) {
     const int cnt = min(C, len - t0);
     const int64_t ch = bh * a.n + t0 / C;
     __syncthreads();  // this chunk is there (and the other buffer has been read)
@@ -907,7 +939,7 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
 #pragma unroll
     for (int s = 0; s < KP / 32; ++s) {
       sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
-      keep<NP, true>(a.ds + (ch * NP * KP + 32 * s) * a.vp + n0, a.vp, (int64_t)KP * a.vp, sf[s]);
+      if (!ACROSS) keep<NP, true>(a.ds + (ch * NP * KP + 32 * s) * a.vp + n0, a.vp, (int64_t)KP * a.vp, sf[s]);
     }
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) {
@@ -982,23 +1014,79 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
       }
       if (i == 0) {
 #pragma unroll
-        for (int rb = 0; rb < NB; ++rb) put_columns<T, WHOLE>(dv + (int64_t)t0 * p.dvs[2], p.dvs[2], V - n0, cnt, 16 * rb, x[rb]);
+        for (int rb = 0; rb < NB; ++rb)
+          if (!ACROSS) put_columns<T, WHOLE>(dv + (int64_t)t0 * p.dvs[2], p.dvs[2], V - n0, cnt, 16 * rb, x[rb]);
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
-          keep<NP, false>(a.x + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, pack<NP>(x[2 * s], x[2 * s + 1]));
+          if (!ACROSS) keep<NP, false>(a.x + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, pack<NP>(x[2 * s], x[2 * s + 1]));
           f[s] = pack<NR>(-x[2 * s] * at(0, 32 * s), -x[2 * s + 1] * at(0, 32 * s + 16));
         }
       }
       phase();
     }
-    if (t0 >= C) {  // as in the forward
+    if (t0 >= lo + C) {  // as in the forward
       if (!DIRECT) __syncthreads();
       arrived(buf ^ DIRECT);
     }
   }
   if (!live) return;
-  if (p.ds_out) store_state<KP>(S, p.ds_out + sb, K, V);
-  for (int64_t t = len + g; t < p.T; t += 4) dv[t * p.dvs[2]] = (T)0.f;
+  if (ACROSS) return store_state<KP>(S, a.dstart + at0 - K * V, K, V);
+  if (p.ds_out && seg == 0) store_state<KP>(S, p.ds_out + sb, K, V);
+  for (int64_t t = max(whole, lo) + g; t < min(p.T, (int64_t)lo + a.seg); t += 4) dv[t * p.dvs[2]] = (T)0.f;
+}
+
+// From segment to segment, a wavefront to 16 columns of a head: start[s + 1] += trans[s] start[s], or with gradients
+// dstart[s - 1] += trans[s]^T dstart[s], on float32 matrix instructions (16x16x4: a lane's result of a row block is its operand
+// of the next product's four steps).
+template <int KP, bool BWD>
+__global__ __launch_bounds__(64) void dr_across(Args a) {
+  const DrProblem& p = a.p;
+  const int nvb = a.vp / 16, K = (int)p.K, V = (int)p.V, lane = threadIdx.x, g = lane / 16, col = lane % 16;
+  const int64_t blk = a.blk0 + blockIdx.x, bh = blk / nvb;
+  const int nn = (int)(blk % nvb) * 16 + col;
+  float* st = (BWD ? a.dstart : a.start) + bh * a.nseg * K * V + nn;
+  auto load = [&](f32x4 (&S)[KP / 16], const float* from) {
+#pragma unroll
+    for (int kb = 0; kb < KP / 16; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * kb + 4 * g + r;
+        S[kb][r] = nn < V && d < K ? from[d * V] : 0.f;
+      }
+  };
+  f32x4 S[KP / 16], N[KP / 16];
+  const int64_t kv = (int64_t)K * V;
+  load(S, st + (BWD ? a.nseg - 2 : 1) * kv);
+  for (int i = 1; i < a.nseg - 1; ++i) {
+    const int s = BWD ? a.nseg - 1 - i : i;
+    float* to = st + (BWD ? s - 1 : s + 1) * kv;
+    const float* M = a.trans + (bh * a.nseg + s) * KP * KP;
+    load(N, to);
+#pragma unroll
+    for (int rb = 0; rb < KP / 16; ++rb) {
+#pragma unroll
+      for (int kb = 0; kb < KP / 16; ++kb) {
+        f32x4 m;
+        if constexpr (BWD) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) m[r] = M[(16 * kb + 4 * g + r) * KP + 16 * rb + col];
+        } else {
+          m = *reinterpret_cast<const f32x4*>(M + (16 * rb + col) * KP + 16 * kb + 4 * g);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) N[rb] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[r], S[kb][r], N[rb], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int kb = 0; kb < KP / 16; ++kb) {
+      S[kb] = N[kb];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * kb + 4 * g + r;
+        if (nn < V && d < K) to[d * V] = N[kb][r];
+      }
+    }
+  }
 }
 
 // The sum of a value over the 16 lanes of a result's row: every lane gets it.
@@ -1269,7 +1357,7 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
 }
 
 // The launches of a type and a number of parts (instantiated in delta_<type>.hip).
-enum Stage { kPrep, kChain, kKeep, kChainBwd, kGrads };
+enum Stage { kPrep, kAhead, kCarry, kChain, kKeepStates, kAheadBwd, kCarryBwd, kChainBwd, kGrads };
 template <typename T, int NP>
 hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
   auto run = [&](auto kernel, int threads, int lds) {
@@ -1279,14 +1367,20 @@ hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
   auto chain = [&](auto kp, auto m) {
     constexpr int KP = decltype(kp)::value, M = decltype(m)::value;
     typedef ChainSize<T, NP, KP, M> Z;
-    if (st == kChain) return run(dr_chain<T, NP, KP, M, false>, kNT, Z::bytes(true));
-    if (st == kKeep) return run(dr_chain<T, NP, KP, M, true>, kNT, Z::bytes(false));
-    return run(dr_chain_bwd<T, NP, KP, M>, kNT, Z::bytes(true));
+    switch (st) {
+      case kAhead: return run(dr_chain<T, NP, KP, M, kAcross>, kNT, Z::bytes(false));
+      case kChain: return run(dr_chain<T, NP, KP, M, kOutputs>, kNT, Z::bytes(true));
+      case kKeepStates: return run(dr_chain<T, NP, KP, M, kKeep>, kNT, Z::bytes(false));
+      case kAheadBwd: return run(dr_chain_bwd<T, NP, KP, M, true>, kNT, Z::bytes(true));
+      default: return run(dr_chain_bwd<T, NP, KP, M, false>, kNT, Z::bytes(true));
+    }
   };
   auto pick = [&](auto kp, auto w) {
     constexpr int KP = decltype(kp)::value;
     constexpr bool W = decltype(w)::value;
     if (st == kPrep) return run(dr_prep<T, NP, KP, W>, 256, 0);
+    if (st == kCarry) return run(dr_across<KP, false>, 64, 0);
+    if (st == kCarryBwd) return run(dr_across<KP, true>, 64, 0);
     if (st == kGrads)
       return a.p.H == a.p.Hk ? run(dr_grads<T, NP, KP, W, true>, 256, 0) : run(dr_grads<T, NP, KP, W, false>, 256, 0);
     if constexpr (W && kHasDirect<T, NP, KP>)
