@@ -62,6 +62,13 @@ struct Abi {
   decltype(&dc_linear_attention_fwd) linear_attention_fwd;
   decltype(&dc_linear_attention_bwd) linear_attention_bwd;
   decltype(&dc_linear_attention_step) linear_attention_step;
+  decltype(&dc_delta_rule_ws_bytes) delta_rule_ws_bytes;
+  decltype(&dc_delta_rule_fwd) delta_rule_fwd;
+  decltype(&dc_delta_rule_bwd) delta_rule_bwd;
+  decltype(&dc_delta_rule_step) delta_rule_step;
+  decltype(&dc_residual_norm_fwd) residual_norm_fwd;
+  decltype(&dc_residual_norm_bwd_ws_bytes) residual_norm_bwd_ws_bytes;
+  decltype(&dc_residual_norm_bwd) residual_norm_bwd;
   decltype(&dc_group_norm_fwd) group_norm_fwd;
   decltype(&dc_group_norm_bwd_ws_bytes) group_norm_bwd_ws_bytes;
   decltype(&dc_group_norm_bwd) group_norm_bwd;
@@ -353,6 +360,136 @@ struct LinearAttentionFn : public Function<LinearAttentionFn> {
   }
 };
 
+// ------------------------------------------------------- gated delta rule
+struct DeltaSizes {
+  int64_t B, Hk, H, T, K, V;
+  int dt, gdt;
+  DeltaSizes(const Tensor& q, const Tensor& v, const Tensor& beta)
+      : B(q.size(0)), Hk(q.size(1)), H(v.size(1)), T(q.size(2)), K(q.size(3)), V(v.size(3)), dt(dtype_code(q)),
+        gdt(dtype_code(beta)) {}
+};
+
+struct GatedDeltaRuleFn : public Function<GatedDeltaRuleFn> {
+  // o over token-major memory, and the final state if it is wanted
+  static variable_list run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& b,
+                           const Tensor& s0, const Tensor& lengths, double scale, double eps, int64_t flags,
+                           bool want_state, Tensor* kept = nullptr) {
+    const DeltaSizes z(q, v, b);
+    Tensor o = at::empty({z.B, z.T, z.H, z.V}, q.options()).transpose(1, 2);
+    Tensor st = want_state ? at::empty({z.B, z.H, z.K, z.V}, q.options().dtype(at::kFloat)) : Tensor();
+    const int64_t n = abi.delta_rule_ws_bytes(z.B, z.Hk, z.H, z.T, z.K, z.V, z.dt, (int)flags, 0);
+    check(n, "gated delta rule workspace query");
+    const Tensor ws = bytes_like(q, n);
+    check(abi.delta_rule_fwd(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(), ptr(g),
+                             g.strides().data(), ptr(b), b.strides().data(), static_cast<float*>(ptr(s0)),
+                             static_cast<int32_t*>(ptr(lengths)), ptr(o), o.strides().data(),
+                             static_cast<float*>(ptr(st)), ptr(ws), n, z.B, z.Hk, z.H, z.T, z.K, z.V, (float)scale,
+                             (float)eps, z.dt, z.gdt, (int)flags, stream_of(q)),
+          "gated delta rule forward");
+    if (kept) *kept = ws;
+    variable_list out{o};
+    if (want_state) out.push_back(st);
+    return out;
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                               const Tensor& b, const std::optional<Tensor>& s0, const std::optional<Tensor>& lengths,
+                               double scale, double eps, int64_t flags, bool want_state) {
+    const Tensor s = s0.value_or(Tensor()), n = lengths.value_or(Tensor());
+    Tensor kept;  // each chunk's triangular systems, a function of the inputs, which the backward takes up again
+    variable_list out = run(q, k, v, g, b, s, n, scale, eps, flags, want_state, &kept);
+    ctx->save_for_backward({q, k, v, g, b, s, n, kept});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["flags"] = flags;
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &g = saved[3], &b = saved[4], &s0 = saved[5],
+                 &lengths = saved[6], &kept = saved[7];
+    const c10::DeviceGuard guard(q.device());
+    const DeltaSizes z(q, v, b);
+    const int flags = (int)ctx->saved_data["flags"].toInt();
+    // an output that did not reach the loss has no gradient
+    Tensor d = grads[0].defined() ? grads[0].to(q.scalar_type()) : at::zeros({z.B, z.H, z.T, z.V}, q.options());
+    if (z.V > 1 && d.stride(3) != 1) d = d.contiguous();
+    const Tensor ds = grads.size() > 1 && grads[1].defined() ? grad_in(grads[1], at::kFloat) : Tensor();
+    Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v), dg = at::empty_like(g), db = at::empty_like(b);
+    Tensor ds0 = s0.defined() && ctx->needs_input_grad(5) ? at::empty_like(s0) : Tensor();
+    const int64_t n = abi.delta_rule_ws_bytes(z.B, z.Hk, z.H, z.T, z.K, z.V, z.dt, flags, kept.defined() ? 2 : 1);
+    check(n, "gated delta rule backward workspace query");
+    const Tensor ws = bytes_like(q, n);
+    check(abi.delta_rule_bwd(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(), ptr(g),
+                             g.strides().data(), ptr(b), b.strides().data(), static_cast<float*>(ptr(s0)),
+                             static_cast<int32_t*>(ptr(lengths)), ptr(d), d.strides().data(),
+                             static_cast<float*>(ptr(ds)), ptr(dq), dq.strides().data(), ptr(dk), dk.strides().data(),
+                             ptr(dv), dv.strides().data(), ptr(dg), dg.strides().data(), ptr(db), db.strides().data(),
+                             static_cast<float*>(ptr(ds0)), ptr(kept), ptr(ws), n, z.B, z.Hk, z.H, z.T, z.K, z.V,
+                             (float)ctx->saved_data["scale"].toDouble(), (float)ctx->saved_data["eps"].toDouble(), z.dt,
+                             z.gdt, flags, stream_of(q)),
+          "gated delta rule backward");
+    return {dq, dk, dv, dg, db, ds0, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// ----------------------------------------------------------- residual norm
+struct ResidualNormFn : public Function<ResidualNormFn> {
+  static int param_code(const Tensor& branch, const Tensor& w, const Tensor& bw, const Tensor& sc) {
+    return dtype_code(w.defined() ? w : bw.defined() ? bw : sc.defined() ? sc : branch);
+  }
+  static variable_list run(const Tensor& x, const Tensor& branch, const Tensor& w, const Tensor& bw, const Tensor& gate,
+                           const Tensor& sc, double constant, int64_t act, double eps) {
+    Tensor y = at::empty_like(branch), h = at::empty_like(x);
+    const int64_t D = x.size(-1);
+    check(abi.residual_norm_fwd(ptr(x), ptr(branch), ptr(w), ptr(bw), ptr(gate), ptr(sc), ptr(y), ptr(h), x.numel() / D, D,
+                                (float)constant, (float)eps, (int)act, dtype_code(branch), dtype_code(x),
+                                param_code(branch, w, bw, sc), stream_of(x)),
+          "residual norm forward");
+    return {y, h};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& branch, const std::optional<Tensor>& w,
+                               const std::optional<Tensor>& bw, const std::optional<Tensor>& gate,
+                               const std::optional<Tensor>& sc, double constant, int64_t act, double eps) {
+    const Tensor wt = w.value_or(Tensor()), bt = bw.value_or(Tensor()), gt = gate.value_or(Tensor()), st = sc.value_or(Tensor());
+    variable_list out = run(x, branch, wt, bt, gt, st, constant, act, eps);
+    ctx->save_for_backward({out[1], branch, wt, bt, gt, st});
+    ctx->saved_data["constant"] = constant;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &h = saved[0], &branch = saved[1], &w = saved[2], &bw = saved[3], &gate = saved[4], &sc = saved[5];
+    const c10::DeviceGuard guard(h.device());
+    const int64_t D = h.size(-1), M = h.numel() / D;
+    // an output that did not reach the loss has no gradient
+    const Tensor dy = grads[0].defined() ? grad_in(grads[0], branch.scalar_type()) : Tensor();
+    const Tensor dh = grads[1].defined() ? grad_in(grads[1], h.scalar_type()) : Tensor();
+    Tensor dx = at::empty_like(h), dbranch = at::empty_like(branch), dgate = gate.defined() ? at::empty_like(gate) : Tensor();
+    // an input that is None has no place among the indexes
+    size_t at = 2;
+    const bool want_w = w.defined() && ctx->needs_input_grad(at++), want_b = bw.defined() && ctx->needs_input_grad(at++);
+    at += gate.defined();
+    const bool want_s = sc.defined() && ctx->needs_input_grad(at);
+    Tensor dw = want_w ? at::empty_like(w) : Tensor(), dbw = want_b ? at::empty_like(bw) : Tensor(),
+           ds = want_s ? at::empty_like(sc) : Tensor();
+    const int dt = dtype_code(branch);
+    const int64_t n = want_w || want_b || want_s ? abi.residual_norm_bwd_ws_bytes(M, D, dt) : 0;
+    check(n, "residual norm backward workspace query");
+    const Tensor ws = bytes_like(h, n);
+    check(abi.residual_norm_bwd(ptr(h), ptr(branch), ptr(w), ptr(bw), ptr(gate), ptr(sc), ptr(dy), ptr(dh), ptr(dx),
+                                ptr(dbranch), ptr(dgate), ptr(dw), ptr(dbw), ptr(ds), ptr(ws), n, M, D,
+                                (float)ctx->saved_data["constant"].toDouble(), (float)ctx->saved_data["eps"].toDouble(),
+                                (int)ctx->saved_data["act"].toInt(), dt, dtype_code(h), param_code(branch, w, bw, sc),
+                                stream_of(h)),
+          "residual norm backward");
+    return {dx, dbranch, dw, dbw, dgate, ds, Tensor(), Tensor(), Tensor()};
+  }
+};
+
 // -------------------------------------------------------------- group norm
 struct GroupNormFn : public Function<GroupNormFn> {
   static int param_code(const Tensor& x, const Tensor& w, const Tensor& b) {
@@ -636,6 +773,127 @@ PyObject* py_linear_attention_step(PyObject*, PyObject* const* args, Py_ssize_t 
   END_HANDLE_TH_ERRORS
 }
 
+// Whether q, k [B, Hk, ..., K], v [B, H, ..., V] and the gates (v's shape without its channels) are of the plain kind, with
+// `rows` axes between heads and channels.
+bool delta_inputs(PyObject* const* args, int rows, Tensor* q, Tensor* k, Tensor* v, Tensor* g, Tensor* b) {
+  if (!plain_tensor(args[0], q) || !plain_tensor(args[1], k, q) || !plain_tensor(args[2], v, q) ||
+      !plain_tensor(args[3], g) || !plain_tensor(args[4], b, g))
+    return false;
+  const int64_t n = 3 + rows;
+  if (dtype_code(*q) < 0 || q->dim() != n || v->dim() != n || k->sizes() != q->sizes() || g->device() != q->device() ||
+      (g->scalar_type() != q->scalar_type() && g->scalar_type() != at::kFloat))
+    return false;
+  if (v->size(0) != q->size(0) || v->size(1) % q->size(1) != 0 || (rows && v->size(2) != q->size(2)) ||
+      q->size(-1) > DC_LA_MAX_DIM || v->size(-1) > DC_LA_MAX_DIM)
+    return false;
+  return g->sizes() == v->sizes().slice(0, n - 1) && b->sizes() == g->sizes() && rows_whole(*q) && rows_whole(*k) &&
+         rows_whole(*v);
+}
+
+// scale (None: 1 / sqrt(K)) and eps; false: an exception is set
+bool scale_and_eps(PyObject* scale, PyObject* eps, const Tensor& q, double* s, double* e) {
+  *s = scale == Py_None ? 1.0 / std::sqrt((double)q.size(-1)) : PyFloat_AsDouble(scale);
+  *e = PyFloat_AsDouble(eps);
+  return !PyErr_Occurred();
+}
+
+// gated_delta_rule(q, k, v, log_decay, beta, scale, initial_state, lengths, return_state, normalize, eps) -> o or (o, state),
+// or None (not taken)
+PyObject* py_gated_delta_rule(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v, g, b, s0, lengths;
+  DC_DECLINE_UNLESS(nargs == 11 && plain_call() && delta_inputs(args, 1, &q, &k, &v, &g, &b));
+  DC_DECLINE_UNLESS(optional_tensor(args[6], &s0, q) && optional_tensor(args[7], &lengths, q) && int_vector(lengths, q.size(0)));
+  DC_DECLINE_UNLESS(!s0.defined() || (s0.scalar_type() == at::kFloat && s0.is_contiguous() && s0.dim() == 4 &&
+                                      s0.size(0) == q.size(0) && s0.size(1) == v.size(1) && s0.size(2) == q.size(3) &&
+                                      s0.size(3) == v.size(3)));
+  double scale = 0, eps = 0;
+  if (!scale_and_eps(args[5], args[10], q, &scale, &eps)) return nullptr;
+  const int want = PyObject_IsTrue(args[8]), unit = PyObject_IsTrue(args[9]);
+  if (want < 0 || unit < 0) return nullptr;
+  // delta._wide_results: whether a result of a call in 16 bits is float32
+  const bool gates = g.scalar_type() == at::kFloat && any_requires_grad({&g, &b});
+  const bool wide = q.scalar_type() != at::kFloat && (want || gates || any_requires_grad({&s0}));
+  const int64_t flags = (unit ? DC_DELTA_NORMALIZE : 0) | (wide ? DC_DELTA_PRECISE : 0);
+  variable_list out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(q.device());
+    out = any_requires_grad({&q, &k, &v, &g, &b, &s0})
+              ? GatedDeltaRuleFn::apply(q, k, v, g, b, opt(s0), opt(lengths), scale, eps, flags, want != 0)
+              : GatedDeltaRuleFn::run(q, k, v, g, b, s0, lengths, scale, eps, flags, want != 0);
+  }
+  return want ? wrap_all(std::move(out)) : THPVariable_Wrap(std::move(out[0]));
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_delta_rule_step(q, k, v, log_decay, beta, state, scale, slots, normalize, eps) -> o, or None (not taken)
+PyObject* py_gated_delta_rule_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v, g, b, state, slots;
+  DC_DECLINE_UNLESS(nargs == 10 && plain_call() && delta_inputs(args, 0, &q, &k, &v, &g, &b) &&
+                    plain_tensor(args[5], &state) && state.device() == q.device());
+  const int64_t B = q.size(0), Hk = q.size(1), K = q.size(2), H = v.size(1), V = v.size(2);
+  DC_DECLINE_UNLESS(!any_requires_grad({&q, &k, &v, &g, &b, &state}));
+  DC_DECLINE_UNLESS(state.scalar_type() == at::kFloat && state.is_contiguous() && state.dim() == 4 && state.size(1) == H &&
+                    state.size(2) == K && state.size(3) == V);
+  DC_DECLINE_UNLESS(optional_tensor(args[7], &slots, q) && int_vector(slots, B) &&
+                    (slots.defined() || B <= state.size(0)));
+  double scale = 0, eps = 0;
+  if (!scale_and_eps(args[6], args[9], q, &scale, &eps)) return nullptr;
+  const int unit = PyObject_IsTrue(args[8]);
+  if (unit < 0) return nullptr;
+  Tensor o;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(q.device());
+    o = at::empty({B, H, V}, q.options());
+    check(abi.delta_rule_step(ptr(q), q.strides().data(), ptr(k), k.strides().data(), ptr(v), v.strides().data(), ptr(g),
+                              g.strides().data(), ptr(b), b.strides().data(), static_cast<float*>(ptr(state)),
+                              static_cast<int32_t*>(ptr(slots)), ptr(o), B, Hk, H, K, V, state.size(0), (float)scale,
+                              (float)eps, dtype_code(q), dtype_code(b), unit ? DC_DELTA_NORMALIZE : 0, stream_of(q)),
+          "gated delta rule step");
+    written(state);
+  }
+  return THPVariable_Wrap(std::move(o));
+  END_HANDLE_TH_ERRORS
+}
+
+// residual_norm(x, branch, weight, branch_weight, gate, activation code, scale, constant, eps) -> (y, h), or None (not taken)
+PyObject* py_residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Tensor x, branch, w, bw, gate, sc;
+  DC_DECLINE_UNLESS(nargs == 9 && plain_call() && plain_tensor(args[0], &x) && plain_tensor(args[1], &branch) &&
+                    branch.device() == x.device() && dtype_code(branch) >= 0 && x.dim() >= 1);
+  DC_DECLINE_UNLESS(x.scalar_type() == branch.scalar_type() || x.scalar_type() == at::kFloat);
+  DC_DECLINE_UNLESS(x.sizes() == branch.sizes() && x.is_contiguous() && branch.is_contiguous() && PyLong_CheckExact(args[5]));
+  DC_DECLINE_UNLESS(optional_tensor(args[2], &w, x) && optional_tensor(args[3], &bw, x) && optional_tensor(args[6], &sc, x));
+  DC_DECLINE_UNLESS(args[4] == Py_None || (plain_tensor(args[4], &gate, &branch) && gate.is_contiguous() &&
+                                           gate.sizes() == x.sizes()));
+  const int64_t D = x.size(-1), act = PyLong_AsLongLong(args[5]);
+  const double constant = PyFloat_AsDouble(args[7]), eps = PyFloat_AsDouble(args[8]);
+  if (PyErr_Occurred()) return nullptr;
+  DC_DECLINE_UNLESS(D <= DC_RN_MAX_DIM && (gate.defined() || act == 0));
+  const Tensor* one = nullptr;
+  for (const Tensor* p : {&w, &bw, &sc}) {
+    if (!p->defined()) continue;
+    DC_DECLINE_UNLESS(p->dim() == 1 && p->size(0) == D && p->is_contiguous() &&
+                      (p->scalar_type() == at::kFloat || p->scalar_type() == branch.scalar_type()) &&
+                      (!one || one->scalar_type() == p->scalar_type()));
+    one = p;
+  }
+  variable_list out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(x.device());
+    out = any_requires_grad({&x, &branch, &w, &bw, &gate, &sc})
+              ? ResidualNormFn::apply(x, branch, opt(w), opt(bw), opt(gate), opt(sc), constant, act, eps)
+              : ResidualNormFn::run(x, branch, w, bw, gate, sc, constant, act, eps);
+  }
+  return wrap_all(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // group_norm(x, groups, weight, bias, gate, activation code, eps) -> y, or None (not taken)
 PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -749,6 +1007,13 @@ PyObject* py_init(PyObject*, PyObject* path) {
   sym(abi.linear_attention_fwd, "dc_linear_attention_fwd");
   sym(abi.linear_attention_bwd, "dc_linear_attention_bwd");
   sym(abi.linear_attention_step, "dc_linear_attention_step");
+  sym(abi.delta_rule_ws_bytes, "dc_delta_rule_ws_bytes");
+  sym(abi.delta_rule_fwd, "dc_delta_rule_fwd");
+  sym(abi.delta_rule_bwd, "dc_delta_rule_bwd");
+  sym(abi.delta_rule_step, "dc_delta_rule_step");
+  sym(abi.residual_norm_fwd, "dc_residual_norm_fwd");
+  sym(abi.residual_norm_bwd_ws_bytes, "dc_residual_norm_bwd_ws_bytes");
+  sym(abi.residual_norm_bwd, "dc_residual_norm_bwd");
   sym(abi.group_norm_fwd, "dc_group_norm_fwd");
   sym(abi.group_norm_bwd_ws_bytes, "dc_group_norm_bwd_ws_bytes");
   sym(abi.group_norm_bwd, "dc_group_norm_bwd");
@@ -768,6 +1033,12 @@ PyMethodDef methods[] = {
      "linear_attention(q, k, v, log_decay, scale, initial_state, lengths, return_state)"},
     {"linear_attention_step", (PyCFunction)(void*)py_linear_attention_step, METH_FASTCALL,
      "linear_attention_step(q, k, v, log_decay, state, scale, slots)"},
+    {"gated_delta_rule", (PyCFunction)(void*)py_gated_delta_rule, METH_FASTCALL,
+     "gated_delta_rule(q, k, v, log_decay, beta, scale, initial_state, lengths, return_state, normalize, eps)"},
+    {"gated_delta_rule_step", (PyCFunction)(void*)py_gated_delta_rule_step, METH_FASTCALL,
+     "gated_delta_rule_step(q, k, v, log_decay, beta, state, scale, slots, normalize, eps)"},
+    {"residual_norm", (PyCFunction)(void*)py_residual_norm, METH_FASTCALL,
+     "residual_norm(x, branch, weight, branch_weight, gate, activation, scale, constant, eps)"},
     {"group_norm", (PyCFunction)(void*)py_group_norm, METH_FASTCALL,
      "group_norm(x, groups, weight, bias, gate, activation, eps)"},
     {"lowrank_step", (PyCFunction)(void*)py_lowrank_step, METH_FASTCALL,

@@ -127,6 +127,10 @@ def gated_delta_rule(
         o [B, H, T, V] in q's dtype, over token-major memory (o.transpose(1, 2).reshape(B, T, H * V) is a view), or
         (o, state [B, H, K, V] float32).  Every input but lengths has a gradient.
     """
+    if _capi.binding is not None:
+        out = _capi.binding.gated_delta_rule(q, k, v, log_decay, beta, scale, initial_state, lengths, return_state, normalize, eps)
+        if out is not None:
+            return out
     assert q.is_cuda and q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k, v must be [B, heads, T, .] on the GPU"
     _check_heads(q, k, v)
     _check_gates(log_decay, beta, v)
@@ -176,6 +180,10 @@ def gated_delta_rule_step(
         o [B, H, V] in q's dtype.  Serving only: no gradients; a backward that has saved `state` from before raises, as
         after torch's own in-place operations.
     """
+    if _capi.binding is not None:
+        o = _capi.binding.gated_delta_rule_step(q, k, v, log_decay, beta, state, scale, slots, normalize, eps)
+        if o is not None:
+            return o
     assert q.is_cuda and q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k, v must be [B, heads, .] on the GPU"
     _check_heads(q, k, v)
     _check_gates(log_decay, beta, v)

@@ -191,6 +191,13 @@ def residual_norm(
         (y, h): the next block's input in branch's dtype, and the residual stream in x's; h is rounded to x's dtype before
         its norm.  Statistics and sums are float32; results are the same run to run.
     """
+    constant = 1.0
+    if scale is not None and not isinstance(scale, torch.Tensor):
+        constant, scale = float(scale), None
+    if _capi.binding is not None and activation in GATE_ACTIVATIONS:
+        out = _capi.binding.residual_norm(x, branch, weight, branch_weight, gate, GATE_ACTIVATIONS[activation], scale, constant, eps)
+        if out is not None:
+            return out
     assert x.is_cuda and x.dim() >= 1 and x.is_contiguous(), "x must be contiguous, on the GPU"
     assert branch.shape == x.shape and branch.device == x.device and branch.is_contiguous(), \
         "branch must be like x, contiguous"
@@ -200,9 +207,6 @@ def residual_norm(
     assert 0 < D <= MAX_ROW, "rows have between 1 and 8192 channels"
     assert activation in GATE_ACTIVATIONS, f"activation must be one of {list(GATE_ACTIVATIONS)}"
     assert gate is not None or activation is None, "an activation is the gate's"
-    constant = 1.0
-    if scale is not None and not isinstance(scale, torch.Tensor):
-        constant, scale = float(scale), None
     params = [p for p in (weight, branch_weight, scale) if p is not None]
     for p in params:
         assert p.device == x.device and p.is_contiguous() and tuple(p.shape) == (D,), \

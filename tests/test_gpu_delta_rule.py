@@ -208,6 +208,19 @@ def test_an_output_that_the_loss_does_not_reach(path):
         _compare([None, None, *got], [None, None, *want], [None, None, *near], dict.fromkeys(NAMES, F32), 2.0**-24)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_one_gradient_alone(dtype, path):
+    """Inputs without a gradient change nothing of the others' (bf16 in float32 results where those are asked for alone)."""
+    (q, k, v, lam, beta, do), S0, _ = _inputs(1, 1, 2, 90, 32, 32, dtype, dtype, True, 11)
+    ts = [t.to(DEV) for t in (q, k, v, lam, beta, S0)]
+    for i in range(6):
+        one = [t.clone().requires_grad_(j == i or (j == 5 and i != 5)) for j, t in enumerate(ts)]
+        full = [t.clone().requires_grad_() for t in ts]
+        f = lambda ls: gated_delta_rule(*ls[:5], initial_state=ls[5], normalize=True)  # noqa: E731
+        (got,), (want,) = torch.autograd.grad(f(one), one[i], do.to(DEV)), torch.autograd.grad(f(full), full[i], do.to(DEV))
+        assert torch.equal(got, want)
+
+
 def test_expanded_inputs_and_views():
     """Heads and batches that are expanded views: their gradients are sums, by autograd."""
     (q, k, v, lam, beta, do), _, _ = _inputs(2, 2, 2, 80, 32, 32, F32, F32, False, 1)

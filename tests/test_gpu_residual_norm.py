@@ -166,6 +166,21 @@ def test_alignment(offset):
     _check((9, 2048), BF, F32, act="silu", offset=offset)
 
 
+@pytest.mark.parametrize("wanted", ["x", "branch", "weight", "branch_weight", "gate", "scale"])
+def test_one_gradient_alone(wanted, path):
+    """Inputs without a gradient change nothing of the others'."""
+    g = gen(3)
+    ts = dict(x=randn(g, 9, 192), branch=randn(g, 9, 192), weight=randn(g, 192), branch_weight=randn(g, 192), gate=randn(g, 9, 192),
+              scale=randn(g, 192))
+    ts = {k: t.to(BF).to(DEV) for k, t in ts.items()}
+    dy, dh = (randn(g, 9, 192).to(BF).to(DEV) for _ in range(2))
+    both = {k: t.clone().requires_grad_() for k, t in ts.items()}
+    (want,) = torch.autograd.grad(residual_norm(**both, activation="silu"), both[wanted], (dy, dh))
+    one = {k: t.clone().requires_grad_(k == wanted) for k, t in ts.items()}
+    (got,) = torch.autograd.grad(residual_norm(**one, activation="silu"), one[wanted], (dy, dh))
+    assert torch.equal(got, want)
+
+
 def test_no_rows(path):
     x = torch.zeros(0, 64, device=DEV, requires_grad=True)
     w = torch.ones(64, device=DEV, requires_grad=True)
