@@ -44,6 +44,31 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[kWaves][4], 
   }
 }
 
+// A row's pieces through buffers of the row's range: channels past it, rows past the last (there: false) and tensors that
+// are not given read as zeros and are not written, without a branch.  Under branches every load was waited for at once, and
+// the next row never was on its way (16384 x 4096 gated bf16 backward 350 -> 210 us).
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void fetch(Row<T, VEC, NV>& r, const Lane<VEC, NV>& L, const void* p, int64_t row, int64_t D, bool there) {
+  const rsrc_t rs = make_rsrc_wave((const T*)p + row * D, p && there ? D * (int64_t)sizeof(T) : 0);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) bload_raw(r.v[i], rs, ((int)L.ch + i * L.step) * (int)sizeof(T));
+}
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void leave(const Lane<VEC, NV>& L, void* p, int64_t row, int64_t D, const float (&v)[NV][VEC]) {
+  const rsrc_t rs = make_rsrc_wave((T*)p + row * D, D * (int64_t)sizeof(T));
+#pragma unroll
+  for (int i = 0; i < NV; ++i) bstore_vals<T, VEC, VEC * sizeof(T) % 16 == 0>(rs, ((int)L.ch + i * L.step) * (int)sizeof(T), v[i]);
+}
+// What was asked for before this row's stores is waited for behind them, where the compiler can count them; at the top of the
+// loop it would wait for the stores too.
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void arrived(Row<T, VEC, NV>& r) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < Raw<T, VEC>::NU; ++j) asm volatile("" : "+v"(r.v[i].u[j]));
+}
+
 // act(a) and its derivative
 __device__ __forceinline__ void activate(int act, float a, float& f, float& d) {
   const float sg = gn::sigmoid(a);
@@ -57,7 +82,7 @@ __device__ __forceinline__ void params(const Lane<VEC, NV>& L, const Args& A, co
   else gn::load_param<T, VEC, NV>(L, p, A.g.param_pieces, 1.f, v);
 }
 
-template <typename T, typename XT, int VEC, int NV, bool WIDE>
+template <typename T, typename XT, int VEC, int NV, bool WIDE, bool GATE>
 __global__ __launch_bounds__(64 * kWaves) void rn_fwd_kernel(Args A) {
   __shared__ float red[2][kWaves][4];
   int slot = 0;
@@ -67,12 +92,12 @@ __global__ __launch_bounds__(64 * kWaves) void rn_fwd_kernel(Args A) {
   if (m >= A.g.M) return;
   Row<XT, VEC, NV> xr;
   Row<T, VEC, NV> br, ar;
-  auto fetch = [&](int64_t row) {
-    br.load(L, A.branch, row * D);
-    xr.load(L, A.x, row * D);
-    if (A.gate) ar.load(L, A.gate, row * D);
+  auto next = [&](int64_t row) {
+    fetch(br, L, A.branch, row, D, row < A.g.M);
+    fetch(xr, L, A.x, row, D, row < A.g.M);
+    if (GATE) fetch(ar, L, A.gate, row, D, row < A.g.M);
   };
-  fetch(m);
+  next(m);
   float w[NV][VEC], bw[NV][VEC], sc[NV][VEC];
   params<T, VEC, NV>(L, A, A.weight, w);
   params<T, VEC, NV>(L, A, A.branch_weight, bw);
@@ -82,8 +107,8 @@ __global__ __launch_bounds__(64 * kWaves) void rn_fwd_kernel(Args A) {
     float x[NV][VEC], b[NV][VEC], a[NV][VEC];
     xr.get(x);
     br.get(b);
-    if (A.gate) ar.get(a);
-    if (m + step < A.g.M) fetch(m + step);
+    if (GATE) ar.get(a);
+    next(m + step);
     float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -97,23 +122,26 @@ __global__ __launch_bounds__(64 * kWaves) void rn_fwd_kernel(Args A) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         float f = 1.f, d;
-        if (A.gate) activate(A.g.act, a[i][j], f, d);
+        if (GATE) activate(A.g.act, a[i][j], f, d);
         x[i][j] = (float)(XT)(x[i][j] + b[i][j] * rb * bw[i][j] * (f * sc[i][j] * A.constant));  // h as it is returned
         s[0] += x[i][j] * x[i][j];
       }
     }
-    gn::store_row<XT, VEC, NV>(L, A.h, m * D, x);
+    leave<XT, VEC, NV>(L, A.h, m, D, x);
     row_sum<WIDE>(s, red, slot);
     const float rh = gn::rsqrt_of(s[0] * inv + A.g.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) x[i][j] *= rh * w[i][j];
-    gn::store_row<T, VEC, NV>(L, A.y, m * D, x);
+    leave<T, VEC, NV>(L, A.y, m, D, x);
+    arrived(br);
+    arrived(xr);
+    if (GATE) arrived(ar);
   }
 }
 
-template <typename T, typename XT, int VEC, int NV, bool WIDE>
+template <typename T, typename XT, int VEC, int NV, bool WIDE, bool GATE>
 __global__ __launch_bounds__(64 * kWaves) void rn_bwd_kernel(Args A) {
   constexpr bool kAhead = VEC * NV <= 16;  // the next row on its way while registers last
   __shared__ float red[2][kWaves][4], sum[WIDE ? 1 : kWaves][WIDE ? 1 : 64 * VEC];
@@ -123,15 +151,14 @@ __global__ __launch_bounds__(64 * kWaves) void rn_bwd_kernel(Args A) {
   int64_t m = WIDE ? (int64_t)blockIdx.y : (int64_t)blockIdx.y * kWaves + wave_id();
   Row<XT, VEC, NV> hr, er;
   Row<T, VEC, NV> br, ar, dr;
-  auto fetch = [&](int64_t row) {
-    if (row >= A.g.M) return;
-    hr.load(L, A.h, row * D);
-    br.load(L, A.branch, row * D);
-    if (A.dy) dr.load(L, A.dy, row * D);
-    if (A.dh) er.load(L, A.dh, row * D);
-    if (A.gate) ar.load(L, A.gate, row * D);
+  auto next = [&](int64_t row) {
+    fetch(hr, L, A.h, row, D, row < A.g.M);
+    fetch(br, L, A.branch, row, D, row < A.g.M);
+    fetch(dr, L, A.dy, row, D, row < A.g.M);
+    fetch(er, L, A.dh, row, D, row < A.g.M);
+    if (GATE) fetch(ar, L, A.gate, row, D, row < A.g.M);
   };
-  if (kAhead) fetch(m);
+  if (kAhead) next(m);
   float w[NV][VEC], bw[NV][VEC], sc[NV][VEC], gw[NV][VEC], gb[NV][VEC], gs[NV][VEC];
   params<T, VEC, NV>(L, A, A.weight, w);
   params<T, VEC, NV>(L, A, A.branch_weight, bw);
@@ -145,16 +172,13 @@ __global__ __launch_bounds__(64 * kWaves) void rn_bwd_kernel(Args A) {
   const float inv = 1.f / A.g.size;
   for (; m < A.g.M; m += step) {
     float h[NV][VEC], b[NV][VEC], a[NV][VEC], d[NV][VEC], e[NV][VEC];
-    if (!kAhead) fetch(m);
+    if (!kAhead) next(m);
     hr.get(h);
     br.get(b);
-    if (A.gate) ar.get(a);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (A.dy) dr.v[i].to_float(d[i]); else zero_vals<VEC>(d[i]);
-      if (A.dh) er.v[i].to_float(e[i]); else zero_vals<VEC>(e[i]);
-    }
-    if (kAhead) fetch(m + step);
+    dr.get(d);
+    er.get(e);
+    if (GATE) ar.get(a);
+    if (kAhead) next(m + step);
     float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -176,7 +200,7 @@ __global__ __launch_bounds__(64 * kWaves) void rn_bwd_kernel(Args A) {
         const float dx = e[i][j] + rh * (d[i][j] * w[i][j] - h[i][j] * c), bh = b[i][j] * rb;
         e[i][j] = dx;
         float f = 1.f, df = 0.f;
-        if (A.gate) activate(A.g.act, a[i][j], f, df);
+        if (GATE) activate(A.g.act, a[i][j], f, df);
         const float n = bh * bw[i][j], dn = dx * (A.constant * sc[i][j]) * f;
         gs[i][j] += A.constant * dx * n * f;
         gb[i][j] += dn * bh;
@@ -185,15 +209,22 @@ __global__ __launch_bounds__(64 * kWaves) void rn_bwd_kernel(Args A) {
         d[i][j] = dn * bw[i][j];
         t[0] += d[i][j] * bh;
       }
-    gn::store_row<XT, VEC, NV>(L, A.dx, m * D, e);
-    if (A.gate) gn::store_row<T, VEC, NV>(L, A.dgate, m * D, a);
+    leave<XT, VEC, NV>(L, A.dx, m, D, e);
+    if (GATE) leave<T, VEC, NV>(L, A.dgate, m, D, a);
     row_sum<WIDE>(t, red, slot);
     const float c2 = t[0] * inv;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) d[i][j] = rb * (d[i][j] - b[i][j] * c2);
-    gn::store_row<T, VEC, NV>(L, A.dbranch, m * D, d);
+    leave<T, VEC, NV>(L, A.dbranch, m, D, d);
+    if (kAhead) {
+      arrived(hr);
+      arrived(br);
+      arrived(dr);
+      arrived(er);
+      if (GATE) arrived(ar);
+    }
   }
   auto write = [&](float* out, float (&v)[NV][VEC]) {
     if (!out) return;
@@ -234,8 +265,9 @@ struct Plan {
 template <typename T, typename XT, int VEC, int NV, bool WIDE>
 hipError_t launch(bool bwd, const Args& a, const Plan& pl, hipStream_t st) {
   const dim3 grid(1, (unsigned)pl.gy);
-  if (bwd) rn_bwd_kernel<T, XT, VEC, NV, WIDE><<<grid, 64 * kWaves, 0, st>>>(a);
-  else rn_fwd_kernel<T, XT, VEC, NV, WIDE><<<grid, 64 * kWaves, 0, st>>>(a);
+  auto run = [&](auto kernel) { kernel<<<grid, 64 * kWaves, 0, st>>>(a); };
+  if (bwd) run(a.gate ? rn_bwd_kernel<T, XT, VEC, NV, WIDE, true> : rn_bwd_kernel<T, XT, VEC, NV, WIDE, false>);
+  else run(a.gate ? rn_fwd_kernel<T, XT, VEC, NV, WIDE, true> : rn_fwd_kernel<T, XT, VEC, NV, WIDE, false>);
   return hipGetLastError();
 }
 

@@ -19,10 +19,11 @@ bool all_aligned(std::initializer_list<const void*> ts, int bytes) {
 // A row of up to 1024 channels lies in a wavefront, a longer one in the workgroup.
 bool wide(const RnProblem& p) { return p.D > 1024; }
 
-// Row blocks: enough wavefronts for every SIMD of 256 CUs eight times over in the forward, four times in the backward (its
-// partial sums grow with them), and no more than there are rows.
+// Row blocks: eight workgroups to a CU in the forward, two in the backward (its registers leave room for one or two, and its
+// partial sums grow with them: 1024 instead of 512 cost 4 us of 230 at 16384 x 4096, 4 of 25 at 4611 x 1000), and no more
+// than there are rows.
 int64_t blocks(const RnProblem& p, bool bwd) {
-  const int64_t want = bwd ? 1024 : 2048, most = wide(p) ? p.M : (p.M + kWaves - 1) / kWaves;
+  const int64_t want = bwd ? 512 : 2048, most = wide(p) ? p.M : (p.M + kWaves - 1) / kWaves;
   return want < most ? want : most;
 }
 
