@@ -169,7 +169,8 @@ hipError_t dr_bwd(const DrProblem& p) {
   if (e == hipSuccess && a.nseg > 1) e = run(dr::kAheadBwd, a, d, columns(a, a.nseg - 1));
   if (e == hipSuccess && a.nseg > 2) e = run(dr::kCarryBwd, a, true, p.B * p.H * (a.vp / 16));
   if (e == hipSuccess) e = run(dr::kChainBwd, a, d, columns(a, a.nseg));
-  return e != hipSuccess ? e : run(dr::kGrads, a, w && whole16(p.d_o, p.dos, p.V, es), p.B * p.Hk * a.n);
+  return e != hipSuccess ? e : run(dr::kGrads, a, w && whole16(p.d_o, p.dos, p.V, es) && whole16(p.dq, p.dqs, p.K, es) &&
+                                                      whole16(p.dk, p.dks, p.K, es), p.B * p.Hk * a.n);
 }
 
 }  // namespace dc

@@ -137,11 +137,15 @@ struct Tile {
     }
     return f;
   }
-  // element (row, c) of spot() order
-  __device__ __forceinline__ float at(int row, int c) const {
-    float v = 0.f;
+  // columns c .. c + 3 (a quad) of a row in spot() order
+  __device__ __forceinline__ f32x4 four(int row, int c) const {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = N - 1; i >= 0; --i) v += (float)t[row * R + spot(c) + i * PL];
+    for (int i = N - 1; i >= 0; --i) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(t + row * R + spot(c) + i * PL);
+      v += f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xFFFF0000u), __uint_as_float(w[1] << 16),
+                 __uint_as_float(w[1] & 0xFFFF0000u)};
+    }
     return v;
   }
 };
@@ -1089,22 +1093,15 @@ __global__ __launch_bounds__(64) void dr_across(Args a) {
   }
 }
 
-// The sum of a value over the 16 lanes of a result's row: every lane gets it.
-__device__ __forceinline__ float sum16(float v) {
-  v += dpp_f<0xB1>(v);
-  v += dpp_f<0x4E>(v);
-  v += dpp_f<0x141>(v);
-  return v + dpp_f<0x140>(v);
-}
-
 // Gradients of q, k and the gates, chunk by chunk: the value heads of one key head to a workgroup, a quarter of the
 // channels to a wavefront.  With the rows' norms in E's place (rq_i rk_j for P, rk_i rk_j for N) the sums are those of q and
-// k themselves, before their part along the row is taken out.  ONE: one value head to a key head, whose sums need no registers
-// of their own.
+// k themselves, before their part along the row is taken out.  Results lie turned over, four neighbouring channels of a
+// token in a lane: sums over a row are of a lane's own and three others', and a store has 8 bytes.  ONE: one value head to a
+// key head, whose sums need no registers of their own.
 template <typename T, int NP, int KP, bool WHOLE, bool ONE>
 __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && parts_of<T>() == 1) ? 2 : 1) void dr_grads(Args a) {
   constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
-  constexpr int NCB = KP / 64, RV = kPiece + 8, PV = C * RV;
+  constexpr int NCB = KP / 64, RV = kPiece + 8, PV = C * RV, NU = NB * NB / 4;
   constexpr int ROWS = (NI + 2 * NP) * PV, KEYS = 2 * NI * PL;
   __shared__ __align__(16) bf16 mem[ROWS > KEYS ? ROWS : KEYS], lm[2 * NP * PC];
   __shared__ __align__(16) float lv[kVecs][C];
@@ -1112,11 +1109,12 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
   const Tile<NI, RV, PV> to{mem};
   const Tile<NP, RV, PV> tu{mem + NI * PV}, tx{mem + (NI + NP) * PV};
   const Tile<NI, R, PL> tk{mem}, tq{mem + NI * PL};
-  const Tile<NP, RC, PC> pe{lm}, ne{lm + NP * PC};
+  const Tile<NP, RC, PC> pe{lm}, ne{lm + NP * PC};  // row j, column i
   const DrProblem& p = a.p;
   const int64_t blk = a.blk0 + blockIdx.x, n = blk % a.n, bhk = blk / a.n, b = bhk / p.Hk, hk = bhk % p.Hk;
   const int t0 = (int)n * C, len = length_of(p, b), cnt = min(C, max(len - t0, 0)), rows = min(C, (int)p.T - t0), t = threadIdx.x;
-  const int K = (int)p.K, V = (int)p.V, group = ONE ? 1 : (int)(p.H / p.Hk), lane = t % 64, g = lane / 16, col = lane % 16, wv = wave_id();
+  const int K = (int)p.K, V = (int)p.V, group = ONE ? 1 : (int)(p.H / p.Hk), lane = t % 64, g = lane / 16, col = lane % 16;
+  const int wv = wave_id();
   T* dq_ = (T*)p.dq + b * p.dqs[0] + hk * p.dqs[1] + (int64_t)t0 * p.dqs[2];
   T* dk_ = (T*)p.dk + b * p.dks[0] + hk * p.dks[1] + (int64_t)t0 * p.dks[2];
   f32x4 sq[NB][NCB], sk[NB][NCB];
@@ -1141,36 +1139,31 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
   for (int hd = 0; hd < group; ++hd) {
     const int64_t h = hk * group + hd, bh = b * p.H + h, ch = bh * a.n + n;
     const T* d_o = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + (int64_t)t0 * p.dos[2];
-    __syncthreads();  // the head before has been read
-    for (int e = t; e < kVecs * C; e += 256) lv[0][e] = a.vec[ch * kVecs * C + e];
+    if (hd > 0) __syncthreads();  // the head before has been read
     f32x4 dq[NB][NCB], dr[NB][NCB], dw[NB][NCB];
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb)
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb) dq[rb][cb] = dr[rb][cb] = dw[rb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // dO U^T and dX U^T: each wavefront has one of them, and of its blocks of rows a small and a large one
-    const int m = wv % 2;
-    f32x4 acc[NB / 2][NB];
-    int rbs[NB / 2];
+    // dO U^T and dX U^T: a block of rows (i) to a wavefront and all blocks of columns (j), those above the diagonal too,
+    // which cost less than the branches that would leave them out; with two blocks of rows one block to a wavefront
+    const int rbu = NB == 4 ? wv : wv % 2;
+    f32x4 accp[NU], accn[NU];
 #pragma unroll
-    for (int i = 0; i < NB / 2; ++i) {
-      rbs[i] = i ? NB - 1 - wv / 2 : wv / 2;
-#pragma unroll
-      for (int cb = 0; cb < NB; ++cb) acc[i][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int i = 0; i < NU; ++i) accp[i] = accn[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float dot = 0.f;
     for (int v0 = 0; v0 < a.vp; v0 += kPiece) {
       const int width = min(kPiece, a.vp - v0);
       if (v0 > 0) __syncthreads();
-      Frag<NP> fs[NCB], fd[NCB];  // the states' operands of a step, the next step's on their way
+      Frag<NP> fs[2][NCB], fd[2][NCB];  // the states' operands of a step and the next
       auto states = [&](int s) {
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
           const int64_t at = ch * NP * KP * a.vp + (int64_t)(wv * NCB * 16 + 16 * cb + col) * a.vp + v0 + 32 * s + 8 * g;
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
-            fs[cb].p[i] = *reinterpret_cast<const u32x4*>(a.s + at + (int64_t)i * KP * a.vp);
-            fd[cb].p[i] = *reinterpret_cast<const u32x4*>(a.ds + at + (int64_t)i * KP * a.vp);
+            fs[s % 2][cb].p[i] = *reinterpret_cast<const u32x4*>(a.s + at + (int64_t)i * KP * a.vp);
+            fd[s % 2][cb].p[i] = *reinterpret_cast<const u32x4*>(a.ds + at + (int64_t)i * KP * a.vp);
           }
         }
       };
@@ -1183,29 +1176,45 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
           ru[i].load(a.u + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
           ru[NP + i].load(a.x + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
         }
+        float vec[(kVecs * C + 255) / 256];
+        if (v0 == 0)
+#pragma unroll
+          for (int i = 0; i * 256 < kVecs * C; ++i) vec[i] = a.vec[ch * kVecs * C + i * 256 + t];
         states(0);
         ro.template store<RV, PV, false>(mem);
 #pragma unroll
         for (int i = 0; i < 2 * NP; ++i) ru[i].template store<RV, PV, false>(mem + (NI + i) * PV);
+        if (v0 == 0)
+#pragma unroll
+          for (int i = 0; i * 256 < kVecs * C; ++i) lv[0][i * 256 + t] = vec[i];
       }
       __syncthreads();
-      for (int s = 0; s < width / 32; ++s) {
-        Frag<NP> gs[NCB], gd[NCB];
 #pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) {
-          gs[cb] = fs[cb];
-          gd[cb] = fd[cb];
+      for (int s = 0; s < kPiece / 32; ++s) {
+        if (s * 32 >= width) break;
+        if ((s + 1) * 32 < width) states(s + 1);
+        const Frag<NP> (&gs)[NCB] = fs[s % 2], (&gd)[NCB] = fd[s % 2];
+        const Frag<NI> uo = to.rows(16 * rbu, s);
+        const Frag<NP> ux = tx.rows(16 * rbu, s);
+        if constexpr (NB == 2) {
+          const Frag<NP> uu = tu.rows(16 * (wv / 2), s);
+          accp[0] = mma(uo, uu, accp[0]);
+          accn[0] = mma(ux, uu, accn[0]);
         }
-        if (s + 1 < width / 32) states(s + 1);
 #pragma unroll
-        for (int i = 0; i < NB / 2; ++i) {
-          auto row = [&](auto f) {
+        for (int rb = 0; rb < NB; ++rb) {
+          const Frag<NI> ro = to.rows(16 * rb, s);
+          const Frag<NP> rx = tx.rows(16 * rb, s), ru = tu.rows(16 * rb, s);
+          if constexpr (NB == 4) {
+            accp[rb] = mma(uo, ru, accp[rb]);
+            accn[rb] = mma(ux, ru, accn[rb]);
+          }
 #pragma unroll
-            for (int cb = 0; cb < NB; ++cb)
-              if (cb <= rbs[i]) acc[i][cb] = mma(f, tu.rows(16 * cb, s), acc[i][cb]);
-          };
-          if (m) row(tx.rows(16 * rbs[i], s));
-          else row(to.rows(16 * rbs[i], s));
+          for (int cb = 0; cb < NCB; ++cb) {
+            dq[rb][cb] = mma(gs[cb], ro, dq[rb][cb]);
+            dr[rb][cb] = mma(gs[cb], rx, dr[rb][cb]);
+            dw[rb][cb] = mma(gd[cb], ru, dw[rb][cb]);
+          }
         }
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb)
@@ -1221,94 +1230,109 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
             }
             dot += x[0] * y[0] + x[1] * y[1];
           }
-#pragma unroll
-        for (int rb = 0; rb < NB; ++rb) {
-          const Frag<NI> ro = to.rows(16 * rb, s);
-          const Frag<NP> rx = tx.rows(16 * rb, s), ru = tu.rows(16 * rb, s);
-#pragma unroll
-          for (int cb = 0; cb < NCB; ++cb) {
-            dq[rb][cb] = mma(ro, gs[cb], dq[rb][cb]);
-            dr[rb][cb] = mma(rx, gs[cb], dr[rb][cb]);
-            dw[rb][cb] = mma(ru, gd[cb], dw[rb][cb]);
-          }
-        }
       }
     }
-    // the pairs' gradients with their decays and norms, as operands
-#pragma unroll
-    for (int i = 0; i < NB / 2; ++i)
-#pragma unroll
-      for (int cb = 0; cb < NB; ++cb) {
-        if (cb / 2 > rbs[i] / 2) continue;  // above the diagonal by whole steps: not read
-        const int j = 16 * cb + col;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int x = 16 * rbs[i] + 4 * g + r;
-          const float E = expf((lv[0][x] - lv[0][j]) + (lv[1][x] - lv[1][j]));
-          const float v = m ? -lv[kRk][x] * lv[kRk][j] * E * acc[i][cb][r] : p.scale * lv[kRq][x] * lv[kRk][j] * E * acc[i][cb][r];
-          if (m && x == j) diag[x] = acc[i][cb][r];
-          uint32_t w[NP];
-          split<NP>(j < x + 1 - m ? v : 0.f, 0.f, w);
-#pragma unroll
-          for (int l = 0; l < NP; ++l)
-            reinterpret_cast<uint16_t*>(lm)[(m * NP + l) * PC + x * RC + spot(j)] = (uint16_t)w[l];
-        }
-      }
     Rows<T, C, KP, 256, WHOLE> rk, rq;
     rk.load((const T*)p.k + b * p.ks[0] + hk * p.ks[1] + (int64_t)t0 * p.ks[2], p.ks[2], K, cnt);
     rq.load((const T*)p.q + b * p.qs[0] + hk * p.qs[1] + (int64_t)t0 * p.qs[2], p.qs[2], K, cnt);
+    // the pairs' gradients with their decays and norms, as operands
+    {
+      auto at = [&](int m) { return *reinterpret_cast<const f32x4*>(&lv[m][16 * rbu + 4 * g]); };
+      const f32x4 hi = at(0), lo = at(1), ki = at(kRk), qi = at(kRq) * p.scale;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        const int cb = NB == 4 ? i : wv / 2, j = 16 * cb + col;
+        const float hj = lv[0][j], lj = lv[1][j], kj = lv[kRk][j];
+        f32x4 vp, vn;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int x = 16 * rbu + 4 * g + r;
+          // e^(c_i - c_j) by the instruction (one last place); above the diagonal the difference is not negative, and unused
+          const float E = kj * __builtin_amdgcn_exp2f(((hi[r] - hj) + (lo[r] - lj)) * 1.44269504088896f);
+          vp[r] = j <= x ? qi[r] * E * accp[i][r] : 0.f;
+          vn[r] = j < x ? -ki[r] * E * accn[i][r] : 0.f;
+          if (x == j) diag[x] = accn[i][r];
+        }
+        const int where = j * RC + spot(16 * rbu + 4 * g);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          uint32_t w0[NP], w1[NP];
+          split<NP>(m ? vn[0] : vp[0], m ? vn[1] : vp[1], w0);
+          split<NP>(m ? vn[2] : vp[2], m ? vn[3] : vp[3], w1);
+#pragma unroll
+          for (int l = 0; l < NP; ++l) *reinterpret_cast<u32x2*>(lm + (m * NP + l) * PC + where) = u32x2{w0[l], w1[l]};
+        }
+      }
+    }
     __syncthreads();  // the rows have been read, the pairs are there
     rk.template store<R, PL, true>(mem);
     rq.template store<R, PL, true>(mem + NI * PL);
     __syncthreads();
-    const float gc = expf(lv[0][C - 1]);
-    float kept = gc * dot;
-    f32x4 sums[3][NB];
+    float kept = expf(lv[0][C - 1]) * dot, sums[3][NB];
+    Frag<NI> fk[NCB][C / 32], fq[NCB][C / 32];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+      for (int s = 0; s < C / 32; ++s) {
+        fk[cb][s] = tk.cols(wv * NCB + cb, s);
+        fq[cb][s] = tq.cols(wv * NCB + cb, s);
+      }
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) {
-      auto at = [&](int m, int row) { return *reinterpret_cast<const f32x4*>(&lv[m][row + 4 * g]); };
-      sums[0][rb] = sums[1][rb] = sums[2][rb] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const f32x4 gq = at(kGq, 16 * rb), gk = at(kGk, 16 * rb), dk = at(kDk, 16 * rb);
+      const int i = 16 * rb + col;
+      const float gq = lv[kGq][i], gk = -lv[kGk][i], dk = lv[kDk][i];
+      sums[0][rb] = sums[1][rb] = sums[2][rb] = 0.f;
+      f32x4 kv[NCB], qv[NCB];
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb) {
-        const int kb = wv * NCB + cb;
-        f32x4 kv, qv;
+        kv[cb] = tk.four(i, 16 * (wv * NCB + cb) + 4 * g);
+        qv[cb] = tq.four(i, 16 * (wv * NCB + cb) + 4 * g);
+        dq[rb][cb] *= gq;
+        dr[rb][cb] *= gk;
+        dw[rb][cb] *= dk;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) kept += kv[cb][r] * dw[rb][cb][r];
+      }
+#pragma unroll
+      for (int s = 0; s < C / 32; ++s) {
+        if (s <= rb / 2) {
+          const Frag<NP> fp = pe.cols(rb, s), fn = ne.cols(rb, s);
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb) {
+            dq[rb][cb] = mma(fk[cb][s], fp, dq[rb][cb]);
+            dr[rb][cb] = mma(fk[cb][s], fn, dr[rb][cb]);
+          }
+        }
+        if (s >= rb / 2) {
+          const Frag<NP> fp = pe.rows(16 * rb, s), fn = ne.rows(16 * rb, s);
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb) {
+            dw[rb][cb] = mma(fq[cb][s], fp, dw[rb][cb]);
+            dw[rb][cb] = mma(fk[cb][s], fn, dw[rb][cb]);
+          }
+        }
+      }
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          kv[r] = tk.at(16 * rb + 4 * g + r, 16 * kb + col);
-          qv[r] = tq.at(16 * rb + 4 * g + r, 16 * kb + col);
+          sums[0][rb] += qv[cb][r] * dq[rb][cb][r];
+          sums[1][rb] += kv[cb][r] * dr[rb][cb][r];
+          sums[2][rb] += kv[cb][r] * dw[rb][cb][r];
         }
-        f32x4 x = dq[rb][cb] * gq, y = -dr[rb][cb] * gk, z = dw[rb][cb] * dk;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) kept += kv[r] * z[r];
-#pragma unroll
-        for (int s = 0; s < C / 32; ++s) {
-          const Frag<NI> fk = tk.cols(kb, s), fq = tq.cols(kb, s);
-          if (s <= rb / 2) {
-            x = mma(pe.rows(16 * rb, s), fk, x);
-            y = mma(ne.rows(16 * rb, s), fk, y);
-          }
-          if (s >= rb / 2) {
-            z = mma(pe.cols(rb, s), fq, z);
-            z = mma(ne.cols(rb, s), fk, z);
-          }
-        }
-        sums[0][rb] += qv * x;
-        sums[1][rb] += kv * y;
-        sums[2][rb] += kv * z;
-        sq[rb][cb] += x;
-        sk[rb][cb] += y + z;
+        sq[rb][cb] += dq[rb][cb];
+        sk[rb][cb] += dr[rb][cb] + dw[rb][cb];
       }
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
+    for (int m = 0; m < 3; ++m)
 #pragma unroll
-      for (int rb = 0; rb < NB; ++rb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float s = sum16(sums[i][rb][r]);
-          if (col == 0) red[i][wv][16 * rb + 4 * g + r] = s;
-        }
+      for (int rb = 0; rb < NB; ++rb) {
+        float s = sums[m][rb];
+        s += __shfl_xor(s, 16);
+        s += __shfl_xor(s, 32);
+        if (g == 0) red[m][wv][16 * rb + col] = s;
+      }
 #pragma unroll
     for (int i = 1; i < 64; i *= 2) kept += __shfl_xor(kept, i);
     if (lane == 0) total[wv] = kept;
@@ -1338,22 +1362,30 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
     }
   }
   __syncthreads();
+  auto out = [&](T* base, int64_t stride, int i, int c, f32x4 v) {  // rows from cnt on are zero
+    if constexpr (WHOLE) {
+      const rsrc_t rs = make_rsrc_wave(base, ((int64_t)(rows - 1) * stride + K) * (int64_t)sizeof(T));
+      const float e[4] = {v[0], v[1], v[2], v[3]};
+      bstore_vals<T, 4>(rs, c < K ? i * (int)stride * (int)sizeof(T) + c * (int)sizeof(T) : kOut, e);
+    } else {
 #pragma unroll
-  for (int rb = 0; rb < NB; ++rb)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 16 * rb + 4 * g + r;
-      if (i >= rows) continue;
-      const float rki = lv[kRk][i], rqi = lv[kRq][i];
-      const float ak = p.normalize ? rki * rki * along[1][i] : 0.f, aq = p.normalize ? rqi * rqi * along[0][i] : 0.f;
-#pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        const int c = 16 * (wv * NCB + cb) + col;
-        if (c >= K) continue;
-        dq_[(int64_t)i * p.dqs[2] + c] = (T)(i < cnt ? sq[rb][cb][r] - tq.at(i, c) * aq : 0.f);
-        dk_[(int64_t)i * p.dks[2] + c] = (T)(i < cnt ? sk[rb][cb][r] - tk.at(i, c) * ak : 0.f);
-      }
+      for (int r = 0; r < 4; ++r)
+        if (i < rows && c + r < K) base[(int64_t)i * stride + c + r] = (T)v[r];
     }
+  };
+#pragma unroll
+  for (int rb = 0; rb < NB; ++rb) {
+    const int i = 16 * rb + col;
+    const float rki = lv[kRk][i], rqi = lv[kRq][i];
+    const float ak = p.normalize ? rki * rki * along[1][i] : 0.f, aq = p.normalize ? rqi * rqi * along[0][i] : 0.f;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+      const int c = 16 * (wv * NCB + cb) + 4 * g;
+      const f32x4 x = sq[rb][cb] - tq.four(i, c) * aq, y = sk[rb][cb] - tk.four(i, c) * ak, zero = {0.f, 0.f, 0.f, 0.f};
+      out(dq_, p.dqs[2], i, c, i < cnt ? x : zero);
+      out(dk_, p.dks[2], i, c, i < cnt ? y : zero);
+    }
+  }
 }
 
 // The launches of a type and a number of parts (instantiated in delta_<type>.hip).
