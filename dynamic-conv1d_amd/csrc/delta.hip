@@ -34,34 +34,40 @@ int chunk(const DrProblem& p) {
   return dr::chunk_of(p.dtype == kFP32 ? 3 : p.dtype == kFP16 ? 2 : 1, np_of(p), dr::cover((int)p.K));
 }
 
-// Segments of the tokens, where heads and columns leave CUs idle: one launch finds what each makes of the state before it, a
-// second carries the states across, and the chains run side by side.  The count with the least estimated time, per chunk of
-// a workgroup in units of the forward's chain: 1 for a chain, 0.8 for one without outputs (twice, with the unit vectors'
-// columns, where K is V), rounds of `fit` workgroups, and the launches.
-int segments(const DrProblem& p, int C, int np) {
-  const int kp = dr::cover((int)p.K), vp = ((int)p.V + 31) / 32 * 32, cols = 2 * 16;
+// How the chains are cut: segments of the tokens, where heads and columns leave CUs idle (one launch finds what each makes of
+// the state before it, a second carries the states across, and the chains run side by side), and wavefronts of a workgroup
+// where its tiles leave room for one on a CU.  The least estimated time: per chunk of a chain `us`, 0.8 of that without
+// outputs (with the unit vectors' columns, twice as many where K is V), in rounds of the workgroups that fit, and the launches.
+struct Cut {
+  int nseg, nw;
+};
+Cut cut_of(const DrProblem& p, int C, int np) {
+  const int kp = dr::cover((int)p.K), vp = ((int)p.V + 31) / 32 * 32;
   const int64_t chunks = (p.T + C - 1) / C, heads = p.B * p.H;
-  // workgroups side by side on 256 CUs, by their LDS
-  const double fit = 256 * (np == 1 && kp > 64 ? 1 : 2), us = np == 1 ? 2.5 : 2.8;
-  double best = 0;
-  int n = 1;
-  for (int s = 1; s <= 64 && s <= chunks; ++s) {
-    const int64_t len = (chunks + s - 1) / s;
-    if ((chunks + len - 1) / len != s) continue;  // the same segments as fewer
-    double t = us * len * __builtin_ceil(heads * s * (vp / cols) / fit);
-    if (s > 1) t += 0.8 * us * len * __builtin_ceil(heads * (s - 1) * ((vp + kp) / cols) / 512.) + 15 + 4 * s;
-    if (s == 1 || t < best) {
-      best = t;
-      n = s;
+  const bool one = np == 1 && kp == 128 && p.dtype == kBF16;  // workgroup on a CU; elsewhere two
+  double best = -1;
+  Cut cut{1, 2};
+  for (int nw = 2; nw <= (one && vp % 64 == 0 ? 4 : 2); nw += 2) {
+    const double fit = one ? 256 : 512, us = (np == 1 ? 2.5 : 2.8) * (nw == 4 ? 1.25 : 1);
+    const int cols = nw * 16;
+    for (int s = 1; s <= 64 && (s == 1 || s <= chunks); ++s) {
+      const int64_t len = (chunks + s - 1) / s;
+      if (s > 1 && (chunks + len - 1) / len != s) continue;  // the same segments as fewer
+      double t = us * len * __builtin_ceil(heads * s * (vp / cols) / fit);
+      if (s > 1) t += 0.8 * us * len * __builtin_ceil(heads * (s - 1) * ((vp + kp) / cols) / 512.) + 15 + 4 * s;
+      if (best < 0 || t < best) {
+        best = t;
+        cut = {s, nw};
+      }
     }
   }
-  return n;
+  return cut;
 }
 
 // The workspace: of the forward vec, Tb, P and the segments' states, of the backward U, dX, the states and their gradients.
 struct Plan {
   int64_t n, vec, sq, rows, st, cut, trans;  // chunks of a head; bytes of each array
-  int vp, seg, nseg;
+  int vp, seg, nseg, nw;
   explicit Plan(const DrProblem& p) {
     const int C = chunk(p), np = np_of(p);
     n = (p.T + C - 1) / C;
@@ -72,7 +78,9 @@ struct Plan {
     rows = chunks * np * C * vp * 2;
     const int kp = dr::cover((int)p.K);
     st = chunks * np * kp * vp * 2;
-    nseg = segments(p, C, np);
+    const Cut cut_ = cut_of(p, C, np);
+    nseg = cut_.nseg;
+    nw = cut_.nw;
     seg = (int)((n + nseg - 1) / nseg) * C;
     cut = nseg > 1 ? (p.B * p.H * nseg * p.K * p.V * 4 + 15) / 16 * 16 : 0;
     trans = nseg > 1 ? p.B * p.H * nseg * kp * kp * 4 : 0;
@@ -89,6 +97,7 @@ Args args_of(const DrProblem& p, bool bwd) {
   a.vp = pl.vp;
   a.seg = pl.seg;
   a.nseg = pl.nseg;
+  a.nw = pl.nw;
   char* f = static_cast<char*>(bwd && p.fwd_ws ? const_cast<void*>(p.fwd_ws) : p.ws);
   a.vec = reinterpret_cast<float*>(f);
   a.tb = reinterpret_cast<bf16*>(f + pl.vec);
@@ -133,7 +142,7 @@ hipError_t run(Stage st, Args a, bool whole, int64_t blocks) {
 }
 
 // Workgroups of the chains over `seg` segments, and `more` columns beside V's.
-int64_t columns(const Args& a, int seg, int more = 0) { return a.p.B * a.p.H * seg * ((a.vp + more) / (dr::kNW * 16)); }
+int64_t columns(const Args& a, int seg, int more = 0) { return a.p.B * a.p.H * seg * ((a.vp + more) / (a.nw * 16)); }
 
 // What the chunks need of their own keys, and the states before the segments.
 hipError_t ahead(const Args& a, bool keys, bool values) {

@@ -42,7 +42,7 @@ struct Args {
   // tokens cut into nseg segments of seg (whole chunks): the states before each but the first [heads][nseg][K][V], the
   // gradients after each but the last, and what a segment makes of the state before it, [heads][nseg][KP][KP]
   float *start, *dstart, *trans;
-  int seg, nseg;
+  int seg, nseg, nw;  // nw: wavefronts of a chain's workgroup, 16 columns each
   int64_t n;           // chunks of a head
   int vp;              // V in whole 32 columns
   int64_t blk0;
@@ -507,7 +507,6 @@ __device__ __forceinline__ void keep(bf16* to, int vp, int64_t plane, const Frag
     }
 }
 
-constexpr int kNW = 2, kNT = kNW * 64;  // wavefronts of the chains, 16 columns each
 
 // Nothing moves across the end of a phase: without it the compiler sinks a batch of operands to its use, which then waits.
 __device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
@@ -538,21 +537,21 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KP / 16], float* to
 }
 
 // The chains' scales of a chunk on their way to LDS: G/|k|, D/|k|, scale G/|q|; top: the whole chunk's decay's logarithm.
-template <int C>
+template <int C, int NT>
 struct Scales {
-  float v[(3 * C + kNT - 1) / kNT], top = 0.f;
+  float v[(3 * C + NT - 1) / NT], top = 0.f;
   __device__ __forceinline__ void load(const float* vec) {
 #pragma unroll
-    for (int i = 0; i * kNT < 3 * C; ++i) {
-      const int e = i * kNT + (int)threadIdx.x;
+    for (int i = 0; i * NT < 3 * C; ++i) {
+      const int e = i * NT + (int)threadIdx.x;
       v[i] = vec[kGk * C + (e < 3 * C ? e : 0)];
     }
     top = vec[C - 1];
   }
   __device__ __forceinline__ void store(float* lds) const {
 #pragma unroll
-    for (int i = 0; i * kNT < 3 * C; ++i) {
-      const int e = i * kNT + (int)threadIdx.x;
+    for (int i = 0; i * NT < 3 * C; ++i) {
+      const int e = i * NT + (int)threadIdx.x;
       if (e < 3 * C) lds[e] = v[i];
     }
   }
@@ -563,20 +562,20 @@ struct Scales {
 // wavefront that has waited for a later load of its own (the scales, which it stores to LDS) has these in LDS too, and the
 // barrier after that makes them everybody's.  Waiting for all, stores among them, took half of the time of the chains that
 // keep states.
-template <int C, int W>
+template <int C, int W, int NW>
 __device__ __forceinline__ void load_direct(const bf16* base, int64_t stride, int cnt, bf16* lds) {
-  constexpr int PR = W / 8, N = C * PR / kNT, RPL = kNT / PR;  // pieces of a row, loads, rows of a load
+  constexpr int PR = W / 8, N = C * PR / (NW * 64), RPL = (NW * 64) / PR;  // pieces of a row, loads, rows of a load
   constexpr int VAR = RPL < 16 ? 16 / RPL : 1;                 // loads after which the rows' turns repeat
-  static_assert(C * PR % kNT == 0 && N % VAR == 0, "whole loads");
+  static_assert(C * PR % (NW * 64) == 0 && N % VAR == 0, "whole loads");
   const rsrc_t rs = make_rsrc_wave(base, ((int64_t)(cnt - 1) * stride + W) * 2);
   const int wv = wave_id(), lane = threadIdx.x % 64, sb = (int)stride * 2;
   const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) bf16*)lds + wv * 1024;
   auto place = [&](int i, int last) {
-    const int row = ((i * kNW + wv) * 64 + lane) / PR;
+    const int row = ((i * NW + wv) * 64 + lane) / PR;
     return min(row, last) * sb + 16 * ((lane % PR) ^ turn<W>(row));
   };
   auto load = [&](int i, int off, int more) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to + i * kNW * 1024), "v"(off),
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to + i * NW * 1024), "v"(off),
                  "s"(rs), "s"(more)
                  : "m0", "memory");
   };
@@ -609,12 +608,16 @@ struct ChainSize {
 template <typename T, int NP, int KP>
 constexpr bool kHasDirect = __is_same(T, bf16) && ChainSize<T, NP, KP, kDirect>::bytes(true) <= 160 * 1024;
 
+// Tiles that leave room for one workgroup on a CU: four wavefronts to it instead of two, where there are columns for them.
+template <typename T, int NP, int KP>
+constexpr bool kHasFour = __is_same(T, bf16) && NP == 1 && KP == 128;
+
 // The states from chunk to chunk, and o (kOutputs); or U and the state before each chunk for the backward (kKeep); or what each
 // segment but the last makes of the state before it (kAcross): its end from zero, and behind those columns its end from each
 // unit vector without values.
 enum What { kOutputs, kKeep, kAcross };
-template <typename T, int NP, int KP, int MODE, int WHAT>
-__global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain(Args a) {
+template <typename T, int NP, int KP, int MODE, int WHAT, int NW>
+__global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
   constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
   constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather, KEEP = WHAT != kOutputs;  // KEEP: no q and no o
@@ -626,15 +629,15 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
   bf16 (*lp)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lq + Z::BUF);
   const DrProblem& p = a.p;
   // columns: V's, and behind them those of the unit vectors
-  const int nvb = (a.vp + (WHAT == kAcross ? KP : 0)) / (kNW * 16), nseg = WHAT == kAcross ? a.nseg - 1 : a.nseg;
+  const int nvb = (a.vp + (WHAT == kAcross ? KP : 0)) / (NW * 16), nseg = WHAT == kAcross ? a.nseg - 1 : a.nseg;
   int64_t blk = a.blk0 + xcd_remap(blockIdx.x, a.nblk);
   const int vb = (int)(blk % nvb);
   blk /= nvb;
   const int seg = (int)(blk % nseg);
   const int64_t bh = blk / nseg, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
   const int lane = threadIdx.x % 64, g = lane / 16, col = lane % 16;
-  const int n0 = vb * kNW * 16 + wave_id() * 16, nn = n0 + col, K = (int)p.K, V = (int)p.V;
-  const bool live = nn < V, unit = WHAT == kAcross && vb * kNW * 16 >= a.vp;
+  const int n0 = vb * NW * 16 + wave_id() * 16, nn = n0 + col, K = (int)p.K, V = (int)p.V;
+  const bool live = nn < V, unit = WHAT == kAcross && vb * NW * 16 >= a.vp;
   if (unit && seg == 0) return;  // the state before the first segment is known
   const int lo = seg * a.seg, len = min(length_of(p, b), lo + a.seg), whole = length_of(p, b);
   const T* q = (const T*)p.q + b * p.qs[0] + hk * p.qs[1];
@@ -653,10 +656,10 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
     const float* from = seg == 0 ? (p.s_in ? p.s_in + sb : nullptr) : WHAT == kAcross ? nullptr : a.start + at0;
     load_state<KP>(S, from, live, K, V);
   }
-  Rows<T, C, KP, kNT, WHOLE> rk, rq;
-  Square<NP, C, kNT> rt, rp;
+  Rows<T, C, KP, NW * 64, WHOLE> rk, rq;
+  Square<NP, C, NW * 64> rt, rp;
   Columns<T, C, WHOLE> cv;
-  Scales<C> vec;
+  Scales<C, NW * 64> vec;
   auto fetch = [&](int t0, int buf) {
     if (t0 >= len) return;
     const int cnt = min(C, len - t0);
@@ -664,11 +667,11 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
     const T *kt = k + (int64_t)t0 * p.ks[2], *qt = q + (int64_t)t0 * p.qs[2];
     const bf16 *tt = a.tb + ch * NP * C * C, *pt = a.pp + ch * NP * C * C;
     if constexpr (DIRECT) {
-      load_direct<C, KP>(kt, p.ks[2], cnt, lk[buf]);
-      load_direct<NP * C, C>(tt, C, NP * C, lt[buf]);
+      load_direct<C, KP, NW>(kt, p.ks[2], cnt, lk[buf]);
+      load_direct<NP * C, C, NW>(tt, C, NP * C, lt[buf]);
       if (!KEEP) {
-        load_direct<C, KP>(qt, p.qs[2], cnt, lq[buf]);
-        load_direct<NP * C, C>(pt, C, NP * C, lp[buf]);
+        load_direct<C, KP, NW>(qt, p.qs[2], cnt, lq[buf]);
+        load_direct<NP * C, C, NW>(pt, C, NP * C, lp[buf]);
       }
     } else {
       rk.load(kt, p.ks[2], K, cnt);
@@ -844,8 +847,8 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
 
 // The states' gradients from the last chunk on, and dv; ACROSS: only what each segment but the first makes of them from zero
 // (from the state after it they come by the transpose of what the forward found).
-template <typename T, int NP, int KP, int MODE, bool ACROSS>
-__global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain_bwd(Args a) {
+template <typename T, int NP, int KP, int MODE, bool ACROSS, int NW>
+__global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain_bwd(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
   constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
   constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
@@ -856,14 +859,14 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
   bf16 (*lq)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lt + Z::BUF);
   bf16 (*lp)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lq + Z::BUF);
   const DrProblem& p = a.p;
-  const int nvb = a.vp / (kNW * 16), nseg = ACROSS ? a.nseg - 1 : a.nseg;
+  const int nvb = a.vp / (NW * 16), nseg = ACROSS ? a.nseg - 1 : a.nseg;
   int64_t blk = a.blk0 + xcd_remap(blockIdx.x, a.nblk);
   const int vb = (int)(blk % nvb);
   blk /= nvb;
   const int seg = (int)(blk % nseg) + ACROSS;
   const int64_t bh = blk / nseg, b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
   const int lane = threadIdx.x % 64, g = lane / 16, col = lane % 16;
-  const int n0 = vb * kNW * 16 + wave_id() * 16, nn = n0 + col, K = (int)p.K, V = (int)p.V;
+  const int n0 = vb * NW * 16 + wave_id() * 16, nn = n0 + col, K = (int)p.K, V = (int)p.V;
   const bool live = nn < V;
   const int lo = seg * a.seg, len = min(length_of(p, b), lo + a.seg), whole = length_of(p, b);
   const T* q = (const T*)p.q + b * p.qs[0] + hk * p.qs[1];
@@ -875,10 +878,10 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
   const int64_t at0 = (bh * a.nseg + seg) * K * V + nn;
   const float* from = seg == a.nseg - 1 ? (p.ds_in ? p.ds_in + sb : nullptr) : ACROSS ? nullptr : a.dstart + at0;
   load_state<KP>(S, from, live, K, V);
-  Rows<T, C, KP, kNT, WHOLE> rk, rq;
-  Square<NP, C, kNT> rt, rp;
+  Rows<T, C, KP, NW * 64, WHOLE> rk, rq;
+  Square<NP, C, NW * 64> rt, rp;
   Columns<T, C, WHOLE> cd;
-  Scales<C> vec;
+  Scales<C, NW * 64> vec;
   auto fetch = [&](int t0, int buf) {
     if (t0 < lo) return;
     const int cnt = min(C, len - t0);
@@ -886,10 +889,10 @@ __global__ __launch_bounds__(kNT, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_c
     const T *kt = k + (int64_t)t0 * p.ks[2], *qt = q + (int64_t)t0 * p.qs[2];
     const bf16 *tt = a.tb + ch * NP * C * C, *pt = a.pp + ch * NP * C * C;
     if constexpr (DIRECT) {
-      load_direct<C, KP>(kt, p.ks[2], cnt, lk[buf]);
-      load_direct<NP * C, C>(tt, C, NP * C, lt[buf]);
-      load_direct<C, KP>(qt, p.qs[2], cnt, lq[buf]);
-      load_direct<NP * C, C>(pt, C, NP * C, lp[buf]);
+      load_direct<C, KP, NW>(kt, p.ks[2], cnt, lk[buf]);
+      load_direct<NP * C, C, NW>(tt, C, NP * C, lt[buf]);
+      load_direct<C, KP, NW>(qt, p.qs[2], cnt, lq[buf]);
+      load_direct<NP * C, C, NW>(pt, C, NP * C, lp[buf]);
     } else {
       rk.load(kt, p.ks[2], K, cnt);
       rt.load(tt);
@@ -1396,17 +1399,19 @@ hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
     kernel<<<(unsigned)a.nblk, threads, lds, stream>>>(a);
     return hipGetLastError();
   };
-  auto chain = [&](auto kp, auto m) {
-    constexpr int KP = decltype(kp)::value, M = decltype(m)::value;
+  auto chain = [&](auto kp, auto m, auto w) {
+    constexpr int KP = decltype(kp)::value, M = decltype(m)::value, NW = decltype(w)::value;
     typedef ChainSize<T, NP, KP, M> Z;
     switch (st) {
-      case kAhead: return run(dr_chain<T, NP, KP, M, kAcross>, kNT, Z::bytes(false));
-      case kChain: return run(dr_chain<T, NP, KP, M, kOutputs>, kNT, Z::bytes(true));
-      case kKeepStates: return run(dr_chain<T, NP, KP, M, kKeep>, kNT, Z::bytes(false));
-      case kAheadBwd: return run(dr_chain_bwd<T, NP, KP, M, true>, kNT, Z::bytes(true));
-      default: return run(dr_chain_bwd<T, NP, KP, M, false>, kNT, Z::bytes(true));
+      case kAhead: return run(dr_chain<T, NP, KP, M, kAcross, NW>, NW * 64, Z::bytes(false));
+      case kChain: return run(dr_chain<T, NP, KP, M, kOutputs, NW>, NW * 64, Z::bytes(true));
+      case kKeepStates: return run(dr_chain<T, NP, KP, M, kKeep, NW>, NW * 64, Z::bytes(false));
+      case kAheadBwd: return run(dr_chain_bwd<T, NP, KP, M, true, NW>, NW * 64, Z::bytes(true));
+      default: return run(dr_chain_bwd<T, NP, KP, M, false, NW>, NW * 64, Z::bytes(true));
     }
   };
+  constexpr std::integral_constant<int, 2> two;
+  constexpr std::integral_constant<int, 4> four;
   auto pick = [&](auto kp, auto w) {
     constexpr int KP = decltype(kp)::value;
     constexpr bool W = decltype(w)::value;
@@ -1416,8 +1421,14 @@ hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
     if (st == kGrads)
       return a.p.H == a.p.Hk ? run(dr_grads<T, NP, KP, W, true>, 256, 0) : run(dr_grads<T, NP, KP, W, false>, 256, 0);
     if constexpr (W && kHasDirect<T, NP, KP>)
-      if (mode == kDirect && a.p.K == KP) return chain(kp, std::integral_constant<int, kDirect>());
-    return chain(kp, std::integral_constant<int, W ? kWhole : kGather>());
+      if (mode == kDirect && a.p.K == KP) {
+        if constexpr (kHasFour<T, NP, KP>)
+          if (a.nw == 4) return chain(kp, std::integral_constant<int, kDirect>(), four);
+        return chain(kp, std::integral_constant<int, kDirect>(), two);
+      }
+    if constexpr (kHasFour<T, NP, KP>)
+      if (a.nw == 4) return chain(kp, std::integral_constant<int, W ? kWhole : kGather>(), four);
+    return chain(kp, std::integral_constant<int, W ? kWhole : kGather>(), two);
   };
   auto size = [&](auto w) {
     switch (cover((int)a.p.K)) {

@@ -177,6 +177,14 @@ def test_many_heads_and_chunks(dtype):
     _check(1, 2, 2, 1537, 100, 100, dtype, "fp32", "token", state=True)
 
 
+@pytest.mark.parametrize("size", [(1, 2, 2, 700, 128, 128), (3, 30, 30, 70, 128, 128), (2, 1, 1, 1100, 128, 64), (1, 4, 8, 400, 128, 96),
+                                  (9, 16, 16, 20, 128, 128), (1, 1, 1, 3000, 64, 64), (2, 1, 2, 500, 256, 128)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_without_float32_results(size, dtype):
+    """Tokens in segments, and workgroups of two and of four wavefronts."""
+    _check(*size, dtype, state=False, lens=[size[3] - 7 * b for b in range(size[0])] if size[0] > 1 else None)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 def test_forward_alone(dtype):
     _check(2, 2, 4, 100, 128, 128, dtype, train=False, state=False)
