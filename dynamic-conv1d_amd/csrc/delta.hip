@@ -37,7 +37,11 @@ int chunk(const DrProblem& p) {
 // How the chains are cut: segments of the tokens, where heads and columns leave CUs idle (one launch finds what each makes of
 // the state before it, a second carries the states across, and the chains run side by side), and wavefronts of a workgroup
 // where its tiles leave room for one on a CU.  The least estimated time: per chunk of a chain `us`, 0.8 of that without
-// outputs (with the unit vectors' columns, twice as many where K is V), in rounds of the workgroups that fit, and the launches.
+// outputs (with the unit vectors' columns, twice as many where K is V), in rounds of the workgroups that fit (small tiles
+// let wavefronts share SIMDs, at 0.65 of a round for another), and the launches.  Measured, bf16, us (* is what it takes):
+// forward of B1 H16 T8192 hd128, 1 segment 379, 2 339, 4 214, 8 171 *, 16 203; B1 H2 T16384 hd128, 8 180, 16 137, 32 135 *;
+// B1 H16 T32768 hd128 with its state, 1 2845, 4 1530, 8 948 *, 16 976; B1 H4 T2048 hd256, 1 245, 4 143, 8 146 *.  Training
+// of B4 H32 T2048 hd128: workgroups of 2 wavefronts 825, of 4 677 *; of B4 H16 T4096: 2 820 *, 4 899.
 struct Cut {
   int nseg, nw;
 };
@@ -48,13 +52,16 @@ Cut cut_of(const DrProblem& p, int C, int np) {
   double best = -1;
   Cut cut{1, 2};
   for (int nw = 2; nw <= (one && vp % 64 == 0 ? 4 : 2); nw += 2) {
-    const double fit = one ? 256 : 512, us = (np == 1 ? 2.5 : 2.8) * (nw == 4 ? 1.25 : 1);
+    auto rounds = [&](double wgs, bool small) {
+      return small ? (wgs <= 512 ? 1 : 0.35 + 0.65 * wgs / 512) : __builtin_ceil(wgs / (one ? 256 : 512));
+    };
+    const double us = (np == 1 ? 2.5 : 2.8) * (nw == 4 ? 1.25 : 1);
     const int cols = nw * 16;
     for (int s = 1; s <= 64 && (s == 1 || s <= chunks); ++s) {
       const int64_t len = (chunks + s - 1) / s;
       if (s > 1 && (chunks + len - 1) / len != s) continue;  // the same segments as fewer
-      double t = us * len * __builtin_ceil(heads * s * (vp / cols) / fit);
-      if (s > 1) t += 0.8 * us * len * __builtin_ceil(heads * (s - 1) * ((vp + kp) / cols) / 512.) + 15 + 4 * s;
+      double t = us * len * rounds((double)heads * s * (vp / cols), np == 3 && kp == 64);
+      if (s > 1) t += 0.8 * us * len * rounds((double)heads * (s - 1) * ((vp + kp) / cols), true) + 15 + 2 * s;
       if (best < 0 || t < best) {
         best = t;
         cut = {s, nw};

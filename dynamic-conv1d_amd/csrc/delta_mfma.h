@@ -1042,57 +1042,77 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
   for (int64_t t = max(whole, lo) + g; t < min(p.T, (int64_t)lo + a.seg); t += 4) dv[t * p.dvs[2]] = (T)0.f;
 }
 
-// From segment to segment, a wavefront to 16 columns of a head: start[s + 1] += trans[s] start[s], or with gradients
-// dstart[s - 1] += trans[s]^T dstart[s], on float32 matrix instructions (16x16x4: a lane's result of a row block is its operand
-// of the next product's four steps).
+// From segment to segment, a workgroup to 16 columns of a head and a quarter of the rows to a wavefront:
+// start[s + 1] += trans[s] start[s], or with gradients dstart[s - 1] += trans[s]^T dstart[s], on float32 matrix instructions
+// (16x16x4).  A step waits for the one before, so what it reads of the transitions is on its way by then, up to 128 channels
+// (one wavefront to the columns, which read as it went, took 9 us a segment at 128 channels and 45 at 256).
 template <int KP, bool BWD>
-__global__ __launch_bounds__(64) void dr_across(Args a) {
+__global__ __launch_bounds__(256) void dr_across(Args a) {
+  constexpr int RB = KP / 64, KB = KP / 16;
+  __shared__ __align__(16) float lds[2][16][KP + 4];  // states, by column
   const DrProblem& p = a.p;
-  const int nvb = a.vp / 16, K = (int)p.K, V = (int)p.V, lane = threadIdx.x, g = lane / 16, col = lane % 16;
+  const int nvb = a.vp / 16, K = (int)p.K, V = (int)p.V, lane = threadIdx.x % 64, g = lane / 16, col = lane % 16, wv = wave_id();
   const int64_t blk = a.blk0 + blockIdx.x, bh = blk / nvb;
   const int nn = (int)(blk % nvb) * 16 + col;
   float* st = (BWD ? a.dstart : a.start) + bh * a.nseg * K * V + nn;
-  auto load = [&](f32x4 (&S)[KP / 16], const float* from) {
+  const int64_t kv = (int64_t)K * V;
+  auto load = [&](f32x4 (&S)[RB], const float* from) {
 #pragma unroll
-    for (int kb = 0; kb < KP / 16; ++kb)
+    for (int i = 0; i < RB; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int d = 16 * kb + 4 * g + r;
-        S[kb][r] = nn < V && d < K ? from[d * V] : 0.f;
+        const int d = 16 * (wv * RB + i) + 4 * g + r;
+        S[i][r] = nn < V && d < K ? from[d * V] : 0.f;
       }
   };
-  f32x4 S[KP / 16], N[KP / 16];
-  const int64_t kv = (int64_t)K * V;
-  load(S, st + (BWD ? a.nseg - 2 : 1) * kv);
-  for (int i = 1; i < a.nseg - 1; ++i) {
-    const int s = BWD ? a.nseg - 1 - i : i;
-    float* to = st + (BWD ? s - 1 : s + 1) * kv;
-    const float* M = a.trans + (bh * a.nseg + s) * KP * KP;
-    load(N, to);
+  auto share = [&](int buf, const f32x4 (&S)[RB]) {
 #pragma unroll
-    for (int rb = 0; rb < KP / 16; ++rb) {
+    for (int i = 0; i < RB; ++i) *reinterpret_cast<f32x4*>(&lds[buf][col][16 * (wv * RB + i) + 4 * g]) = S[i];
+  };
+  auto segment = [&](int i) { return BWD ? a.nseg - 1 - i : i; };
+  auto row = [&](f32x4 (&m)[KB], int i, int rb) {  // a block of rows of the transition of step i
+    const float* M = a.trans + (bh * a.nseg + segment(i)) * KP * KP;
 #pragma unroll
-      for (int kb = 0; kb < KP / 16; ++kb) {
-        f32x4 m;
-        if constexpr (BWD) {
+    for (int kb = 0; kb < KB; ++kb) {
+      if constexpr (BWD) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) m[r] = M[(16 * kb + 4 * g + r) * KP + 16 * rb + col];
-        } else {
-          m = *reinterpret_cast<const f32x4*>(M + (16 * rb + col) * KP + 16 * kb + 4 * g);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) N[rb] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[r], S[kb][r], N[rb], 0, 0, 0);
+        for (int r = 0; r < 4; ++r) m[kb][r] = M[(16 * kb + 4 * g + r) * KP + 16 * rb + col];
+      } else {
+        m[kb] = *reinterpret_cast<const f32x4*>(M + (16 * rb + col) * KP + 16 * kb + 4 * g);
       }
     }
+  };
+  constexpr bool AHEAD = KP <= 128;
+  f32x4 S[RB], N[RB], m[AHEAD ? RB : 1][KB];
+  load(S, st + segment(1) * kv);
+  share(1, S);
+  if (AHEAD)
 #pragma unroll
-    for (int kb = 0; kb < KP / 16; ++kb) {
-      S[kb] = N[kb];
+    for (int i = 0; i < RB; ++i) row(m[AHEAD ? i : 0], 1, wv * RB + i);
+  for (int i = 1; i < a.nseg - 1; ++i) {
+    float* to = st + (segment(i) + (BWD ? -1 : 1)) * kv;
+    load(N, to);
+    __syncthreads();
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      f32x4 (&mr)[KB] = m[AHEAD ? rb : 0];
+      if (!AHEAD) row(mr, i, wv * RB + rb);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(&lds[i % 2][col][16 * kb + 4 * g]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) N[rb] = __builtin_amdgcn_mfma_f32_16x16x4f32(mr[kb][r], s[r], N[rb], 0, 0, 0);
+      }
+      if (AHEAD && i + 1 < a.nseg - 1) row(mr, i + 1, wv * RB + rb);
+    }
+    share((i + 1) % 2, N);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int d = 16 * kb + 4 * g + r;
-        if (nn < V && d < K) to[d * V] = N[kb][r];
+        const int d = 16 * (wv * RB + rb) + 4 * g + r;
+        if (nn < V && d < K) to[d * V] = N[rb][r];
       }
-    }
   }
 }
 
@@ -1416,8 +1436,8 @@ hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
     constexpr int KP = decltype(kp)::value;
     constexpr bool W = decltype(w)::value;
     if (st == kPrep) return run(dr_prep<T, NP, KP, W>, 256, 0);
-    if (st == kCarry) return run(dr_across<KP, false>, 64, 0);
-    if (st == kCarryBwd) return run(dr_across<KP, true>, 64, 0);
+    if (st == kCarry) return run(dr_across<KP, false>, 256, 0);
+    if (st == kCarryBwd) return run(dr_across<KP, true>, 256, 0);
     if (st == kGrads)
       return a.p.H == a.p.Hk ? run(dr_grads<T, NP, KP, W, true>, 256, 0) : run(dr_grads<T, NP, KP, W, false>, 256, 0);
     if constexpr (W && kHasDirect<T, NP, KP>)
