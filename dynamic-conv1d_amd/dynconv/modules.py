@@ -12,6 +12,9 @@ proj_in GEMM for all groups, and one launch per direction that reads the fused
 DynamicLinearAttention is a layer around it: the q, k and v convolutions, linear
 attention with a decay for each head, the heads' gated group norm, and the
 projections, for training, for prompts in pieces and for single tokens.
+DynamicDeltaRule has the gated delta rule in linear attention's place, with a decay
+and a strength of each token's own; DynamicDeltaStack is layers of it with norms
+before and after each, a residual scale and the residual stream.
 
 The proj_in GEMM (README.md:67, 75) runs on libdynconv.so's own matrix-core
 kernels (dc_proj_in_fwd / dc_proj_in_bwd): skinny products bound by streaming
@@ -30,10 +33,11 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import _capi
+from .delta import gated_delta_rule, gated_delta_rule_step
 from .linattn import MAX_DIM, linear_attention, linear_attention_step
 from .lowrank import (lowrank_dynamic_convolution, lowrank_dynamic_convolution_grouped,
                       lowrank_dynamic_convolution_step_grouped)
-from .norm import group_norm
+from .norm import group_norm, residual_norm
 
 
 class _ProjInFn(torch.autograd.Function):
@@ -185,29 +189,26 @@ class GroupedLowRankDynamicShortConvolution(nn.Module):
 
 
 class LayerState(NamedTuple):
-    """What DynamicLinearAttention keeps of each sequence (a row each)."""
+    """What DynamicLinearAttention and DynamicDeltaRule keep of each sequence (a row each)."""
 
     conv: torch.Tensor  # [rows, W - 1, 3 * d_model]: the last projected rows, oldest first
     attn: torch.Tensor  # [rows, heads, head_dim, head_dim] float32: the heads' states
 
 
-class DynamicLinearAttention(nn.Module):
-    """A layer of linear attention over convolved q, k and v:
+class _RecurrentLayer(nn.Module):
+    """What the layers with a recurrent state share:
 
         q, k, v = GroupedLowRankDynamicShortConvolution(c_attn(x), x), in heads
-        o       = linear_attention(q, k, v) with a fixed decay for each head
+        o       = _sequences(x, q, k, v, ...) or _tokens(x, q, k, v, ...) of the subclass
         out     = c_proj(group_norm(o, heads, gate=c_gate(x)))
-
-    forward(x) takes whole sequences [B, T, d_model]; step(x, state) one token [N, d_model] of each sequence.
-    Decays run from 1 - 2^-5 to 1 - 2^-12 over the heads; they are not trained and stay float32.
     """
 
-    def __init__(self, d_model: int, heads: int, R: int, W: int, eps: float = 1e-5):
+    def __init__(self, d_model: int, heads: int, R: int, W: int, eps: float, what: str):
         super().__init__()
         if heads <= 0 or d_model % heads != 0:
             raise ValueError("heads must divide d_model")
         if d_model // heads > MAX_DIM:
-            raise ValueError(f"linear attention's heads have at most {MAX_DIM} channels")
+            raise ValueError(f"{what}'s heads have at most {MAX_DIM} channels")
         self.d_model, self.heads, self.head_dim, self.W, self.eps = d_model, heads, d_model // heads, W, eps
         self.c_attn = nn.Linear(d_model, 3 * d_model, bias=False)
         self.conv = GroupedLowRankDynamicShortConvolution(d_model, R, W, groups=3, head_dim=self.head_dim)
@@ -215,19 +216,6 @@ class DynamicLinearAttention(nn.Module):
         self.norm_bias = nn.Parameter(torch.zeros(d_model))
         self.c_gate = nn.Linear(d_model, d_model, bias=False)
         self.c_proj = nn.Linear(d_model, d_model, bias=False)
-        self.register_buffer("log_decay", self._log_decay(self.c_attn.weight.device), persistent=False)
-
-    def _log_decay(self, device):
-        u = 5 + 7 * torch.arange(self.heads, dtype=torch.float64, device="cpu") / max(self.heads - 1, 1)
-        return torch.log1p(-torch.exp2(-u)).to(device=device, dtype=torch.float32)
-
-    def _apply(self, fn, recurse=True):
-        old = self.log_decay
-        super()._apply(fn, recurse)
-        # .to(bfloat16) and its like leave the decays as they are, and so does to_empty, whose memory holds anything
-        device = self.log_decay.device
-        self.log_decay = self._log_decay(device) if old.is_meta else old.to(device)
-        return self
 
     def new_state(self, rows: int) -> LayerState:
         """States of sequences without a token yet."""
@@ -256,8 +244,7 @@ class DynamicLinearAttention(nn.Module):
             past = self.W - 1
             qkv = torch.cat([state.conv, qkv], 1)
             q, k, v = (t[:, :, past:] for t in self.conv(qkv, F.pad(x, (0, 0, past, 0))))
-        o = linear_attention(q, k, v, self.log_decay, initial_state=None if state is None else state.attn, lengths=lengths,
-                             return_state=return_state)
+        o = self._sequences(x, q, k, v, None if state is None else state.attn, lengths, return_state)
         o, attn = o if return_state else (o, None)
         out = self.c_proj(self._norm(o.transpose(1, 2).reshape(B, T, D), self.c_gate(x)))
         if not return_state:
@@ -281,5 +268,123 @@ class DynamicLinearAttention(nn.Module):
             self.c_attn(x), [t.view(N, -1) for t in z], list(U.unbind(0)), state.conv, static_w=list(sw.unbind(0)),
             residual=True, slots=slots)
         heads = (N, self.heads, self.head_dim)
-        o = linear_attention_step(q.view(heads), k.view(heads), v.view(heads), self.log_decay, state.attn, slots=slots)
+        o = self._tokens(x, q.view(heads), k.view(heads), v.view(heads), state.attn, slots)
         return self.c_proj(self._norm(o.view(N, D), self.c_gate(x)))
+
+
+class DynamicLinearAttention(_RecurrentLayer):
+    """A layer of linear attention over convolved q, k and v:
+
+        q, k, v = GroupedLowRankDynamicShortConvolution(c_attn(x), x), in heads
+        o       = linear_attention(q, k, v) with a fixed decay for each head
+        out     = c_proj(group_norm(o, heads, gate=c_gate(x)))
+
+    forward(x) takes whole sequences [B, T, d_model]; step(x, state) one token [N, d_model] of each sequence.
+    Decays run from 1 - 2^-5 to 1 - 2^-12 over the heads; they are not trained and stay float32.
+    """
+
+    def __init__(self, d_model: int, heads: int, R: int, W: int, eps: float = 1e-5):
+        super().__init__(d_model, heads, R, W, eps, "linear attention")
+        self.register_buffer("log_decay", self._log_decay(self.c_attn.weight.device), persistent=False)
+
+    def _log_decay(self, device):
+        u = 5 + 7 * torch.arange(self.heads, dtype=torch.float64, device="cpu") / max(self.heads - 1, 1)
+        return torch.log1p(-torch.exp2(-u)).to(device=device, dtype=torch.float32)
+
+    def _apply(self, fn, recurse=True):
+        old = self.log_decay
+        super()._apply(fn, recurse)
+        # .to(bfloat16) and its like leave the decays as they are, and so does to_empty, whose memory holds anything
+        device = self.log_decay.device
+        self.log_decay = self._log_decay(device) if old.is_meta else old.to(device)
+        return self
+
+    def _sequences(self, x, q, k, v, initial, lengths, return_state):
+        return linear_attention(q, k, v, self.log_decay, initial_state=initial, lengths=lengths, return_state=return_state)
+
+    def _tokens(self, x, q, k, v, state, slots):
+        return linear_attention_step(q, k, v, self.log_decay, state, slots=slots)
+
+
+class DynamicDeltaRule(_RecurrentLayer):
+    """A layer of the gated delta rule over convolved q, k and v, with a decay and a strength of each token's own:
+
+        q, k, v   = GroupedLowRankDynamicShortConvolution(c_attn(x), x), in heads
+        log_decay = -exp(log_rate) softplus(c_decay(x) + decay_bias),   beta = sigmoid(c_beta(x))     of each head
+        o         = gated_delta_rule(q, k, v, log_decay, beta, normalize=True)
+        out       = c_proj(group_norm(o, heads, gate=c_gate(x)))
+
+    forward(x) takes whole sequences [B, T, d_model]; step(x, state) one token [N, d_model] of each sequence.  The gates
+    are computed in float32 and passed on in x's type, so that in 16 bits no gradient is float32.
+    """
+
+    def __init__(self, d_model: int, heads: int, R: int, W: int, eps: float = 1e-5):
+        super().__init__(d_model, heads, R, W, eps, "the gated delta rule")
+        self.c_decay = nn.Linear(d_model, heads, bias=False)
+        self.c_beta = nn.Linear(d_model, heads, bias=False)
+        # rates from 1 to 2^-9 over the heads
+        self.log_rate = nn.Parameter(torch.arange(heads, dtype=torch.get_default_dtype()) * (-9 * math.log(2) / max(heads - 1, 1)))
+        self.decay_bias = nn.Parameter(torch.zeros(heads))
+
+    def _gates(self, x):
+        """log_decay, beta [..., heads] of the tokens x [..., d_model]."""
+        log_decay = -torch.exp(self.log_rate.float()) * F.softplus(self.c_decay(x).float() + self.decay_bias.float())
+        return log_decay.to(x.dtype), torch.sigmoid(self.c_beta(x).float()).to(x.dtype)
+
+    def _sequences(self, x, q, k, v, initial, lengths, return_state):
+        log_decay, beta = (t.transpose(1, 2) for t in self._gates(x))
+        return gated_delta_rule(q, k, v, log_decay.to(q.dtype), beta.to(q.dtype), initial_state=initial, lengths=lengths,
+                                return_state=return_state, normalize=True)
+
+    def _tokens(self, x, q, k, v, state, slots):
+        log_decay, beta = self._gates(x)
+        return gated_delta_rule_step(q, k, v, log_decay.to(q.dtype), beta.to(q.dtype), state, slots=slots, normalize=True)
+
+
+class DynamicDeltaStack(nn.Module):
+    """Layers of DynamicDeltaRule on a residual stream, with norms before and after each and a residual scale:
+
+        y = norm(x),  h = x;   for each layer   y, h = residual_norm(h, layer(y), ...)
+
+    forward(x) and step(x, states) return the last y, the stream normed; `stream` is the type that h is kept in
+    (None: x's), e.g. torch.float32 around layers in bfloat16.
+    """
+
+    def __init__(self, d_model: int, heads: int, layers: int, R: int, W: int, eps: float = 1e-6, stream: torch.dtype | None = None):
+        super().__init__()
+        self.d_model, self.eps, self.stream = d_model, eps, stream
+        self.layers = nn.ModuleList(DynamicDeltaRule(d_model, heads, R, W) for _ in range(layers))
+        self.weight = nn.Parameter(torch.ones(layers + 1, d_model))   # of the norms before the layers, and the last one
+        self.branch_weight = nn.Parameter(torch.ones(layers, d_model))
+        self.scale = nn.Parameter(torch.ones(layers, d_model))
+
+    def new_state(self, rows: int) -> list:
+        return [layer.new_state(rows) for layer in self.layers]
+
+    def _run(self, x, call):
+        h = x.contiguous() if self.stream is None else x.to(self.stream).contiguous()
+        y = F.rms_norm(x, (self.d_model,), self.weight[0], self.eps)
+        for i in range(len(self.layers)):
+            y, h = residual_norm(h, call(i, y), weight=self.weight[i + 1], branch_weight=self.branch_weight[i],
+                                 scale=self.scale[i], eps=self.eps)
+        return y
+
+    def forward(self, x: torch.Tensor, states: list | None = None, lengths: torch.Tensor | None = None,
+                return_state: bool = False):
+        """x [B, T, d_model] -> y like x, or (y, the layers' states after it); the others as in DynamicDeltaRule.forward."""
+        after = []
+
+        def call(i, y):
+            out = self.layers[i](y, None if states is None else states[i], lengths, return_state)
+            if return_state:
+                after.append(out[1])
+                return out[0]
+            return out
+
+        y = self._run(x, call)
+        return (y, after) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, states: list, slots: torch.Tensor | None = None) -> torch.Tensor:
+        """One token x [N, d_model] of each of N sequences -> y [N, d_model]; `states` are updated in place."""
+        return self._run(x, lambda i, y: self.layers[i].step(y, states[i], slots))

@@ -1,7 +1,7 @@
 """Import path of the operators behind the convolutions, beside headwise.py and lowrank.py.
 
     from linattn import linear_attention, linear_attention_step, group_norm, DynamicLinearAttention
-    from linattn import gated_delta_rule, gated_delta_rule_step, residual_norm
+    from linattn import gated_delta_rule, gated_delta_rule_step, residual_norm, DynamicDeltaRule, DynamicDeltaStack
 
 resolves to dynamic-conv1d_amd/dynconv/linattn.py, delta.py, norm.py and modules.py.
 """
@@ -16,4 +16,4 @@ if _PKG_DIR not in _sys.path:
 from dynconv.linattn import linear_attention, linear_attention_step  # noqa: E402,F401
 from dynconv.delta import gated_delta_rule, gated_delta_rule_step  # noqa: E402,F401
 from dynconv.norm import group_norm, residual_norm  # noqa: E402,F401
-from dynconv.modules import DynamicLinearAttention, LayerState  # noqa: E402,F401
+from dynconv.modules import DynamicDeltaRule, DynamicDeltaStack, DynamicLinearAttention, LayerState  # noqa: E402,F401
