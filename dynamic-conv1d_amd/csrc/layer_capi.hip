@@ -260,6 +260,7 @@ static int check_dr(int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int6
   if (s != DC_OK) return s;
   if (gdtype != dtype && gdtype != DC_DTYPE_FP32) return DC_ERR_DTYPE;
   if (Hk <= 0 || H % Hk != 0) return DC_ERR_SHAPE;
+  if (B * H * T > int64_t(1) << 40) return DC_ERR_SHAPE;  // workspaces past 64 bits, and past any memory
   return (flags & ~(DC_DELTA_NORMALIZE | DC_DELTA_PRECISE)) ? DC_ERR_UNSUPPORTED : DC_OK;
 }
 
@@ -296,6 +297,7 @@ int dc_delta_rule_fwd(const void* q, const int64_t* q_strides, const void* k, co
       !aligned_to(log_decay, gs) || !aligned_to(beta, gs) || !aligned_to(initial_state, 4) ||
       !aligned_to(final_state, 4) || !aligned_to(lengths, 4))
     return DC_ERR_ALIGN;
+  if (final_state && final_state == initial_state) return DC_ERR_UNSUPPORTED;
   dc::DrProblem p = dr_sizes(B, Hk, H, T, K, V, dtype, gate_dtype, flags);
   const int64_t need = dc::dr_ws_bytes(p, 0);
   if (need > 0 && (!workspace || ws_bytes < need || !aligned_to(workspace, 16))) return DC_ERR_WORKSPACE;
@@ -330,6 +332,7 @@ int dc_delta_rule_bwd(const void* q, const int64_t* q_strides, const void* k, co
   for (const void* t : {(const void*)initial_state, (const void*)d_final_state, (const void*)d_initial_state,
                         (const void*)lengths})
     if (!aligned_to(t, 4)) return DC_ERR_ALIGN;
+  if (d_initial_state && d_initial_state == d_final_state) return DC_ERR_UNSUPPORTED;
   dc::DrProblem p = dr_sizes(B, Hk, H, T, K, V, dtype, gate_dtype, flags);
   const int64_t need = dc::dr_ws_bytes(p, fwd_workspace ? 2 : 1);
   if (need > 0 && (!workspace || ws_bytes < need || !aligned_to(workspace, 16))) return DC_ERR_WORKSPACE;

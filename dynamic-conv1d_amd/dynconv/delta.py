@@ -126,6 +126,11 @@ def gated_delta_rule(
     Returns:
         o [B, H, T, V] in q's dtype, over token-major memory (o.transpose(1, 2).reshape(B, T, H * V) is a view), or
         (o, state [B, H, K, V] float32).  Every input but lengths has a gradient.
+
+    Values are finite: an infinity or NaN reaches its head's outputs from the start of its block of up to 64 tokens on.  In 16
+    bits products run on matrix cores with float32 sums; what they take of the states and corrections is rounded to the inputs'
+    type (fp16: to 16 bits), unless a result is float32: a returned state, or a gradient of float32 gates or of the initial
+    state.  Then everything is as good as float32, at about twice the time.
     """
     if _capi.binding is not None:
         out = _capi.binding.gated_delta_rule(q, k, v, log_decay, beta, scale, initial_state, lengths, return_state, normalize, eps)

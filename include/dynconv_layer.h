@@ -83,9 +83,12 @@ typedef enum dc_delta_flags {
  *   q, k [B, Hk, T, K], v, o [B, H, T, V], log_decay, beta [B, H, T], with strides (batch, head, row) each, those of
  *   log_decay and beta for the whole of their axes; Hk divides H, and head h reads q and k of head h / (H / Hk);
  *   log_decay <= 0 (-inf forgets at once), beta and log_decay in gate_dtype: dtype or float32;
- *   initial_state, final_state, lengths as in dc_linear_attention_fwd.
- * T may be 0.  Both calls need a workspace of dc_delta_rule_ws_bytes bytes (0: none), 16-byte aligned; bwd: 0 the
- * forward, 1 the backward, 2 the backward that is given the forward's workspace (of the same flags). */
+ *   initial_state, final_state, lengths as in dc_linear_attention_fwd, but the two states are not the same memory
+ *   (refused), which segments of a sequence read and write side by side.
+ * B * H * T is at most 2^40.  Values are finite: one that is not reaches its head's outputs from the start of its chunk of
+ * up to 64 tokens on (rows past the lengths may hold anything).  T may be 0.  Both calls need a workspace of
+ * dc_delta_rule_ws_bytes bytes (0: none), 16-byte aligned; bwd: 0 the forward, 1 the backward, 2 the backward that is given
+ * the forward's workspace (of the same flags). */
 int64_t dc_delta_rule_ws_bytes(int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int64_t V, int dtype, int flags,
                                int bwd);
 int dc_delta_rule_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
@@ -96,8 +99,8 @@ int dc_delta_rule_fwd(const void* q, const int64_t* q_strides, const void* k, co
                       int dtype, int gate_dtype, int flags, void* stream);
 
 /* Gradients of dc_delta_rule_fwd: dq, dk, dv, dlog_decay, dbeta from d_o and d_final_state (NULL: zero), and
- * d_initial_state (NULL: not wanted).  Rows past a sequence's length get zero.  fwd_workspace is NULL or the
- * workspace of the forward of the same inputs, as that call left it (trusted, not checked). */
+ * d_initial_state (NULL: not wanted; not d_final_state's memory).  Rows past a sequence's length get zero.  fwd_workspace
+ * is NULL or the workspace of the forward of the same inputs, as that call left it (trusted, not checked). */
 int dc_delta_rule_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                       const int64_t* v_strides, const void* log_decay, const int64_t* log_decay_strides,
                       const void* beta, const int64_t* beta_strides, const float* initial_state, const int32_t* lengths,

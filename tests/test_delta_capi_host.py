@@ -47,6 +47,28 @@ def test_delta_rule_refusals(lib, call):
         assert call(lib) == E_DEV and call(lib, nws=need) == E_DEV
 
 
+def test_delta_rule_sizes_past_any_memory(lib):
+    """Workspaces are counted in 64 bits: sizes that would pass them are refused, the largest others give a count."""
+    q = lambda B, H, T, dt, flags, which: lib.dc_delta_rule_ws_bytes(B, 1, H, T, 256, 256, dt, flags, which)  # noqa: E731
+    for dt in (0, 1, 2):
+        for which in (0, 1, 2):
+            assert q(1 << 20, 1, (1 << 20) + 1, dt, 3, which) == E_SHAPE
+            assert q(1 << 20, 1, 1 << 20, dt, 3, which) > 1 << 40
+            assert q(1 << 10, 1 << 10, 1 << 20, dt, 0, which) > 1 << 40
+
+
+def test_delta_rule_states_are_apart(lib):
+    s, gs = st(1, 1, 1), st(1, 1, 1)
+    call = lambda a, b: lib.dc_delta_rule_fwd(P, s, P, s, P, s, P, gs, P, gs, a, None, P, s, b, P, 1 << 40, 1, 1, 2, 8, 16, 16, 1.0,  # noqa: E731
+                                              1e-6, 0, 2, 1, None)
+    assert call(P, P) == E_UNSUP
+    back = lambda a, b: lib.dc_delta_rule_bwd(P, s, P, s, P, s, P, gs, P, gs, None, None, P, s, a, P, s, P, s, P, s, P, gs, P, gs, b,  # noqa: E731
+                                              None, P, 1 << 40, 1, 1, 2, 8, 16, 16, 1.0, 1e-6, 0, 2, 1, None)
+    assert back(P, P) == E_UNSUP
+    if NO_DEV:
+        assert call(P, P + 16) == E_DEV and call(None, P) == E_DEV and back(P, P + 16) == E_DEV
+
+
 def test_delta_rule_pointers(lib):
     assert fwd(lib, q=None) == E_NULL and fwd(lib, o=None) == E_NULL and fwd(lib, g=None) == E_NULL
     assert fwd(lib, q=P + 1) == E_ALIGN and fwd(lib, g=P + 2) == E_ALIGN and fwd(lib, g=P + 1, gdt=0) == E_ALIGN
