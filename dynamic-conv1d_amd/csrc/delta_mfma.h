@@ -47,6 +47,7 @@ struct Args {
   int vp;              // V in whole 32 columns
   int64_t blk0;
   int nblk;
+  bool kept;  // the forward keeps U and the states
 };
 
 // Where column c of a row lies: of each 32 the quads of both halves side by side.
@@ -612,20 +613,21 @@ constexpr bool kHasDirect = __is_same(T, bf16) && ChainSize<T, NP, KP, kDirect>:
 template <typename T, int NP, int KP>
 constexpr bool kHasFour = __is_same(T, bf16) && NP == 1 && KP == 128;
 
-// The states from chunk to chunk, and o (kOutputs); or U and the state before each chunk for the backward (kKeep); or what each
-// segment but the last makes of the state before it (kAcross): its end from zero, and behind those columns its end from each
-// unit vector without values.
-enum What { kOutputs, kKeep, kAcross };
+// The states from chunk to chunk, and o (kOutputs); or U and the state before each chunk for the backward (kKeep); or all of
+// these (kBoth); or what each segment but the last makes of the state before it (kAcross): its end from zero, and behind those
+// columns its end from each unit vector without values.
+enum What { kOutputs, kKeep, kBoth, kAcross };
 template <typename T, int NP, int KP, int MODE, int WHAT, int NW>
 __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
   constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
-  constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather, KEEP = WHAT != kOutputs;  // KEEP: no q and no o
+  constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
+  constexpr bool OUT = WHAT == kOutputs || WHAT == kBoth, KEEP = WHAT == kKeep || WHAT == kBoth;  // !OUT: no q and no o
   extern __shared__ __align__(16) unsigned char chain_lds[];
   float (*lv)[3][C] = reinterpret_cast<float (*)[3][C]>(chain_lds);
   bf16 (*lk)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lv + Z::BUF);
   bf16 (*lt)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lk + Z::BUF);
-  bf16 (*lq)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lt + Z::BUF);  // not there if KEEP
+  bf16 (*lq)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lt + Z::BUF);  // there if OUT
   bf16 (*lp)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lq + Z::BUF);
   const DrProblem& p = a.p;
   // columns: V's, and behind them those of the unit vectors
@@ -669,14 +671,14 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
     if constexpr (DIRECT) {
       load_direct<C, KP, NW>(kt, p.ks[2], cnt, lk[buf]);
       load_direct<NP * C, C, NW>(tt, C, NP * C, lt[buf]);
-      if (!KEEP) {
+      if (OUT) {
         load_direct<C, KP, NW>(qt, p.qs[2], cnt, lq[buf]);
         load_direct<NP * C, C, NW>(pt, C, NP * C, lp[buf]);
       }
     } else {
       rk.load(kt, p.ks[2], K, cnt);
       rt.load(tt);
-      if (!KEEP) {
+      if (OUT) {
         rq.load(qt, p.qs[2], K, cnt);
         rp.load(pt);
       }
@@ -688,7 +690,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
     if constexpr (!DIRECT) {
       rk.template store<R, PL, false>(lk[buf]);
       rt.store(lt[buf]);
-      if (!KEEP) {
+      if (OUT) {
         rq.template store<R, PL, false>(lq[buf]);
         rp.store(lp[buf]);
       }
@@ -728,7 +730,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
 #pragma unroll
     for (int s = 0; s < KP / 32; ++s) {
       sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
-      if (WHAT == kKeep) keep<NP, true>(a.s + (ch * NP * KP + 32 * s) * a.vp + n0, a.vp, (int64_t)KP * a.vp, sf[s]);
+      if (KEEP) keep<NP, true>(a.s + (ch * NP * KP + 32 * s) * a.vp + n0, a.vp, (int64_t)KP * a.vp, sf[s]);
     }
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) y[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -777,7 +779,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) {
       f[s] = pack<NR>(x[2 * s], x[2 * s + 1]);
-      if (WHAT == kKeep) keep<NP, false>(a.u + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, first<NP>(f[s]));
+      if (KEEP) keep<NP, false>(a.u + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, first<NP>(f[s]));
       d[s] = pack<NR>(x[2 * s] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 4 * g]),
                       x[2 * s + 1] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 16 + 4 * g]));
     }
@@ -786,7 +788,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
 #pragma unroll
     for (int e0 = 0; e0 < NK; e0 += 8) {
       if (e0 + 8 < NK) keys(e0 + 8);
-      else if (!KEEP) rows(tq, even, 0);
+      else if (OUT) rows(tq, even, 0);
 #pragma unroll
       for (int e = 0; e < 8 && e < NK; ++e) {
         const int kb = (e0 + e) % KN, s = (e0 + e) / KN;
@@ -795,7 +797,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
       phase();
     }
     // O^T = G S^T q^T + U^T P^T: four neighbouring channels of a token in a lane
-    if constexpr (!KEEP) {
+    if constexpr (OUT) {
 #pragma unroll
       for (int rb = 0; rb < NB; ++rb) y[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -840,7 +842,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
   if (unit) store_state<KP>(S, a.trans + (bh * a.nseg + seg) * KP * KP + nn - a.vp, KP, KP);
   if (!live) return;
   if (WHAT == kAcross) store_state<KP>(S, a.start + at0 + K * V, K, V);
-  if (WHAT != kOutputs) return;
+  if (!OUT) return;
   if (p.s_out && (lo < whole ? whole <= lo + a.seg : seg == 0 && whole == 0)) store_state<KP>(S, p.s_out + sb, K, V);
   for (int64_t t = max(whole, lo) + g; t < min(p.T, (int64_t)lo + a.seg); t += 4) o[t * p.os[2] + col] = (T)0.f;
 }
@@ -1412,7 +1414,7 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
 }
 
 // The launches of a type and a number of parts (instantiated in delta_<type>.hip).
-enum Stage { kPrep, kAhead, kCarry, kChain, kKeepStates, kAheadBwd, kCarryBwd, kChainBwd, kGrads };
+enum Stage { kPrep, kAhead, kCarry, kChain, kChainKeep, kKeepStates, kAheadBwd, kCarryBwd, kChainBwd, kGrads };
 template <typename T, int NP>
 hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
   auto run = [&](auto kernel, int threads, int lds) {
@@ -1425,6 +1427,7 @@ hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
     switch (st) {
       case kAhead: return run(dr_chain<T, NP, KP, M, kAcross, NW>, NW * 64, Z::bytes(false));
       case kChain: return run(dr_chain<T, NP, KP, M, kOutputs, NW>, NW * 64, Z::bytes(true));
+      case kChainKeep: return run(dr_chain<T, NP, KP, M, kBoth, NW>, NW * 64, Z::bytes(true));
       case kKeepStates: return run(dr_chain<T, NP, KP, M, kKeep, NW>, NW * 64, Z::bytes(false));
       case kAheadBwd: return run(dr_chain_bwd<T, NP, KP, M, true, NW>, NW * 64, Z::bytes(true));
       default: return run(dr_chain_bwd<T, NP, KP, M, false, NW>, NW * 64, Z::bytes(true));

@@ -261,7 +261,7 @@ static int check_dr(int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int6
   if (gdtype != dtype && gdtype != DC_DTYPE_FP32) return DC_ERR_DTYPE;
   if (Hk <= 0 || H % Hk != 0) return DC_ERR_SHAPE;
   if (B * H * T > int64_t(1) << 40) return DC_ERR_SHAPE;  // workspaces past 64 bits, and past any memory
-  return (flags & ~(DC_DELTA_NORMALIZE | DC_DELTA_PRECISE)) ? DC_ERR_UNSUPPORTED : DC_OK;
+  return (flags & ~(DC_DELTA_NORMALIZE | DC_DELTA_PRECISE | DC_DELTA_KEEP)) ? DC_ERR_UNSUPPORTED : DC_OK;
 }
 
 static dc::DrProblem dr_sizes(int64_t B, int64_t Hk, int64_t H, int64_t T, int64_t K, int64_t V, int dtype, int gdtype,
@@ -271,6 +271,7 @@ static dc::DrProblem dr_sizes(int64_t B, int64_t Hk, int64_t H, int64_t T, int64
   p.dtype = dtype; p.gdtype = gdtype;
   p.normalize = (flags & DC_DELTA_NORMALIZE) != 0;
   p.precise = (flags & DC_DELTA_PRECISE) != 0;
+  p.keep = (flags & DC_DELTA_KEEP) != 0;
   return p;
 }
 

@@ -80,7 +80,7 @@ struct DrProblem {
   void* ws;
   int64_t B, Hk, H, T, K, V;
   float scale, eps;
-  int dtype, gdtype, normalize, precise;
+  int dtype, gdtype, normalize, precise, keep;
   hipStream_t stream;
 };
 int64_t dr_ws_bytes(const DrProblem& p, int bwd);

@@ -814,12 +814,13 @@ PyObject* py_gated_delta_rule(PyObject*, PyObject* const* args, Py_ssize_t nargs
   // delta._wide_results: whether a result of a call in 16 bits is float32
   const bool gates = g.scalar_type() == at::kFloat && any_requires_grad({&g, &b});
   const bool wide = q.scalar_type() != at::kFloat && (want || gates || any_requires_grad({&s0}));
-  const int64_t flags = (unit ? DC_DELTA_NORMALIZE : 0) | (wide ? DC_DELTA_PRECISE : 0);
+  const bool grads = any_requires_grad({&q, &k, &v, &g, &b, &s0});
+  const int64_t flags = (unit ? DC_DELTA_NORMALIZE : 0) | (wide ? DC_DELTA_PRECISE : 0) | (grads ? DC_DELTA_KEEP : 0);
   variable_list out;
   {
     pybind11::gil_scoped_release no_gil;
     const c10::DeviceGuard guard(q.device());
-    out = any_requires_grad({&q, &k, &v, &g, &b, &s0})
+    out = grads
               ? GatedDeltaRuleFn::apply(q, k, v, g, b, opt(s0), opt(lengths), scale, eps, flags, want != 0)
               : GatedDeltaRuleFn::run(q, k, v, g, b, s0, lengths, scale, eps, flags, want != 0);
   }

@@ -16,7 +16,7 @@ import torch
 from . import _capi
 from .linattn import MAX_DIM, _index, _like, _rows, _strides
 
-_NORMALIZE, _PRECISE = 1, 2  # dc_delta_flags
+_NORMALIZE, _PRECISE, _KEEP = 1, 2, 4  # dc_delta_flags
 
 
 class _GatedDeltaRuleFn(torch.autograd.Function):
@@ -41,7 +41,7 @@ class _GatedDeltaRuleFn(torch.autograd.Function):
             _capi.ptr(lengths), _capi.ptr(o), _strides(o, 3), _capi.ptr(state), _capi.ptr(ws), nws, B, Hk, H, T, K, V,
             scale, eps, dtype, gdtype, flags, _capi.stream_of(q))
         _capi.check(status, "gated delta rule forward")
-        # ws: each chunk's triangular systems, a function of the inputs, which the backward takes up again
+        # ws: each chunk's triangular systems and states, a function of the inputs, which the backward takes up again
         ctx.save_for_backward(q, k, v, log_decay, beta, initial, lengths, ws)
         ctx.args = scale, eps, flags
         ctx.set_materialize_grads(False)
@@ -148,6 +148,8 @@ def gated_delta_rule(
     lengths = _index(lengths, B, q.device, "lengths")
     scale = K ** -0.5 if scale is None else float(scale)
     flags = (_NORMALIZE if normalize else 0) | (_PRECISE if _wide_results(q, log_decay, beta, initial_state, return_state) else 0)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, beta, initial_state)):
+        flags |= _KEEP
     return _GatedDeltaRuleFn.apply(_rows(q), _rows(k), _rows(v), log_decay, beta, initial_state, lengths, scale, float(eps),
                                    flags, bool(return_state))
 

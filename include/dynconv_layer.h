@@ -74,7 +74,9 @@ int dc_linear_attention_step(const void* q, const int64_t* q_strides, const void
 /* Flags of the gated delta rule. */
 typedef enum dc_delta_flags {
   DC_DELTA_NORMALIZE = 1, /* the rows of q and k are divided by sqrt(|row|^2 + eps) */
-  DC_DELTA_PRECISE = 2    /* bf16, fp16: products as good as float32's, for the results that are float32 */
+  DC_DELTA_PRECISE = 2,   /* bf16, fp16: products as good as float32's, for the results that are float32 */
+  DC_DELTA_KEEP = 4       /* a backward follows, with the forward's workspace: the forward keeps its states for it there where
+                             they take no more than twice the memory of q, k, v and o */
 } dc_delta_flags;
 
 /* The gated delta rule: with a = exp(log_decay_t), b = beta_t, for each sequence and head,

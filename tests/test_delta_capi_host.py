@@ -37,7 +37,7 @@ def test_delta_rule_refusals(lib, call):
     for bad in (dict(B=0), dict(H=0), dict(Hk=0), dict(Hk=3), dict(T=-1), dict(K=0), dict(V=-5), dict(B=1 << 31),
                 dict(B=1 << 20, H=1 << 20), dict(Hk=4, H=2)):
         assert call(lib, **bad) == E_SHAPE, bad
-    assert call(lib, K=257) == E_UNSUP and call(lib, V=257) == E_UNSUP and call(lib, flags=4) == E_UNSUP
+    assert call(lib, K=257) == E_UNSUP and call(lib, V=257) == E_UNSUP and call(lib, flags=8) == E_UNSUP
     assert call(lib, s=None) == E_NULL and call(lib, gs=None) == E_NULL
     which = 1 if call is bwd else 0
     need = lib.dc_delta_rule_ws_bytes(1, 1, 2, 8, 16, 16, 0, 1, which)
@@ -55,6 +55,19 @@ def test_delta_rule_sizes_past_any_memory(lib):
             assert q(1 << 20, 1, (1 << 20) + 1, dt, 3, which) == E_SHAPE
             assert q(1 << 20, 1, 1 << 20, dt, 3, which) > 1 << 40
             assert q(1 << 10, 1 << 10, 1 << 20, dt, 0, which) > 1 << 40
+
+
+def test_delta_rule_states_kept_for_a_backward(lib):
+    """What the forward keeps the backward need not hold; it is kept where it is at most twice q, k, v and o."""
+    q = lambda flags, which, T=640, H=4, K=128, V=128, dt=0: lib.dc_delta_rule_ws_bytes(2, 2, H, T, K, V, dt, flags, which)  # noqa: E731
+    n = 10 * 8  # chunks of 64 tokens, of all heads
+    kept = n * (64 * 128 + 128 * 128) * 2
+    assert q(5, 0) == q(1, 0) + kept and q(5, 2) == q(1, 2) - kept and q(5, 1) == q(1, 1)
+    for flags, sizes in ((3, {}), (1, dict(K=256, V=64, H=2)), (1, dict(K=256, V=256, dt=1)), (1, dict(K=256, V=256, dt=2))):
+        if sizes.get("dt", 0) or flags == 3:  # 32 tokens to a chunk and two or three parts of everything
+            assert q(flags | 4, 0, **sizes) == q(flags, 0, **sizes) and q(flags | 4, 2, **sizes) == q(flags, 2, **sizes)
+        else:
+            assert q(flags | 4, 0, **sizes) > q(flags, 0, **sizes)
 
 
 def test_delta_rule_states_are_apart(lib):
