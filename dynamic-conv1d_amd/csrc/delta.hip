@@ -41,7 +41,8 @@ int chunk(const DrProblem& p) {
 // let wavefronts share SIMDs, at 0.65 of a round for another), and the launches.  Measured, bf16, us (* is what it takes):
 // forward of B1 H16 T8192 hd128, 1 segment 379, 2 339, 4 214, 8 171 *, 16 203; B1 H2 T16384 hd128, 8 180, 16 137, 32 135 *;
 // B1 H16 T32768 hd128 with its state, 1 2845, 4 1530, 8 948 *, 16 976; B1 H4 T2048 hd256, 1 245, 4 143, 8 146 *.  Training
-// of B4 H32 T2048 hd128: workgroups of 2 wavefronts 825, of 4 677 *; of B4 H16 T4096: 2 820 *, 4 899.
+// of B4 H32 T2048 hd128: workgroups of 2 wavefronts 717, of 4 558 *; of B4 H16 T4096, before the forward kept its states, 2
+// 820 *, 4 899.
 struct Cut {
   int nseg, nw;
 };
@@ -93,7 +94,7 @@ struct Plan {
     seg = (int)((n + nseg - 1) / nseg) * C;
     cut = nseg > 1 ? (p.B * p.H * nseg * p.K * p.V * 4 + 15) / 16 * 16 : 0;
     trans = nseg > 1 ? p.B * p.H * nseg * kp * kp * 4 : 0;
-    // saves the backward a launch: training of B4 H16 T4096 hd128 in bf16 824 -> 730 us for 168 MB, 0.6 of q, k, v and o;
+    // saves the backward a launch: training of B4 H16 T4096 hd128 in bf16 824 -> 730 us for 201 MB, 0.75 of q, k, v and o;
     // of B2 T2048 with 8 | 16 heads of 64 x 128 and float32 gates 47 of 390 us would take 3.6 times their memory
     kept = p.keep && rows + st <= 2 * p.B * p.T * (p.Hk * 2 * p.K + p.H * 2 * p.V) * dtype_size(p.dtype);
   }

@@ -628,6 +628,13 @@ constexpr bool kHasFour = __is_same(T, bf16) && NP == 1 && KP == 128;
 // The states from chunk to chunk, and o (kOutputs); or U and the state before each chunk for the backward (kKeep); or all of
 // these (kBoth); or what each segment but the last makes of the state before it (kAcross): its end from zero, and behind those
 // columns its end from each unit vector without values.
+//
+// A chunk waits for the one before it, so a chain's time is its chunks': 2.8 us each at 128 x 128 in bf16, 3.5 with the
+// states' stores (B4 T4096 H16: 64 chunks, 180 and 225 us, 2.4 TB/s of what the latter moves).  Of that 0.6 us are matrix
+// instructions and 1.7 all instructions of a wavefront that has its SIMD to itself; the rest are latencies, of operands
+// from LDS within a chunk, and of the next chunk's loads, for which a second buffer leaves the time of one chunk and LDS has
+// no third.  Beside each wavefront another for the outputs and one for the loads took 146 us without the stores, but the
+// same 222 with them, and lost to four wavefronts where heads abound (B4 T2048 H32 forward 219 us for 175): not here.
 enum What { kOutputs, kKeep, kBoth, kAcross };
 template <typename T, int NP, int KP, int MODE, int WHAT, int NW>
 __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain(Args a) {
@@ -860,7 +867,8 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
 }
 
 // The states' gradients from the last chunk on, and dv; ACROSS: only what each segment but the first makes of them from zero
-// (from the state after it they come by the transpose of what the forward found).
+// (from the state after it they come by the transpose of what the forward found).  As the forward's, with twice its products
+// that the state waits for: 3.7 us a chunk at 128 x 128 in bf16, 238 us at B4 T4096 H16.
 template <typename T, int NP, int KP, int MODE, bool ACROSS, int NW>
 __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain_bwd(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
@@ -1134,7 +1142,9 @@ __global__ __launch_bounds__(256) void dr_across(Args a) {
 // channels to a wavefront.  With the rows' norms in E's place (rq_i rk_j for P, rk_i rk_j for N) the sums are those of q and
 // k themselves, before their part along the row is taken out.  Results lie turned over, four neighbouring channels of a
 // token in a lane: sums over a row are of a lane's own and three others', and a store has 8 bytes.  ONE: one value head to a
-// key head, whose sums need no registers of their own.
+// key head, whose sums need no registers of their own.  The memory path bounds it: B4 T4096 H16 hd128 bf16 170 us for 0.74 GB,
+// of which the states and their gradients are 0.27 (4.3 TB/s); with two value heads to a key head, whose sums leave one
+// workgroup to a CU for two, 455 us for B2 T8192 H32 (1.3 GB, 2.9 TB/s).
 template <typename T, int NP, int KP, bool WHOLE, bool ONE>
 __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && parts_of<T>() == 1) ? 2 : 1) void dr_grads(Args a) {
   constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;

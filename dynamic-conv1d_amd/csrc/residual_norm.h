@@ -9,6 +9,8 @@
 // dgate out, each once.  A row's channels stay in the registers of a wavefront (up to 16 to a lane) or of a workgroup's 256
 // lanes, which walk rows with the parameters, and backward the sums of their gradients, in registers; each workgroup writes
 // those sums once, and reduce_partials adds them in a fixed order.  The backward forms the norms' factors again.
+// 16384 x 4096, gate, scale, bf16: forward 124 us (0.67 GB, 5.4 TB/s), backward 193 (1.07 GB, 5.6 TB/s) and 7 of sums;
+// 8 x 2048 forward 4.2 us, the launch.
 #pragma once
 
 #include "group_norm.h"
