@@ -72,12 +72,12 @@ Cut cut_of(const DrProblem& p, int C, int np) {
   return cut;
 }
 
-// The workspace: of the forward vec, Tb, P and the segments' states, of the backward dX and the states' gradients; U and the
-// states, of the forward where it keeps them, else of the backward.
+// The workspace: of the forward vec, Tb, P and the segments' states, of the backward dX, where it is not dv, and the states'
+// gradients; U and the states, of the forward where it keeps them, else of the backward.
 struct Plan {
   int64_t n, vec, sq, rows, st, cut, trans;  // chunks of a head; bytes of each array
   int vp, seg, nseg, nw;
-  bool kept;
+  bool kept, from_dv;
   explicit Plan(const DrProblem& p) {
     const int C = chunk(p), np = np_of(p);
     n = (p.T + C - 1) / C;
@@ -96,10 +96,11 @@ struct Plan {
     trans = nseg > 1 ? p.B * p.H * nseg * kp * kp * 4 : 0;
     // saves the backward a launch: training of B4 H16 T4096 hd128 in bf16 824 -> 730 us for 201 MB, 0.75 of q, k, v and o;
     // of B2 T2048 with 8 | 16 heads of 64 x 128 and float32 gates 47 of 390 us would take 3.6 times their memory
+    from_dv = p.dtype == kBF16 && np == 1;
     kept = p.keep && rows + st <= 2 * p.B * p.T * (p.Hk * 2 * p.K + p.H * 2 * p.V) * dtype_size(p.dtype);
   }
   int64_t fwd() const { return vec + 2 * sq + trans + cut + (kept ? rows + st : 0); }
-  int64_t bwd() const { return (kept ? 1 : 2) * (rows + st) + cut; }
+  int64_t bwd() const { return (kept ? 0 : rows + st) + (from_dv ? 0 : rows) + st + cut; }
 };
 
 Args args_of(const DrProblem& p, bool bwd) {
@@ -126,8 +127,9 @@ Args args_of(const DrProblem& p, bool bwd) {
   if (bwd) {
     if (!pl.kept) w += pl.rows + pl.st;
     a.x = reinterpret_cast<bf16*>(w);
-    a.ds = reinterpret_cast<bf16*>(w + pl.rows);
-    a.dstart = reinterpret_cast<float*>(w + pl.rows + pl.st);
+    if (!pl.from_dv) w += pl.rows;
+    a.ds = reinterpret_cast<bf16*>(w);
+    a.dstart = reinterpret_cast<float*>(w + pl.st);
   }
   return a;
 }
@@ -195,8 +197,9 @@ hipError_t dr_bwd(const DrProblem& p) {
   if (e == hipSuccess && a.nseg > 1) e = run(dr::kAheadBwd, a, d, columns(a, a.nseg - 1));
   if (e == hipSuccess && a.nseg > 2) e = run(dr::kCarryBwd, a, true, p.B * p.H * (a.vp / 16));
   if (e == hipSuccess) e = run(dr::kChainBwd, a, d, columns(a, a.nseg));
-  return e != hipSuccess ? e : run(dr::kGrads, a, w && whole16(p.d_o, p.dos, p.V, es) && whole16(p.dq, p.dqs, p.K, es) &&
-                                                      whole16(p.dk, p.dks, p.K, es), p.B * p.Hk * a.n);
+  const bool g = w && whole16(p.d_o, p.dos, p.V, es) && whole16(p.dv, p.dvs, p.V, es) && whole16(p.dq, p.dqs, p.K, es) &&
+                 whole16(p.dk, p.dks, p.K, es);
+  return e != hipSuccess ? e : run(dr::kGrads, a, g, p.B * p.Hk * a.n);
 }
 
 }  // namespace dc

@@ -30,6 +30,8 @@ constexpr int kPiece = 128;  // columns of v that the gradients' launch holds at
 
 template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __is_same(T, fp16) ? 2 : 1; }
 constexpr int held(int np) { return np == 1 ? 2 : np; }  // parts of operands that stay in registers
+// dX for the gradients' launch is dv itself, where both are one bf16 (B4 T4096 H16 hd128: 67 MB less to write).
+template <typename T, int NP> constexpr bool kFromDv = __is_same(T, bf16) && NP == 1;
 // Tokens of a chunk: 64, or 32 where tiles of 64 would pass the LDS (np: parts of what is computed, ni: of q and k).
 __host__ __device__ constexpr int chunk_of(int ni, int np, int kp) { return np == 3 || ni * kp > 256 ? 32 : 64; }
 __host__ __device__ constexpr int cover(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : 256; }
@@ -38,7 +40,7 @@ struct Args {
   DrProblem p;
   float* vec;          // [chunks][kVecs][C]
   bf16 *tb, *pp;       // [chunks][NP][C][C], spot() order
-  bf16 *u, *x, *s, *ds;  // [chunks][NP][C][VP] U and dX, [chunks][NP][KP][VP] states before and their gradients after
+  bf16 *u, *x, *s, *ds;  // [chunks][NP][C][VP] U and dX (not if kFromDv), [chunks][NP][KP][VP] states before and their gradients after
   // tokens cut into nseg segments of seg (whole chunks): the states before each but the first [heads][nseg][K][V], the
   // gradients after each but the last, and what a segment makes of the state before it, [heads][nseg][KP][KP]
   float *start, *dstart, *trans;
@@ -1047,7 +1049,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
           if (!ACROSS) put_columns<T, WHOLE>(dv + (int64_t)t0 * p.dvs[2], p.dvs[2], V - n0, cnt, 16 * rb, x[rb]);
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
-          if (!ACROSS) keep<NP, false>(a.x + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, pack<NP>(x[2 * s], x[2 * s + 1]));
+          if (!ACROSS && !kFromDv<T, NP>) keep<NP, false>(a.x + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, pack<NP>(x[2 * s], x[2 * s + 1]));
           f[s] = pack<NR>(-x[2 * s] * at(0, 32 * s), -x[2 * s + 1] * at(0, 32 * s + 16));
         }
       }
@@ -1186,6 +1188,7 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
   for (int hd = 0; hd < group; ++hd) {
     const int64_t h = hk * group + hd, bh = b * p.H + h, ch = bh * a.n + n;
     const T* d_o = (const T*)p.d_o + b * p.dos[0] + h * p.dos[1] + (int64_t)t0 * p.dos[2];
+    const T* dv = (const T*)p.dv + b * p.dvs[0] + h * p.dvs[1] + (int64_t)t0 * p.dvs[2];
     if (hd > 0) __syncthreads();  // the head before has been read
     f32x4 dq[NB][NCB], dr[NB][NCB], dw[NB][NCB];
 #pragma unroll
@@ -1215,13 +1218,15 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
         }
       };
       {
-        Rows<T, C, kPiece, 256, WHOLE> ro;
-        Rows<bf16, C, kPiece, 256, true> ru[2 * NP];
+        constexpr bool DV = kFromDv<T, NP>;
+        Rows<T, C, kPiece, 256, WHOLE> ro, rv;
+        Rows<bf16, C, kPiece, 256, true> ru[DV ? 1 : 2 * NP];
         ro.load(d_o + v0, p.dos[2], V - v0, cnt);
+        if constexpr (DV) rv.load(dv + v0, p.dvs[2], V - v0, cnt);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           ru[i].load(a.u + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
-          ru[NP + i].load(a.x + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
+          if constexpr (!DV) ru[NP + i].load(a.x + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
         }
         float vec[(kVecs * C + 255) / 256];
         if (v0 == 0)
@@ -1229,8 +1234,9 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
           for (int i = 0; i * 256 < kVecs * C; ++i) vec[i] = a.vec[ch * kVecs * C + i * 256 + t];
         states(0);
         ro.template store<RV, PV, false>(mem);
+        if constexpr (DV) rv.template store<RV, PV, false>(mem + 2 * PV);
 #pragma unroll
-        for (int i = 0; i < 2 * NP; ++i) ru[i].template store<RV, PV, false>(mem + (NI + i) * PV);
+        for (int i = 0; i < (DV ? 1 : 2 * NP); ++i) ru[i].template store<RV, PV, false>(mem + (NI + i) * PV);
         if (v0 == 0)
 #pragma unroll
           for (int i = 0; i * 256 < kVecs * C; ++i) lv[0][i * 256 + t] = vec[i];
