@@ -40,7 +40,7 @@ int chunk(const DrProblem& p) {
 // outputs (with the unit vectors' columns, twice as many where K is V), in rounds of the workgroups that fit (small tiles
 // let wavefronts share SIMDs, at 0.65 of a round for another), and the launches.  Measured, bf16, us (* is what it takes):
 // forward of B1 H16 T8192 hd128, 1 segment 379, 2 339, 4 214, 8 171 *, 16 203; B1 H2 T16384 hd128, 8 180, 16 137, 32 135 *;
-// B1 H16 T32768 hd128 with its state, 1 2845, 4 1530, 8 948 *, 16 976; B1 H4 T2048 hd256, 1 245, 4 143, 8 146 *.  Training
+// B1 H16 T32768 hd128 with its state, 1 2845, 4 1530, 8 950, 16 835 *; B1 H4 T2048 hd256, 1 245, 4 143, 8 146 *.  Training
 // of B4 H32 T2048 hd128: workgroups of 2 wavefronts 717, of 4 558 *; of B4 H16 T4096, before the forward kept its states, 2
 // 820 *, 4 899.
 struct Cut {
@@ -50,19 +50,23 @@ Cut cut_of(const DrProblem& p, int C, int np) {
   const int kp = dr::cover((int)p.K), vp = ((int)p.V + 31) / 32 * 32;
   const int64_t chunks = (p.T + C - 1) / C, heads = p.B * p.H;
   const bool one = np == 1 && kp == 128 && p.dtype == kBF16;  // workgroup on a CU; elsewhere two
+  const bool shares = np == 3 && kp == 128 && p.dtype == kBF16;  // two or, of more than 512, four (delta_mfma.h)
   double best = -1;
   Cut cut{1, 2};
   for (int nw = 2; nw <= (one && vp % 64 == 0 ? 4 : 2); nw += 2) {
     auto rounds = [&](double wgs, bool small) {
+      if (shares && !small) return wgs <= 512 ? 1 : 1.6 * wgs / 1024 > 0.6 + wgs / 1024 ? 1.6 * wgs / 1024 : 0.6 + wgs / 1024;
       return small ? (wgs <= 512 ? 1 : 0.35 + 0.65 * wgs / 512) : __builtin_ceil(wgs / (one ? 256 : 512));
     };
-    const double us = (np == 1 ? 2.5 : 2.8) * (nw == 4 ? 1.25 : 1);
+    const double us = (np == 1 ? 2.5 : shares ? 3.2 : 2.8) * (nw == 4 ? 1.25 : 1);
     const int cols = nw * 16;
     for (int s = 1; s <= 64 && (s == 1 || s <= chunks); ++s) {
       const int64_t len = (chunks + s - 1) / s;
       if (s > 1 && (chunks + len - 1) / len != s) continue;  // the same segments as fewer
       double t = us * len * rounds((double)heads * s * (vp / cols), np == 3 && kp == 64);
-      if (s > 1) t += 0.8 * us * len * rounds((double)heads * (s - 1) * ((vp + kp) / cols), true) + 15 + 2 * s;
+      if (s > 1)
+        t += (shares ? 0.65 : 0.8) * us * len * rounds((double)heads * (s - 1) * ((vp + kp) / cols), true) +
+             (shares ? 5 + 3 * s : 15 + 2 * s);
       if (best < 0 || t < best) {
         best = t;
         cut = {s, nw};
@@ -148,6 +152,7 @@ hipError_t run(Stage st, Args a, bool whole, int64_t blocks) {
   const int mode = whole ? dr::kDirect : dr::kGather;
   const DrProblem& p = a.p;
   constexpr int64_t most = most_workgroups(256);
+  a.blocks = blocks;
   for (a.blk0 = 0; a.blk0 < blocks; a.blk0 += most) {
     a.nblk = (int)(blocks - a.blk0 < most ? blocks - a.blk0 : most);
     const hipError_t e = p.dtype == kFP32 ? dr::launch<float, 3>(st, a, mode, p.stream)

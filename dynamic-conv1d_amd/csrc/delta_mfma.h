@@ -47,7 +47,7 @@ struct Args {
   int seg, nseg, nw;  // nw: wavefronts of a chain's workgroup, 16 columns each
   int64_t n;           // chunks of a head
   int vp;              // V in whole 32 columns
-  int64_t blk0;
+  int64_t blk0, blocks;  // of this launch the first workgroup, of all its launches their number
   int nblk;
   bool kept;  // the forward keeps U and the states
 };
@@ -606,6 +606,14 @@ __device__ __forceinline__ void load_direct(const bf16* base, int64_t stride, in
 // How rows reach the chains' tiles.
 enum Mode { kGather, kWhole, kDirect };
 
+// Tiles of one buffer that leave room for four workgroups on a CU, two wavefronts to a SIMD, where those of two leave two
+// (bf16 with float32 results at 128 channels): with workgroups enough they hide each other's latencies, and the chains take
+// rows through registers (B1 T32768 H16: outputs 416 -> 322 us, segments 405 -> 363; B2 T4096 H16 backward's segments 133 ->
+// 93). With fewer the second buffer does (512 workgroups of outputs 113 us, 128 through registers), and in the backward's
+// chain, whose registers are a wavefront's alone (250 us, 260).
+template <typename T, int NP, int KP>
+constexpr bool kShares = __is_same(T, bf16) && NP == 3 && KP == 128;
+
 // What the chains share: the sizes of their tiles in LDS, k, q, Tb, P and the scales, twice where loads write them directly.
 // The memory is asked for at the launch: with its size in sight the compiler takes one wavefront to a SIMD for granted, and
 // 512 registers, of which half are accumulation registers, whose moves were 300 of 490 vector instructions a chunk.
@@ -616,7 +624,7 @@ struct ChainSize {
                        RC = C + (DIRECT ? 0 : 8), PC = C * RC;
   static constexpr int BUF = DIRECT ? 2 : 1, KEYS = NI * PL, SQUARE = NP * PC;
   static constexpr int bytes(bool both) { return BUF * ((both ? 2 : 1) * (KEYS + SQUARE) * 2 + 3 * C * 4); }
-  static constexpr int WAVES = DIRECT && NP == 1 ? 2 : 1;
+  static constexpr int WAVES = DIRECT && NP == 1 || kShares<T, NP, KP> && MODE == kWhole ? 2 : 1;
 };
 
 // bf16 rows of whole tiles, where two buffers fit.
@@ -872,7 +880,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
 // (from the state after it they come by the transpose of what the forward found).  As the forward's, with twice its products
 // that the state waits for: 3.7 us a chunk at 128 x 128 in bf16, 238 us at B4 T4096 H16.
 template <typename T, int NP, int KP, int MODE, bool ACROSS, int NW>
-__global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain_bwd(Args a) {
+__global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, NP, KP, MODE>::WAVES : 1)) void dr_chain_bwd(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
   constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
   constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
@@ -1472,7 +1480,8 @@ hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
     if (st == kGrads)
       return a.p.H == a.p.Hk ? run(dr_grads<T, NP, KP, W, true>, 256, 0) : run(dr_grads<T, NP, KP, W, false>, 256, 0);
     if constexpr (W && kHasDirect<T, NP, KP>)
-      if (mode == kDirect && a.p.K == KP) {
+      if (mode == kDirect && a.p.K == KP &&
+          !(kShares<T, NP, KP> && st != kChainBwd && a.blocks > (st == kChain || st == kChainKeep ? 512 : 256))) {
         if constexpr (kHasFour<T, NP, KP>)
           if (a.nw == 4) return chain(kp, std::integral_constant<int, kDirect>(), four);
         return chain(kp, std::integral_constant<int, kDirect>(), two);

@@ -185,6 +185,13 @@ def test_without_float32_results(size, dtype):
     _check(*size, dtype, state=False, lens=[size[3] - 7 * b for b in range(size[0])] if size[0] > 1 else None)
 
 
+@pytest.mark.parametrize("size", [(3, 48, 48, 70, 128, 128), (2, 8, 16, 1300, 128, 128), (1, 24, 24, 1000, 128, 120)])
+@pytest.mark.parametrize("state", [False, True])
+def test_workgroups_past_two_to_a_cu(size, state):
+    """bf16 with float32 results at 128 channels: more than 512 workgroups, of chains and of segments."""
+    _check(*size, BF, "fp32", state=state, lens=[size[3] - 35 * b for b in range(size[0])])
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 def test_forward_alone(dtype):
     _check(2, 2, 4, 100, 128, 128, dtype, train=False, state=False)
