@@ -878,7 +878,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
 
 // The states' gradients from the last chunk on, and dv; ACROSS: only what each segment but the first makes of them from zero
 // (from the state after it they come by the transpose of what the forward found).  As the forward's, with twice its products
-// that the state waits for: 3.7 us a chunk at 128 x 128 in bf16, 238 us at B4 T4096 H16.
+// that the state waits for: 3.5 us a chunk at 128 x 128 in bf16, 221 us at B4 T4096 H16.
 template <typename T, int NP, int KP, int MODE, bool ACROSS, int NW>
 __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, NP, KP, MODE>::WAVES : 1)) void dr_chain_bwd(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
@@ -1152,8 +1152,8 @@ __global__ __launch_bounds__(256) void dr_across(Args a) {
 // channels to a wavefront.  With the rows' norms in E's place (rq_i rk_j for P, rk_i rk_j for N) the sums are those of q and
 // k themselves, before their part along the row is taken out.  Results lie turned over, four neighbouring channels of a
 // token in a lane: sums over a row are of a lane's own and three others', and a store has 8 bytes.  ONE: one value head to a
-// key head, whose sums need no registers of their own.  The memory path bounds it: B4 T4096 H16 hd128 bf16 170 us for 0.74 GB,
-// of which the states and their gradients are 0.27 (4.3 TB/s); with two value heads to a key head, whose sums leave one
+// key head, whose sums need no registers of their own.  The memory path bounds it: B4 T4096 H16 hd128 bf16 177 us for 0.74 GB,
+// of which the states and their gradients are 0.27 (4.2 TB/s); with two value heads to a key head, whose sums leave one
 // workgroup to a CU for two, 455 us for B2 T8192 H32 (1.3 GB, 2.9 TB/s).
 template <typename T, int NP, int KP, bool WHOLE, bool ONE>
 __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && parts_of<T>() == 1) ? 2 : 1) void dr_grads(Args a) {

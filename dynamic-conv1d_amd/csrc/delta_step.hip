@@ -5,7 +5,8 @@
 // Bound by the state, K x V floats read and written for each sequence and head.  A workgroup takes 8 lanes of VEC columns
 // times 32 rows of one head's state, as linear attention's step does; k S and q S come from the same pass over it, so the
 // rows' parts of both meet once (lane exchanges, then LDS), and the state, kept in registers, is written with its
-// correction.  256 sequences of 32 heads of 128 x 128: 242 us for 1.08 GB, 4.5 TB/s; 8 of 16 heads 6.5 us, the launch.
+// correction.  256 sequences of 32 heads of 128 x 128: 242 us for 1.08 GB, 4.5 TB/s (16 lanes 258,
+// 32 280, 4 328); 8 of 16 heads 6.5 us, the launch.
 #include "dc_common.h"
 #include "layer_launch.h"
 
