@@ -552,12 +552,15 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KP / 16], float* to
 }
 
 // The chains' scales of a chunk on their way to LDS: G/|k|, D/|k|, scale G/|q|; top: the whole chunk's decay's logarithm.
+// Every thread loads and stores as many, those past the 3 C for their wavefront's sake (load_direct): 4 C lie in LDS.
 template <int C, int NT>
 struct Scales {
-  float v[(3 * C + NT - 1) / NT], top = 0.f;
+  static_assert(4 * C % NT == 0, "every wavefront loads scales and stores them");
+  static constexpr int N = 4 * C / NT;
+  float v[N], top = 0.f;
   __device__ __forceinline__ void load(const float* vec) {
 #pragma unroll
-    for (int i = 0; i * NT < 3 * C; ++i) {
+    for (int i = 0; i < N; ++i) {
       const int e = i * NT + (int)threadIdx.x;
       v[i] = vec[kGk * C + (e < 3 * C ? e : 0)];
     }
@@ -565,18 +568,15 @@ struct Scales {
   }
   __device__ __forceinline__ void store(float* lds) const {
 #pragma unroll
-    for (int i = 0; i * NT < 3 * C; ++i) {
-      const int e = i * NT + (int)threadIdx.x;
-      if (e < 3 * C) lds[e] = v[i];
-    }
+    for (int i = 0; i < N; ++i) lds[i * NT + (int)threadIdx.x] = v[i];
   }
 };
 
 // C rows of W channels from memory into a turned tile, by loads that write LDS themselves (16 bytes a lane, 1 KB of the tile
 // a wavefront): no registers hold them.  Rows from cnt on repeat the last one.  Memory operations complete in order: a
-// wavefront that has waited for a later load of its own (the scales, which it stores to LDS) has these in LDS too, and the
-// barrier after that makes them everybody's.  Waiting for all, stores among them, took half of the time of the chains that
-// keep states.
+// wavefront that has waited for a later load of its own has these in LDS too, and the barrier after that makes them
+// everybody's.  That load is the scales', which every wavefront issues behind these and stores to LDS before the barrier.
+// Waiting for all, stores among them, took half of the time of the chains that keep states.
 template <int C, int W, int NW>
 __device__ __forceinline__ void load_direct(const bf16* base, int64_t stride, int cnt, bf16* lds) {
   constexpr int PR = W / 8, N = C * PR / (NW * 64), RPL = (NW * 64) / PR;  // pieces of a row, loads, rows of a load
@@ -623,7 +623,7 @@ struct ChainSize {
   static constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + (DIRECT ? 0 : 24), PL = C * R,
                        RC = C + (DIRECT ? 0 : 8), PC = C * RC;
   static constexpr int BUF = DIRECT ? 2 : 1, KEYS = NI * PL, SQUARE = NP * PC;
-  static constexpr int bytes(bool both) { return BUF * ((both ? 2 : 1) * (KEYS + SQUARE) * 2 + 3 * C * 4); }
+  static constexpr int bytes(bool both) { return BUF * ((both ? 2 : 1) * (KEYS + SQUARE) * 2 + 4 * C * 4); }
   static constexpr int WAVES = DIRECT && NP == 1 || kShares<T, NP, KP> && MODE == kWhole ? 2 : 1;
 };
 
@@ -653,7 +653,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
   constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
   constexpr bool OUT = WHAT == kOutputs || WHAT == kBoth, KEEP = WHAT == kKeep || WHAT == kBoth;  // !OUT: no q and no o
   extern __shared__ __align__(16) unsigned char chain_lds[];
-  float (*lv)[3][C] = reinterpret_cast<float (*)[3][C]>(chain_lds);
+  float (*lv)[4][C] = reinterpret_cast<float (*)[4][C]>(chain_lds);
   bf16 (*lk)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lv + Z::BUF);
   bf16 (*lt)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lk + Z::BUF);
   bf16 (*lq)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lt + Z::BUF);  // there if OUT
@@ -885,7 +885,7 @@ __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, 
   constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
   constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
   extern __shared__ __align__(16) unsigned char chain_lds[];
-  float (*lv)[3][C] = reinterpret_cast<float (*)[3][C]>(chain_lds);
+  float (*lv)[4][C] = reinterpret_cast<float (*)[4][C]>(chain_lds);
   bf16 (*lk)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lv + Z::BUF);
   bf16 (*lt)[Z::SQUARE] = reinterpret_cast<bf16 (*)[Z::SQUARE]>(lk + Z::BUF);
   bf16 (*lq)[Z::KEYS] = reinterpret_cast<bf16 (*)[Z::KEYS]>(lt + Z::BUF);
