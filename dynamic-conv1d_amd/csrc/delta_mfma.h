@@ -24,7 +24,8 @@ namespace dc {
 namespace dr {
 
 constexpr float kTiny = 0x1p-60f;  // stands for a b of zero
-// What a token's chunk keeps of it, floats: c in two parts, b, 1/|k|, 1/|q|, G/|k|, D/|k|, scale G/|q|.
+// What a token's chunk keeps of it, floats: c in two parts, b, 1/|k|, 1/|q|, G/|k|, D/|k|, scale G/|q| (the last five zero
+// behind the last token).
 constexpr int kC = 0, kB = 2, kRk = 3, kRq = 4, kGk = 5, kDk = 6, kGq = 7, kVecs = 8;
 constexpr int kPiece = 128;  // columns of v that the gradients' launch holds at once
 
@@ -307,7 +308,9 @@ __global__ __launch_bounds__(256) void dr_prep(Args a) {
       s[1] += __shfl_xor(s[1], m);
     }
     if (t % TPR == 0) {
-      const float ik = p.normalize ? 1.f / sqrtf(s[0] + p.eps) : 1.f, iq = p.normalize ? 1.f / sqrtf(s[1] + p.eps) : 1.f;
+      // rows from cnt on are no tokens: factors of zero keep them out of everything, also where eps is zero
+      const float one = row < cnt ? 1.f : 0.f, ik = row < cnt && p.normalize ? 1.f / sqrtf(s[0] + p.eps) : one,
+                  iq = row < cnt && p.normalize ? 1.f / sqrtf(s[1] + p.eps) : one;
       rk[row] = ik;
       rq[row] = iq;
       by[0][row] = be[row] * ik;
@@ -573,7 +576,7 @@ struct Scales {
 };
 
 // C rows of W channels from memory into a turned tile, by loads that write LDS themselves (16 bytes a lane, 1 KB of the tile
-// a wavefront): no registers hold them.  Rows from cnt on repeat the last one.  Memory operations complete in order: a
+// a wavefront): no registers hold them.  Rows from cnt on repeat the last one; their scales are zero.  Memory operations complete in order: a
 // wavefront that has waited for a later load of its own has these in LDS too, and the barrier after that makes them
 // everybody's.  That load is the scales', which every wavefront issues behind these and stores to LDS before the barrier.
 // Waiting for all, stores among them, took half of the time of the chains that keep states.

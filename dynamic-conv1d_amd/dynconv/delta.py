@@ -120,8 +120,9 @@ def gated_delta_rule(
         lengths:       [B] int32 on the device: sequence b has its first lengths[b] rows (0 .. T).  Rows past them
                        are not used, whatever they hold; their outputs and gradients are zero.
         return_state:  return the state after each sequence's last token too.
-        normalize:     divide each row of q and k by sqrt(|row|^2 + eps).  The rule wants keys of at most about that
-                       length: a state grows without bound where beta |k|^2 passes 2.
+        normalize:     divide each row of q and k by sqrt(|row|^2 + eps) (eps >= 0; with 0 no row of a sequence may be
+                       zero).  The rule wants keys of at most about that length: a state grows without bound where
+                       beta |k|^2 passes 2.
 
     Returns:
         o [B, H, T, V] in q's dtype, over token-major memory (o.transpose(1, 2).reshape(B, T, H * V) is a view), or

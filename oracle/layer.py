@@ -65,7 +65,8 @@ def gated_delta_rule_ref(q, k, v, log_decay, beta, scale, initial=None, lengths=
         return torch.where(live[:, None, :, None], t.double(), zero)
 
     def unit(t):
-        return t / torch.sqrt((t * t).sum(-1, keepdim=True) + eps) if normalize else t
+        n = torch.sqrt((t * t).sum(-1, keepdim=True) + eps)
+        return t / torch.where(live[:, None, :, None], n, zero + 1) if normalize else t
 
     q, k = (unit(rows(t)).repeat_interleave(H // Hk, 1) for t in (q, k))
     v = rows(v)
@@ -101,9 +102,12 @@ def gated_delta_rule_chunked(q, k, v, log_decay, beta, scale, do, initial=None, 
     def whole(t):
         return t.flatten(2, 3)[:, :, :T]
 
+    tokens = cut(torch.ones(B, 1, T)) > 0  # rows behind the last are none: whatever eps is, nothing comes of them
+
     def heads(t):
         t = cut(t)
-        n = 1 / torch.sqrt((t * t).sum(-1, keepdim=True) + eps) if normalize else torch.ones_like(t[..., :1])
+        n = torch.where(tokens[..., None], torch.sqrt((t * t).sum(-1, keepdim=True) + eps), torch.inf)
+        n = 1 / n if normalize else torch.ones_like(t[..., :1])
         return (t * n).repeat_interleave(H // Hk, 1), n
 
     (qh, nq), (kh, nk) = heads(q), heads(k)
