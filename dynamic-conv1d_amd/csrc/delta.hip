@@ -5,21 +5,23 @@
 // in chunks of C tokens.  With the state S before a chunk, c_i the sum of its logarithms of decays up to token i,
 // G_i = e^{c_i}, E_ij = e^{c_i - c_j}, D_i = e^{c_C - c_i}, and q, k normed and q scaled:
 //
-//   A_ij = b_i E_ij k_i.k_j (j < i),   P_ij = E_ij q_i.k_j (j <= i),   Tb = (1 + A)^-1 diag(b)
-//   X = V - G k S,   U = Tb X,   O = G q S + P U,   S <- G_C S + k^T D U
+//   A_ij = E_ij k_i.k_j b_j (j < i),   P_ij = E_ij q_i.k_j b_j (j <= i),   T = (1 + A)^-1
+//   X = V - G k S,   Z = T X (what the state gets wrong of each token, u = b Z),   O = G q S + P Z,   S <- G_C S + k^T D b Z
 //
-// and backward, dS the gradient of the state after the chunk:
+// and backward, dS the gradient of the state after the chunk, Y that of Z:
 //
-//   dU = P^T dO + D k dS,   dX = Tb^T dU = dV,   dS <- G_C dS + q^T G dO - k^T G dX
-//   dP = dO U^T (j <= i),   N = -dX U^T (j < i)
+//   Y = P^T dO + b D k dS,   dX = T^T Y = dV,   dS <- G_C dS + q^T G dO - k^T G dX
+//   dP = dO Z^T b (j <= i),   N = -dX Z^T b (j < i)                                    (b of the columns)
 //   dq = G dO S^T + (dP E) k
-//   W  = (dP E)^T q + D U dS^T + (N E)^T k,   R = -G dX S^T + (N E) k,   dk = W + R
-//   db_i = (dX_i . U_i) / b_i^2
+//   W  = (dP E)^T q + D b Z dS^T + (N E)^T k,   R = -G dX S^T + (N E) k,   dk = W + R
+//   db_i = (dX_i . Z_i) / b_i
 //   dc_i = q_i.dq_i + k_i.(R_i - W_i),   dc_C += <S after the chunk, dS>;   dlog_decay_i = sum_{l >= i} dc_l
 //
-// Launches: what each chunk needs of its own keys (Tb, P and the decays); the states from chunk to chunk with the outputs, and
-// in the backward with U and the states themselves; the same against time for the states' gradients; and the gradients chunk
-// by chunk.  A b of zero counts as 2^-60, so that db has its quotient.
+// Launches: what each chunk needs of its own keys (T, P and the decays); the states from chunk to chunk with the outputs, and
+// in the backward with Z and the states themselves; the same against time for the states' gradients; and the gradients chunk
+// by chunk.  A b below 2^-60 counts as that, so that db has its quotient: dX is b times a gradient, and what is summed in
+// dX.Z stays a normal float32 where it is above 2^-66 without b (with U = b Z kept instead of Z it was b^2 times that, and
+// nothing was left of gradients below 2^-29).
 #include "delta_mfma.h"
 
 namespace dc {
@@ -76,8 +78,8 @@ Cut cut_of(const DrProblem& p, int C, int np) {
   return cut;
 }
 
-// The workspace: of the forward vec, Tb, P and the segments' states, of the backward dX, where it is not dv, and the states'
-// gradients; U and the states, of the forward where it keeps them, else of the backward.
+// The workspace: of the forward vec, T, P and the segments' states, of the backward dX, where it is not dv, and the states'
+// gradients; Z and the states, of the forward where it keeps them, else of the backward.
 struct Plan {
   int64_t n, vec, sq, rows, st, cut, trans;  // chunks of a head; bytes of each array
   int vp, seg, nseg, nw;
@@ -118,14 +120,14 @@ Args args_of(const DrProblem& p, bool bwd) {
   a.nw = pl.nw;
   char* f = static_cast<char*>(bwd && p.fwd_ws ? const_cast<void*>(p.fwd_ws) : p.ws);
   a.vec = reinterpret_cast<float*>(f);
-  a.tb = reinterpret_cast<bf16*>(f + pl.vec);
+  a.tt = reinterpret_cast<bf16*>(f + pl.vec);
   a.pp = reinterpret_cast<bf16*>(f + pl.vec + pl.sq);
   a.trans = reinterpret_cast<float*>(f + pl.vec + 2 * pl.sq);
   f += pl.vec + 2 * pl.sq + pl.trans;
   a.start = reinterpret_cast<float*>(f);
   char* w = static_cast<char*>(p.ws) + (p.fwd_ws ? 0 : pl.fwd());  // the backward's
   char* kept = pl.kept ? f + pl.cut : w;
-  a.u = reinterpret_cast<bf16*>(kept);
+  a.z = reinterpret_cast<bf16*>(kept);
   a.s = reinterpret_cast<bf16*>(kept + pl.rows);
   a.kept = pl.kept;
   if (bwd) {

@@ -3,13 +3,13 @@
 // Operands and results.  v_mfma_f32_16x16x32 leaves element (row, col) of its result in lane col + 16 (row/4), register
 // row%4; an operand wants 8 values of the summed index in a lane.  Products sum in the order that two results of 16 rows
 // come in (step s: 32 s + 16 (e/4) + 4 (lane/16) + e%4 for element e), so that the chain from the state to the next one,
-// k S, Tb X, k^T U, goes from results to operands without leaving the lane: a wavefront keeps 16 columns of S.  Rows of
+// k S, T X, k^T Z, goes from results to operands without leaving the lane: a wavefront keeps 16 columns of S.  Rows of
 // tiles lie in LDS so that a lane's 8 values of that order are neighbours (spot()); columns are read through transposing
 // reads.
 //
 // Precision.  Operands are bf16 parts: q, k, v and dO one part (bf16), two (fp16: all of its bits) or three (float32); what is
 // computed NP parts: three where a result is float32 (24 bits), two in fp16 (16 bits, results have 11), one in bf16 (8 bits)
-// of what goes through memory (Tb, P, S, dS, U, dX) and two of what does not (X, U, dU and their scaled forms: NR).  Were
+// of what goes through memory (T, P, S, dS, Z, dX) and two of what does not (X, Z, Y and their scaled forms: NR).  Were
 // those one part too, a dozen roundings of a result's own size would add up to 2-3 of its roundings (o 3.2e-3 of its norm,
 // dlog_decay 4.5-8e-3; two parts cost the chains 10%).  A product of parts keeps those down to the last part's size.
 // Sums, S and dS, decays and norms are float32; sums of logarithms of decays are float64.
@@ -24,7 +24,7 @@ namespace dc {
 namespace dr {
 
 constexpr float kTiny = 0x1p-60f;  // stands for a b of zero
-// What a token's chunk keeps of it, floats: c in two parts, b, 1/|k|, 1/|q|, G/|k|, D/|k|, scale G/|q| (the last five zero
+// What a token's chunk keeps of it, floats: c in two parts, b, 1/|k|, 1/|q|, G/|k|, D b/|k|, scale G/|q| (the last five zero
 // behind the last token).
 constexpr int kC = 0, kB = 2, kRk = 3, kRq = 4, kGk = 5, kDk = 6, kGq = 7, kVecs = 8;
 constexpr int kPiece = 128;  // columns of v that the gradients' launch holds at once
@@ -40,8 +40,8 @@ __host__ __device__ constexpr int cover(int n) { return n <= 64 ? 64 : n <= 128 
 struct Args {
   DrProblem p;
   float* vec;          // [chunks][kVecs][C]
-  bf16 *tb, *pp;       // [chunks][NP][C][C], spot() order
-  bf16 *u, *x, *s, *ds;  // [chunks][NP][C][VP] U and dX (not if kFromDv), [chunks][NP][KP][VP] states before and their gradients after
+  bf16 *tt, *pp;       // T and P, [chunks][NP][C][C], spot() order
+  bf16 *z, *x, *s, *ds;  // [chunks][NP][C][VP] Z and dX (not if kFromDv), [chunks][NP][KP][VP] states before and their gradients after
   // tokens cut into nseg segments of seg (whole chunks): the states before each but the first [heads][nseg][K][V], the
   // gradients after each but the last, and what a segment makes of the state before it, [heads][nseg][KP][KP]
   float *start, *dstart, *trans;
@@ -50,7 +50,7 @@ struct Args {
   int vp;              // V in whole 32 columns
   int64_t blk0, blocks;  // of this launch the first workgroup, of all its launches their number
   int nblk;
-  bool kept;  // the forward keeps U and the states
+  bool kept;  // the forward keeps Z and the states
 };
 
 // Where column c of a row lies: of each 32 the quads of both halves side by side.
@@ -243,8 +243,8 @@ __global__ __launch_bounds__(256) void dr_prep(Args a) {
   constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RA = C + 4;
   constexpr int TILES = 2 * NI * PL * 2, MATS = 2 * C * RA * 4;
   __shared__ __align__(16) unsigned char mem[TILES > MATS ? TILES : MATS];
-  // of each token: c in two parts, b, 1/|k|, 1/|q|, and the factors of A's and P's rows b/|k| and scale/|q|
-  __shared__ __align__(16) float chi[C], clo[C], be[C], rk[C], rq[C], by[2][C];
+  // of each token: c in two parts, b, 1/|k|, 1/|q|, the factors of A's and P's rows 1/|k| and scale/|q| and of their columns b/|k|
+  __shared__ __align__(16) float chi[C], clo[C], be[C], rk[C], rq[C], by[2][C], bk[C];
   bf16 *lk = reinterpret_cast<bf16*>(mem), *lq = lk + NI * PL;
   float (*A)[RA] = reinterpret_cast<float (*)[RA]>(mem), (*X)[RA] = A + C;
   const DrProblem& p = a.p;
@@ -313,8 +313,9 @@ __global__ __launch_bounds__(256) void dr_prep(Args a) {
                   iq = row < cnt && p.normalize ? 1.f / sqrtf(s[1] + p.eps) : one;
       rk[row] = ik;
       rq[row] = iq;
-      by[0][row] = be[row] * ik;
+      by[0][row] = ik;
       by[1][row] = p.scale * iq;
+      bk[row] = be[row] * ik;
     }
   }
   // blocks on and below the diagonal, k k^T and q k^T, round the wavefronts
@@ -345,7 +346,7 @@ __global__ __launch_bounds__(256) void dr_prep(Args a) {
     vec[kRk * C] = rk[t];
     vec[kRq * C] = rq[t];
     vec[kGk * C] = G * rk[t];
-    vec[kDk * C] = D * rk[t];
+    vec[kDk * C] = D * bk[t];
     vec[kGq * C] = p.scale * G * rq[t];
   }
 #pragma unroll
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(256) void dr_prep(Args a) {
     const int j = 16 * cb + col, x = 16 * rb + 4 * g;
     const f32x4 hi = *reinterpret_cast<const f32x4*>(&chi[x]), lo = *reinterpret_cast<const f32x4*>(&clo[x]),
                 row = *reinterpret_cast<const f32x4*>(&by[m][x]);
-    const float hj = chi[j], lj = clo[j], kj = rk[j];
+    const float hj = chi[j], lj = clo[j], kj = bk[j];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float c = ((hi[r] - hj) + (lo[r] - lj)) * 1.44269504088896f;
@@ -417,18 +418,17 @@ __global__ __launch_bounds__(256) void dr_prep(Args a) {
       for (int w = 0; w < 2; ++w) {
         const int j = j0 + 16 * w;
         v[w] = *reinterpret_cast<const f32x4*>(&(m ? A : X)[x][j]);
-        if (!m) v[w] *= *reinterpret_cast<const f32x4*>(&be[j]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[w][r] = j + r > x ? 0.f : v[w][r];
       }
       const Frag<NP> f = pack<NP>(v[0], v[1]);
 #pragma unroll
       for (int i = 0; i < NP; ++i)
-        *reinterpret_cast<u32x4*>((m ? a.pp : a.tb) + ((blk * NP + i) * C + x) * C + c) = f.p[i];
+        *reinterpret_cast<u32x4*>((m ? a.pp : a.tt) + ((blk * NP + i) * C + x) * C + c) = f.p[i];
     }
 }
 
-// A chunk's Tb or P on its way to LDS.
+// A chunk's T or P on its way to LDS.
 template <int NP, int C, int NT>
 struct Square {
   static constexpr int NV = NP * C * C / 8 / NT;
@@ -554,7 +554,7 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KP / 16], float* to
     }
 }
 
-// The chains' scales of a chunk on their way to LDS: G/|k|, D/|k|, scale G/|q|; top: the whole chunk's decay's logarithm.
+// The chains' scales of a chunk on their way to LDS: G/|k|, D b/|k|, scale G/|q|; top: the whole chunk's decay's logarithm.
 // Every thread loads and stores as many, those past the 3 C for their wavefront's sake (load_direct): 4 C lie in LDS.
 template <int C, int NT>
 struct Scales {
@@ -617,7 +617,7 @@ enum Mode { kGather, kWhole, kDirect };
 template <typename T, int NP, int KP>
 constexpr bool kShares = __is_same(T, bf16) && NP == 3 && KP == 128;
 
-// What the chains share: the sizes of their tiles in LDS, k, q, Tb, P and the scales, twice where loads write them directly.
+// What the chains share: the sizes of their tiles in LDS, k, q, T, P and the scales, twice where loads write them directly.
 // The memory is asked for at the launch: with its size in sight the compiler takes one wavefront to a SIMD for granted, and
 // 512 registers, of which half are accumulation registers, whose moves were 300 of 490 vector instructions a chunk.
 template <typename T, int NP, int KP, int MODE>
@@ -638,7 +638,7 @@ constexpr bool kHasDirect = __is_same(T, bf16) && ChainSize<T, NP, KP, kDirect>:
 template <typename T, int NP, int KP>
 constexpr bool kHasFour = __is_same(T, bf16) && NP == 1 && KP == 128;
 
-// The states from chunk to chunk, and o (kOutputs); or U and the state before each chunk for the backward (kKeep); or all of
+// The states from chunk to chunk, and o (kOutputs); or Z and the state before each chunk for the backward (kKeep); or all of
 // these (kBoth); or what each segment but the last makes of the state before it (kAcross): its end from zero, and behind those
 // columns its end from each unit vector without values.
 //
@@ -699,7 +699,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
     const int cnt = min(C, len - t0);
     const int64_t ch = bh * a.n + t0 / C;
     const T *kt = k + (int64_t)t0 * p.ks[2], *qt = q + (int64_t)t0 * p.qs[2];
-    const bf16 *tt = a.tb + ch * NP * C * C, *pt = a.pp + ch * NP * C * C;
+    const bf16 *tt = a.tt + ch * NP * C * C, *pt = a.pp + ch * NP * C * C;
     if constexpr (DIRECT) {
       load_direct<C, KP, NW>(kt, p.ks[2], cnt, lk[buf]);
       load_direct<NP * C, C, NW>(tt, C, NP * C, lt[buf]);
@@ -799,7 +799,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
     Frag<NR> f[C / 32], d[C / 32];
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) f[s] = pack<NR>(x[2 * s], x[2 * s + 1]);
-    // U = Tb X
+    // Z = T X
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -811,12 +811,12 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) {
       f[s] = pack<NR>(x[2 * s], x[2 * s + 1]);
-      if (KEEP) keep<NP, false>(a.u + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, first<NP>(f[s]));
+      if (KEEP) keep<NP, false>(a.z + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, first<NP>(f[s]));
       d[s] = pack<NR>(x[2 * s] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 4 * g]),
                       x[2 * s + 1] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 16 + 4 * g]));
     }
     phase();
-    // S <- G_C S + k^T D U
+    // S <- G_C S + k^T D b Z
 #pragma unroll
     for (int e0 = 0; e0 < NK; e0 += 8) {
       if (e0 + 8 < NK) keys(e0 + 8);
@@ -828,7 +828,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
       }
       phase();
     }
-    // O^T = G S^T q^T + U^T P^T: four neighbouring channels of a token in a lane
+    // O^T = G S^T q^T + Z^T P^T: four neighbouring channels of a token in a lane
     if constexpr (OUT) {
 #pragma unroll
       for (int rb = 0; rb < NB; ++rb) y[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -922,7 +922,7 @@ __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, 
     const int cnt = min(C, len - t0);
     const int64_t ch = bh * a.n + t0 / C;
     const T *kt = k + (int64_t)t0 * p.ks[2], *qt = q + (int64_t)t0 * p.qs[2];
-    const bf16 *tt = a.tb + ch * NP * C * C, *pt = a.pp + ch * NP * C * C;
+    const bf16 *tt = a.tt + ch * NP * C * C, *pt = a.pp + ch * NP * C * C;
     if constexpr (DIRECT) {
       load_direct<C, KP, NW>(kt, p.ks[2], cnt, lk[buf]);
       load_direct<NP * C, C, NW>(tt, C, NP * C, lt[buf]);
@@ -988,7 +988,7 @@ __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, 
       df[s] = pack<NI>(x[2 * s], x[2 * s + 1]);
       gd[s] = pack<NR>(x[2 * s] * at(2, 32 * s), x[2 * s + 1] * at(2, 32 * s + 16));
     }
-    // dU = P^T dO + D k dS
+    // Y = P^T dO + b D k dS
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
     Frag<NP> tc[NB][NB / 2];
@@ -1017,7 +1017,7 @@ __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, 
 #pragma unroll
       for (int rb = 0; rb < 2 * s + 2; ++rb) x[rb] = mma(tc[rb][s], df[s], x[rb]);
     phase();
-    // dS <- G_C dS + q^T G dO - k^T G dX: its first part, beside dX = Tb^T dU
+    // dS <- G_C dS + q^T G dO - k^T G dX: its first part, beside dX = T^T Y
     square(tt);
     constexpr int KN = KP / 16, NK = KN * (C / 32);
     Frag<NI> kc[2][NK < 8 ? NK : 8];
@@ -1206,7 +1206,7 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
     for (int rb = 0; rb < NB; ++rb)
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb) dq[rb][cb] = dr[rb][cb] = dw[rb][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // dO U^T and dX U^T: a block of rows (i) to a wavefront and all blocks of columns (j), those above the diagonal too,
+    // dO Z^T and dX Z^T: a block of rows (i) to a wavefront and all blocks of columns (j), those above the diagonal too,
     // which cost less than the branches that would leave them out; with two blocks of rows one block to a wavefront
     const int rbu = NB == 4 ? wv : wv % 2;
     f32x4 accp[NU], accn[NU];
@@ -1236,7 +1236,7 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
         if constexpr (DV) rv.load(dv + v0, p.dvs[2], V - v0, cnt);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          ru[i].load(a.u + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
+          ru[i].load(a.z + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
           if constexpr (!DV) ru[NP + i].load(a.x + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
         }
         float vec[(kVecs * C + 255) / 256];
@@ -1299,14 +1299,14 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
     Rows<T, C, KP, 256, WHOLE> rk, rq;
     rk.load((const T*)p.k + b * p.ks[0] + hk * p.ks[1] + (int64_t)t0 * p.ks[2], p.ks[2], K, cnt);
     rq.load((const T*)p.q + b * p.qs[0] + hk * p.qs[1] + (int64_t)t0 * p.qs[2], p.qs[2], K, cnt);
-    // the pairs' gradients with their decays and norms, as operands
+    // the pairs' gradients with their decays, strengths and norms, as operands
     {
       auto at = [&](int m) { return *reinterpret_cast<const f32x4*>(&lv[m][16 * rbu + 4 * g]); };
       const f32x4 hi = at(0), lo = at(1), ki = at(kRk), qi = at(kRq) * p.scale;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         const int cb = NB == 4 ? i : wv / 2, j = 16 * cb + col;
-        const float hj = lv[0][j], lj = lv[1][j], kj = lv[kRk][j];
+        const float hj = lv[0][j], lj = lv[1][j], kj = lv[kRk][j] * lv[kB][j];
         f32x4 vp, vn;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -1421,7 +1421,7 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
         c += (total[0] + total[1]) + (total[2] + total[3]);
         const float be = lv[kB][i];
         put_gate(p.dg, p.gdtype, b * p.dgs[0] + h * p.dgs[1] + (t0 + lane) * p.dgs[2], in ? c : 0.f);
-        put_gate(p.db, p.gdtype, b * p.dbs[0] + h * p.dbs[1] + (t0 + lane) * p.dbs[2], in ? diag[i] / be / be : 0.f);
+        put_gate(p.db, p.gdtype, b * p.dbs[0] + h * p.dbs[1] + (t0 + lane) * p.dbs[2], in ? diag[i] / be : 0.f);
       }
     }
   }

@@ -117,42 +117,42 @@ def gated_delta_rule_chunked(q, k, v, log_decay, beta, scale, do, initial=None, 
     low = torch.ones(chunk, chunk, dtype=torch.bool).tril()
     E = torch.exp(torch.where(low, c[..., :, None] - c[..., None, :], -torch.inf)).to(dtype)
     G, D, Gl = (torch.exp(t).to(dtype) for t in (c[..., None], (c[..., -1:] - c)[..., None], c[..., -1][..., None, None]))
-    P = r((qh @ kh.transpose(3, 4)) * E)
-    A = b * ((kh @ kh.transpose(3, 4)) * E).tril(-1)
-    Tb = torch.linalg.solve_triangular(A + torch.eye(chunk, dtype=dtype), torch.eye(chunk, dtype=dtype).expand_as(A),
-                                       upper=False, unitriangular=True)
-    Tb = r(Tb * b.transpose(3, 4))
+    bj = b.transpose(3, 4)
+    P = r((qh @ kh.transpose(3, 4)) * E * bj)
+    A = ((kh @ kh.transpose(3, 4)) * E * bj).tril(-1)
+    M = r(torch.linalg.solve_triangular(A + torch.eye(chunk, dtype=dtype), torch.eye(chunk, dtype=dtype).expand_as(A),
+                                        upper=False, unitriangular=True))
     S = torch.zeros(B, H, K, V, dtype=dtype) if initial is None else initial.to(dtype)
-    states, Us, o = [], [], []
+    states, Zs, o = [], [], []
     for n in range(N):
         states.append(r(S))
-        U = Tb[:, :, n] @ r(v[:, :, n] - G[:, :, n] * (kh[:, :, n] @ states[-1]))
-        Us.append(U)
-        o.append(G[:, :, n] * (qh[:, :, n] @ states[-1]) + P[:, :, n] @ r(U))
-        S = Gl[:, :, n] * S + kh[:, :, n].transpose(2, 3) @ r(D[:, :, n] * U)
+        Z = M[:, :, n] @ r(v[:, :, n] - G[:, :, n] * (kh[:, :, n] @ states[-1]))
+        Zs.append(Z)
+        o.append(G[:, :, n] * (qh[:, :, n] @ states[-1]) + P[:, :, n] @ r(Z))
+        S = Gl[:, :, n] * S + kh[:, :, n].transpose(2, 3) @ r((D * b)[:, :, n] * Z)
     if N == 0:
         return (torch.zeros(B, H, 0, V, dtype=dtype), S), None
-    Ss, U, o = torch.stack(states, 2), torch.stack(Us, 2), torch.stack(o, 2)
+    Ss, Z, o = torch.stack(states, 2), torch.stack(Zs, 2), torch.stack(o, 2)
     dS = torch.zeros_like(S) if dstate is None else dstate.to(dtype)
     last, dX = [None] * N, [None] * N
     for n in reversed(range(N)):
         last[n] = r(dS)
-        dU = P[:, :, n].transpose(2, 3) @ do[:, :, n] + D[:, :, n] * (kh[:, :, n] @ last[n])
-        dX[n] = Tb[:, :, n].transpose(2, 3) @ r(dU)
+        Y = P[:, :, n].transpose(2, 3) @ do[:, :, n] + (D * b)[:, :, n] * (kh[:, :, n] @ last[n])
+        dX[n] = M[:, :, n].transpose(2, 3) @ r(Y)
         dS = (Gl[:, :, n] * dS + qh[:, :, n].transpose(2, 3) @ r(G[:, :, n] * do[:, :, n])
               - kh[:, :, n].transpose(2, 3) @ r(G[:, :, n] * dX[n]))
     last, dX = torch.stack(last, 2), torch.stack(dX, 2)
     after = torch.cat([Ss[:, :, 1:], S[:, :, None]], 2)
-    Ur, Xr = r(U), r(dX)
-    PE = r((do @ Ur.transpose(3, 4)).tril() * E)
-    NU = -(Xr @ Ur.transpose(3, 4))
-    NE = r(NU.tril(-1) * E)
+    Zr, Xr = r(Z), r(dX)
+    PE = r((do @ Zr.transpose(3, 4)).tril() * E * bj)
+    NZ = -(Xr @ Zr.transpose(3, 4))
+    NE = r(NZ.tril(-1) * E * bj)
     dq = G * (do @ Ss.transpose(3, 4)) + PE @ kh
-    W = PE.transpose(3, 4) @ qh + D * (Ur @ last.transpose(3, 4)) + NE.transpose(3, 4) @ kh
+    W = PE.transpose(3, 4) @ qh + D * b * (Zr @ last.transpose(3, 4)) + NE.transpose(3, 4) @ kh
     R = NE @ kh - G * (Xr @ Ss.transpose(3, 4))
     dc = (qh * dq).sum(-1) + (kh * (R - W)).sum(-1)
     dg = dc.flip(-1).cumsum(-1).flip(-1) + (after * last).sum((-1, -2))[..., None]
-    db = -torch.diagonal(NU, dim1=-2, dim2=-1) / b[..., 0] / b[..., 0]
+    db = -torch.diagonal(NZ, dim1=-2, dim2=-1) / b[..., 0]
 
     def back(dt, t, n, s=1.0):
         dt, t = (x.unflatten(1, (Hk, H // Hk)) for x in (dt * s, t / s))
