@@ -368,8 +368,9 @@ class DynamicDeltaStack(nn.Module):
         return [layer.new_state(rows) for layer in self.layers]
 
     def _run(self, x, call):
-        h = x.contiguous() if self.stream is None else x.to(self.stream).contiguous()
-        y = F.rms_norm(x, (self.d_model,), self.weight[0], self.eps)
+        x = x.contiguous()
+        # the first norm has no branch before it: x takes its place, with no weight in the sum
+        y, h = residual_norm(x if self.stream is None else x.to(self.stream), x, weight=self.weight[0], scale=0.0, eps=self.eps)
         for i in range(len(self.layers)):
             y, h = residual_norm(h, call(i, y), weight=self.weight[i + 1], branch_weight=self.branch_weight[i],
                                  scale=self.scale[i], eps=self.eps)
