@@ -14,7 +14,7 @@
 //   dP = dO Z^T b (j <= i),   N = -dX Z^T b (j < i)                                    (b of the columns)
 //   dq = G dO S^T + (dP E) k
 //   W  = (dP E)^T q + D b Z dS^T + (N E)^T k,   R = -G dX S^T + (N E) k,   dk = W + R
-//   db_i = (dX_i . Z_i) / b_i
+//   db_i = (dX_i . Z_i) / b_i = k_i.W_i / b_i (the former where dX keeps more bits than dv)
 //   dc_i = q_i.dq_i + k_i.(R_i - W_i),   dc_C += <S after the chunk, dS>;   dlog_decay_i = sum_{l >= i} dc_l
 //
 // Launches: what each chunk needs of its own keys (T, P and the decays); the states from chunk to chunk with the outputs, and
@@ -31,7 +31,9 @@ using dr::Args;
 using dr::Stage;
 
 // Parts of what is computed (delta_mfma.h).
-int np_of(const DrProblem& p) { return p.dtype == kFP32 || p.precise ? 3 : p.dtype == kFP16 ? 2 : 1; }
+int np_of(const DrProblem& p) { return p.dtype == kFP32 || p.precise ? 3 : 2; }
+// Halves in memory (delta_mfma.h).
+bool halves(const DrProblem& p) { return p.dtype == kBF16 && !p.precise; }
 int chunk(const DrProblem& p) {
   return dr::chunk_of(p.dtype == kFP32 ? 3 : p.dtype == kFP16 ? 2 : 1, np_of(p), dr::cover((int)p.K));
 }
@@ -41,17 +43,16 @@ int chunk(const DrProblem& p) {
 // where its tiles leave room for one on a CU.  The least estimated time: per chunk of a chain `us`, 0.8 of that without
 // outputs (with the unit vectors' columns, twice as many where K is V), in rounds of the workgroups that fit (small tiles
 // let wavefronts share SIMDs, at 0.65 of a round for another), and the launches.  Measured, bf16, us (* is what it takes):
-// forward of B1 H16 T8192 hd128, 1 segment 379, 2 339, 4 214, 8 171 *, 16 203; B1 H2 T16384 hd128, 8 180, 16 137, 32 135 *;
-// B1 H16 T32768 hd128 with its state, 1 2845, 4 1530, 8 950, 16 835 *; B1 H4 T2048 hd256, 1 245, 4 143, 8 146 *.  Training
-// of B4 H32 T2048 hd128: workgroups of 2 wavefronts 717, of 4 558 *; of B4 H16 T4096, before the forward kept its states, 2
-// 820 *, 4 899.
+// forward of B1 H16 T8192 hd128, 1 segment 427, 2 383, 4 231, 8 176 *, 16 202; B1 H2 T16384 hd128, 8 205, 16 151, 26 154 *,
+// 32 159; B1 H16 T32768 hd128 with its state, 1 2845, 4 1530, 8 950, 16 816 *; B1 H4 T2048 hd256, 1 456, 4 198, 8 177 *.
+// Training of B4 H32 T2048 hd128: workgroups of 2 wavefronts 864, of 4 624 *; of B4 H16 T4096, 2 818 *, 4 891.
 struct Cut {
   int nseg, nw;
 };
 Cut cut_of(const DrProblem& p, int C, int np) {
   const int kp = dr::cover((int)p.K), vp = ((int)p.V + 31) / 32 * 32;
   const int64_t chunks = (p.T + C - 1) / C, heads = p.B * p.H;
-  const bool one = np == 1 && kp == 128 && p.dtype == kBF16;  // workgroup on a CU; elsewhere two
+  const bool one = halves(p) && kp == 128;  // workgroup on a CU; elsewhere two
   const bool shares = np == 3 && kp == 128 && p.dtype == kBF16;  // two or, of more than 512, four (delta_mfma.h)
   double best = -1;
   Cut cut{1, 2};
@@ -60,7 +61,7 @@ Cut cut_of(const DrProblem& p, int C, int np) {
       if (shares && !small) return wgs <= 512 ? 1 : 1.6 * wgs / 1024 > 0.6 + wgs / 1024 ? 1.6 * wgs / 1024 : 0.6 + wgs / 1024;
       return small ? (wgs <= 512 ? 1 : 0.35 + 0.65 * wgs / 512) : __builtin_ceil(wgs / (one ? 256 : 512));
     };
-    const double us = (np == 1 ? 2.5 : shares ? 3.2 : 2.8) * (nw == 4 ? 1.25 : 1);
+    const double us = (shares ? 3.2 : 2.8) * (nw == 4 ? 1.25 : 1);
     const int cols = nw * 16;
     for (int s = 1; s <= 64 && (s == 1 || s <= chunks); ++s) {
       const int64_t len = (chunks + s - 1) / s;
@@ -79,9 +80,10 @@ Cut cut_of(const DrProblem& p, int C, int np) {
 }
 
 // The workspace: of the forward vec, T, P and the segments' states, of the backward dX, where it is not dv, and the states'
-// gradients; Z and the states, of the forward where it keeps them, else of the backward.
+// gradients; Z and the states with their exponents, of the forward where it keeps them, else of the backward (the exponents, a
+// byte for 8 to 64 values, have room in both, so that keeping moves Z and the states alone).
 struct Plan {
-  int64_t n, vec, sq, rows, st, cut, trans;  // chunks of a head; bytes of each array
+  int64_t n, vec, sq, rows, st, ex, cut, trans;  // chunks of a head; bytes of each array
   int vp, seg, nseg, nw;
   bool kept, from_dv;
   explicit Plan(const DrProblem& p) {
@@ -91,9 +93,11 @@ struct Plan {
     const int64_t chunks = p.B * p.H * n;
     vec = chunks * dr::kVecs * C * 4;
     sq = chunks * np * C * C * 2;
-    rows = chunks * np * C * vp * 2;
+    const int nd = dr::planes(halves(p), np);
+    rows = chunks * nd * C * vp * 2;
     const int kp = dr::cover((int)p.K);
-    st = chunks * np * kp * vp * 2;
+    st = chunks * nd * kp * vp * 2;
+    ex = halves(p) ? chunks * 4 * vp : 0;
     const Cut cut_ = cut_of(p, C, np);
     nseg = cut_.nseg;
     nw = cut_.nw;
@@ -102,11 +106,11 @@ struct Plan {
     trans = nseg > 1 ? p.B * p.H * nseg * kp * kp * 4 : 0;
     // saves the backward a launch: training of B4 H16 T4096 hd128 in bf16 824 -> 730 us for 201 MB, 0.75 of q, k, v and o;
     // of B2 T2048 with 8 | 16 heads of 64 x 128 and float32 gates 47 of 390 us would take 3.6 times their memory
-    from_dv = p.dtype == kBF16 && np == 1;
+    from_dv = halves(p);
     kept = p.keep && rows + st <= 2 * p.B * p.T * (p.Hk * 2 * p.K + p.H * 2 * p.V) * dtype_size(p.dtype);
   }
-  int64_t fwd() const { return vec + 2 * sq + trans + cut + (kept ? rows + st : 0); }
-  int64_t bwd() const { return (kept ? 0 : rows + st) + (from_dv ? 0 : rows) + st + cut; }
+  int64_t fwd() const { return vec + 2 * sq + trans + cut + 2 * ex + (kept ? rows + st : 0); }
+  int64_t bwd() const { return (kept ? 0 : rows + st) + (from_dv ? 0 : rows) + st + 3 * ex + cut; }
 };
 
 Args args_of(const DrProblem& p, bool bwd) {
@@ -125,8 +129,11 @@ Args args_of(const DrProblem& p, bool bwd) {
   a.trans = reinterpret_cast<float*>(f + pl.vec + 2 * pl.sq);
   f += pl.vec + 2 * pl.sq + pl.trans;
   a.start = reinterpret_cast<float*>(f);
+  f += pl.cut;
+  uint8_t* ex = reinterpret_cast<uint8_t*>(f);
+  f += 2 * pl.ex;
   char* w = static_cast<char*>(p.ws) + (p.fwd_ws ? 0 : pl.fwd());  // the backward's
-  char* kept = pl.kept ? f + pl.cut : w;
+  char* kept = pl.kept ? f : w;
   a.z = reinterpret_cast<bf16*>(kept);
   a.s = reinterpret_cast<bf16*>(kept + pl.rows);
   a.kept = pl.kept;
@@ -135,8 +142,12 @@ Args args_of(const DrProblem& p, bool bwd) {
     a.x = reinterpret_cast<bf16*>(w);
     if (!pl.from_dv) w += pl.rows;
     a.ds = reinterpret_cast<bf16*>(w);
-    a.dstart = reinterpret_cast<float*>(w + pl.st);
+    a.eds = reinterpret_cast<uint8_t*>(w + pl.st);
+    if (!pl.kept) ex = a.eds + pl.ex;
+    a.dstart = reinterpret_cast<float*>(w + pl.st + 3 * pl.ex);
   }
+  a.es = ex;
+  a.ez = ex + pl.ex;
   return a;
 }
 
@@ -161,7 +172,7 @@ hipError_t run(Stage st, Args a, bool whole, int64_t blocks) {
                          : p.dtype == kFP16 && p.precise ? dr::launch<fp16, 3>(st, a, mode, p.stream)
                          : p.dtype == kFP16              ? dr::launch<fp16, 2>(st, a, mode, p.stream)
                          : p.precise                     ? dr::launch<bf16, 3>(st, a, mode, p.stream)
-                                                         : dr::launch<bf16, 1>(st, a, mode, p.stream);
+                                                         : dr::launch<bf16, 2>(st, a, mode, p.stream);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;

@@ -8,10 +8,12 @@
 // reads.
 //
 // Precision.  Operands are bf16 parts: q, k, v and dO one part (bf16), two (fp16: all of its bits) or three (float32); what is
-// computed NP parts: three where a result is float32 (24 bits), two in fp16 (16 bits, results have 11), one in bf16 (8 bits)
-// of what goes through memory (T, P, S, dS, Z, dX) and two of what does not (X, Z, Y and their scaled forms: NR).  Were
-// those one part too, a dozen roundings of a result's own size would add up to 2-3 of its roundings (o 3.2e-3 of its norm,
-// dlog_decay 4.5-8e-3; two parts cost the chains 10%).  A product of parts keeps those down to the last part's size.
+// computed NP parts: three where a result is float32 (24 bits), else two (16 bits; results have 8 or 11).  In bf16 what goes
+// through memory for the gradients takes 16 bits a value all the same: S, dS and Z are halves of 11 bits over a power of two
+// of each lane's own (Half), and dX is dv, whose own rounding it is.  That leaves o, dq and dv at one rounding of their norm
+// (1.7e-3 of it), dk and dlog_decay at 1.1 and dbeta (by k.W: dX.Z would have dX's rounding whole, 1.4) at 1.2.  With one bf16
+// part of each (8 bits) they were 1.5, 1.7, 1.5, 1.9, 2.4 and 2.1 roundings off, in 0.8 of the time (B4 T4096 H16 hd128 training
+// 663 us, 818).  A product of parts keeps those down to the last part's size.
 // Sums, S and dS, decays and norms are float32; sums of logarithms of decays are float64.
 #pragma once
 
@@ -27,12 +29,11 @@ constexpr float kTiny = 0x1p-60f;  // stands for a b of zero
 // What a token's chunk keeps of it, floats: c in two parts, b, 1/|k|, 1/|q|, G/|k|, D b/|k|, scale G/|q| (the last five zero
 // behind the last token).
 constexpr int kC = 0, kB = 2, kRk = 3, kRq = 4, kGk = 5, kDk = 6, kGq = 7, kVecs = 8;
-constexpr int kPiece = 128;  // columns of v that the gradients' launch holds at once
 
 template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __is_same(T, fp16) ? 2 : 1; }
-constexpr int held(int np) { return np == 1 ? 2 : np; }  // parts of operands that stay in registers
-// dX for the gradients' launch is dv itself, where both are one bf16 (B4 T4096 H16 hd128: 67 MB less to write).
-template <typename T, int NP> constexpr bool kFromDv = __is_same(T, bf16) && NP == 1;
+// What goes through memory for the gradients is halves, and dX dv itself (B4 T4096 H16 hd128: 67 MB less to write).
+template <typename T, int NP> constexpr bool kHalves = __is_same(T, bf16) && NP == 2;
+constexpr int planes(bool halves, int np) { return halves ? 1 : np; }  // 16-bit words of a value there
 // Tokens of a chunk: 64, or 32 where tiles of 64 would pass the LDS (np: parts of what is computed, ni: of q and k).
 __host__ __device__ constexpr int chunk_of(int ni, int np, int kp) { return np == 3 || ni * kp > 256 ? 32 : 64; }
 __host__ __device__ constexpr int cover(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : 256; }
@@ -41,7 +42,10 @@ struct Args {
   DrProblem p;
   float* vec;          // [chunks][kVecs][C]
   bf16 *tt, *pp;       // T and P, [chunks][NP][C][C], spot() order
-  bf16 *z, *x, *s, *ds;  // [chunks][NP][C][VP] Z and dX (not if kFromDv), [chunks][NP][KP][VP] states before and their gradients after
+  // Z and dX (not if kHalves) [chunks][planes][C][VP], states before and their gradients after [chunks][planes][KP][VP]; and if
+  // kHalves the lanes' exponents of Z, states and gradients, [chunks][4][VP]
+  bf16 *z, *x, *s, *ds;
+  uint8_t *ez, *es, *eds;
   // tokens cut into nseg segments of seg (whole chunks): the states before each but the first [heads][nseg][K][V], the
   // gradients after each but the last, and what a segment makes of the state before it, [heads][nseg][KP][KP]
   float *start, *dstart, *trans;
@@ -105,14 +109,48 @@ __device__ __forceinline__ int turn(int row) {
   return W == 32 ? row >> 2 & 3 : W == 64 ? (row << 1 & 4) | (row >> 2 & 3) : (row << 2 & 12) | (row >> 2 & 3);
 }
 
-// The first parts of an operand.
-template <int N, int M>
-__device__ __forceinline__ Frag<N> first(const Frag<M>& f) {
-  Frag<N> t;
+// Float32 values of a lane in halves over a power of two of the lane's own, which takes the largest of them to 2^14 .. 2^15:
+// 11 bits of each that is not below 2^-28 of it.  A byte holds the power as a float's exponent bits.
+struct Half {
+  uint32_t byte;
+  float by;
+  template <int N>
+  __device__ __forceinline__ explicit Half(const f32x4 (&v)[N]) {
+    float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) t.p[i] = f.p[i];
-  return t;
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(v[i][r]));
+    byte = max((int)(__float_as_uint(m) >> 23) - 14, 1);
+    by = __uint_as_float((254 - byte) << 23);
+  }
+  // as pack()
+  __device__ __forceinline__ Frag<1> operator()(f32x4 a, f32x4 b) const {
+    Frag<1> f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f.p[0][e] = e < 2 ? pack2<fp16>(a[2 * e] * by, a[2 * e + 1] * by) : pack2<fp16>(b[2 * e - 4] * by, b[2 * e - 3] * by);
+    return f;
+  }
+};
+// Eight such halves over the powers `by`, in two bf16 parts (8 and 3 bits, exact); `v`: their values.
+__device__ __forceinline__ Frag<2> halves(u32x4 w, const f32x4 (&by)[2], float (&v)[8]) {
+  Frag<2> f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t lo[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = 2 * e + i;
+      v[j] = Mma16<fp16>::to_f(i ? w[e] >> 16 : w[e] & 0xFFFFu) * by[j / 4][j % 4];
+      lo[i] = __float_as_uint(v[j] - __uint_as_float(__float_as_uint(v[j]) & 0xFFFF0000u));
+    }
+    f.p[0][e] = __builtin_amdgcn_perm(__float_as_uint(v[2 * e + 1]), __float_as_uint(v[2 * e]), 0x07060302u);
+    f.p[1][e] = __builtin_amdgcn_perm(lo[1], lo[0], 0x07060302u);
+  }
+  return f;
 }
+// The power of a byte.
+__device__ __forceinline__ float power(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // A tile in LDS: R elements from a row to the next, PL from a part to the next; TURN: its pieces turned, R of them whole.
 template <int N, int R, int PL, bool TURN = false>
@@ -447,6 +485,19 @@ struct Square {
   }
 };
 
+// Rows of halves (Rows<bf16>, as they are) over the powers of their columns into a tile of two parts.
+template <int R, int PL, typename ROWS>
+__device__ __forceinline__ void store_halves(const ROWS& rows, const f32x4 (&by)[2], bf16* lds) {
+  bf16* to = lds + (int)threadIdx.x / ROWS::PR * R + (int)threadIdx.x % ROWS::PR * 8;
+#pragma unroll
+  for (int i = 0; i < ROWS::NV; ++i, to += ROWS::RPI * R) {
+    float v[8];
+    const Frag<2> f = halves(rows.v[i], by, v);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) *reinterpret_cast<u32x4*>(to + j * PL) = f.p[j];
+  }
+}
+
 // 16 columns of C rows as results lie: element r of v[rb] is row 16 rb + 4 (lane/16) + r, column lane%16.
 template <typename T, int C, bool WHOLE>
 struct Columns {
@@ -514,17 +565,33 @@ __device__ __forceinline__ void put_columns(T* base, int64_t stride, int left, i
 template <int NP, bool STATE>
 __device__ __forceinline__ void keep(bf16* to, int vp, int64_t plane, const Frag<NP>& f) {
   const int g = threadIdx.x % 64 / 16, col = threadIdx.x % 16, odd = col % 2;
-  uint32_t* q = reinterpret_cast<uint32_t*>(to + ((STATE ? 8 : 4) * g + odd) * vp + col - odd);
+  const rsrc_t rs = make_rsrc_wave(to, ((NP - 1) * plane + 32 * vp) * 2);
+  const int off = (((STATE ? 8 : 4) * g + odd) * vp + col - odd) * 2;
   const uint32_t sel = odd ? 0x03020706u : 0x05040100u;  // (the neighbour's, own) high halves, or (own, its) low halves
 #pragma unroll
   for (int i = 0; i < NP; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t own = f.p[i][e], its = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)own, 0xB1, 0xF, 0xF, false);
-      q[(i * plane + (STATE ? 2 * e : 16 * (e / 2) + 2 * (e % 2)) * vp) / 2] = __builtin_amdgcn_perm(its, own, sel);
+      const int more = ((int)(i * plane) + (STATE ? 2 * e : 16 * (e / 2) + 2 * (e % 2)) * vp) * 2;
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_amdgcn_perm(its, own, sel), rs, off, more, 0);
     }
 }
 
+// A chunk's states (or their gradients) of this wavefront's columns into memory: halves, or the parts that are there.
+template <typename T, int NP, int KP>
+__device__ __forceinline__ void keep_state(bf16* to, uint8_t* exponents, int64_t ch, int vp, int n0, const f32x4 (&S)[KP / 16],
+                                           const Frag<NP> (&parts)[KP / 32]) {
+  if constexpr (kHalves<T, NP>) {
+    const Half half(S);
+#pragma unroll
+    for (int s = 0; s < KP / 32; ++s) keep<1, true>(to + (ch * KP + 32 * s) * vp + n0, vp, 0, half(S[2 * s], S[2 * s + 1]));
+    exponents[(ch * 4 + threadIdx.x % 64 / 16) * vp + n0 + threadIdx.x % 16] = (uint8_t)half.byte;
+  } else {
+#pragma unroll
+    for (int s = 0; s < KP / 32; ++s) keep<NP, true>(to + (ch * NP * KP + 32 * s) * vp + n0, vp, (int64_t)KP * vp, parts[s]);
+  }
+}
 
 // Nothing moves across the end of a phase: without it the compiler sinks a batch of operands to its use, which then waits.
 __device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
@@ -625,9 +692,11 @@ struct ChainSize {
   static constexpr bool DIRECT = MODE == kDirect;
   static constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + (DIRECT ? 0 : 24), PL = C * R,
                        RC = C + (DIRECT ? 0 : 8), PC = C * RC;
+  // steps of an operands' batch, one ahead of the products: two parts' products of one step take as long as one part's of two
+  static constexpr int STEPS = NP == 2 ? 1 : 2;
   static constexpr int BUF = DIRECT ? 2 : 1, KEYS = NI * PL, SQUARE = NP * PC;
   static constexpr int bytes(bool both) { return BUF * ((both ? 2 : 1) * (KEYS + SQUARE) * 2 + 4 * C * 4); }
-  static constexpr int WAVES = DIRECT && NP == 1 || kShares<T, NP, KP> && MODE == kWhole ? 2 : 1;
+  static constexpr int WAVES = DIRECT && NP == 2 || kShares<T, NP, KP> && MODE == kWhole ? 2 : 1;
 };
 
 // bf16 rows of whole tiles, where two buffers fit.
@@ -636,7 +705,7 @@ constexpr bool kHasDirect = __is_same(T, bf16) && ChainSize<T, NP, KP, kDirect>:
 
 // Tiles that leave room for one workgroup on a CU: four wavefronts to it instead of two, where there are columns for them.
 template <typename T, int NP, int KP>
-constexpr bool kHasFour = __is_same(T, bf16) && NP == 1 && KP == 128;
+constexpr bool kHasFour = kHalves<T, NP> && KP == 128;
 
 // The states from chunk to chunk, and o (kOutputs); or Z and the state before each chunk for the backward (kKeep); or all of
 // these (kBoth); or what each segment but the last makes of the state before it (kAcross): its end from zero, and behind those
@@ -652,7 +721,7 @@ enum What { kOutputs, kKeep, kBoth, kAcross };
 template <typename T, int NP, int KP, int MODE, int WHAT, int NW>
 __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void dr_chain(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
-  constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
+  constexpr int NI = Z::NI, C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
   constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
   constexpr bool OUT = WHAT == kOutputs || WHAT == kBoth, KEEP = WHAT == kKeep || WHAT == kBoth;  // !OUT: no q and no o
   extern __shared__ __align__(16) unsigned char chain_lds[];
@@ -749,10 +818,11 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
     fetch(t0 + C, buf ^ DIRECT);
     f32x4 y[NB];
     // X = V - G k S
-    Frag<NI> even[2][NB], odd[2][NB];
-    auto rows = [&](const Tile<NI, R, PL, DIRECT>& t, Frag<NI> (&f)[2][NB], int s) {
+    constexpr int ST = Z::STEPS;
+    Frag<NI> even[ST][NB], odd[ST][NB];
+    auto rows = [&](const Tile<NI, R, PL, DIRECT>& t, Frag<NI> (&f)[ST][NB], int s) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < ST; ++i)
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) f[i][rb] = t.rows(16 * rb, s + i);
       phase();
@@ -760,10 +830,8 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
     rows(tk, even, 0);
     Frag<NP> sf[KP / 32];
 #pragma unroll
-    for (int s = 0; s < KP / 32; ++s) {
-      sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
-      if (KEEP) keep<NP, true>(a.s + (ch * NP * KP + 32 * s) * a.vp + n0, a.vp, (int64_t)KP * a.vp, sf[s]);
-    }
+    for (int s = 0; s < KP / 32; ++s) sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
+    if constexpr (KEEP) keep_state<T, NP, KP>(a.s, a.es, ch, a.vp, n0, S, sf);
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) y[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
     Frag<NP> tr[NB][NB / 2];
@@ -775,12 +843,12 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
       phase();
     };
 #pragma unroll
-    for (int s = 0; s < KP / 32; s += 2) {
-      Frag<NI> (&now)[2][NB] = s % 4 ? odd : even, (&then)[2][NB] = s % 4 ? even : odd;
-      if (s + 2 < KP / 32) rows(tk, then, s + 2);
+    for (int s = 0; s < KP / 32; s += ST) {
+      Frag<NI> (&now)[ST][NB] = s / ST % 2 ? odd : even, (&then)[ST][NB] = s / ST % 2 ? even : odd;
+      if (s + ST < KP / 32) rows(tk, then, s + ST);
       else square(tt);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < ST; ++i)
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) y[rb] = mma(now[i][rb], sf[s + i], y[rb]);
       phase();
@@ -793,12 +861,12 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
       for (int e = 0; e < 8 && e < NK; ++e) kc[e0 / 8 % 2][e] = tk.cols((e0 + e) % KN, (e0 + e) / KN);
       phase();
     };
-    keys(0);
+    if (ST > 1) keys(0);
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] -= *reinterpret_cast<const f32x4*>(&sc[0][16 * rb + 4 * g]) * y[rb];
-    Frag<NR> f[C / 32], d[C / 32];
+    Frag<NP> f[C / 32], d[C / 32];
 #pragma unroll
-    for (int s = 0; s < C / 32; ++s) f[s] = pack<NR>(x[2 * s], x[2 * s + 1]);
+    for (int s = 0; s < C / 32; ++s) f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
     // Z = T X
 #pragma unroll
     for (int rb = 0; rb < NB; ++rb) x[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -806,14 +874,21 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
     for (int s = 0; s < NB / 2; ++s)
 #pragma unroll
       for (int rb = 2 * s; rb < NB; ++rb) x[rb] = mma(tr[rb][s], f[s], x[rb]);
+    if (ST == 1) keys(0);  // two parts' T has left its registers by now
 #pragma unroll
     for (int kb = 0; kb < KN; ++kb) S[kb] *= gc;
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) {
-      f[s] = pack<NR>(x[2 * s], x[2 * s + 1]);
-      if (KEEP) keep<NP, false>(a.z + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, first<NP>(f[s]));
-      d[s] = pack<NR>(x[2 * s] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 4 * g]),
+      f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
+      if constexpr (KEEP && !kHalves<T, NP>) keep<NP, false>(a.z + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, f[s]);
+      d[s] = pack<NP>(x[2 * s] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 4 * g]),
                       x[2 * s + 1] * *reinterpret_cast<const f32x4*>(&sc[1][32 * s + 16 + 4 * g]));
+    }
+    if constexpr (KEEP && kHalves<T, NP>) {
+      const Half half(x);
+#pragma unroll
+      for (int s = 0; s < C / 32; ++s) keep<1, false>(a.z + (ch * C + 32 * s) * a.vp + n0, a.vp, 0, half(x[2 * s], x[2 * s + 1]));
+      a.ez[(ch * 4 + g) * a.vp + nn] = (uint8_t)half.byte;
     }
     phase();
     // S <- G_C S + k^T D b Z
@@ -833,12 +908,12 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
 #pragma unroll
       for (int rb = 0; rb < NB; ++rb) y[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < KP / 32; s += 2) {
-        Frag<NI> (&now)[2][NB] = s % 4 ? odd : even, (&then)[2][NB] = s % 4 ? even : odd;
-        if (s + 2 < KP / 32) rows(tq, then, s + 2);
+      for (int s = 0; s < KP / 32; s += ST) {
+        Frag<NI> (&now)[ST][NB] = s / ST % 2 ? odd : even, (&then)[ST][NB] = s / ST % 2 ? even : odd;
+        if (s + ST < KP / 32) rows(tq, then, s + ST);
         else square(tp);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < ST; ++i)
 #pragma unroll
           for (int rb = 0; rb < NB; ++rb) y[rb] = mma(sf[s + i], now[i][rb], y[rb]);
         phase();
@@ -885,7 +960,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
 template <typename T, int NP, int KP, int MODE, bool ACROSS, int NW>
 __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, NP, KP, MODE>::WAVES : 1)) void dr_chain_bwd(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
-  constexpr int NI = Z::NI, NR = held(NP), C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
+  constexpr int NI = Z::NI, C = Z::C, NB = Z::NB, R = Z::R, PL = Z::PL, RC = Z::RC, PC = Z::PC;
   constexpr bool DIRECT = Z::DIRECT, WHOLE = MODE != kGather;
   extern __shared__ __align__(16) unsigned char chain_lds[];
   float (*lv)[4][C] = reinterpret_cast<float (*)[4][C]>(chain_lds);
@@ -966,27 +1041,26 @@ __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, 
     const float gc = expf(vec.top);
     fetch(t0 - C, buf ^ DIRECT);
     auto at = [&](int m, int row) { return *reinterpret_cast<const f32x4*>(&sc[m][row + 4 * g]); };
-    Frag<NI> even[2][NB], odd[2][NB];
-    auto rows = [&](Frag<NI> (&f)[2][NB], int s) {
+    constexpr int ST = Z::STEPS;
+    Frag<NI> even[ST][NB], odd[ST][NB];
+    auto rows = [&](Frag<NI> (&f)[ST][NB], int s) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < ST; ++i)
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) f[i][rb] = tk.rows(16 * rb, s + i);
       phase();
     };
     rows(even, 0);
     Frag<NP> sf[KP / 32];
-    Frag<NR> gd[C / 32], f[C / 32];
+    Frag<NP> gd[C / 32], f[C / 32];
     Frag<NI> df[C / 32];
 #pragma unroll
-    for (int s = 0; s < KP / 32; ++s) {
-      sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
-      if (!ACROSS) keep<NP, true>(a.ds + (ch * NP * KP + 32 * s) * a.vp + n0, a.vp, (int64_t)KP * a.vp, sf[s]);
-    }
+    for (int s = 0; s < KP / 32; ++s) sf[s] = pack<NP>(S[2 * s], S[2 * s + 1]);
+    if constexpr (!ACROSS) keep_state<T, NP, KP>(a.ds, a.eds, ch, a.vp, n0, S, sf);
 #pragma unroll
     for (int s = 0; s < C / 32; ++s) {
       df[s] = pack<NI>(x[2 * s], x[2 * s + 1]);
-      gd[s] = pack<NR>(x[2 * s] * at(2, 32 * s), x[2 * s + 1] * at(2, 32 * s + 16));
+      gd[s] = pack<NP>(x[2 * s] * at(2, 32 * s), x[2 * s + 1] * at(2, 32 * s + 16));
     }
     // Y = P^T dO + b D k dS
 #pragma unroll
@@ -1000,12 +1074,12 @@ __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, 
       phase();
     };
 #pragma unroll
-    for (int s = 0; s < KP / 32; s += 2) {
-      Frag<NI> (&now)[2][NB] = s % 4 ? odd : even, (&then)[2][NB] = s % 4 ? even : odd;
-      if (s + 2 < KP / 32) rows(then, s + 2);
+    for (int s = 0; s < KP / 32; s += ST) {
+      Frag<NI> (&now)[ST][NB] = s / ST % 2 ? odd : even, (&then)[ST][NB] = s / ST % 2 ? even : odd;
+      if (s + ST < KP / 32) rows(then, s + ST);
       else square(tp);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < ST; ++i)
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) x[rb] = mma(now[i][rb], sf[s + i], x[rb]);
       phase();
@@ -1028,7 +1102,7 @@ __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, 
     };
     keys(tq, 0);
 #pragma unroll
-    for (int s = 0; s < C / 32; ++s) f[s] = pack<NR>(x[2 * s], x[2 * s + 1]);
+    for (int s = 0; s < C / 32; ++s) f[s] = pack<NP>(x[2 * s], x[2 * s + 1]);
 #pragma unroll
     for (int kb = 0; kb < KN; ++kb) S[kb] *= gc;
 #pragma unroll
@@ -1060,8 +1134,8 @@ __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, 
           if (!ACROSS) put_columns<T, WHOLE>(dv + (int64_t)t0 * p.dvs[2], p.dvs[2], V - n0, cnt, 16 * rb, x[rb]);
 #pragma unroll
         for (int s = 0; s < C / 32; ++s) {
-          if (!ACROSS && !kFromDv<T, NP>) keep<NP, false>(a.x + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, pack<NP>(x[2 * s], x[2 * s + 1]));
-          f[s] = pack<NR>(-x[2 * s] * at(0, 32 * s), -x[2 * s + 1] * at(0, 32 * s + 16));
+          if (!ACROSS && !kHalves<T, NP>) keep<NP, false>(a.x + (ch * NP * C + 32 * s) * a.vp + n0, a.vp, (int64_t)C * a.vp, pack<NP>(x[2 * s], x[2 * s + 1]));
+          f[s] = pack<NP>(-x[2 * s] * at(0, 32 * s), -x[2 * s + 1] * at(0, 32 * s + 16));
         }
       }
       phase();
@@ -1159,15 +1233,20 @@ __global__ __launch_bounds__(256) void dr_across(Args a) {
 // of which the states and their gradients are 0.27 (4.2 TB/s); with two value heads to a key head, whose sums leave one
 // workgroup to a CU for two, 455 us for B2 T8192 H32 (1.3 GB, 2.9 TB/s).
 template <typename T, int NP, int KP, bool WHOLE, bool ONE>
-__global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && parts_of<T>() == 1) ? 2 : 1) void dr_grads(Args a) {
+__global__ __launch_bounds__(256, ONE && KP <= 128 && parts_of<T>() == 1 ? 2 : 1) void dr_grads(Args a) {
   constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
-  constexpr int NCB = KP / 64, RV = kPiece + 8, PV = C * RV, NU = NB * NB / 4;
-  constexpr int ROWS = (NI + 2 * NP) * PV, KEYS = 2 * NI * PL;
+  constexpr bool HALF = kHalves<T, NP>;
+  // columns of v at once: 64 where LDS then has room for two workgroups and registers have too
+  constexpr int PIECE = HALF && ONE && KP <= 128 ? 64 : 128, NX = HALF ? 1 : NP, ND = planes(HALF, NP);
+  constexpr int NCB = KP / 64, RV = PIECE + 8, PV = C * RV, NU = NB * NB / 4;
+  constexpr int ROWS = (NI + NP + NX) * PV, KEYS = 2 * NI * PL;
   __shared__ __align__(16) bf16 mem[ROWS > KEYS ? ROWS : KEYS], lm[2 * NP * PC];
   __shared__ __align__(16) float lv[kVecs][C];
   __shared__ float diag[C], red[3][4][C], total[4], along[2][C];
+  __shared__ __align__(16) float powers[2][4][HALF ? PIECE : 4];  // of the states' and their gradients' lanes
   const Tile<NI, RV, PV> to{mem};
-  const Tile<NP, RV, PV> tu{mem + NI * PV}, tx{mem + (NI + NP) * PV};
+  const Tile<NP, RV, PV> tz{mem + NI * PV};
+  const Tile<NX, RV, PV> tx{mem + (NI + NP) * PV};
   const Tile<NI, R, PL> tk{mem}, tq{mem + NI * PL};
   const Tile<NP, RC, PC> pe{lm}, ne{lm + NP * PC};  // row j, column i
   const DrProblem& p = a.p;
@@ -1213,31 +1292,42 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
 #pragma unroll
     for (int i = 0; i < NU; ++i) accp[i] = accn[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float dot = 0.f;
-    for (int v0 = 0; v0 < a.vp; v0 += kPiece) {
-      const int width = min(kPiece, a.vp - v0);
+    for (int v0 = 0; v0 < a.vp; v0 += PIECE) {
+      const int width = min(PIECE, a.vp - v0);
       if (v0 > 0) __syncthreads();
-      Frag<NP> fs[2][NCB], fd[2][NCB];  // the states' operands of a step and the next
+      Frag<ND> fs[2][NCB], fd[2][NCB];  // the states of a step and the next, as they lie in memory
       auto states = [&](int s) {
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
-          const int64_t at = ch * NP * KP * a.vp + (int64_t)(wv * NCB * 16 + 16 * cb + col) * a.vp + v0 + 32 * s + 8 * g;
+          const int64_t at = ch * ND * KP * a.vp + (int64_t)(wv * NCB * 16 + 16 * cb + col) * a.vp + v0 + 32 * s + 8 * g;
 #pragma unroll
-          for (int i = 0; i < NP; ++i) {
+          for (int i = 0; i < ND; ++i) {
             fs[s % 2][cb].p[i] = *reinterpret_cast<const u32x4*>(a.s + at + (int64_t)i * KP * a.vp);
             fd[s % 2][cb].p[i] = *reinterpret_cast<const u32x4*>(a.ds + at + (int64_t)i * KP * a.vp);
           }
         }
       };
       {
-        constexpr bool DV = kFromDv<T, NP>;
-        Rows<T, C, kPiece, 256, WHOLE> ro, rv;
-        Rows<bf16, C, kPiece, 256, true> ru[DV ? 1 : 2 * NP];
+        Rows<T, C, PIECE, 256, WHOLE> ro, rv;
+        Rows<bf16, C, PIECE, 256, true> rz[HALF ? 1 : 2 * NP];
         ro.load(d_o + v0, p.dos[2], V - v0, cnt);
-        if constexpr (DV) rv.load(dv + v0, p.dvs[2], V - v0, cnt);
+        if constexpr (HALF) rv.load(dv + v0, p.dvs[2], V - v0, cnt);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          ru[i].load(a.z + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
-          if constexpr (!DV) ru[NP + i].load(a.x + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
+        for (int i = 0; i < ND; ++i) {
+          rz[i].load(a.z + (ch * ND + i) * C * a.vp + v0, a.vp, width, C);
+          if constexpr (!HALF) rz[NP + i].load(a.x + (ch * NP + i) * C * a.vp + v0, a.vp, width, C);
+        }
+        u32x2 ez = {0, 0};
+        uint32_t ep[HALF ? 2 * PIECE / 64 : 1];
+        if constexpr (HALF) {  // exponents: Z's of this thread's columns (its rows are of one lane's kind), the states' shared
+          const int c0 = t % (PIECE / 8) * 8, kind = t / (PIECE / 8) % 16 / 4;
+          static_assert(256 / (PIECE / 8) % 16 == 0, "a thread's rows");
+          if (c0 < width) ez = *reinterpret_cast<const u32x2*>(a.ez + (ch * 4 + kind) * a.vp + v0 + c0);
+#pragma unroll
+          for (int i = 0; i < 2 * PIECE / 64; ++i) {
+            const int e = i * 256 + t, c = e % PIECE, m = e / PIECE;
+            ep[i] = c < width ? (m < 4 ? a.es : a.eds)[(ch * 4 + m % 4) * a.vp + v0 + c] : 0;
+          }
         }
         float vec[(kVecs * C + 255) / 256];
         if (v0 == 0)
@@ -1245,55 +1335,79 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
           for (int i = 0; i * 256 < kVecs * C; ++i) vec[i] = a.vec[ch * kVecs * C + i * 256 + t];
         states(0);
         ro.template store<RV, PV, false>(mem);
-        if constexpr (DV) rv.template store<RV, PV, false>(mem + 2 * PV);
+        if constexpr (HALF) {
+          rv.template store<RV, PV, false>(mem + (NI + NP) * PV);
+          const f32x4 by[2] = {{power(ez[0] & 0xFF), power(ez[0] >> 8 & 0xFF), power(ez[0] >> 16 & 0xFF), power(ez[0] >> 24)},
+                               {power(ez[1] & 0xFF), power(ez[1] >> 8 & 0xFF), power(ez[1] >> 16 & 0xFF), power(ez[1] >> 24)}};
+          store_halves<RV, PV>(rz[0], by, mem + NI * PV);
 #pragma unroll
-        for (int i = 0; i < (DV ? 1 : 2 * NP); ++i) ru[i].template store<RV, PV, false>(mem + (NI + i) * PV);
+          for (int i = 0; i < 2 * PIECE / 64; ++i) (&powers[0][0][0])[i * 256 + t] = power(ep[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2 * NP; ++i) rz[i].template store<RV, PV, false>(mem + (NI + i) * PV);
+        }
         if (v0 == 0)
 #pragma unroll
           for (int i = 0; i * 256 < kVecs * C; ++i) lv[0][i * 256 + t] = vec[i];
       }
       __syncthreads();
 #pragma unroll
-      for (int s = 0; s < kPiece / 32; ++s) {
+      for (int s = 0; s < PIECE / 32; ++s) {
         if (s * 32 >= width) break;
         if ((s + 1) * 32 < width) states(s + 1);
-        const Frag<NP> (&gs)[NCB] = fs[s % 2], (&gd)[NCB] = fd[s % 2];
+        Frag<NP> gs[NCB], gd[NCB];
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+          if constexpr (HALF) {
+            auto by = [&](int m) { return &powers[m][((wv * NCB + cb) % 2 * 16 + col) / 8][32 * s + 8 * g]; };  // of this channel's lanes
+            float x[8], y[8];
+            f32x4 w[2];
+            __builtin_memcpy(w, __builtin_assume_aligned(by(0), 16), 32);
+            gs[cb] = halves(fs[s % 2][cb].p[0], w, x);
+            __builtin_memcpy(w, __builtin_assume_aligned(by(1), 16), 32);
+            gd[cb] = halves(fd[s % 2][cb].p[0], w, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dot += x[e] * y[e];
+          } else {
+            gs[cb] = fs[s % 2][cb];
+            gd[cb] = fd[s % 2][cb];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float x[2] = {0.f, 0.f}, y[2] = {0.f, 0.f};
+#pragma unroll
+              for (int i = NP - 1; i >= 0; --i) {
+                x[0] += __uint_as_float(gs[cb].p[i][e] << 16);
+                x[1] += __uint_as_float(gs[cb].p[i][e] & 0xFFFF0000u);
+                y[0] += __uint_as_float(gd[cb].p[i][e] << 16);
+                y[1] += __uint_as_float(gd[cb].p[i][e] & 0xFFFF0000u);
+              }
+              dot += x[0] * y[0] + x[1] * y[1];
+            }
+          }
+        }
         const Frag<NI> uo = to.rows(16 * rbu, s);
-        const Frag<NP> ux = tx.rows(16 * rbu, s);
+        const Frag<NX> ux = tx.rows(16 * rbu, s);
         if constexpr (NB == 2) {
-          const Frag<NP> uu = tu.rows(16 * (wv / 2), s);
-          accp[0] = mma(uo, uu, accp[0]);
-          accn[0] = mma(ux, uu, accn[0]);
+          const Frag<NP> uz = tz.rows(16 * (wv / 2), s);
+          accp[0] = mma(uo, uz, accp[0]);
+          accn[0] = mma(ux, uz, accn[0]);
         }
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
           const Frag<NI> ro = to.rows(16 * rb, s);
-          const Frag<NP> rx = tx.rows(16 * rb, s), ru = tu.rows(16 * rb, s);
+          const Frag<NX> rx = tx.rows(16 * rb, s);
+          const Frag<NP> rz = tz.rows(16 * rb, s);
           if constexpr (NB == 4) {
-            accp[rb] = mma(uo, ru, accp[rb]);
-            accn[rb] = mma(ux, ru, accn[rb]);
+            accp[rb] = mma(uo, rz, accp[rb]);
+            accn[rb] = mma(ux, rz, accn[rb]);
           }
 #pragma unroll
           for (int cb = 0; cb < NCB; ++cb) {
             dq[rb][cb] = mma(gs[cb], ro, dq[rb][cb]);
             dr[rb][cb] = mma(gs[cb], rx, dr[rb][cb]);
-            dw[rb][cb] = mma(gd[cb], ru, dw[rb][cb]);
+            dw[rb][cb] = mma(gd[cb], rz, dw[rb][cb]);
           }
         }
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x[2] = {0.f, 0.f}, y[2] = {0.f, 0.f};
-#pragma unroll
-            for (int i = NP - 1; i >= 0; --i) {
-              x[0] += __uint_as_float(gs[cb].p[i][e] << 16);
-              x[1] += __uint_as_float(gs[cb].p[i][e] & 0xFFFF0000u);
-              y[0] += __uint_as_float(gd[cb].p[i][e] << 16);
-              y[1] += __uint_as_float(gd[cb].p[i][e] & 0xFFFF0000u);
-            }
-            dot += x[0] * y[0] + x[1] * y[1];
-          }
       }
     }
     Rows<T, C, KP, 256, WHOLE> rk, rq;
@@ -1315,7 +1429,7 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
           const float E = kj * __builtin_amdgcn_exp2f(((hi[r] - hj) + (lo[r] - lj)) * 1.44269504088896f);
           vp[r] = j <= x ? qi[r] * E * accp[i][r] : 0.f;
           vn[r] = j < x ? -ki[r] * E * accn[i][r] : 0.f;
-          if (x == j) diag[x] = accn[i][r];
+          if (!HALF && x == j) diag[x] = accn[i][r];
         }
         const int where = j * RC + spot(16 * rbu + 4 * g);
 #pragma unroll
@@ -1421,7 +1535,7 @@ __global__ __launch_bounds__(256, ONE && KP <= 128 && (NP == 1 || NP == 3 && par
         c += (total[0] + total[1]) + (total[2] + total[3]);
         const float be = lv[kB][i];
         put_gate(p.dg, p.gdtype, b * p.dgs[0] + h * p.dgs[1] + (t0 + lane) * p.dgs[2], in ? c : 0.f);
-        put_gate(p.db, p.gdtype, b * p.dbs[0] + h * p.dbs[1] + (t0 + lane) * p.dbs[2], in ? diag[i] / be : 0.f);
+        put_gate(p.db, p.gdtype, b * p.dbs[0] + h * p.dbs[1] + (t0 + lane) * p.dbs[2], in ? (HALF ? s[2] : diag[i]) / be : 0.f);
       }
     }
   }
@@ -1502,7 +1616,7 @@ hipError_t launch(Stage st, const Args& a, int mode, hipStream_t stream) {
   };
   return mode != kGather ? size(std::true_type()) : size(std::false_type());
 }
-extern template hipError_t launch<bf16, 1>(Stage, const Args&, int, hipStream_t);
+extern template hipError_t launch<bf16, 2>(Stage, const Args&, int, hipStream_t);
 extern template hipError_t launch<bf16, 3>(Stage, const Args&, int, hipStream_t);
 extern template hipError_t launch<fp16, 2>(Stage, const Args&, int, hipStream_t);
 extern template hipError_t launch<fp16, 3>(Stage, const Args&, int, hipStream_t);

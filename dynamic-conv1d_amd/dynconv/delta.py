@@ -129,10 +129,11 @@ def gated_delta_rule(
         (o, state [B, H, K, V] float32).  Every input but lengths has a gradient.
 
     Values are finite: an infinity or NaN reaches its head's outputs from the start of its block of up to 64 tokens on.  In 16
-    bits products run on matrix cores with float32 sums; what they take of the states and corrections is rounded to the inputs'
-    type (fp16: to 16 bits), unless a result is float32: a returned state, or a gradient of float32 gates or of the initial
-    state.  Then everything is as good as float32, at about twice the time.  Where a backward may follow, the states of each block
-    stay in memory for it if they take at most twice that of q, k, v and o.
+    bits products run on matrix cores with float32 sums; what they take of the states and corrections has 16 bits (for a backward
+    in bf16 11, and v's gradients their own 8), so that results are good to little more than their own rounding, unless a
+    result is float32: a returned state, or a gradient of float32 gates or of the initial state.  Then everything is as good as
+    float32, at two to three times the time.  A |beta| below 2^-60 counts as 2^-60.  Where a backward may follow, the states of
+    each block stay in memory for it if they take at most twice that of q, k, v and o.
     """
     if _capi.binding is not None:
         out = _capi.binding.gated_delta_rule(q, k, v, log_decay, beta, scale, initial_state, lengths, return_state, normalize, eps)

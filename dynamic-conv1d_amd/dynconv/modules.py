@@ -316,7 +316,7 @@ class DynamicDeltaRule(_RecurrentLayer):
 
     forward(x) takes whole sequences [B, T, d_model]; step(x, state) one token [N, d_model] of each sequence.  The gates
     are computed in float32 and passed on in the type `gates`: None, x's (in 16 bits they are rounded to it, and no gradient
-    is float32), or torch.float32, which keeps their bits, at about twice the rule's time in training.
+    is float32), or torch.float32, which keeps their bits, at two to three times the rule's time in training.
     """
 
     def __init__(self, d_model: int, heads: int, R: int, W: int, eps: float = 1e-5, gates: torch.dtype | None = None):
