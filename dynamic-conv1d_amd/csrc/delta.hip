@@ -34,9 +34,7 @@ using dr::Stage;
 int np_of(const DrProblem& p) { return p.dtype == kFP32 || p.precise ? 3 : 2; }
 // Halves in memory (delta_mfma.h).
 bool halves(const DrProblem& p) { return p.dtype == kBF16 && !p.precise; }
-int chunk(const DrProblem& p) {
-  return dr::chunk_of(p.dtype == kFP32 ? 3 : p.dtype == kFP16 ? 2 : 1, np_of(p), dr::cover((int)p.K));
-}
+int chunk(const DrProblem& p) { return dr::chunk_of(np_of(p), dr::cover((int)p.K)); }
 
 // How the chains are cut: segments of the tokens, where heads and columns leave CUs idle (one launch finds what each makes of
 // the state before it, a second carries the states across, and the chains run side by side), and wavefronts of a workgroup
@@ -44,7 +42,8 @@ int chunk(const DrProblem& p) {
 // outputs (with the unit vectors' columns, twice as many where K is V), in rounds of the workgroups that fit (small tiles
 // let wavefronts share SIMDs, at 0.65 of a round for another), and the launches.  Measured, bf16, us (* is what it takes):
 // forward of B1 H16 T8192 hd128, 1 segment 427, 2 383, 4 231, 8 176 *, 16 202; B1 H2 T16384 hd128, 8 205, 16 151, 26 154 *,
-// 32 159; B1 H16 T32768 hd128 with its state, 1 2845, 4 1530, 8 950, 16 816 *; B1 H4 T2048 hd256, 1 456, 4 198, 8 177 *.
+// 32 159; B1 H16 T32768 hd128 with its state, 1 2845, 4 1530, 8 950, 16 816 *; B1 H4 T2048 hd256, 1 237, 4 141 *, 8 147,
+// 16 235 (its transitions are carried at 12 us a segment).
 // Training of B4 H32 T2048 hd128: workgroups of 2 wavefronts 864, of 4 624 *; of B4 H16 T4096, 2 818 *, 4 891.
 struct Cut {
   int nseg, nw;
@@ -52,11 +51,11 @@ struct Cut {
 Cut cut_of(const DrProblem& p, int C, int np) {
   const int kp = dr::cover((int)p.K), vp = ((int)p.V + 31) / 32 * 32;
   const int64_t chunks = (p.T + C - 1) / C, heads = p.B * p.H;
-  const bool one = halves(p) && kp == 128;  // workgroup on a CU; elsewhere two
+  const bool one = halves(p) && kp >= 128;  // workgroup on a CU; elsewhere two
   const bool shares = np == 3 && kp == 128 && p.dtype == kBF16;  // two or, of more than 512, four (delta_mfma.h)
   double best = -1;
   Cut cut{1, 2};
-  for (int nw = 2; nw <= (one && vp % 64 == 0 ? 4 : 2); nw += 2) {
+  for (int nw = 2; nw <= (one && kp == 128 && vp % 64 == 0 ? 4 : 2); nw += 2) {
     auto rounds = [&](double wgs, bool small) {
       if (shares && !small) return wgs <= 512 ? 1 : 1.6 * wgs / 1024 > 0.6 + wgs / 1024 ? 1.6 * wgs / 1024 : 0.6 + wgs / 1024;
       return small ? (wgs <= 512 ? 1 : 0.35 + 0.65 * wgs / 512) : __builtin_ceil(wgs / (one ? 256 : 512));
@@ -69,7 +68,7 @@ Cut cut_of(const DrProblem& p, int C, int np) {
       double t = us * len * rounds((double)heads * s * (vp / cols), np == 3 && kp == 64);
       if (s > 1)
         t += (shares ? 0.65 : 0.8) * us * len * rounds((double)heads * (s - 1) * ((vp + kp) / cols), true) +
-             (shares ? 5 + 3 * s : 15 + 2 * s);
+             (shares ? 5 + 3 * s : 15 + (kp == 256 && np == 2 ? 12 : 2) * s);
       if (best < 0 || t < best) {
         best = t;
         cut = {s, nw};

@@ -34,8 +34,9 @@ template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __i
 // What goes through memory for the gradients is halves, and dX dv itself (B4 T4096 H16 hd128: 67 MB less to write).
 template <typename T, int NP> constexpr bool kHalves = __is_same(T, bf16) && NP == 2;
 constexpr int planes(bool halves, int np) { return halves ? 1 : np; }  // 16-bit words of a value there
-// Tokens of a chunk: 64, or 32 where tiles of 64 would pass the LDS (np: parts of what is computed, ni: of q and k).
-__host__ __device__ constexpr int chunk_of(int ni, int np, int kp) { return np == 3 || ni * kp > 256 ? 32 : 64; }
+// Tokens of a chunk: 64, or 32 where tiles of 64 would pass the LDS (three parts) or it and the registers (256 channels: B2 T4096
+// H8 training in bf16 2509 us with 64, 1410 with 32).  np: parts of what is computed.
+__host__ __device__ constexpr int chunk_of(int np, int kp) { return np == 3 || kp == 256 ? 32 : 64; }
 __host__ __device__ constexpr int cover(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : 256; }
 
 struct Args {
@@ -278,7 +279,7 @@ __device__ __forceinline__ void put_gate(void* t, int gdtype, int64_t i, float v
 // what it waits for is the substitution's 16 steps and the barriers around them, and the four hide each other's.
 template <typename T, int NP, int KP, bool WHOLE>
 __global__ __launch_bounds__(256) void dr_prep(Args a) {
-  constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RA = C + 4;
+  constexpr int NI = parts_of<T>(), C = chunk_of(NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RA = C + 4;
   constexpr int TILES = 2 * NI * PL * 2, MATS = 2 * C * RA * 4;
   __shared__ __align__(16) unsigned char mem[TILES > MATS ? TILES : MATS];
   // of each token: c in two parts, b, 1/|k|, 1/|q|, the factors of A's and P's rows 1/|k| and scale/|q| and of their columns b/|k|
@@ -690,7 +691,7 @@ constexpr bool kShares = __is_same(T, bf16) && NP == 3 && KP == 128;
 template <typename T, int NP, int KP, int MODE>
 struct ChainSize {
   static constexpr bool DIRECT = MODE == kDirect;
-  static constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + (DIRECT ? 0 : 24), PL = C * R,
+  static constexpr int NI = parts_of<T>(), C = chunk_of(NP, KP), NB = C / 16, R = KP + (DIRECT ? 0 : 24), PL = C * R,
                        RC = C + (DIRECT ? 0 : 8), PC = C * RC;
   // steps of an operands' batch, one ahead of the products: two parts' products of one step take as long as one part's of two
   static constexpr int STEPS = NP == 2 ? 1 : 2;
@@ -1234,7 +1235,7 @@ __global__ __launch_bounds__(256) void dr_across(Args a) {
 // workgroup to a CU for two, 455 us for B2 T8192 H32 (1.3 GB, 2.9 TB/s).
 template <typename T, int NP, int KP, bool WHOLE, bool ONE>
 __global__ __launch_bounds__(256, ONE && KP <= 128 && parts_of<T>() == 1 ? 2 : 1) void dr_grads(Args a) {
-  constexpr int NI = parts_of<T>(), C = chunk_of(NI, NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
+  constexpr int NI = parts_of<T>(), C = chunk_of(NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
   constexpr bool HALF = kHalves<T, NP>;
   // columns of v at once: 64 where LDS then has room for two workgroups and registers have too
   constexpr int PIECE = HALF && ONE && KP <= 128 ? 64 : 128, NX = HALF ? 1 : NP, ND = planes(HALF, NP);
