@@ -103,9 +103,9 @@ struct Plan {
     seg = (int)((n + nseg - 1) / nseg) * C;
     cut = nseg > 1 ? (p.B * p.H * nseg * p.K * p.V * 4 + 15) / 16 * 16 : 0;
     trans = nseg > 1 ? p.B * p.H * nseg * kp * kp * 4 : 0;
-    // saves the backward a launch: training of B4 H16 T4096 hd128 in bf16 824 -> 730 us for 201 MB, 0.75 of q, k, v and o;
-    // of B2 T2048 with 8 | 16 heads of 64 x 128 and float32 gates 47 of 390 us would take 3.6 times their memory
     from_dv = halves(p);
+    // saves the backward a launch: training of B4 H16 T4096 hd128 in bf16 956 -> 816 us for 201 MB, 0.75 of q, k, v and o;
+    // of B2 T2048 with 8 | 16 heads of 64 x 128 and float32 gates 48 of 377 us would take 3.6 times their memory
     kept = p.keep && rows + st <= 2 * p.B * p.T * (p.Hk * 2 * p.K + p.H * 2 * p.V) * dtype_size(p.dtype);
   }
   int64_t fwd() const { return vec + 2 * sq + trans + cut + 2 * ex + (kept ? rows + st : 0); }

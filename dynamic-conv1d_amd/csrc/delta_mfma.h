@@ -13,7 +13,7 @@
 // of each lane's own (Half), and dX is dv, whose own rounding it is.  That leaves o, dq and dv at one rounding of their norm
 // (1.7e-3 of it), dk and dlog_decay at 1.1 and dbeta (by k.W: dX.Z would have dX's rounding whole, 1.4) at 1.2.  With one bf16
 // part of each (8 bits) they were 1.5, 1.7, 1.5, 1.9, 2.4 and 2.1 roundings off, in 0.8 of the time (B4 T4096 H16 hd128 training
-// 663 us, 818).  A product of parts keeps those down to the last part's size.
+// 663 us, 814).  A product of parts keeps those down to the last part's size.
 // Sums, S and dS, decays and norms are float32; sums of logarithms of decays are float64.
 #pragma once
 
@@ -35,7 +35,7 @@ template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : __i
 template <typename T, int NP> constexpr bool kHalves = __is_same(T, bf16) && NP == 2;
 constexpr int planes(bool halves, int np) { return halves ? 1 : np; }  // 16-bit words of a value there
 // Tokens of a chunk: 64, or 32 where tiles of 64 would pass the LDS (three parts) or it and the registers (256 channels: B2 T4096
-// H8 training in bf16 2509 us with 64, 1410 with 32).  np: parts of what is computed.
+// H8 training in bf16 2509 us with 64, 1416 with 32).  np: parts of what is computed.
 __host__ __device__ constexpr int chunk_of(int np, int kp) { return np == 3 || kp == 256 ? 32 : 64; }
 __host__ __device__ constexpr int cover(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : 256; }
 
@@ -275,7 +275,7 @@ __device__ __forceinline__ void put_gate(void* t, int gdtype, int64_t i, float v
 }
 
 // What each chunk needs of its own keys: a workgroup of four wavefronts to a chunk of one head, four workgroups to a CU.
-// B4 T4096 H16 hd128 bf16 63 us for 209 MB (3.3 TB/s; 85 before its products' factors came in quads and without branches):
+// B4 T4096 H16 hd128 bf16 68 us for 277 MB (4.1 TB/s; a third slower before its products' factors came in quads, unbranched):
 // what it waits for is the substitution's 16 steps and the barriers around them, and the four hide each other's.
 template <typename T, int NP, int KP, bool WHOLE>
 __global__ __launch_bounds__(256) void dr_prep(Args a) {
@@ -712,11 +712,11 @@ constexpr bool kHasFour = kHalves<T, NP> && KP == 128;
 // these (kBoth); or what each segment but the last makes of the state before it (kAcross): its end from zero, and behind those
 // columns its end from each unit vector without values.
 //
-// A chunk waits for the one before it, so a chain's time is its chunks': 2.8 us each at 128 x 128 in bf16, 3.5 with the
-// states' stores (B4 T4096 H16: 64 chunks, 180 and 225 us, 2.4 TB/s of what the latter moves).  Of that 0.6 us are matrix
-// instructions and 1.7 all instructions of a wavefront that has its SIMD to itself; the rest are latencies, of operands
-// from LDS within a chunk, and of the next chunk's loads, for which a second buffer leaves the time of one chunk and LDS has
-// no third.  Beside each wavefront another for the outputs and one for the loads took 146 us without the stores, but the
+// A chunk waits for the one before it, so a chain's time is its chunks': 3.7 us each at 128 x 128 in bf16, 4.5 with the
+// states' stores (B4 T4096 H16: 64 chunks, 235 and 289 us).  Of that 0.9 us are matrix instructions and about half all
+// instructions of a wavefront that has its SIMD to itself; the rest are latencies, of operands from LDS within a chunk, and of
+// the next chunk's loads, for which a second buffer leaves the time of one chunk and LDS has no third.  With one part of each
+// operand, another wavefront beside each for the outputs and one for the loads took 146 us for 180 without the stores, but the
 // same 222 with them, and lost to four wavefronts where heads abound (B4 T2048 H32 forward 219 us for 175): not here.
 enum What { kOutputs, kKeep, kBoth, kAcross };
 template <typename T, int NP, int KP, int MODE, int WHAT, int NW>
@@ -957,7 +957,7 @@ __global__ __launch_bounds__(NW * 64, (ChainSize<T, NP, KP, MODE>::WAVES)) void 
 
 // The states' gradients from the last chunk on, and dv; ACROSS: only what each segment but the first makes of them from zero
 // (from the state after it they come by the transpose of what the forward found).  As the forward's, with twice its products
-// that the state waits for: 3.5 us a chunk at 128 x 128 in bf16, 221 us at B4 T4096 H16.
+// that the state waits for: 4.2 us a chunk at 128 x 128 in bf16, 267 us at B4 T4096 H16.
 template <typename T, int NP, int KP, int MODE, bool ACROSS, int NW>
 __global__ __launch_bounds__(NW * 64, (ACROSS || MODE == kDirect ? ChainSize<T, NP, KP, MODE>::WAVES : 1)) void dr_chain_bwd(Args a) {
   typedef ChainSize<T, NP, KP, MODE> Z;
@@ -1230,9 +1230,10 @@ __global__ __launch_bounds__(256) void dr_across(Args a) {
 // channels to a wavefront.  With the rows' norms in E's place (rq_i rk_j for P, rk_i rk_j for N) the sums are those of q and
 // k themselves, before their part along the row is taken out.  Results lie turned over, four neighbouring channels of a
 // token in a lane: sums over a row are of a lane's own and three others', and a store has 8 bytes.  ONE: one value head to a
-// key head, whose sums need no registers of their own.  The memory path bounds it: B4 T4096 H16 hd128 bf16 177 us for 0.74 GB,
-// of which the states and their gradients are 0.27 (4.2 TB/s); with two value heads to a key head, whose sums leave one
-// workgroup to a CU for two, 455 us for B2 T8192 H32 (1.3 GB, 2.9 TB/s).
+// key head, whose sums need no registers of their own.  The memory path bounds it, and the halves' way into parts: B4 T4096
+// H16 hd128 bf16 212 us for 0.74 GB, of which the states and their gradients are 0.27 (3.5 TB/s; 177 from one part of each, which
+// needs no way); with two value heads to a key head, whose sums leave one workgroup to a CU for two, 566 us for B2 T8192 H32
+// (1.3 GB, 2.3 TB/s).
 template <typename T, int NP, int KP, bool WHOLE, bool ONE>
 __global__ __launch_bounds__(256, ONE && KP <= 128 && parts_of<T>() == 1 ? 2 : 1) void dr_grads(Args a) {
   constexpr int NI = parts_of<T>(), C = chunk_of(NP, KP), NB = C / 16, R = KP + 8, PL = C * R, RC = C + 8, PC = C * RC;
